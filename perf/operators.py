@@ -254,11 +254,11 @@ def _plain_w4_pack(s):
     g = w.view(w.shape[0], -1, s["G"])
     if s["zeros"]:
         lo, hi = g.amin(2).clamp_max(0.0), g.amax(2).clamp_min(0.0)
-        scales = ((hi - lo) / 15.0).half()
+        scales = ((hi - lo) * (1.0 / 15.0)).half()
         st = scales.float()
         z = torch.where(st > 0, torch.round(-lo / st), 0.0).clamp(0, 15)[:, :, None]
     else:
-        scales = (g.abs().amax(2) / 7.0).half()
+        scales = (g.abs().amax(2) * (1.0 / 7.0)).half()
         st = scales.float()
         z = torch.full_like(st, 8.0)[:, :, None]
     st = st[:, :, None]
@@ -285,7 +285,7 @@ def _plain_written(codes, scale, rows, s):
     before = (torch.arange(J * T, device=dev) < off[:, None]).view(B, J, 1, T, 1)   # rows that the first page held already
     old_codes, old_scale = codes[page], scale[page]
     touched, begun = is_new.any(3)[:, :, :, 0], before.any(3)[:, :, :, 0]
-    new_scale = (grid.abs().amax((3, 4)) / 127.0).clamp_min(1e-30)
+    new_scale = (grid.abs().amax((3, 4)) * (1.0 / 127.0)).clamp_min(1e-30)
     sc = torch.where(begun, torch.maximum(old_scale, new_scale), new_scale)
     q = torch.round(grid / sc[..., None, None]).clamp(-127, 127)
     kept = torch.round(old_codes.float() * (old_scale / sc)[..., None, None])
