@@ -1,0 +1,367 @@
+// Attention next to the quantized linears: cross attention to an encoder's states, and attention over a cache of int8 keys and values.
+//
+//   gpu_cross_attention   q rows of one sequence, k and v rows of another, 16-bit
+//   gpu_kv8_attention     q rows over pages of int8 keys and values, one f32 scale for each page and head
+//
+// o[i] = sum_t p[i, t] v[t] / sum_t p[i, t],  p[i, t] = exp(scale q[i] . k[t] - m[i]), m[i] the largest exponent seen so far; a row that sees
+// no key is zeros. One pass over the keys: the sums are scaled when m grows. Exponents, m and both sums are f32; p is rounded to the type
+// of the matrix product (as its operands have to be) after it entered the sum of p, so that the rounding is at most half a step of each term.
+#include "common.cuh"
+#include "mma.cuh"
+
+#include <type_traits>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTiny = 1e-30f;          // the smallest scale of a page; smaller ones are taken for it
+
+struct AttnParams {
+    const void *q, *k, *v;
+    void* out;
+    int64_t qs[3], ks[3], vs[3], os[3];      // strides of batch, row, head in elements (k and v: 16-bit rows only)
+    const float *k_scale, *v_scale;          // pages: [pages, Hkv]
+    const int32_t* table;                    // [B, max_pages]
+    int64_t table_stride, pages;
+    const int32_t* kv_len;                   // keys of each sequence, or null: Lkv
+    const int32_t* q_len;                    // query rows of each sequence, or null: Lq
+    const uint8_t* mask;                     // [B, Lkv], 0 = not seen, or null
+    int64_t mask_stride;
+    int B, Lq, Lkv, H, Hkv, D, T, causal, splits, row_tiles;
+    float scale;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float dsmem_f32(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, rank)) : "memory");
+    return v;
+}
+
+// Eight int8 codes as eight halves, exact: each byte, its sign bit turned, becomes the low byte of 1024 + (code + 128), and 1152 is taken away.
+__device__ __forceinline__ uint4 halves_of(uint2 w) {
+    const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u, off = 0x64806480u;
+    uint4 r;
+    uint32_t* o = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t v = __byte_perm(i < 2 ? a : b, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
+        const half2 h = __hsub2(*reinterpret_cast<const half2*>(&v), *reinterpret_cast<const half2*>(&off));
+        o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return r;
+}
+
+// 64 query rows (a kv head's queries: row r is query r / ratio, head r % ratio of its group), 64 keys a step, four warps of 16 rows.
+constexpr int kRows = 64, kKeys = 64, kThreads = 128;
+
+template <typename QT, int DP, bool KV8> struct Tile {
+    using T = typename std::conditional<KV8, half, QT>::type;      // of the products
+    static constexpr int kRowBytes = DP * 2, kBytes = kKeys * DP * 2;
+    static constexpr int kStage = KV8 ? kKeys * DP : kBytes;       // K or V of a step as it is loaded
+    // Q | loaded K, V x 2 | (int8: K, V as halves) | per key: factor, offset, weight x 2 | m, l of every row
+    static constexpr int kLoaded = kRows * kRowBytes, kHalves = kLoaded + 4 * kStage, kKeyInfo = kHalves + (KV8 ? 2 * kBytes : 0);
+    static constexpr int kStats = kKeyInfo + 2 * 3 * kKeys * 4, kSmem = kStats + 2 * kRows * 4;
+    static __device__ __forceinline__ uint32_t at(int row, int c) { return (uint32_t)(row * kRowBytes + ((c ^ (row & 7)) * 16)); }
+};
+
+template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThreads) attention_tile_kernel(const AttnParams p) {
+    using L = Tile<QT, DP, KV8>;
+    using T = typename L::T;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits % p.row_tiles, bh = blockIdx.x / p.splits / p.row_tiles;
+    const int b = bh / p.Hkv, kvh = bh % p.Hkv, ratio = p.H / p.Hkv;
+    const int D = p.D, chunks = DP / 8;
+    pdl_wait();
+    const int limit = p.Lkv;
+    const int len = p.kv_len ? min(max(gload(p.kv_len + b), 0), limit) : limit;
+    const int ql = p.q_len ? min(max(gload(p.q_len + b), 0), p.Lq) : p.Lq;
+    const int r0 = rt * kRows, live = min(kRows, ql * ratio - r0);      // rows of this tile that exist
+    if (live <= 0) return;                                              // the same for every CTA of the cluster
+    // keys that the tile's last row sees
+    const int seen = p.causal ? max(0, min(len, len - ql + (r0 + live - 1) / ratio + 1)) : len;
+    const int steps = (seen + kKeys - 1) / kKeys, per = (steps + p.splits - 1) / p.splits;
+    const int first = min(split * per, steps), last = min(first + per, steps);
+
+    const uint32_t base = smem_u32(smem);
+    float* key_mul = reinterpret_cast<float*>(smem + L::kKeyInfo);      // [stage][factor, offset, weight][key]
+    // ---- queries: into shared memory, for int8 keys as halves times a power of two per row (so that bf16's range does no harm)
+    float row_factor[2] = {1.f, 1.f};
+    {
+        const int row = tid >> 1, i = (r0 + row) / ratio, h = kvh * ratio + (r0 + row) % ratio;
+        const QT* src = reinterpret_cast<const QT*>(p.q) + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
+        float mult = 1.f;
+        if constexpr (KV8 && std::is_same<QT, bf16>::value) {
+            float top = 0.f;
+            if (row < live)
+                for (int c = tid & 1; c < D / 8; c += 2) {
+                    const uint4 w = gload(reinterpret_cast<const uint4*>(src) + c);
+                    const QT* x = reinterpret_cast<const QT*>(&w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f<QT>(x[e])));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            // 2^(14 - exponent): the largest lands in [2^14, 2^15). Both it and its inverse are f32 numbers for exponents within 100.
+            const int e = top > 0.f && top <= FLT_MAX ? min(100, max(-100, 14 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+            mult = __uint_as_float((uint32_t)(127 + e) << 23);
+            if ((tid & 1) == 0) reinterpret_cast<float*>(smem + L::kStats)[row] = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+        for (int c = tid & 1; c < chunks; c += 2) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (row < live && c * 8 < D) {
+                w = gload(reinterpret_cast<const uint4*>(src) + c);
+                if constexpr (KV8 && std::is_same<QT, bf16>::value) {
+                    const QT* x = reinterpret_cast<const QT*>(&w);
+                    uint4 y;
+                    uint32_t* o = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = pack2<half>(to_f<QT>(x[2 * e]) * mult, to_f<QT>(x[2 * e + 1]) * mult);
+                    w = y;
+                }
+            }
+            *reinterpret_cast<uint4*>(smem + L::at(row, c)) = w;
+        }
+    }
+    // ---- one step's keys and values on their way
+    auto load = [&](int step, int stage) {
+        const uint32_t ks = base + L::kLoaded + stage * 2 * L::kStage, vs = ks + L::kStage;
+        if constexpr (KV8) {
+            for (int i = tid; i < kKeys * DP / 16; i += kThreads) {
+                const int key = i / (DP / 16), c = i % (DP / 16), at = step * kKeys + key;
+                int64_t page = at < seen ? gload(p.table + b * p.table_stride + at / p.T) : -1;
+                const bool valid = page >= 0 && page < p.pages && c * 16 < D;
+                const int64_t off = valid ? ((page * p.Hkv + kvh) * p.T + at % p.T) * D + c * 16 : 0;
+                cp_async16(ks + i * 16, reinterpret_cast<const int8_t*>(p.k) + off, valid);
+                cp_async16(vs + i * 16, reinterpret_cast<const int8_t*>(p.v) + off, valid);
+            }
+        } else {
+            for (int i = tid; i < kKeys * chunks; i += kThreads) {
+                const int key = i / chunks, c = i % chunks, at = step * kKeys + key;
+                const bool valid = at < seen && c * 8 < D && (!p.mask || gload(p.mask + b * p.mask_stride + at));
+                const QT* k = reinterpret_cast<const QT*>(p.k) + (valid ? b * p.ks[0] + at * p.ks[1] + kvh * p.ks[2] + c * 8 : 0);
+                const QT* v = reinterpret_cast<const QT*>(p.v) + (valid ? b * p.vs[0] + at * p.vs[1] + kvh * p.vs[2] + c * 8 : 0);
+                cp_async16(ks + L::at(key, c), k, valid);
+                cp_async16(vs + L::at(key, c), v, valid);
+            }
+        }
+        // logit (base 2) = product * factor + offset; an offset of -inf is a key that is not seen. With pages the offset is log2 of the
+        // value's scale, so that p carries it and the products take the codes as they are; `weight` takes it out of the sum of p.
+        if (tid < kKeys) {
+            const int at = step * kKeys + tid;
+            bool valid = at < seen;
+            float mul = p.scale * kLog2e, add = 0.f, wt = 1.f;
+            if constexpr (KV8) {
+                const int64_t page = valid ? gload(p.table + b * p.table_stride + at / p.T) : -1;
+                valid = page >= 0 && page < p.pages;
+                if (valid) {
+                    const float s = fmaxf(gload(p.v_scale + page * p.Hkv + kvh), kTiny);
+                    mul *= gload(p.k_scale + page * p.Hkv + kvh), add = log2f(s), wt = 1.f / s;
+                }
+            } else if (valid && p.mask) valid = gload(p.mask + b * p.mask_stride + at) != 0;
+            float* info = key_mul + stage * 3 * kKeys + tid;
+            info[0] = mul, info[kKeys] = valid ? add : -INFINITY, info[2 * kKeys] = valid ? wt : 0.f;
+        }
+    };
+    float o[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+    int bound[2];      // keys that rows g and g + 8 of this warp see
+#pragma unroll
+    for (int h = 0; h < 2; ++h) bound[h] = p.causal ? len - ql + (r0 + warp * 16 + g + 8 * h) / ratio + 1 : len;
+    if (first < last) load(first, 0);
+    cp_async_commit();
+    __syncthreads();
+    if constexpr (KV8 && std::is_same<QT, bf16>::value) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) row_factor[h] = reinterpret_cast<const float*>(smem + L::kStats)[warp * 16 + g + 8 * h];
+    }
+    for (int step = first; step < last; ++step) {
+        const int stage = (step - first) & 1;
+        if (step + 1 < last) load(step + 1, stage ^ 1);
+        cp_async_commit();
+        cp_async_wait<1>();
+        __syncthreads();
+        uint32_t ks = base + L::kLoaded + stage * 2 * L::kStage, vs = ks + L::kStage;
+        if constexpr (KV8) {      // codes -> halves
+            const uint8_t* src = smem + L::kLoaded + stage * 2 * L::kStage;
+            for (int i = tid; i < 2 * kKeys * DP / 8; i += kThreads) {
+                const int which = i / (kKeys * DP / 8), j = i % (kKeys * DP / 8);
+                *reinterpret_cast<uint4*>(smem + L::kHalves + which * L::kBytes + L::at(j / chunks, j % chunks)) =
+                    halves_of(*reinterpret_cast<const uint2*>(src + which * L::kStage + j * 8));
+            }
+            __syncthreads();
+            ks = base + L::kHalves, vs = ks + L::kBytes;
+        }
+        float s[8][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+            uint32_t a[4];
+            ldmatrix4(a, base + L::at(warp * 16 + (lane & 15), 2 * kk + (lane >> 4)));
+#pragma unroll
+            for (int n = 0; n < 8; n += 2) {
+                uint32_t k4[4];
+                ldmatrix4(k4, ks + L::at(n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+                mma16816<T>(s[n], a[0], a[1], a[2], a[3], k4[0], k4[1]);
+                mma16816<T>(s[n + 1], a[0], a[1], a[2], a[3], k4[2], k4[3]);
+            }
+        }
+        const float* info = key_mul + stage * 3 * kKeys;
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = n * 8 + 2 * t + (i & 1), h = i >> 1;
+                const float add = info[kKeys + key];
+                const bool valid = add != -INFINITY && step * kKeys + key < bound[h];
+                s[n][i] = valid ? __fmaf_rn(s[n][i] * row_factor[h], info[key], add) : -INFINITY;
+                top[h] = fmaxf(top[h], s[n][i]);
+            }
+        float keep[2], shift[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+            shift[h] = top[h] == -INFINITY ? 0.f : top[h];
+            keep[h] = exp2_fast(m[h] - shift[h]);
+            m[h] = top[h], l[h] *= keep[h];
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= keep[i >> 1];
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk) {
+            uint32_t a[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = 2 * kk + j;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[n][i] = exp2_fast(s[n][i] - shift[i >> 1]);
+                    l[i >> 1] = __fmaf_rn(s[n][i], KV8 ? info[2 * kKeys + n * 8 + 2 * t + (i & 1)] : 1.f, l[i >> 1]);
+                }
+                a[2 * j] = pack2<T>(s[n][0], s[n][1]), a[2 * j + 1] = pack2<T>(s[n][2], s[n][3]);
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 8; n += 2) {
+                uint32_t v4[4];
+                ldmatrix4_t(v4, vs + L::at(kk * 16 + (lane & 15), n + (lane >> 4)));
+                mma16816<T>(o[n], a[0], a[1], a[2], a[3], v4[0], v4[1]);
+                mma16816<T>(o[n + 1], a[0], a[1], a[2], a[3], v4[2], v4[3]);
+            }
+        }
+        __syncthreads();
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1), l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    // ---- rows out, by way of shared memory; with several CTAs to a row tile each finishes its share of the rows from all of them
+    constexpr int kPitch = DP;
+    float* part = reinterpret_cast<float*>(smem + L::kLoaded);          // [64][DP], over the loaded tiles
+    float* stats = reinterpret_cast<float*>(smem + L::kStats);
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = warp * 16 + g + 8 * h;
+        if (t == 0) stats[row] = m[h], stats[kRows + row] = l[h];
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+            *reinterpret_cast<float2*>(part + row * kPitch + ((n ^ (g & 3)) * 8 + 2 * t)) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    if (p.splits > 1) cluster_sync_all();
+    else __syncthreads();
+    const uint32_t part_at = smem_u32(part), stats_at = smem_u32(stats);
+    const int pieces = (D + 7) / 8;
+    for (int i = tid + split * kThreads; i < live * pieces; i += kThreads * p.splits) {
+        const int row = i / pieces, n = i % pieces;
+        float y[8] = {}, total = 0.f;
+        if (p.splits == 1) {
+            total = stats[kRows + row];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = part[row * kPitch + (n ^ (row & 3)) * 8 + e];
+        } else {
+            float top = -INFINITY;
+            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, dsmem_f32(stats_at + row * 4, s));
+            for (int s = 0; s < p.splits; ++s) {
+                const float w = top == -INFINITY ? 0.f : exp2_fast(dsmem_f32(stats_at + row * 4, s) - top);
+                total = __fmaf_rn(dsmem_f32(stats_at + (kRows + row) * 4, s), w, total);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = __fmaf_rn(dsmem_f32(part_at + (row * kPitch + (n ^ (row & 3)) * 8 + e) * 4, s), w, y[e]);
+            }
+        }
+        const float inv = total > 0.f || total != total ? 1.f / total : 0.f;      // no key seen: zeros; NaN stays
+        uint4 w;
+        uint32_t* ow = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ow[e] = pack2<QT>(y[2 * e] * inv, y[2 * e + 1] * inv);
+        QT* dst = reinterpret_cast<QT*>(p.out) + b * p.os[0] + (int64_t)((r0 + row) / ratio) * p.os[1] + (kvh * ratio + (r0 + row) % ratio) * p.os[2] + n * 8;
+        *reinterpret_cast<uint4*>(dst) = w;
+    }
+    if (p.splits > 1) cluster_sync_all();      // nobody leaves while its shared memory is read
+}
+
+template <typename QT, int DP, bool KV8> int launch_tile(AttnParams& p, cudaStream_t st) {
+    using L = Tile<QT, DP, KV8>;
+    auto kern = attention_tile_kernel<QT, DP, KV8>;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
+    const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + kRows - 1) / kRows, base = tiles * p.B * p.Hkv;
+    p.row_tiles = (int)tiles;
+    // CTAs to a row tile: as long as the device has room for twice as many and each keeps 256 keys
+    p.splits = 1;
+    while (p.splits < 8 && base * p.splits * 2 <= 296 && (int64_t)p.Lkv >= (int64_t)p.splits * 2 * 256) p.splits *= 2;
+    if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
+    return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kThreads, L::kSmem, st, p.splits, p);
+}
+template <typename QT, bool KV8> int launch_width(AttnParams& p, cudaStream_t st) {
+    if (p.D <= 64) return launch_tile<QT, 64, KV8>(p, st);
+    if (p.D <= 128) return launch_tile<QT, 128, KV8>(p, st);
+    if (p.D <= 192) return launch_tile<QT, 192, KV8>(p, st);
+    return launch_tile<QT, 256, KV8>(p, st);
+}
+
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+// Strides in elements of 16 bits: whole 16-byte pieces
+bool ragged(const int64_t* s, int n) {
+    for (int i = 0; i < n; ++i)
+        if (s[i] % 8 != 0) return true;
+    return false;
+}
+
+}  // namespace
+
+GPU_API int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides, const int32_t* kv_len,
+                                const uint8_t* key_mask, int64_t mask_stride, int B, int Lq, int Lkv, int H, int Hkv, int D, float scale, void* stream) {
+    if (B < 0 || Lq < 0 || Lkv < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || D % 8 != 0 || D > 256) return -1;
+    if (dtype != DT_F16 && dtype != DT_BF16) return -4;
+    if (B == 0 || Lq == 0) return 0;
+    if (!q || !out || !strides || (Lkv > 0 && (!k || !v)) || off16(q) || off16(k) || off16(v) || off16(out) || ragged(strides, 12)) return -5;
+    AttnParams p = {};
+    p.q = q, p.k = k, p.v = v, p.out = out, p.kv_len = kv_len, p.mask = key_mask, p.mask_stride = mask_stride;
+    for (int i = 0; i < 3; ++i) p.qs[i] = strides[i], p.ks[i] = strides[3 + i], p.vs[i] = strides[6 + i], p.os[i] = strides[9 + i];
+    p.B = B, p.Lq = Lq, p.Lkv = Lkv, p.H = H, p.Hkv = Hkv, p.D = D, p.T = 1, p.scale = scale;
+    cudaStream_t st = (cudaStream_t)stream;
+    return dtype == DT_F16 ? launch_width<half, false>(p, st) : launch_width<bf16, false>(p, st);
+}
+
+GPU_API int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t* strides, const int8_t* k8, const int8_t* v8, const float* k_scale,
+                              const float* v_scale, const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* q_len, int causal, int B,
+                              int Lq, int H, int Hkv, int D, int T, int64_t pages, int max_pages, float scale, void* stream) {
+    if (B < 0 || Lq < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || D % 16 != 0 || D > 256 || pages < 0 || max_pages < 0) return -1;
+    if (T != 16 && T != 32 && T != 64 && T != 128) return -206;
+    if (dtype != DT_F16 && dtype != DT_BF16) return -4;
+    if ((int64_t)max_pages * T > INT32_MAX - 256) return -1;
+    if (B == 0 || Lq == 0) return 0;
+    if (!q || !out || !strides || !lengths || off16(q) || off16(out) || off16(k8) || off16(v8) || ragged(strides, 6)) return -5;
+    if (max_pages > 0 && pages > 0 && (!k8 || !v8 || !k_scale || !v_scale || !table)) return -5;
+    AttnParams p = {};
+    p.q = q, p.k = k8, p.v = v8, p.out = out, p.k_scale = k_scale, p.v_scale = v_scale, p.table = table, p.table_stride = table_stride, p.pages = pages;
+    for (int i = 0; i < 3; ++i) p.qs[i] = strides[i], p.os[i] = strides[3 + i];
+    p.kv_len = lengths, p.q_len = q_len, p.causal = causal;
+    p.B = B, p.Lq = Lq, p.Lkv = pages > 0 ? max_pages * T : 0, p.H = H, p.Hkv = Hkv, p.D = D, p.T = T, p.scale = scale;
+    cudaStream_t st = (cudaStream_t)stream;
+    return dtype == DT_F16 ? launch_width<half, true>(p, st) : launch_width<bf16, true>(p, st);
+}

@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -242,9 +243,144 @@ FAST(w6a8_gemm, 12)
     return wrap(a[10], D);
 END
 
+// ---- operators that check their tensors: shapes, types and devices before anything is launched ---------------------------------
+
+void check(bool ok, const char* text) {
+    if (!ok) raise(PyExc_ValueError, text);
+}
+// On the device of x whichever is current, on that device's current stream.
+struct On {
+    c10::cuda::CUDAGuard guard;
+    c10::Device device;
+    explicit On(const at::Tensor& x) : guard(x.device()), device(x.device()) {}
+    void same(std::initializer_list<const at::Tensor*> all) const {
+        for (const at::Tensor* t : all)
+            if (t) check(t->device() == device, "the tensors of a call lie on one device");
+    }
+};
+bool shaped(const at::Tensor& t, std::initializer_list<int64_t> sizes) { return t.sizes() == at::IntArrayRef(sizes); }
+bool plain(const at::Tensor& t, at::ScalarType dt, std::initializer_list<int64_t> sizes) { return t.scalar_type() == dt && t.is_contiguous() && shaped(t, sizes); }
+int attention_dtype(const at::Tensor& t) {
+    check(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, "attention takes fp16 or bf16 rows");
+    return dtype_code(t);
+}
+// Strides of batch, row and head; a dimension of one has none.
+void put_strides(const at::Tensor& t, int64_t* s) {
+    check(t.dim() == 4 && (t.size(3) <= 1 || t.stride(3) == 1), "expected [B, L, heads, D] with the values of a head side by side");
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+int small(int64_t v) {
+    check(v <= INT32_MAX, "a dimension does not fit 32 bits");
+    return (int)v;
+}
+
+// x, packed, scales, zeros, bias, out, beta, out_dtype
+FAST(w4_linear, 8)
+    const at::Tensor &x = on_gpu(a[0]), &W = ten(a[1]), &sc = ten(a[2]);
+    const at::Tensor *z = opt(a[3]), *bias = opt(a[4]), *given = opt(a[5]);
+    const On on(x);
+    on.same({&W, &sc, z, bias, given});
+    int64_t M, K;
+    rows_cols(x, M, K);
+    check(W.dim() == 2 && sc.dim() == 2 && sc.size(1) > 0 && K > 0 && K % sc.size(1) == 0, "expected packed [N, K / 2] and scales [N, K / G]");
+    const int64_t N = W.size(0), groups = sc.size(1);
+    check(plain(W, at::kByte, {N, K / 2}) && K % 2 == 0 && shaped(sc, {N, groups}) && sc.is_contiguous(), "packed is uint8 [N, K / 2], scales [N, K / G], both contiguous");
+    check(sc.scalar_type() == at::kHalf || sc.scalar_type() == at::kBFloat16, "scales are fp16 or bf16");
+    check(!z || plain(*z, at::kByte, {N, groups}), "zero points are uint8 [N, K / G]");
+    check(x.stride(1) == 1 || K == 1, "the values of a row of x lie side by side");
+    const float beta = real(a[6]);
+    check(beta == 0.f || given, "beta needs the out that it scales");
+    at::Tensor D = given ? *given : matrix(x, M, N, a[7] == Py_None ? x.scalar_type() : out_dtype(a[7]));
+    check(shaped(D, {M, N}) && (D.stride(1) == 1 || N == 1), "out is [M, N], the values of a row side by side");
+    check(!bias || plain(*bias, D.scalar_type(), {N}), "bias is [N] in the type of out");
+    CALL(gpu_w4_linear, dtype_code(x), ptr(x), M > 1 ? x.stride(0) : K, ptr(W), dtype_code(sc), ptr(sc), ptr(z), ptr(bias), dtype_code(D), ptr(D),
+                        M > 1 ? D.stride(0) : N, beta, small(M), small(N), small(K), small(K / groups), stream());
+    return wrap(a[5], D);
+END
+// q, k, v, kv_len, key_mask, scale, out
+FAST(cross_attention, 7)
+    const at::Tensor &q = on_gpu(a[0]), &k = ten(a[1]), &v = ten(a[2]);
+    const at::Tensor *kv_len = opt(a[3]), *mask = opt(a[4]), *given = opt(a[6]);
+    const On on(q);
+    on.same({&k, &v, kv_len, mask, given});
+    const int dt = attention_dtype(q);
+    int64_t st[12];
+    put_strides(q, st), put_strides(k, st + 3), put_strides(v, st + 6);
+    const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), D = q.size(3), Lkv = k.size(1), Hkv = k.size(2);
+    check(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v have one type");
+    check(shaped(k, {B, Lkv, Hkv, D}) && shaped(v, {B, Lkv, Hkv, D}) && Hkv > 0 && H % Hkv == 0, "expected k and v [B, Lkv, Hkv, D], H a multiple of Hkv");
+    check(!kv_len || plain(*kv_len, at::kInt, {B}), "kv_len is int32 [B]");
+    check(!mask || ((mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte) && shaped(*mask, {B, Lkv}) && (mask->stride(1) == 1 || Lkv <= 1)),
+          "key_mask is bool [B, Lkv]");
+    at::Tensor out = given ? *given : at::empty(q.sizes(), q.options());
+    check(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out has the shape and type of q");
+    put_strides(out, st + 9);
+    CALL(gpu_cross_attention, dt, ptr(q), ptr(k), ptr(v), ptr(out), st, ptr<int32_t>(kv_len), ptr<uint8_t>(mask), mask && B > 1 ? mask->stride(0) : 0, small(B),
+                              small(Lq), small(Lkv), small(H), small(Hkv), small(D), real(a[5]), stream());
+    return wrap(a[6], out);
+END
+
+// k, v, k_scale, v_scale of a cache
+struct Cache {
+    const at::Tensor &k, &v, &ks, &vs;
+    int64_t pages, Hkv, T, D;
+    explicit Cache(PyObject* const* a) : k(on_gpu(a[0])), v(ten(a[1])), ks(ten(a[2])), vs(ten(a[3])) {
+        check(k.dim() == 4, "a cache's keys and values are int8 [pages, Hkv, T, D]");
+        pages = k.size(0), Hkv = k.size(1), T = k.size(2), D = k.size(3);
+        check(plain(k, at::kChar, {pages, Hkv, T, D}) && plain(v, at::kChar, {pages, Hkv, T, D}), "a cache's keys and values are int8 [pages, Hkv, T, D]");
+        check(plain(ks, at::kFloat, {pages, Hkv}) && plain(vs, at::kFloat, {pages, Hkv}), "a cache's scales are f32 [pages, Hkv]");
+    }
+};
+void check_table(const at::Tensor& t, int64_t B) {
+    check(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == B && (t.stride(1) == 1 || t.size(1) <= 1), "table is int32 [B, pages to a sequence]");
+}
+int64_t table_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+
+// cache (4), k, v, table, start, count
+FAST(kv8_append, 9)
+    const Cache c(a);
+    const at::Tensor &k = ten(a[4]), &v = ten(a[5]), &table = ten(a[6]), &start = ten(a[7]);
+    const at::Tensor* count = opt(a[8]);
+    const On on(c.k);
+    on.same({&c.v, &c.ks, &c.vs, &k, &v, &table, &start, count});
+    int64_t st[6];
+    put_strides(k, st), put_strides(v, st + 3);
+    const int64_t B = k.size(0), L = k.size(1);
+    check(shaped(k, {B, L, c.Hkv, c.D}) && shaped(v, {B, L, c.Hkv, c.D}) && k.scalar_type() == v.scalar_type(), "expected k and v [B, L, Hkv, D] of one type");
+    check_table(table, B);
+    check(plain(start, at::kInt, {B}) && (!count || plain(*count, at::kInt, {B})), "start and count are int32 [B]");
+    CALL(gpu_kv8_append, dtype_code(k), ptr(k), ptr(v), st, ptr<int8_t>(c.k), ptr<int8_t>(c.v), ptr<float>(c.ks), ptr<float>(c.vs), ptr<int32_t>(table),
+                         table_stride(table), ptr<int32_t>(start), ptr<int32_t>(count), small(B), small(L), small(c.Hkv), small(c.D), small(c.T), c.pages,
+                         small(table.size(1)), stream());
+    Py_RETURN_NONE;
+END
+// cache (4), q, table, lengths, q_len, causal, scale, out
+FAST(kv8_attention, 11)
+    const Cache c(a);
+    const at::Tensor &q = on_gpu(a[4]), &table = ten(a[5]), &len = ten(a[6]);
+    const at::Tensor *q_len = opt(a[7]), *given = opt(a[10]);
+    const On on(q);
+    on.same({&c.k, &c.v, &c.ks, &c.vs, &table, &len, q_len, given});
+    const int dt = attention_dtype(q);
+    int64_t st[6];
+    put_strides(q, st);
+    const int64_t B = q.size(0), L = q.size(1), H = q.size(2), D = q.size(3);
+    check(D == c.D && c.Hkv > 0 && H % c.Hkv == 0, "expected q [B, L, H, D] with the cache's D, H a multiple of its heads");
+    check_table(table, B);
+    check(plain(len, at::kInt, {B}) && (!q_len || plain(*q_len, at::kInt, {B})), "lengths and q_len are int32 [B]");
+    at::Tensor out = given ? *given : q_len ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
+    check(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out has the shape and type of q");
+    put_strides(out, st + 3);
+    CALL(gpu_kv8_attention, dt, ptr(q), ptr(out), st, ptr<int8_t>(c.k), ptr<int8_t>(c.v), ptr<float>(c.ks), ptr<float>(c.vs), ptr<int32_t>(table),
+                            table_stride(table), ptr<int32_t>(len), ptr<int32_t>(q_len), integer32(a[8]), small(B), small(L), small(H), small(c.Hkv), small(D),
+                            small(c.T), c.pages, small(table.size(1)), real(a[9]), stream());
+    return wrap(a[10], out);
+END
+
 #define M(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {M(quant_rows), M(sd_quant_rows), M(sd_ln_quant_rows), M(sd_geglu_quant_rows), M(sd_group_norm_quant_rows),
                          M(sd_unpad_quant_rows), M(int8_gemm), M(int8_gemm_act_rot), M(quant_rows_rotated), M(w6a8_gemm),
+                         M(w4_linear), M(cross_attention), M(kv8_append), M(kv8_attention),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

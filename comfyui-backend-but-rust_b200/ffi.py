@@ -54,6 +54,13 @@ SIGNATURES = {
     "gpu_convrot_dequant": [i32, P, P, P, i64, i32, P],
     "gpu_dequant_i8": [P, P, P, i64, i64, P],
     "gpu_embed_dequant": [P, P, P, i32, i32, i32, P],
+    "gpu_w4_requant": [i32, P, i64, P, i32, P, P, i64, i32, i32, P],
+    "gpu_w4_dequant": [i32, P, i32, P, P, P, i64, i32, i32, P],
+    "gpu_w4_linear": [i32, P, i64, P, i32, P, P, P, i32, P, i64, f32, i32, i32, i32, i32, P],
+    "gpu_kv8_append": [i32, P, P, C.POINTER(i64), P, P, P, P, P, i64, P, P, i32, i32, i32, i32, i32, i64, i32, P],
+    "gpu_kv8_dequant": [i32, P, P, P, P, P, i64, P, P, P, i32, i64, i32, i32, i32, i64, i32, P],
+    "gpu_kv8_attention": [i32, P, P, C.POINTER(i64), P, P, P, P, P, i64, P, P, i32, i32, i32, i32, i32, i32, i32, i64, i32, f32, P],
+    "gpu_cross_attention": [i32, P, P, P, P, C.POINTER(i64), P, P, i64, i32, i32, i32, i32, i32, i32, f32, P],
     "gpu_wddm_budget": [C.POINTER(u64), C.POINTER(u64)],
     "gpu_kernels_status": [C.POINTER(i32)],
 }

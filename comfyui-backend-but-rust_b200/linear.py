@@ -39,6 +39,12 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _one_device(*tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != tensors[0].device):
+            raise ValueError("this path runs on CUDA tensors only, those of a call on one device")
+
+
 def _cuda(t: torch.Tensor) -> torch.Tensor:
     if not t.is_cuda:
         raise ValueError("this path runs on CUDA tensors only")
@@ -205,6 +211,47 @@ def w6_requant(w: torch.Tensor, seed: int = 1):
     s_ch = torch.empty((N,), dtype=torch.float32, device=w.device)
     ok(_lib().gpu_w6_requant(_ptr(w), _ptr(packed), _ptr(s_rel), _ptr(s_ch), N, K, seed, _stream()), "gpu_w6_requant")
     return packed, s_rel, s_ch
+
+
+def w4_requant(w: torch.Tensor, group: int = 128, *, zero_points: bool = False, scale_dtype=torch.float16):
+    """gpu_w4_requant: f32 / f16 / bf16 [N, K] -> (packed u8 [N, K/2], scales [N, K/group], zeros u8 [N, K/group] or None). A group of
+    32, 64, 128 or 256 columns has one scale (fp16 or bf16) and, with `zero_points`, one zero point."""
+    _one_device(w)
+    if w.dim() != 2 or w.stride(1) != 1:
+        raise ValueError("expected a matrix whose rows' values lie side by side")
+    N, K = w.shape
+    if group not in (32, 64, 128, 256) or K == 0 or K % group:
+        raise ValueError("K has to be a multiple of the group, the group 32, 64, 128 or 256")
+    with torch.cuda.device(w.device):
+        packed = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
+        scales = torch.empty((N, K // group), dtype=scale_dtype, device=w.device)
+        zeros = torch.empty((N, K // group), dtype=torch.uint8, device=w.device) if zero_points else None
+        ok(_lib().gpu_w4_requant(_DT[w.dtype], _ptr(w), w.stride(0) if N > 1 else K, _ptr(packed), _DT[scale_dtype], _ptr(scales), _ptr(zeros), N, K,
+                                 group, _stream()), "gpu_w4_requant")
+    return packed, scales, zeros
+
+
+def w4_dequant(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *, dtype=torch.float32) -> torch.Tensor:
+    """gpu_w4_dequant: the weight [N, K] that w4_requant's codes, scales and zero points stand for."""
+    _one_device(packed, scales, zeros)
+    N, K = packed.shape[0], packed.shape[1] * 2
+    groups = scales.shape[1]
+    if packed.dtype != torch.uint8 or scales.shape[0] != N or groups == 0 or K % groups or not (packed.is_contiguous() and scales.is_contiguous()):
+        raise ValueError("expected packed uint8 [N, K / 2] and scales [N, K / G], both contiguous")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape or not zeros.is_contiguous()):
+        raise ValueError("zero points are uint8 [N, K / G]")
+    with torch.cuda.device(packed.device):
+        out = torch.empty((N, K), dtype=dtype, device=packed.device)
+        ok(_lib().gpu_w4_dequant(_DT[dtype], _ptr(packed), _DT[scales.dtype], _ptr(scales), _ptr(zeros), _ptr(out), N, K, K // groups, _stream()),
+           "gpu_w4_dequant")
+    return out
+
+
+def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+              out: Optional[torch.Tensor] = None, beta: float = 0.0, out_dtype=None) -> torch.Tensor:
+    """gpu_w4_linear: out = beta * out + x @ W^T + bias from w4_requant's codes. x [M, K] f32 / f16 / bf16; out [M, N] in x's type or
+    f32 (`out_dtype`, or the type of the `out` given); bias [N] in out's type; beta 0 or 1."""
+    return _h.w4_linear(x, packed, scales, zeros, bias, out, beta, out_dtype)
 
 
 def int8_gemm(A, W, xs, ws, bias=None, *, out_dtype=torch.bfloat16, act: int = 0, rscale=None, resid=None, out=None):

@@ -211,6 +211,65 @@ int gpu_dequant_i8(const int8_t* q, const float* s, float* out, int64_t N, int64
  * Replaces csrc/kernels.cu:633-638 (src/ffi.rs:82). */
 int gpu_embed_dequant(const int8_t* q, const float* s, float* out, int M, int K, int rotate, void* stream);
 
+/* ---- 4-bit weights with group scales ---------------------------------------------------------------------- */
+
+/* New (the reference's smallest weight has 6 bits and int8 activations): linears whose weight has 4 bits and a scale for each
+ * group of G columns, W[n,k] = (c[n,k] - z[n,k/G]) * s[n,k/G], activations in floating point. Codes c in 0..15: Wq4 [N, K/2],
+ * column 2i in the low nibble of byte i, 2i + 1 in the high one (the order of the W6 nibble plane); scales [N, K/G] f16 or bf16
+ * (scale_dt); zeros u8 [N, K/G] in 0..15, or NULL: 8. G is 32, 64, 128 or 256 and divides K (-1).
+ *
+ * gpu_w4_requant   w [N, K] (f32, f16 or bf16, rows w_stride apart) -> codes and scales, nearest even. Without zeros: s = amax * (1/7)
+ *                  rounded to its type, c = clamp(rint(w / s), -8, 7) + 8. With: s = (max(w, 0) - min(w, 0)) * (1/15),
+ *                  z = clamp(rint(-min / s), 0, 15), c = clamp(rint(w / s) + z, 0, 15). A group of zeros has s = 0. Weights in another
+ *                  basis: gpu_rotate_rows_f32 first.
+ * gpu_w4_dequant   the way back, out [N, K] in dtype.
+ * gpu_w4_linear    out[m,n] = beta * out[m,n] + sum_k x[m,k] W[n,k] + bias[n], beta 0 or 1 (-207). x [M, K] f32, f16 or bf16, out [M, N]
+ *                  in x's type or f32, bias [N] in out's type or NULL. Codes and x enter the products exactly (an f32 x as three
+ *                  bf16 terms), sums are f32, one rounding to out's type. M from one token up; out must not overlap x.
+ * Errors: -4 types, -5 a NULL, a row of x or w, Wq4 or out of gpu_w4_dequant off a 16-byte boundary (packed of the packer: 8). */
+int gpu_w4_requant(int dtype, const void* w, int64_t w_stride, void* packed, int scale_dt, void* scales, void* zeros, int64_t N,
+                   int K, int G, void* stream);
+int gpu_w4_dequant(int dtype, const void* packed, int scale_dt, const void* scales, const void* zeros, void* out, int64_t N, int K,
+                   int G, void* stream);
+int gpu_w4_linear(int dtype, const void* x, int64_t x_stride, const void* Wq4, int scale_dt, const void* scales, const void* zeros,
+                  const void* bias, int out_dt, void* out, int64_t out_stride, float beta, int M, int N, int K, int G, void* stream);
+
+/* ---- attention between the linears --------------------------------------------------------------------------- */
+
+/* New: a cache of keys and values in 8 bits. k8, v8 int8 [pages, Hkv, T, D], k_scale, v_scale f32 [pages, Hkv]; a value is
+ * code * scale. T is 16, 32, 64 or 128 tokens (-206), D a multiple of 16 up to 256 (-1). Token i of sequence b is row i % T of page
+ * table[b * table_stride + i / T]; a sequence has at most max_pages pages, and an index outside [0, pages) is a page that there is
+ * not: rows for it are dropped, keys on it are not seen.
+ *
+ * gpu_kv8_append     k, v [B, L, Hkv, D] (f32, f16 or bf16; strides = 6 HOST values, in elements: batch, row, head of k, then of v): row i < count[b]
+ *                    (NULL: L) becomes token start[b] + i. A page's scale is amax * (1/127) of its rows, at least 1e-30; a page begun
+ *                    before keeps a larger one, and when the new rows raise it its old codes become rint(code * (old / new)). Codes are
+ *                    rint(value / scale) within +-127, NaN gives 0. No two sequences of a call may write the same page.
+ * gpu_kv8_dequant    k, v [B, rows, Hkv, D] in dtype, zeros from lengths[b] on.
+ * gpu_kv8_attention  q, out [B, Lq, H, D] f16 or bf16 (strides = 6 HOST values: of q, then of out; H % Hkv == 0): out = softmax(scale q k^T) v over
+ *                    tokens < lengths[b]. Rows i < q_len[b] (NULL: Lq) are the sequence's last tokens: with causal != 0 row i sees
+ *                    tokens <= lengths[b] - q_len[b] + i. Rows from q_len[b] on are not written; a row that sees no token is zeros.
+ *                    Needs no workspace. bf16 queries are taken as fp16 times a power of two per row (values below 2^-29 of their row's largest lose bits).
+ * Errors: -1 sizes, -4 types, -5 a NULL or rows off a 16-byte boundary (strides in whole 16 bytes). */
+int gpu_kv8_append(int dtype, const void* k, const void* v, const int64_t* strides, int8_t* k8, int8_t* v8, float* k_scale,
+                   float* v_scale, const int32_t* table, int64_t table_stride, const int32_t* start, const int32_t* count, int B, int L,
+                   int Hkv, int D, int T, int64_t pages, int max_pages, void* stream);
+int gpu_kv8_dequant(int dtype, const int8_t* k8, const int8_t* v8, const float* k_scale, const float* v_scale, const int32_t* table,
+                    int64_t table_stride, const int32_t* lengths, void* k, void* v, int B, int64_t rows, int Hkv, int D, int T,
+                    int64_t pages, int max_pages, void* stream);
+int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t* strides, const int8_t* k8, const int8_t* v8,
+                      const float* k_scale, const float* v_scale, const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                      const int32_t* q_len, int causal, int B, int Lq, int H, int Hkv, int D, int T, int64_t pages, int max_pages,
+                      float scale, void* stream);
+
+/* New: cross attention to an encoder's states, out = softmax(scale q k^T) v without the scores in memory. q, out [B, Lq, H, D], k, v
+ * [B, Lkv, Hkv, D], f16 or bf16 (strides = 12 HOST values, in elements: batch, row, head of q, k, v, out); D a multiple of 8 up to 256; H % Hkv == 0. Keys >= kv_len[b] and keys
+ * with key_mask[b * mask_stride + t] == 0 (either may be NULL) are not seen, whatever they hold; a row that sees none is zeros.
+ * Errors as above. Stands between gpu_int8_gemm of q, k, v and gpu_sd_quant_rows / gpu_quant_rows of its result. */
+int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides,
+                        const int32_t* kv_len, const uint8_t* key_mask, int64_t mask_stride, int B, int Lq, int Lkv, int H, int Hkv,
+                        int D, float scale, void* stream);
+
 /* Windows video-memory budget query the Rust side imports unconditionally (src/cuda.rs:136-153; the reference
  * defines it in csrc/wddm.cu). HOST pointers. Always returns non-zero here: no budget is known. */
 int gpu_wddm_budget(uint64_t* budget, uint64_t* usage);
