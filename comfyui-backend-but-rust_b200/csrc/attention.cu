@@ -42,18 +42,30 @@ __device__ __forceinline__ float dsmem_f32(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// Eight int8 codes as eight halves, exact: each byte, its sign bit turned, becomes the low byte of 1024 + (code + 128), and 1152 is taken away.
-__device__ __forceinline__ uint4 halves_of(uint2 w) {
-    const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u, off = 0x64806480u;
-    uint4 r;
-    uint32_t* o = reinterpret_cast<uint32_t*>(&r);
+// Four int8 codes as four halves, exact: each byte, its sign bit turned, becomes the low byte of 1024 + (code + 128), and 1152 is taken away.
+__device__ __forceinline__ uint2 halves_of4(uint32_t w) {
+    const uint32_t off = 0x64806480u, a = w ^ 0x80808080u;
+    const uint32_t lo = __byte_perm(a, 0x64646464u, 0x4140), hi = __byte_perm(a, 0x64646464u, 0x4342);
+    const half2 x = __hsub2(*reinterpret_cast<const half2*>(&lo), *reinterpret_cast<const half2*>(&off));
+    const half2 y = __hsub2(*reinterpret_cast<const half2*>(&hi), *reinterpret_cast<const half2*>(&off));
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// bf16 queries over int8 keys are taken as halves times a power of two: 2^e brings a row's largest magnitude to [2^14, 2^15). 2^e and 2^-e are
+// f32 numbers.
+__device__ __forceinline__ int row_exponent(float top) {
+    return top > 0.f && top <= FLT_MAX ? min(100, max(-100, 14 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+}
+
+// Eight columns of a finished row; one that saw no key is zeros, NaN stays.
+template <typename QT> __device__ __forceinline__ void store_row(const AttnParams& p, const float (&y)[8], float total, int b, int row, int kvh, int ratio, int d, QT) {
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+    uint4 w;
+    uint32_t* ow = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t v = __byte_perm(i < 2 ? a : b, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
-        const half2 h = __hsub2(*reinterpret_cast<const half2*>(&v), *reinterpret_cast<const half2*>(&off));
-        o[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return r;
+    for (int e = 0; e < 4; ++e) ow[e] = pack2<QT>(y[2 * e] * inv, y[2 * e + 1] * inv);
+    QT* dst = reinterpret_cast<QT*>(p.out) + b * p.os[0] + (int64_t)(row / ratio) * p.os[1] + (kvh * ratio + row % ratio) * p.os[2] + d;
+    *reinterpret_cast<uint4*>(dst) = w;
 }
 
 // 64 query rows (a kv head's queries: row r is query r / ratio, head r % ratio of its group), 64 keys a step, four warps of 16 rows.
@@ -106,8 +118,7 @@ template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThre
                     for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f<QT>(x[e])));
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            // 2^(14 - exponent): the largest lands in [2^14, 2^15). Both it and its inverse are f32 numbers for exponents within 100.
-            const int e = top > 0.f && top <= FLT_MAX ? min(100, max(-100, 14 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+            const int e = row_exponent(top);
             mult = __uint_as_float((uint32_t)(127 + e) << 23);
             if ((tid & 1) == 0) reinterpret_cast<float*>(smem + L::kStats)[row] = __uint_as_float((uint32_t)(127 - e) << 23);
         }
@@ -189,8 +200,8 @@ template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThre
             const uint8_t* src = smem + L::kLoaded + stage * 2 * L::kStage;
             for (int i = tid; i < 2 * kKeys * DP / 8; i += kThreads) {
                 const int which = i / (kKeys * DP / 8), j = i % (kKeys * DP / 8);
-                *reinterpret_cast<uint4*>(smem + L::kHalves + which * L::kBytes + L::at(j / chunks, j % chunks)) =
-                    halves_of(*reinterpret_cast<const uint2*>(src + which * L::kStage + j * 8));
+                const uint2 w = *reinterpret_cast<const uint2*>(src + which * L::kStage + j * 8), x = halves_of4(w.x), y = halves_of4(w.y);
+                *reinterpret_cast<uint4*>(smem + L::kHalves + which * L::kBytes + L::at(j / chunks, j % chunks)) = make_uint4(x.x, x.y, y.x, y.y);
             }
             __syncthreads();
             ks = base + L::kHalves, vs = ks + L::kBytes;
@@ -293,13 +304,7 @@ template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThre
                 for (int e = 0; e < 8; ++e) y[e] = __fmaf_rn(dsmem_f32(part_at + (row * kPitch + (n ^ (row & 3)) * 8 + e) * 4, s), w, y[e]);
             }
         }
-        const float inv = total > 0.f || total != total ? 1.f / total : 0.f;      // no key seen: zeros; NaN stays
-        uint4 w;
-        uint32_t* ow = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ow[e] = pack2<QT>(y[2 * e] * inv, y[2 * e + 1] * inv);
-        QT* dst = reinterpret_cast<QT*>(p.out) + b * p.os[0] + (int64_t)((r0 + row) / ratio) * p.os[1] + (kvh * ratio + (r0 + row) % ratio) * p.os[2] + n * 8;
-        *reinterpret_cast<uint4*>(dst) = w;
+        store_row(p, y, total, b, r0 + row, kvh, ratio, n * 8, QT());
     }
     if (p.splits > 1) cluster_sync_all();      // nobody leaves while its shared memory is read
 }
@@ -316,7 +321,304 @@ template <typename QT, int DP, bool KV8> int launch_tile(AttnParams& p, cudaStre
     if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kThreads, L::kSmem, st, p.splits, p);
 }
+// ---- few rows over the cache ---------------------------------------------------------------------------------------------------------
+// Up to 16 rows to a kv head (a token's query heads, or a few tokens'): bound by the cache's bytes. A CTA's eight warps take 16 keys each
+// in turn, and every warp is on its own until the end: its ring of stages, its m, l and sums. The operands of the products come out of the
+// codes as they lie in memory, because the order of a product's inner index is free as long as both operands have it: a lane multiplies 16
+// neighbouring values of a key with the same 16 of its query row, and in p . v its column 16 g + j of every key stands for column g of the
+// product's j-th tile. So codes are read from shared memory in 16-byte pieces and nothing is transposed.
+constexpr int kRowsWarps = 8, kRowsStages = 3;
+
+template <int DP> struct RowsTile {
+    static constexpr int kHalf = 16 * DP, kStage = 2 * kHalf, kRing = kRowsWarps * kRowsStages * kStage;
+    static constexpr int kPitch = DP + 8;                              // floats to a row of sums
+    static constexpr int kParts = kRowsWarps * 16 * kPitch * 4, kSmem0 = kParts + 16 * kPitch * 4 > kRing ? kParts + 16 * kPitch * 4 : kRing;
+    static constexpr int kStats = kSmem0, kInfo = kStats + (kRowsWarps + 1) * 32 * 4, kSmem = kInfo + kRowsWarps * kRowsStages * 16;
+};
+
+// Four int8 codes (sign bits turned) of each of two rows as four registers of halves (row a's value, row b's value)
+__device__ __forceinline__ void half_pairs(uint32_t a, uint32_t b, uint32_t (&r)[4]) {
+    const uint32_t off = 0x64806480u, lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t v = __byte_perm(i < 2 ? lo : hi, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
+        const half2 h = __hsub2(*reinterpret_cast<const half2*>(&v), *reinterpret_cast<const half2*>(&off));
+        r[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
+template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32, DP <= 128 ? 2 : 1) kv8_rows_kernel(const AttnParams p) {
+    using R = RowsTile<DP>;
+    constexpr bool kBf16 = std::is_same<QT, bf16>::value;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits % p.row_tiles, bh = blockIdx.x / p.splits / p.row_tiles;
+    const int b = bh / p.Hkv, kvh = bh % p.Hkv, ratio = p.H / p.Hkv, D = p.D;
+    pdl_wait();
+    const int len = min(max(gload(p.kv_len + b), 0), p.Lkv);
+    const int ql = p.q_len ? min(max(gload(p.q_len + b), 0), p.Lq) : p.Lq;
+    const int r0 = rt * 16, live = min(16, ql * ratio - r0);
+    if (live <= 0) return;                                              // the same for every CTA of the cluster
+    const int seen = p.causal ? max(0, min(len, len - ql + (r0 + live - 1) / ratio + 1)) : len;
+    // blocks of 16 keys: a CTA's share is at least one for each of its warps
+    const int blocks = (seen + 15) / 16, per = max((blocks + p.splits - 1) / p.splits, kRowsWarps);
+    const int first = min(split * per, blocks), last = min(first + per, blocks);
+    const int mine = (last - first - warp + kRowsWarps - 1) / kRowsWarps;      // blocks first + warp + 8 i, i < mine
+    const uint32_t ring = smem_u32(smem) + warp * kRowsStages * R::kStage;
+    float4* info = reinterpret_cast<float4*>(smem + R::kInfo) + warp * kRowsStages;      // factor, offset, weight of a stage's page
+
+    // Pages and scales of the next 32 blocks, one to a lane
+    int64_t page_off = -1;
+    float mul_l = 0.f, add_l = -INFINITY, wt_l = 0.f;
+    auto look_up = [&](int i0) {
+        page_off = -1, mul_l = 0.f, add_l = -INFINITY, wt_l = 0.f;
+        const int i = i0 + lane;
+        if (i < mine) {
+            const int key = (first + warp + i * kRowsWarps) * 16;
+            const int64_t page = gload(p.table + b * p.table_stride + key / p.T);
+            if (page >= 0 && page < p.pages) {
+                const float s = fmaxf(gload(p.v_scale + page * p.Hkv + kvh), kTiny);
+                mul_l = gload(p.k_scale + page * p.Hkv + kvh) * (p.scale * kLog2e), add_l = log2f(s), wt_l = 1.f / s;
+                page_off = ((page * p.Hkv + kvh) * p.T + key % p.T) * D;
+            }
+        }
+    };
+    // 16 rows of K, then of V. K's 16-byte pieces are read four to a row by two rows at a time, V's two to a row by four pairs of rows: the
+    // piece's number is turned so that either lies in all 32 banks.
+    auto load = [&](int i, int slot) {
+        const int64_t off = __shfl_sync(0xffffffffu, page_off, i & 31);
+        const int key = (first + warp + i * kRowsWarps) * 16;
+        const uint32_t dst = ring + slot * R::kStage;
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j) {
+            const int x = j * 32 + lane, row = x / (DP / 16), c = x % (DP / 16);
+            const bool valid = off >= 0 && c * 16 < D && key + row < seen;
+            const int64_t o = valid ? off + row * D + c * 16 : 0;
+            cp_async16(dst + row * DP + ((c ^ ((row & 1) << 2)) & (DP / 16 - 1)) * 16, reinterpret_cast<const int8_t*>(p.k) + o, valid);
+            cp_async16(dst + R::kHalf + row * DP + ((c ^ (row & 6)) & (DP / 16 - 1)) * 16, reinterpret_cast<const int8_t*>(p.v) + o, valid);
+        }
+        if (lane == (i & 31)) info[slot] = make_float4(mul_l, add_l, wt_l, page_off >= 0 ? 1.f : 0.f);
+    };
+    float o[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+    uint32_t q[DP / 16][4];
+    float factor[2] = {1.f, 1.f};
+    look_up(0);
+#pragma unroll
+    for (int i = 0; i < kRowsStages - 1; ++i) {
+        if (i < mine) load(i, i);
+        cp_async_commit();
+    }
+    int bound[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = g + 8 * h;
+        bound[h] = p.causal ? len - ql + (r0 + row) / ratio + 1 : len;
+        const QT* src = reinterpret_cast<const QT*>(p.q) + b * p.qs[0] + (int64_t)((r0 + row) / ratio) * p.qs[1] + (kvh * ratio + (r0 + row) % ratio) * p.qs[2];
+        uint4 w[DP / 64][2];
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = c * 64 + t * 16 + e * 8;
+                w[c][e] = row < live && d < D ? gload(reinterpret_cast<const uint4*>(src + d)) : make_uint4(0, 0, 0, 0);
+                if (kBf16)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(to_f<QT>(reinterpret_cast<const QT*>(&w[c][e])[x])));
+            }
+        float mult = 1.f;
+        if (kBf16) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = row_exponent(top);
+            mult = __uint_as_float((uint32_t)(127 + e) << 23), factor[h] = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t v = reinterpret_cast<const uint32_t*>(&w[c][j >> 1])[(j & 1) * 2 + e];
+                    const QT* x = reinterpret_cast<const QT*>(&v);
+                    q[c * 4 + j][2 * e + h] = kBf16 ? pack2<half>(to_f<QT>(x[0]) * mult, to_f<QT>(x[1]) * mult) : v;
+                }
+    }
+    const int lowest = p.causal ? len - ql + r0 / ratio + 1 : len;      // keys that every row sees
+    int slot = 0;
+    for (int i = 0; i < mine; ++i) {
+        cp_async_wait<kRowsStages - 2>();
+        __syncwarp();
+        const uint32_t ks = ring + slot * R::kStage, vs = ks + R::kHalf;
+        const float4 in = info[slot];
+        const int key0 = (first + warp + i * kRowsWarps) * 16;
+        if (in.w != 0.f) {      // the page exists
+            float s[2][4] = {};
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int row = n * 8 + g;
+                    const uint4 w = lds128(ks + row * DP + (((4 * c + t) ^ ((row & 1) << 2)) & (DP / 16 - 1)) * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint2 k2 = halves_of4(reinterpret_cast<const uint32_t*>(&w)[j]);
+                        mma16816<half>(s[n], q[c * 4 + j][0], q[c * 4 + j][1], q[c * 4 + j][2], q[c * 4 + j][3], k2.x, k2.y);
+                    }
+                }
+            float top[2] = {m[0], m[1]};
+            const bool all = key0 + 16 <= lowest;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int h = x >> 1;
+                    s[n][x] = __fmaf_rn(s[n][x] * factor[h], in.x, in.y);
+                    if (!all && key0 + n * 8 + 2 * t + (x & 1) >= bound[h]) s[n][x] = -INFINITY;
+                    top[h] = fmaxf(top[h], s[n][x]);
+                }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {      // a larger exponent: the sums follow it
+                float keep[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) keep[h] = exp2_fast(m[h] - (top[h] == -INFINITY ? 0.f : top[h])), m[h] = top[h], l[h] *= keep[h];
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[n][x] *= keep[x >> 1];
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    s[n][x] = exp2_fast(s[n][x] - (m[x >> 1] == -INFINITY ? 0.f : m[x >> 1]));
+                    l[x >> 1] = __fmaf_rn(s[n][x], in.z, l[x >> 1]);
+                }
+            const uint32_t a0 = pack2<half>(s[0][0], s[0][1]), a1 = pack2<half>(s[0][2], s[0][3]), a2 = pack2<half>(s[1][0], s[1][1]), a3 = pack2<half>(s[1][2], s[1][3]);
+            constexpr int kWide = DP >= 128 ? 16 : 8;      // neighbouring columns of a lane: 16 g + j, or 8 g + j
+#pragma unroll
+            for (int u = 0; u < DP / 8 / kWide; ++u) {
+                uint32_t w[4][kWide / 4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 2 * t + (r & 1) + (r >> 1) * 8;
+                    if (kWide == 16) {
+                        const uint4 v = lds128(vs + row * DP + (((8 * u + g) ^ (row & 6)) & (DP / 16 - 1)) * 16);
+                        w[r][0] = v.x, w[r][1] = v.y, w[r][kWide / 4 - 2] = v.z, w[r][kWide / 4 - 1] = v.w;
+                    } else {
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[r][0]), "=r"(w[r][1])
+                                     : "r"(vs + row * DP + (((g >> 1) ^ (row & 6)) & (DP / 16 - 1)) * 16 + (g & 1) * 8) : "memory");
+                    }
+#pragma unroll
+                    for (int j = 0; j < kWide / 4; ++j) w[r][j] ^= 0x80808080u;
+                }
+#pragma unroll
+                for (int j = 0; j < kWide / 4; ++j) {
+                    uint32_t b0[4], b1[4];
+                    half_pairs(w[0][j], w[1][j], b0);
+                    half_pairs(w[2][j], w[3][j], b1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mma16816<half>(o[u * kWide + j * 4 + e], a0, a1, a2, a3, b0[e], b1[e]);
+                }
+            }
+        }
+        __syncwarp();
+        const int ahead = i + kRowsStages - 1;
+        if (ahead < mine) {
+            if ((ahead & 31) == 0) look_up(ahead);
+            load(ahead, slot == 0 ? kRowsStages - 1 : slot - 1);
+        }
+        cp_async_commit();
+        slot = slot + 1 == kRowsStages ? 0 : slot + 1;
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1), l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    // ---- the warps' sums into the CTA's, the CTAs' into the row: m, l and o of each, in this order
+    __syncthreads();                                                  // every ring is done with
+    float* part = reinterpret_cast<float*>(smem);                     // [warp][16][pitch] in the products' order of columns, then the CTA's
+    float* stats = reinterpret_cast<float*>(smem + R::kStats);        // [warp][m, l][16], then the CTA's
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = g + 8 * h;
+        if (t == 0) stats[warp * 32 + row] = m[h], stats[warp * 32 + 16 + row] = l[h];
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+            *reinterpret_cast<float2*>(part + (warp * 16 + row) * R::kPitch + n * 8 + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    __syncthreads();
+    float* all = part + kRowsWarps * 16 * R::kPitch;
+    float* all_stats = stats + kRowsWarps * 32;
+    for (int x = tid; x < live * (DP / 4); x += kRowsWarps * 32) {
+        const int row = x / (DP / 4), c = x % (DP / 4) * 4;
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, stats[w * 32 + row]);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) {
+            const float k = top == -INFINITY ? 0.f : exp2_fast(stats[w * 32 + row] - top);
+            const float4 v = *reinterpret_cast<const float4*>(part + (w * 16 + row) * R::kPitch + c);
+            total = __fmaf_rn(stats[w * 32 + 16 + row], k, total);
+            y.x = __fmaf_rn(v.x, k, y.x), y.y = __fmaf_rn(v.y, k, y.y), y.z = __fmaf_rn(v.z, k, y.z), y.w = __fmaf_rn(v.w, k, y.w);
+        }
+        *reinterpret_cast<float4*>(all + row * R::kPitch + c) = y;
+        if (c == 0) all_stats[row] = top, all_stats[16 + row] = total;
+    }
+    if (p.splits > 1) cluster_sync_all();
+    else __syncthreads();
+    constexpr int kWide = DP >= 128 ? 16 : 8;
+    const uint32_t part_at = smem_u32(all), stats_at = smem_u32(all_stats);
+    const int pieces = D / 8;
+    for (int x = tid + split * kRowsWarps * 32; x < live * pieces; x += kRowsWarps * 32 * p.splits) {
+        const int row = x / pieces, d = x % pieces * 8;
+        // column d + e = kWide g + j of unit u lies at (kWide u + j) * 8 + g
+        const int col = (d / (8 * kWide) * kWide + d % kWide) * 8 + d % (8 * kWide) / kWide;
+        float y[8] = {}, total = 0.f;
+        if (p.splits == 1) {
+            total = all_stats[16 + row];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = all[row * R::kPitch + col + e * 8];
+        } else {
+            float top = -INFINITY;
+            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, dsmem_f32(stats_at + row * 4, s));
+            for (int s = 0; s < p.splits; ++s) {
+                const float k = top == -INFINITY ? 0.f : exp2_fast(dsmem_f32(stats_at + row * 4, s) - top);
+                total = __fmaf_rn(dsmem_f32(stats_at + (16 + row) * 4, s), k, total);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = __fmaf_rn(dsmem_f32(part_at + (row * R::kPitch + col + e * 8) * 4, s), k, y[e]);
+            }
+        }
+        store_row(p, y, total, b, r0 + row, kvh, ratio, d, QT());
+    }
+    if (p.splits > 1) cluster_sync_all();      // nobody leaves while its shared memory is read
+}
+
+template <typename QT, int DP> int launch_rows(AttnParams& p, cudaStream_t st) {
+    using R = RowsTile<DP>;
+    auto kern = kv8_rows_kernel<QT, DP>;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kSmem)) return (int)e;
+    const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + 15) / 16, base = tiles * p.B * p.Hkv;
+    p.row_tiles = (int)tiles;
+    p.splits = 1;
+    while (p.splits < 8 && base * p.splits < 148 * 8 && (int64_t)p.Lkv > (int64_t)p.splits * 16 * kRowsWarps) p.splits *= 2;
+    if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
+    return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kRowsWarps * 32, R::kSmem, st, p.splits, p);
+}
+
 template <typename QT, bool KV8> int launch_width(AttnParams& p, cudaStream_t st) {
+    if constexpr (KV8)
+        if ((int64_t)p.Lq * (p.H / p.Hkv) <= 16)
+            return p.D <= 64 ? launch_rows<QT, 64>(p, st) : p.D <= 128 ? launch_rows<QT, 128>(p, st) : launch_rows<QT, 256>(p, st);
     if (p.D <= 64) return launch_tile<QT, 64, KV8>(p, st);
     if (p.D <= 128) return launch_tile<QT, 128, KV8>(p, st);
     if (p.D <= 192) return launch_tile<QT, 192, KV8>(p, st);
