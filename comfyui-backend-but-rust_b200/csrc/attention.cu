@@ -6,66 +6,16 @@
 // o[i] = sum_t p[i, t] v[t] / sum_t p[i, t],  p[i, t] = exp(scale q[i] . k[t] - m[i]), m[i] the largest exponent seen so far; a row that sees
 // no key is zeros. One pass over the keys: the sums are scaled when m grows. Exponents, m and both sums are f32; p is rounded to the type
 // of the matrix product (as its operands have to be) after it entered the sum of p, so that the rounding is at most half a step of each term.
-#include "common.cuh"
-#include "mma.cuh"
-
-#include <type_traits>
+#include "attention.cuh"
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kTiny = 1e-30f;          // the smallest scale of a page; smaller ones are taken for it
+using namespace b200q;
 
-struct AttnParams {
-    const void *q, *k, *v;
-    void* out;
-    int64_t qs[3], ks[3], vs[3], os[3];      // strides of batch, row, head in elements (k and v: 16-bit rows only)
-    const float *k_scale, *v_scale;          // pages: [pages, Hkv]
-    const int32_t* table;                    // [B, max_pages]
-    int64_t table_stride, pages;
-    const int32_t* kv_len;                   // keys of each sequence, or null: Lkv
-    const int32_t* q_len;                    // query rows of each sequence, or null: Lq
-    const uint8_t* mask;                     // [B, Lkv], 0 = not seen, or null
-    int64_t mask_stride;
-    int B, Lq, Lkv, H, Hkv, D, T, causal, splits, row_tiles;
-    float scale;
-};
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float dsmem_f32(uint32_t addr, uint32_t rank) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, rank)) : "memory");
     return v;
-}
-
-// Four int8 codes as four halves, exact: each byte, its sign bit turned, becomes the low byte of 1024 + (code + 128), and 1152 is taken away.
-__device__ __forceinline__ uint2 halves_of4(uint32_t w) {
-    const uint32_t off = 0x64806480u, a = w ^ 0x80808080u;
-    const uint32_t lo = __byte_perm(a, 0x64646464u, 0x4140), hi = __byte_perm(a, 0x64646464u, 0x4342);
-    const half2 x = __hsub2(*reinterpret_cast<const half2*>(&lo), *reinterpret_cast<const half2*>(&off));
-    const half2 y = __hsub2(*reinterpret_cast<const half2*>(&hi), *reinterpret_cast<const half2*>(&off));
-    return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-}
-
-// bf16 queries over int8 keys are taken as halves times a power of two: 2^e brings a row's largest magnitude to [2^14, 2^15). 2^e and 2^-e are
-// f32 numbers.
-__device__ __forceinline__ int row_exponent(float top) {
-    return top > 0.f && top <= FLT_MAX ? min(100, max(-100, 14 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
-}
-
-// Eight columns of a finished row; one that saw no key is zeros, NaN stays.
-template <typename QT> __device__ __forceinline__ void store_row(const AttnParams& p, const float (&y)[8], float total, int b, int row, int kvh, int ratio, int d, QT) {
-    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-    uint4 w;
-    uint32_t* ow = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ow[e] = pack2<QT>(y[2 * e] * inv, y[2 * e + 1] * inv);
-    QT* dst = reinterpret_cast<QT*>(p.out) + b * p.os[0] + (int64_t)(row / ratio) * p.os[1] + (kvh * ratio + row % ratio) * p.os[2] + d;
-    *reinterpret_cast<uint4*>(dst) = w;
 }
 
 // 64 query rows (a kv head's queries: row r is query r / ratio, head r % ratio of its group), 64 keys a step, four warps of 16 rows.
@@ -616,6 +566,7 @@ template <typename QT, int DP> int launch_rows(AttnParams& p, cudaStream_t st) {
 }
 
 template <typename QT, bool KV8> int launch_width(AttnParams& p, cudaStream_t st) {
+    if (attention_tc_takes(p, KV8)) return attention_tc(std::is_same<QT, half>::value ? DT_F16 : DT_BF16, KV8, p, st);
     if constexpr (KV8)
         if ((int64_t)p.Lq * (p.H / p.Hkv) <= 16)
             return p.D <= 64 ? launch_rows<QT, 64>(p, st) : p.D <= 128 ? launch_rows<QT, 128>(p, st) : launch_rows<QT, 256>(p, st);

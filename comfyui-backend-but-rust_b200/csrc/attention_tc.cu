@@ -1,0 +1,584 @@
+// Attention with many query rows, on tcgen05: the kernel behind gpu_cross_attention and gpu_kv8_attention where tiles of 128 rows fill.
+//
+// A CTA an SM, persistent, two tiles of 128 query rows at a time over tiles of 128 keys. Per key tile and query tile: S = Q K^T into tensor
+// memory (128 columns of f32), p = exp2(S c - m) by one thread a row, p back into the same columns as 16-bit values, O += p V with p as the
+// operand from tensor memory. While the softmax warps of one query tile work, the tensor cores multiply for the other. Tensor memory: S of
+// both tiles in columns 0..255, O in 256..511.
+//
+// Warps 0-3 and 4-7: softmax and the rows' way out, for the two tiles. Warp 8 issues the products (one thread), in the order S0 S1 | O0 S0'
+// O1 S1' | ..., in which the tensor cores execute them: S' of the next key tile overwrites p only behind the product that read it. Warp 9
+// loads 16-bit Q, K and V by TMA; for the int8 cache warps 9-12 load codes, turn them into halves and write them as TMA would.
+// m follows the running maximum only when that has grown by 2^8: until then p is at most 256 and the sums need no rescaling; O is then scaled
+// in tensor memory by the row's own thread, which nothing else touches between the two products of its tile.
+// Keys that are not seen get p = 0; what V holds there (16-bit V comes as it lies in memory, NaN perhaps) is overwritten with zeros in shared
+// memory before the product.
+// Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "attention.cuh"
+
+namespace {
+
+using namespace b200q;
+
+__device__ int g_attention_status = 0;
+
+constexpr int kTileKeys = 128, kSlots = 4, kBox = 128 * 128;       // a box: 128 rows of 128 bytes, 128-byte swizzle
+constexpr float kSlack = 8.f;                                      // by how much (a power of two) p may exceed 1
+
+template <int DP, bool KV8> struct Tc {
+    static constexpr int kTile = DP / 64 * kBox;                   // 128 rows of Q, K or V
+    static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + 8 * 2048;
+    static constexpr int kWords = kTail + 160, kInfo = kWords + kSlots * 16, kFactor = kInfo + kSlots * 96;
+    static constexpr int kEnd = kFactor + (KV8 ? 2048 : 0), kSmem = kEnd + 1024;
+    static constexpr int kThreads = KV8 ? 416 : 320;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// kind::f16: D f32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1), B's rows along N when `n_major` (bit 16)
+__host__ __device__ constexpr uint32_t umma_idesc_16(bool is_bf16, bool n_major, int m, int n) {
+    return (1u << 4) | ((is_bf16 ? 1u : 0u) << 7) | ((is_bf16 ? 1u : 0u) << 10) | ((n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Both operands from shared memory, K-major boxes
+__device__ __forceinline__ void umma_16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128) : "memory");
+}
+// A from tensor memory, B from shared memory
+__device__ __forceinline__ void umma_16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128) : "memory");
+}
+// V lies with its columns side by side: rows of 64 columns, 8 keys to a swizzle atom (1024 bytes apart, the stride offset); the next 64
+// columns are a box further on (the leading offset).
+__device__ __forceinline__ uint32_t umma_desc_lo_n_major(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | ((uint32_t)(kBox >> 4) << 16); }
+
+struct TcParams {
+    AttnParams a;
+    int q_tiles;             // pairs of tiles: 256 rows
+    int64_t items;
+    int kv_batch, kv_head;   // 0: the batch's (the heads') keys and values are one
+    int q_batch, q_head;
+};
+struct Item {
+    int b, h, row0, rows, len, ql, seen, n;      // h: query head, or kv head of packed rows; rows from row0 on; n key tiles
+};
+template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, int64_t i) {
+    Item x;
+    const int heads = KV8 ? p.a.Hkv : p.a.H, bhs = p.a.B * heads;
+    // 16-bit: the tiles of a head next to one another (its keys stay in L2); cache: long causal tiles first
+    const int bh = KV8 ? (int)(i % bhs) : (int)(i / p.q_tiles), qt = KV8 ? p.q_tiles - 1 - (int)(i / bhs) : (int)(i % p.q_tiles);
+    x.b = bh / heads, x.h = bh % heads, x.row0 = qt * 256;
+    x.len = p.a.kv_len ? min(max(gload(p.a.kv_len + x.b), 0), p.a.Lkv) : p.a.Lkv;
+    x.ql = p.a.Lq;
+    x.seen = x.len;
+    if (KV8) {
+        const int ratio = p.a.H / p.a.Hkv;
+        if (p.a.q_len) x.ql = min(max(gload(p.a.q_len + x.b), 0), p.a.Lq);
+        x.rows = min(256, x.ql * ratio - x.row0);
+        if (p.a.causal) x.seen = max(0, min(x.len, x.len - x.ql + (x.row0 + x.rows - 1) / ratio + 1));
+    } else x.rows = min(256, p.a.Lq - x.row0);
+    x.n = x.rows > 0 ? (x.seen + kTileKeys - 1) / kTileKeys : 0;
+    return x;
+}
+
+template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(Tc<DP, KV8>::kThreads, 1)
+attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                    const TcParams p) {
+    using L = Tc<DP, KV8>;
+    constexpr bool kBf16 = std::is_same<QT, bf16>::value, kBf16Mma = kBf16 && !KV8;
+    using T = typename std::conditional<KV8, half, QT>::type;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* sm = smem_raw + (base - raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bars = base + L::kTail;
+    const uint32_t kv_full = bars, kv_empty = bars + 32, q_full = bars + 64, q_empty = bars + 80, s_full = bars + 96, p_full = bars + 112;
+    uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 128);
+    volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
+    uint32_t* words = reinterpret_cast<uint32_t*>(sm + L::kWords);            // [key tile % 4][4]: bit = key is seen
+    float* info = reinterpret_cast<float*>(sm + L::kInfo);                    // [key tile % 4][factor, offset, weight][16 keys]
+    float* factors = reinterpret_cast<float*>(sm + L::kFactor);               // [item % 2][tile][row]: bf16 queries' power of two
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
+        for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4);
+        *abort_s = 0;
+        fence_mbar_init();
+        if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(tmem_s), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_s;
+    pdl_wait();
+    const int D = p.a.D;
+
+    if (warp < 8) {
+        // ---- softmax of tile t, one row a thread
+        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, ratio = KV8 ? p.a.H / p.a.Hkv : 1;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+        const float c = p.a.scale * kLog2e;
+        uint8_t* stage = sm + L::kStaging + warp * 2048;
+        uint32_t s_phase = 0, tile_no = 0, item_no = 0;
+        bool ok = true;
+        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            const Item x = item_at<KV8>(p, i);
+            if (x.n > 0 && t * 128 >= x.rows) {
+                tile_no += x.n, ++item_no;
+                continue;
+            }
+            if (x.rows <= 0) continue;
+            float m = -INFINITY, l = 0.f, factor = 1.f;
+            // keys that this row sees
+            const int bound = KV8 && p.a.causal ? x.len - x.ql + (x.row0 + t * 128 + row) / ratio + 1 : x.seen;
+            for (int j = 0; j < x.n; ++j, ++tile_no) {
+                if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) { ok = false; break; }
+                s_phase ^= 1;
+                tc_fence_after();
+                const uint32_t* w = words + (tile_no & 3) * 4;
+                const float* in = info + (tile_no & 3) * 24;
+                if (KV8 && kBf16 && j == 0) factor = factors[(item_no & 1) * 256 + t * 128 + row];
+                const int limit = bound - j * kTileKeys;
+                const bool all = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu && (!KV8 || __all_sync(0xffffffffu, limit >= kTileKeys));
+                // logit of key e of quarter q, in powers of two (16-bit: without the factor c, which the exponent's product applies)
+                auto value = [&](uint32_t bits, int q, int e, uint32_t wq) {
+                    float v = __uint_as_float(bits);
+                    if (KV8) v = __fmaf_rn(v, in[q * 2 + (e >> 4)] * factor, in[8 + q * 2 + (e >> 4)]);
+                    if (!all && (!(wq >> e & 1) || (KV8 && q * 32 + e >= limit))) v = -INFINITY;
+                    return v;
+                };
+                float top = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t r[32];
+                    tmem_ld32(s_at + q * 32, r);
+                    tmem_ld_wait();
+                    const uint32_t wq = w[q];
+                    float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) a = fmaxf(a, value(r[e], q, e, wq)), b = fmaxf(b, value(r[e + 1], q, e + 1, wq));
+                    top = fmaxf(top, fmaxf(a, b));
+                }
+                if (!KV8) top *= c;
+                const bool grew = top > m + kSlack;
+                if (__any_sync(0xffffffffu, grew)) {
+                    const float keep = grew ? exp2_fast(m - top) : 1.f;
+                    if (grew) m = top;
+                    l *= keep;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int q = 0; q < DP / 32; ++q) {
+                            uint32_t r[32];
+                            tmem_ld32(o_at + q * 32, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * keep);
+                            tmem_st32(o_at + q * 32, r);
+                        }
+                    }
+                }
+                const float shift = m == -INFINITY ? 0.f : m;
+                float sum[4] = {};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t r[32], out[16];
+                    tmem_ld32(s_at + q * 32, r);
+                    tmem_ld_wait();
+                    const uint32_t wq = w[q];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float y[2];
+#pragma unroll
+                        for (int f = 0; f < 2; ++f) {
+                            const float v = value(r[e + f], q, e + f, wq);
+                            y[f] = exp2_fast(KV8 ? v - shift : __fmaf_rn(v, c, -shift));
+                            if (KV8) sum[(e & 2) + f] = __fmaf_rn(y[f], in[16 + q * 2 + (e >> 4)], sum[(e & 2) + f]);
+                            else sum[(e & 2) + f] += y[f];
+                        }
+                        out[e >> 1] = pack2<T>(y[0], y[1]);
+                    }
+                    tmem_st16(s_at + q * 16, out);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * t);
+            }
+            if (!ok) break;
+            // ---- the rows out: 32 columns at a time through this warp's staging, so that a row's pieces are stored together
+            if (x.n > 0) {
+                if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
+                s_phase ^= 1, ++item_no;
+                tc_fence_after();
+            }
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            for (int q = 0; q * 32 < D; ++q) {
+                uint32_t r[32] = {};
+                if (x.n > 0) {
+                    tmem_ld32(o_at + q * 32, r);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint4 v;
+                    uint32_t* o = reinterpret_cast<uint32_t*>(&v);
+                    // (l = 0: the columns may hold anything, an earlier row's infinity among it)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                        o[f] = inv == 0.f && l == 0.f ? 0u : pack2<QT>(__uint_as_float(r[e * 8 + 2 * f]) * inv, __uint_as_float(r[e * 8 + 2 * f + 1]) * inv);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ (lane >> 1)) & 3) * 16) = v;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rr = k * 8 + (lane >> 2), e = lane & 3, at = t * 128 + quarter * 32 + rr, d = q * 32 + e * 8;
+                    if (at < x.rows && d < D) {
+                        const int gr = x.row0 + at, query = KV8 ? gr / ratio : gr, head = KV8 ? x.h * ratio + gr % ratio : x.h;
+                        QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + query * p.a.os[1] + head * p.a.os[2] + d;
+                        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((e ^ (rr >> 1)) & 3) * 16);
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+        }
+    } else if (warp == 8) {
+        // ---- products
+        const uint32_t idesc_s = umma_idesc_16(kBf16Mma, false, 128, kTileKeys), idesc_o = umma_idesc_16(kBf16Mma, true, 128, DP);
+        const bool one = elect_one();
+        uint32_t kv_no = 0, q_no[2] = {}, p_phase[2] = {}, tile_no = 0;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity, int code) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, code)); };
+        auto issue_s = [&](int t, uint32_t slot) {
+            const uint32_t q = umma_desc_lo(base + t * L::kTile), k = umma_desc_lo(base + L::kRing + slot * L::kTile);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t step = (kk & 3) * 2 + (kk >> 2) * (kBox >> 4);
+                umma_16_ss(tmem + t * 128, q + step, k + step, idesc_s, kk > 0);
+            }
+        };
+        auto ready = [&](int t) {      // one arrival when the products are done, one that orders what this warp has seen in shared memory
+            umma_commit(s_full + 8 * t);
+            mbar_arrive(s_full + 8 * t);
+        };
+        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            const Item x = item_at<KV8>(p, i);
+            if (x.n == 0) continue;
+            const int tiles = x.rows > 128 ? 2 : 1;
+            uint32_t ks = kv_no & 3, k_phase = kv_no >> 2 & 1;
+            if (!wait(kv_full + 8 * ks, k_phase, ST_TIMEOUT_FULL)) break;
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait(q_full + 8 * t, q_no[t] & 1, ST_TIMEOUT_FULL)) break;
+                ++q_no[t];
+                tc_fence_after();
+                if (one) {
+                    issue_s(t, ks);
+                    if (x.n == 1) umma_commit(q_empty + 8 * t);
+                    ready(t);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (one) umma_commit(kv_empty + 8 * ks);
+            for (int j = 0; j < x.n; ++j, ++tile_no) {
+                const uint32_t v_no = kv_no + 1, vs = v_no & 3;
+                const bool more = j + 1 < x.n;
+                if (!wait(kv_full + 8 * vs, v_no >> 2 & 1, ST_TIMEOUT_FULL)) break;
+                if (!KV8) {      // rows of V behind keys that are not seen
+                    const uint32_t* w = words + (tile_no & 3) * 4;
+                    if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
+                        for (int key = lane >> 3; key < min(kTileKeys, p.a.Lkv - j * kTileKeys); key += 4)
+                            if (!(w[key >> 5] >> (key & 31) & 1))
+#pragma unroll
+                                for (int box = 0; box < DP / 64; ++box)
+                                    *reinterpret_cast<uint4*>(sm + L::kRing + vs * L::kTile + box * kBox + key * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                ks = (kv_no + 2) & 3, k_phase = (kv_no + 2) >> 2 & 1;
+                for (int t = 0; t < tiles; ++t) {
+                    if (!wait(p_full + 8 * t, p_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
+                    p_phase[t] ^= 1;
+                    if (more && t == 0 && !wait(kv_full + 8 * ks, k_phase, ST_TIMEOUT_FULL)) break;
+                    tc_fence_after();
+                    if (one) {
+                        const uint32_t v = umma_desc_lo_n_major(base + L::kRing + vs * L::kTile);
+#pragma unroll
+                        for (int kk = 0; kk < kTileKeys / 16; ++kk)      // 16 keys: 8 columns of p, two swizzle atoms of V
+                            umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0);
+                        if (more) {
+                            issue_s(t, ks);
+                            if (j + 2 == x.n) umma_commit(q_empty + 8 * t);
+                        }
+                        ready(t);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (one) {
+                    umma_commit(kv_empty + 8 * vs);
+                    if (more) umma_commit(kv_empty + 8 * ks);
+                }
+                kv_no += 2;
+            }
+        }
+    } else if (!KV8) {
+        // ---- loads
+        uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
+        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            const Item x = item_at<KV8>(p, i);
+            if (x.n == 0) continue;
+            const int tiles = x.rows > 128 ? 2 : 1, kvh = x.h / (p.a.H / p.a.Hkv);
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait(q_empty + 8 * t, (q_no[t] & 1) ^ 1)) break;
+                ++q_no[t];
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(q_full + 8 * t, L::kTile);
+#pragma unroll
+                    for (int box = 0; box < DP / 64; ++box)
+                        tma_load_4d(base + t * L::kTile + box * kBox, &tmap_q, box * 64, x.row0 + t * 128, x.h * p.q_head, x.b * p.q_batch, q_full + 8 * t);
+                }
+                __syncwarp();
+            }
+            for (int j = 0; j < x.n && ok; ++j, ++tile_no)
+                for (int which = 0; which < 2; ++which, ++kv_no) {
+                    const uint32_t slot = kv_no & 3;
+                    if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
+                    if (which == 0) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int key = j * kTileKeys + q * 32 + lane;
+                            const bool seen = key < x.seen && (!p.a.mask || gload(p.a.mask + x.b * p.a.mask_stride + key) != 0);
+                            const uint32_t w = __ballot_sync(0xffffffffu, seen);
+                            if (lane == 0) words[(tile_no & 3) * 4 + q] = w;
+                        }
+                    }
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(kv_full + 8 * slot, L::kTile);
+#pragma unroll
+                        for (int box = 0; box < DP / 64; ++box)
+                            tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
+                                        kv_full + 8 * slot);
+                    }
+                    __syncwarp();
+                }
+        }
+    } else {
+        // ---- codes to halves: four warps of 32 keys (or query rows) each
+        const int w = warp - 9;
+        uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0, item_no = 0;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
+        auto done = [&](uint32_t bar) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto put = [&](uint8_t* tile, int row, int piece, uint4 v) {      // 8 values: piece `piece` of a row of 16-bit values
+            *reinterpret_cast<uint4*>(tile + (piece >> 3) * kBox + row * 128 + ((piece ^ row) & 7) * 16) = v;
+        };
+        const int ratio = p.a.H / p.a.Hkv;
+        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            const Item x = item_at<KV8>(p, i);
+            if (x.n == 0) continue;
+            const int tiles = x.rows > 128 ? 2 : 1;
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait(q_empty + 8 * t, (q_no[t] & 1) ^ 1)) break;
+                ++q_no[t];
+                constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes;        // lanes to a row, rows to an instruction
+#pragma unroll 4
+                for (int k = 0; k < 32 / kAtOnce; ++k) {
+                    const int row = w * 32 + k * kAtOnce + lane / kLanes, piece = lane % kLanes, at = t * 128 + row, gr = x.row0 + at;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (at < x.rows && piece * 8 < D)
+                        v = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const QT*>(p.a.q) + x.b * p.a.qs[0] + (gr / ratio) * p.a.qs[1] +
+                                                                 (x.h * ratio + gr % ratio) * p.a.qs[2]) + piece);
+                    if (kBf16) {
+                        const QT* y = reinterpret_cast<const QT*>(&v);
+                        float top = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f<QT>(y[e])));
+#pragma unroll
+                        for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int e2 = row_exponent(top);
+                        const float mult = __uint_as_float((uint32_t)(127 + e2) << 23);
+                        if (piece == 0) factors[(item_no & 1) * 256 + t * 128 + row] = __uint_as_float((uint32_t)(127 - e2) << 23);
+                        uint4 z;
+                        uint32_t* o = reinterpret_cast<uint32_t*>(&z);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = pack2<half>(to_f<QT>(y[2 * e]) * mult, to_f<QT>(y[2 * e + 1]) * mult);
+                        v = z;
+                    }
+                    put(sm + t * L::kTile, row, piece, v);
+                }
+                done(q_full + 8 * t);
+            }
+            ++item_no;
+            for (int j = 0; j < x.n && ok; ++j, ++tile_no) {
+                // this warp's 32 keys: one to a lane
+                const int key0 = j * kTileKeys + w * 32, key = key0 + lane;
+                int64_t page = key < x.seen ? gload(p.a.table + x.b * p.a.table_stride + key / p.a.T) : -1;
+                const bool there = page >= 0 && page < p.a.pages;
+                const int64_t off = there ? ((page * p.a.Hkv + x.h) * p.a.T + key % p.a.T) * D : -1;
+                for (int which = 0; which < 2; ++which, ++kv_no) {
+                    constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
+                    uint4 code[32 / kAtOnce];
+#pragma unroll
+                    for (int k = 0; k < 32 / kAtOnce; ++k) {
+                        const int64_t o = __shfl_sync(0xffffffffu, off, k * kAtOnce + lane / kLanes);
+                        const int piece = lane % kLanes;
+                        code[k] = make_uint4(0x0, 0x0, 0x0, 0x0);
+                        if (o >= 0 && piece * 16 < D) code[k] = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const int8_t*>(which ? p.a.v : p.a.k) + o) + piece);
+                    }
+                    const uint32_t slot = kv_no & 3;
+                    if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
+                    if (which == 0) {
+                        const uint32_t seen = __ballot_sync(0xffffffffu, there);
+                        if (lane == 0) words[(tile_no & 3) * 4 + w] = seen;
+                        if ((lane & 15) == 0) {
+                            float* in = info + (tile_no & 3) * 24 + w * 2 + (lane >> 4);
+                            float mul = 0.f, add = 0.f, wt = 0.f;
+                            if (there) {
+                                const float s = fmaxf(gload(p.a.v_scale + page * p.a.Hkv + x.h), kTiny);
+                                mul = gload(p.a.k_scale + page * p.a.Hkv + x.h) * (p.a.scale * kLog2e), add = log2f(s), wt = 1.f / s;
+                            }
+                            in[0] = mul, in[8] = add, in[16] = wt;
+                        }
+                    }
+                    uint8_t* tile = sm + L::kRing + slot * L::kTile;
+#pragma unroll
+                    for (int k = 0; k < 32 / kAtOnce; ++k) {
+                        const int row = w * 32 + k * kAtOnce + lane / kLanes, piece = lane % kLanes;
+                        const uint2 a = halves_of4(code[k].x), b = halves_of4(code[k].y), e = halves_of4(code[k].z), f = halves_of4(code[k].w);
+                        put(tile, row, 2 * piece, make_uint4(a.x, a.y, b.x, b.y));
+                        put(tile, row, 2 * piece + 1, make_uint4(e.x, e.y, f.x, f.y));
+                    }
+                    done(kv_full + 8 * slot);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_s != 0) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);      // leave time for copies and products still in flight, then report
+        if (threadIdx.x == 0) atomicCAS(&g_attention_status, 0, *abort_s);
+        __syncthreads();
+    }
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static std::atomic<EncodeTiledFn> fn{nullptr};
+    EncodeTiledFn f = fn.load(std::memory_order_acquire);
+    if (f) return f;
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess || !sym)
+        return nullptr;
+    f = reinterpret_cast<EncodeTiledFn>(sym);
+    fn.store(f, std::memory_order_release);
+    return f;
+}
+// Rows [B, L, H, D] of 16-bit values as boxes of 64 columns by 128 rows; columns and rows outside read as zeros. A dimension without a
+// stride is one entry.
+bool make_rows_map(CUtensorMap* tm, const void* ptr, const int64_t (&s)[3], int B, int L, int H, int D) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    auto dim = [](int64_t stride, int n) { return (cuuint64_t)(stride ? n : 1); };
+    auto pitch = [](int64_t stride) { return (cuuint64_t)(stride ? stride * 2 : 16); };
+    const cuuint64_t dims[4] = {(cuuint64_t)D, dim(s[1], L), dim(s[2], H), dim(s[0], B)}, strides[3] = {pitch(s[1]), pitch(s[2]), pitch(s[0])};
+    const cuuint32_t box[4] = {64, 128, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return n;
+}
+
+template <typename QT, int DP, bool KV8> int launch_tc(const CUtensorMap (&tm)[3], const TcParams& p, cudaStream_t st) {
+    using L = Tc<DP, KV8>;
+    auto kern = attention_tc_kernel<QT, DP, KV8>;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
+    const int sms = sm_count();
+    if (sms <= 0) return (int)cudaErrorInvalidDevice;
+    return launch_pdl(kern, dim3((unsigned)(p.items < sms ? p.items : sms)), L::kThreads, L::kSmem, st, tm[0], tm[1], tm[2], p);
+}
+
+}  // namespace
+
+bool b200q::attention_tc_takes(const AttnParams& p, bool kv8) {
+    if (p.D > 128 || !(p.scale > 0.f) || p.Lkv <= 0) return false;
+    const int64_t rows = kv8 ? (int64_t)p.Lq * (p.H / p.Hkv) : p.Lq;
+    if (rows < 128) return false;
+    // rows without a stride between them have no tensor map
+    return kv8 || ((p.Lq == 1 || p.qs[1] > 0) && (p.Lkv == 1 || (p.ks[1] > 0 && p.vs[1] > 0)) && p.qs[0] >= 0 && p.qs[2] >= 0 && p.ks[0] >= 0 &&
+                   p.ks[2] >= 0 && p.vs[0] >= 0 && p.vs[2] >= 0 && (p.ks[0] == 0) == (p.vs[0] == 0) && (p.ks[2] == 0) == (p.vs[2] == 0));
+}
+
+int b200q::attention_tc(int dtype, bool kv8, AttnParams& a, cudaStream_t st) {
+    TcParams p = {};
+    p.a = a;
+    const int64_t rows = kv8 ? (int64_t)a.Lq * (a.H / a.Hkv) : a.Lq, tiles = (rows + 255) / 256;
+    if (rows > INT32_MAX - 512) return -1;
+    p.q_tiles = (int)tiles, p.items = tiles * a.B * (kv8 ? a.Hkv : a.H);
+    p.q_batch = a.qs[0] != 0, p.q_head = a.qs[2] != 0, p.kv_batch = a.ks[0] != 0, p.kv_head = a.ks[2] != 0;
+    CUtensorMap tm[3] = {};
+    if (!kv8 && (!make_rows_map(&tm[0], a.q, a.qs, a.B, a.Lq, a.H, a.D) || !make_rows_map(&tm[1], a.k, a.ks, a.B, a.Lkv, a.Hkv, a.D) ||
+                 !make_rows_map(&tm[2], a.v, a.vs, a.B, a.Lkv, a.Hkv, a.D)))
+        return -203;
+    const bool h = dtype == DT_F16, wide = a.D > 64;
+    if (kv8) return h ? (wide ? launch_tc<half, 128, true>(tm, p, st) : launch_tc<half, 64, true>(tm, p, st))
+                      : (wide ? launch_tc<bf16, 128, true>(tm, p, st) : launch_tc<bf16, 64, true>(tm, p, st));
+    return h ? (wide ? launch_tc<half, 128, false>(tm, p, st) : launch_tc<half, 64, false>(tm, p, st))
+             : (wide ? launch_tc<bf16, 128, false>(tm, p, st) : launch_tc<bf16, 64, false>(tm, p, st));
+}
+
+int b200q::attention_status_read_clear(int* out) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_attention_status, sizeof(int));
+    if (e != cudaSuccess) return (int)e;
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return (int)e;
+    *out = v;
+    return 0;
+}
