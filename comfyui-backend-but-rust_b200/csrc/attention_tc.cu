@@ -7,7 +7,7 @@
 //
 // Warps 0-3 and 4-7: softmax and the rows' way out, for the two tiles. Warp 8 issues the products (one thread), in the order S0 S1 | O0 S0'
 // O1 S1' | ..., in which the tensor cores execute them: S' of the next key tile overwrites p only behind the product that read it. Warp 9
-// loads 16-bit Q, K and V by TMA; for the int8 cache warps 9-12 load codes, turn them into halves and write them as TMA would.
+// loads 16-bit Q, K and V by TMA; for the int8 cache warps 12-15 load codes, turn them into halves and write them as TMA would.
 // m follows the running maximum only when that has grown by 2^8: until then p is at most 256 and the sums need no rescaling; O is then scaled
 // in tensor memory by the row's own thread, which nothing else touches between the two products of its tile.
 // Keys that are not seen get p = 0; what V holds there (16-bit V comes as it lies in memory, NaN perhaps) is overwritten with zeros in shared
@@ -33,13 +33,19 @@ template <int DP, bool KV8> struct Tc {
     static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + 8 * 2048;
     static constexpr int kWords = kTail + 160, kInfo = kWords + kSlots * 16, kFactor = kInfo + kSlots * 96;
     static constexpr int kEnd = kFactor + (KV8 ? 2048 : 0), kSmem = kEnd + 1024;
-    static constexpr int kThreads = KV8 ? 416 : 320;
+    static constexpr int kThreads = KV8 ? 512 : 384;
+    // Registers of the warpgroups (softmax twice, products and loads, codes): a softmax thread holds a row of 128 logits. Their sum over the
+    // threads is what the launch has: 384 x 168, 512 x 128.
+    static constexpr int kSoftmaxRegs = KV8 ? 176 : 208, kIssueRegs = KV8 ? 48 : 88, kCodeRegs = 112;
+    static_assert(KV8 ? 2 * kSoftmaxRegs + kIssueRegs + kCodeRegs == 4 * 128 : 2 * kSoftmaxRegs + kIssueRegs == 3 * 168, "register split");
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int w, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
@@ -137,6 +143,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int D = p.a.D;
 
     if (warp < 8) {
+        more_registers<L::kSoftmaxRegs>();
         // ---- softmax of tile t, one row a thread
         const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, ratio = KV8 ? p.a.H / p.a.Hkv : 1;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
@@ -163,25 +170,36 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (KV8 && kBf16 && j == 0) factor = factors[(item_no & 1) * 256 + t * 128 + row];
                 const int limit = bound - j * kTileKeys;
                 const bool all = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu && (!KV8 || __all_sync(0xffffffffu, limit >= kTileKeys));
-                // logit of key e of quarter q, in powers of two (16-bit: without the factor c, which the exponent's product applies)
-                auto value = [&](uint32_t bits, int q, int e, uint32_t wq) {
-                    float v = __uint_as_float(bits);
-                    if (KV8) v = __fmaf_rn(v, in[q * 2 + (e >> 4)] * factor, in[8 + q * 2 + (e >> 4)]);
-                    if (!all && (!(wq >> e & 1) || (KV8 && q * 32 + e >= limit))) v = -INFINITY;
-                    return v;
-                };
-                float top = -INFINITY;
+                // logits: in powers of two for the cache, without the factor c for 16-bit keys (the exponent's product applies it)
+                float v[128];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t r[32];
-                    tmem_ld32(s_at + q * 32, r);
-                    tmem_ld_wait();
-                    const uint32_t wq = w[q];
-                    float a = -INFINITY, b = -INFINITY;
+                for (int q = 0; q < 4; ++q) tmem_ld32(s_at + q * 32, reinterpret_cast<uint32_t(&)[32]>(v[q * 32]));
+                tmem_ld_wait();
+                if (KV8) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) a = fmaxf(a, value(r[e], q, e, wq)), b = fmaxf(b, value(r[e + 1], q, e + 1, wq));
-                    top = fmaxf(top, fmaxf(a, b));
+                    for (int q = 0; q < 8; ++q) {
+                        const float mul = in[q] * factor, add = in[8 + q];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[q * 16 + e] = __fmaf_rn(v[q * 16 + e], mul, add);
+                    }
                 }
+                if (!all) {
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        uint32_t bits = w[q >> 2] >> (q & 3) * 8 & 255u;
+                        if (KV8) bits &= limit - q * 8 >= 8 ? 255u : limit - q * 8 <= 0 ? 0u : (1u << (limit - q * 8)) - 1u;
+                        if (KV8 || bits != 255u) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[q * 8 + e] = bits >> e & 1 ? v[q * 8 + e] : -INFINITY;
+                        }
+                    }
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 128; e += 8)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) tops[f] = fmaxf(tops[f], fmaxf(v[e + 2 * f], v[e + 2 * f + 1]));
+                float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 if (!KV8) top *= c;
                 const bool grew = top > m + kSlack;
                 if (__any_sync(0xffffffffu, grew)) {
@@ -204,17 +222,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 float sum[4] = {};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    uint32_t r[32], out[16];
-                    tmem_ld32(s_at + q * 32, r);
-                    tmem_ld_wait();
-                    const uint32_t wq = w[q];
+                    uint32_t out[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         float y[2];
 #pragma unroll
                         for (int f = 0; f < 2; ++f) {
-                            const float v = value(r[e + f], q, e + f, wq);
-                            y[f] = exp2_fast(KV8 ? v - shift : __fmaf_rn(v, c, -shift));
+                            y[f] = exp2_fast(KV8 ? v[q * 32 + e + f] - shift : __fmaf_rn(v[q * 32 + e + f], c, -shift));
                             if (KV8) sum[(e & 2) + f] = __fmaf_rn(y[f], in[16 + q * 2 + (e >> 4)], sum[(e & 2) + f]);
                             else sum[(e & 2) + f] += y[f];
                         }
@@ -266,7 +280,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             tc_fence_before();
         }
-    } else if (warp == 8) {
+    } else if (warp < 12) {
+      fewer_registers<L::kIssueRegs>();
+      if (warp == 8) {
         // ---- products
         const uint32_t idesc_s = umma_idesc_16(kBf16Mma, false, 128, kTileKeys), idesc_o = umma_idesc_16(kBf16Mma, true, 128, DP);
         const bool one = elect_one();
@@ -347,7 +363,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 kv_no += 2;
             }
         }
-    } else if (!KV8) {
+      } else if (!KV8 && warp == 9) {
         // ---- loads
         uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0;
         bool ok = true;
@@ -390,9 +406,11 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     __syncwarp();
                 }
         }
+      }
     } else {
+        fewer_registers<L::kCodeRegs>();
         // ---- codes to halves: four warps of 32 keys (or query rows) each
-        const int w = warp - 9;
+        const int w = warp - 12;
         uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0, item_no = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
@@ -441,47 +459,64 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 done(q_full + 8 * t);
             }
             ++item_no;
-            for (int j = 0; j < x.n && ok; ++j, ++tile_no) {
-                // this warp's 32 keys: one to a lane
-                const int key0 = j * kTileKeys + w * 32, key = key0 + lane;
-                int64_t page = key < x.seen ? gload(p.a.table + x.b * p.a.table_stride + key / p.a.T) : -1;
-                const bool there = page >= 0 && page < p.a.pages;
-                const int64_t off = there ? ((page * p.a.Hkv + x.h) * p.a.T + key % p.a.T) * D : -1;
-                for (int which = 0; which < 2; ++which, ++kv_no) {
-                    constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
-                    uint4 code[32 / kAtOnce];
-#pragma unroll
-                    for (int k = 0; k < 32 / kAtOnce; ++k) {
-                        const int64_t o = __shfl_sync(0xffffffffu, off, k * kAtOnce + lane / kLanes);
-                        const int piece = lane % kLanes;
-                        code[k] = make_uint4(0x0, 0x0, 0x0, 0x0);
-                        if (o >= 0 && piece * 16 < D) code[k] = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const int8_t*>(which ? p.a.v : p.a.k) + o) + piece);
-                    }
-                    const uint32_t slot = kv_no & 3;
-                    if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
-                    if (which == 0) {
-                        const uint32_t seen = __ballot_sync(0xffffffffu, there);
-                        if (lane == 0) words[(tile_no & 3) * 4 + w] = seen;
-                        if ((lane & 15) == 0) {
-                            float* in = info + (tile_no & 3) * 24 + w * 2 + (lane >> 4);
-                            float mul = 0.f, add = 0.f, wt = 0.f;
-                            if (there) {
-                                const float s = fmaxf(gload(p.a.v_scale + page * p.a.Hkv + x.h), kTiny);
-                                mul = gload(p.a.k_scale + page * p.a.Hkv + x.h) * (p.a.scale * kLog2e), add = log2f(s), wt = 1.f / s;
-                            }
-                            in[0] = mul, in[8] = add, in[16] = wt;
-                        }
-                    }
-                    uint8_t* tile = sm + L::kRing + slot * L::kTile;
-#pragma unroll
-                    for (int k = 0; k < 32 / kAtOnce; ++k) {
-                        const int row = w * 32 + k * kAtOnce + lane / kLanes, piece = lane % kLanes;
-                        const uint2 a = halves_of4(code[k].x), b = halves_of4(code[k].y), e = halves_of4(code[k].z), f = halves_of4(code[k].w);
-                        put(tile, row, 2 * piece, make_uint4(a.x, a.y, b.x, b.y));
-                        put(tile, row, 2 * piece + 1, make_uint4(e.x, e.y, f.x, f.y));
-                    }
-                    done(kv_full + 8 * slot);
+            // Pages are looked up a tile ahead, codes requested a step (K or V of a tile) ahead of their conversion.
+            constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
+            int64_t off = -1, off_next = -1;
+            float mul = 0.f, add = 0.f, wt = 0.f, mul_next = 0.f, add_next = 0.f, wt_next = 0.f;
+            auto look_up = [&](int j) {      // this warp's 32 keys of a tile: one to a lane
+                const int key = j * kTileKeys + w * 32 + lane;
+                const int64_t page = key < x.seen ? gload(p.a.table + x.b * p.a.table_stride + key / p.a.T) : -1;
+                off_next = -1, mul_next = 0.f, add_next = 0.f, wt_next = 0.f;
+                if (page >= 0 && page < p.a.pages) {
+                    off_next = ((page * p.a.Hkv + x.h) * p.a.T + key % p.a.T) * D;
+                    const float s = fmaxf(gload(p.a.v_scale + page * p.a.Hkv + x.h), kTiny);
+                    mul_next = gload(p.a.k_scale + page * p.a.Hkv + x.h) * (p.a.scale * kLog2e), add_next = log2f(s), wt_next = 1.f / s;
                 }
+            };
+            auto request = [&](uint4 (&code)[32 / kAtOnce], int64_t offs, int which) {
+                const int8_t* src = reinterpret_cast<const int8_t*>(which ? p.a.v : p.a.k);
+                const int piece = lane % kLanes;
+#pragma unroll
+                for (int k = 0; k < 32 / kAtOnce; ++k) {
+                    const int64_t o = __shfl_sync(0xffffffffu, offs, k * kAtOnce + lane / kLanes);
+                    code[k] = o >= 0 && piece * 16 < D ? gload(reinterpret_cast<const uint4*>(src + o) + piece) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            auto convert = [&](const uint4 (&code)[32 / kAtOnce], uint32_t slot) {
+                uint8_t* tile = sm + L::kRing + slot * L::kTile;
+                const int piece = lane % kLanes;
+#pragma unroll
+                for (int k = 0; k < 32 / kAtOnce; ++k) {
+                    const int row = w * 32 + k * kAtOnce + lane / kLanes;
+                    const uint2 a = halves_of4(code[k].x), b = halves_of4(code[k].y), e = halves_of4(code[k].z), f = halves_of4(code[k].w);
+                    put(tile, row, 2 * piece, make_uint4(a.x, a.y, b.x, b.y));
+                    put(tile, row, 2 * piece + 1, make_uint4(e.x, e.y, f.x, f.y));
+                }
+                done(kv_full + 8 * slot);
+            };
+            uint4 kc[32 / kAtOnce], vc[32 / kAtOnce];
+            look_up(0);
+            off = off_next, mul = mul_next, add = add_next, wt = wt_next;
+            request(kc, off, 0);
+            for (int j = 0; j < x.n && ok; ++j, ++tile_no) {
+                request(vc, off, 1);
+                if (j + 1 < x.n) look_up(j + 1);
+                uint32_t slot = kv_no & 3;
+                if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
+                ++kv_no;
+                const uint32_t seen = __ballot_sync(0xffffffffu, off >= 0);
+                if (lane == 0) words[(tile_no & 3) * 4 + w] = seen;
+                if ((lane & 15) == 0) {
+                    float* in = info + (tile_no & 3) * 24 + w * 2 + (lane >> 4);
+                    in[0] = mul, in[8] = add, in[16] = wt;
+                }
+                convert(kc, slot);
+                off = off_next, mul = mul_next, add = add_next, wt = wt_next;
+                if (j + 1 < x.n) request(kc, off, 0);
+                slot = kv_no & 3;
+                if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
+                ++kv_no;
+                convert(vc, slot);
             }
         }
     }
