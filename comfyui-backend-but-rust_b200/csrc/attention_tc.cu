@@ -30,16 +30,21 @@ constexpr float kSlack = 8.f;                                      // by how muc
 
 template <int DP, bool KV8> struct Tc {
     static constexpr int kTile = DP / 64 * kBox;                   // 128 rows of Q, K or V
-    static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + 8 * 2048;
-    static constexpr int kWords = kTail + 160, kInfo = kWords + kSlots * 16, kFactor = kInfo + kSlots * 96;
-    static constexpr int kEnd = kFactor + (KV8 ? 2048 : 0), kSmem = kEnd + 1024;
-    static constexpr int kThreads = KV8 ? 512 : 384;
-    // Registers of the warpgroups (softmax twice, products and loads, codes): a softmax thread holds a row of 128 logits. Their sum over the
-    // threads is what the launch has: 384 x 168, 512 x 128.
-    static constexpr int kSoftmaxRegs = KV8 ? 176 : 208, kIssueRegs = KV8 ? 48 : 88, kCodeRegs = 112;
-    static_assert(KV8 ? 2 * kSoftmaxRegs + kIssueRegs + kCodeRegs == 4 * 128 : 2 * kSoftmaxRegs + kIssueRegs == 3 * 168, "register split");
+    static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + (KV8 ? 8 * 2048 : 4 * 4096);
+    // barriers and two words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
+    // item % 2: 1 / l of every row (16-bit), or bf16 queries' powers of two
+    static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
+    static constexpr int kEnd = kRowInfo + 2048, kSmem = kEnd + 1024;
+    static constexpr int kThreads = 512;
+    // Registers of the warpgroups (softmax twice, products and loads, codes or rows out): a softmax thread holds a row of 128 logits. Their
+    // sum over the threads is what the launch has, 512 x 128.
+    static constexpr int kSoftmaxRegs = KV8 ? 176 : 184, kIssueRegs = KV8 ? 48 : 56, kLastRegs = KV8 ? 112 : 88;
+    static_assert(2 * kSoftmaxRegs + kIssueRegs + kLastRegs == 4 * 128, "register split");
 };
 
+__device__ __forceinline__ void tma_prefetch_4d(const void* tmap, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int w, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
@@ -50,6 +55,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// Two f32 operations in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {      // (x, y) = (a, b) * m + c
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(m), "f"(c));
+}
+__device__ __forceinline__ void fma2_into(float (&s)[2], float a, float b, float m) {                  // s += (a, b) * m
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%0, %1};\n\tfma.rn.f32x2 w, u, v, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b), "f"(m));
+}
+__device__ __forceinline__ void add2_into(float (&s)[2], float a, float b) {
+    asm("{\n\t.reg .b64 u, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 w, {%0, %1};\n\tadd.rn.f32x2 w, u, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b));
 }
 // kind::f16: D f32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1), B's rows along N when `n_major` (bit 16)
 __host__ __device__ constexpr uint32_t umma_idesc_16(bool is_bf16, bool n_major, int m, int n) {
@@ -90,10 +108,12 @@ struct Item {
 };
 template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, int64_t i) {
     Item x;
-    const int heads = KV8 ? p.a.Hkv : p.a.H, bhs = p.a.B * heads;
-    // 16-bit: the tiles of a head next to one another (its keys stay in L2); cache: long causal tiles first
-    const int bh = KV8 ? (int)(i % bhs) : (int)(i / p.q_tiles), qt = KV8 ? p.q_tiles - 1 - (int)(i / bhs) : (int)(i % p.q_tiles);
-    x.b = bh / heads, x.h = bh % heads, x.row0 = qt * 256;
+    const int heads = KV8 ? p.a.Hkv : p.a.H;
+    // heads next to one another: together they read and write whole rows of Q and of the result. Cache: long causal tiles first.
+    const int rest = (int)(i / heads);
+    x.h = (int)(i - (int64_t)rest * heads);
+    const int qt = KV8 ? p.q_tiles - 1 - rest / p.a.B : rest % p.q_tiles;
+    x.b = KV8 ? rest % p.a.B : rest / p.q_tiles, x.row0 = qt * 256;
     x.len = p.a.kv_len ? min(max(gload(p.a.kv_len + x.b), 0), p.a.Lkv) : p.a.Lkv;
     x.ql = p.a.Lq;
     x.seen = x.len;
@@ -118,15 +138,18 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint8_t* sm = smem_raw + (base - raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t bars = base + L::kTail;
-    const uint32_t kv_full = bars, kv_empty = bars + 32, q_full = bars + 64, q_empty = bars + 80, s_full = bars + 96, p_full = bars + 112;
-    uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 128);
+    const uint32_t kv_full = bars, kv_empty = bars + 32, q_full = bars + 64, q_empty = bars + 80, s_full = bars + 96, p_full = bars + 112,
+                   o_full = bars + 128, o_empty = bars + 144, p_half = bars + 160, v_ready = bars + 176;
+    uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
     uint32_t* words = reinterpret_cast<uint32_t*>(sm + L::kWords);            // [key tile % 4][4]: bit = key is seen
-    float* info = reinterpret_cast<float*>(sm + L::kInfo);                    // [key tile % 4][factor, offset, weight][16 keys]
-    float* factors = reinterpret_cast<float*>(sm + L::kFactor);               // [item % 2][tile][row]: bf16 queries' power of two
+    // [key tile % 4]: 16-bit: [key] +inf, or -inf where a key is not seen; cache: [factor, offset, weight][16 keys]
+    float* info = reinterpret_cast<float*>(sm + L::kInfo);
+    float* row_info = reinterpret_cast<float*>(sm + L::kRowInfo);             // [item % 2][tile][row]
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
-        for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4);
+        for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
+            mbar_init(o_full + 8 * t, 5), mbar_init(o_empty + 8 * t, 4), mbar_init(p_half + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
         *abort_s = 0;
         fence_mbar_init();
         if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
@@ -157,7 +180,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 tile_no += x.n, ++item_no;
                 continue;
             }
-            if (x.rows <= 0) continue;
+            if (x.rows <= 0 || (!KV8 && x.n == 0)) continue;
             float m = -INFINITY, l = 0.f, factor = 1.f;
             // keys that this row sees
             const int bound = KV8 && p.a.causal ? x.len - x.ql + (x.row0 + t * 128 + row) / ratio + 1 : x.seen;
@@ -166,8 +189,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 s_phase ^= 1;
                 tc_fence_after();
                 const uint32_t* w = words + (tile_no & 3) * 4;
-                const float* in = info + (tile_no & 3) * 24;
-                if (KV8 && kBf16 && j == 0) factor = factors[(item_no & 1) * 256 + t * 128 + row];
+                const float* in = info + (tile_no & 3) * (KV8 ? 24 : 128);
+                if (KV8 && kBf16 && j == 0) factor = row_info[(item_no & 1) * 256 + t * 128 + row];
                 const int limit = bound - j * kTileKeys;
                 const bool all = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu && (!KV8 || __all_sync(0xffffffffu, limit >= kTileKeys));
                 // logits: in powers of two for the cache, without the factor c for 16-bit keys (the exponent's product applies it)
@@ -180,17 +203,23 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     for (int q = 0; q < 8; ++q) {
                         const float mul = in[q] * factor, add = in[8 + q];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[q * 16 + e] = __fmaf_rn(v[q * 16 + e], mul, add);
+                        for (int e = 0; e < 16; e += 2) fma2(v[q * 16 + e], v[q * 16 + e + 1], v[q * 16 + e], v[q * 16 + e + 1], mul, add);
                     }
                 }
                 if (!all) {
+                    if (KV8) {      // pages that there are not: groups of 16 keys; then the row's own bound
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        uint32_t bits = w[q >> 2] >> (q & 3) * 8 & 255u;
-                        if (KV8) bits &= limit - q * 8 >= 8 ? 255u : limit - q * 8 <= 0 ? 0u : (1u << (limit - q * 8)) - 1u;
-                        if (KV8 || bits != 255u) {
+                        for (int q = 0; q < 8; ++q) {
+                            const int end = w[q >> 1] >> (q & 1) * 16 & 1 ? limit - q * 16 : 0;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) v[q * 8 + e] = bits >> e & 1 ? v[q * 8 + e] : -INFINITY;
+                            for (int e = 0; e < 16; ++e) v[q * 16 + e] = e < end ? v[q * 16 + e] : -INFINITY;
+                        }
+                    } else {        // the smaller of logit and limit: -inf also for what is no number
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) {
+                            const float4 f = reinterpret_cast<const float4*>(in)[q];
+                            v[q * 4] = fminf(v[q * 4], f.x), v[q * 4 + 1] = fminf(v[q * 4 + 1], f.y);
+                            v[q * 4 + 2] = fminf(v[q * 4 + 2], f.z), v[q * 4 + 3] = fminf(v[q * 4 + 3], f.w);
                         }
                     }
                 }
@@ -219,30 +248,36 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     }
                 }
                 const float shift = m == -INFINITY ? 0.f : m;
-                float sum[4] = {};
+                float sum[2][2] = {};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t out[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        float y[2];
-#pragma unroll
-                        for (int f = 0; f < 2; ++f) {
-                            y[f] = exp2_fast(KV8 ? v[q * 32 + e + f] - shift : __fmaf_rn(v[q * 32 + e + f], c, -shift));
-                            if (KV8) sum[(e & 2) + f] = __fmaf_rn(y[f], in[16 + q * 2 + (e >> 4)], sum[(e & 2) + f]);
-                            else sum[(e & 2) + f] += y[f];
-                        }
-                        out[e >> 1] = pack2<T>(y[0], y[1]);
+                        float a, b;
+                        fma2(a, b, v[q * 32 + e], v[q * 32 + e + 1], KV8 ? 1.f : c, -shift);
+                        a = exp2_fast(a), b = exp2_fast(b);
+                        if (KV8) fma2_into(sum[e >> 1 & 1], a, b, in[16 + q * 2 + (e >> 4)]);
+                        else add2_into(sum[e >> 1 & 1], a, b);
+                        out[e >> 1] = pack2<T>(a, b);
                     }
                     tmem_st16(s_at + q * 16, out);
+                    if (q & 1) {      // the products of half the keys start while the other half is on its way
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive((q == 1 ? p_half : p_full) + 8 * t);
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * t);
+                l += (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
             }
             if (!ok) break;
+            if (!KV8) {      // 1 / l for the rows' way out; 0: zeros, whatever the sums hold
+                row_info[(item_no++ & 1) * 256 + t * 128 + row] = l > 0.f || l != l ? 1.f / l : 0.f;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_full + 8 * t);
+                continue;
+            }
             // ---- the rows out: 32 columns at a time through this warp's staging, so that a row's pieces are stored together
             if (x.n > 0) {
                 if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
@@ -286,7 +321,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         // ---- products
         const uint32_t idesc_s = umma_idesc_16(kBf16Mma, false, 128, kTileKeys), idesc_o = umma_idesc_16(kBf16Mma, true, 128, DP);
         const bool one = elect_one();
-        uint32_t kv_no = 0, q_no[2] = {}, p_phase[2] = {}, tile_no = 0;
+        uint32_t kv_no = 0, q_no[2] = {}, p_phase[2] = {}, tile_no = 0, o_phase[2] = {1, 1};
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity, int code) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, code)); };
         auto issue_s = [&](int t, uint32_t slot) {
@@ -324,34 +359,35 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 const uint32_t v_no = kv_no + 1, vs = v_no & 3;
                 const bool more = j + 1 < x.n;
                 if (!wait(kv_full + 8 * vs, v_no >> 2 & 1, ST_TIMEOUT_FULL)) break;
-                if (!KV8) {      // rows of V behind keys that are not seen
-                    const uint32_t* w = words + (tile_no & 3) * 4;
-                    if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-                        for (int key = lane >> 3; key < min(kTileKeys, p.a.Lkv - j * kTileKeys); key += 4)
-                            if (!(w[key >> 5] >> (key & 31) & 1))
-#pragma unroll
-                                for (int box = 0; box < DP / 64; ++box)
-                                    *reinterpret_cast<uint4*>(sm + L::kRing + vs * L::kTile + box * kBox + key * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                }
+                if (!KV8 && !wait(v_ready + 8 * (vs >> 1), v_no >> 2 & 1, ST_TIMEOUT_UNPACK)) break;
                 ks = (kv_no + 2) & 3, k_phase = (kv_no + 2) >> 2 & 1;
                 for (int t = 0; t < tiles; ++t) {
+                    if (!wait(p_half + 8 * t, p_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
+                    if (!KV8 && j == 0) {      // the rows before have left O
+                        if (!wait(o_empty + 8 * t, o_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
+                        o_phase[t] ^= 1;
+                    }
+                    const uint32_t v = umma_desc_lo_n_major(base + L::kRing + vs * L::kTile);
+                    tc_fence_after();
+                    if (one) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)      // 16 keys: 8 columns of p, two swizzle atoms of V
+                            umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0);
+                    }
+                    __syncwarp();
                     if (!wait(p_full + 8 * t, p_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
                     p_phase[t] ^= 1;
                     if (more && t == 0 && !wait(kv_full + 8 * ks, k_phase, ST_TIMEOUT_FULL)) break;
                     tc_fence_after();
                     if (one) {
-                        const uint32_t v = umma_desc_lo_n_major(base + L::kRing + vs * L::kTile);
 #pragma unroll
-                        for (int kk = 0; kk < kTileKeys / 16; ++kk)      // 16 keys: 8 columns of p, two swizzle atoms of V
-                            umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0);
+                        for (int kk = 4; kk < 8; ++kk) umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, 1);
                         if (more) {
                             issue_s(t, ks);
                             if (j + 2 == x.n) umma_commit(q_empty + 8 * t);
                         }
-                        ready(t);
+                        if (KV8 || more) ready(t);
+                        else umma_commit(o_full + 8 * t);
                     }
                     __syncwarp();
                 }
@@ -372,7 +408,32 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             const Item x = item_at<KV8>(p, i);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1, kvh = x.h / (p.a.H / p.a.Hkv);
-            for (int t = 0; t < tiles; ++t) {
+            auto load_kv = [&](int j, int which) {
+                const uint32_t slot = kv_no & 3;
+                if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) return;
+                if (which == 0) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int key = j * kTileKeys + q * 32 + lane;
+                        const bool seen = key < x.seen && (!p.a.mask || gload(p.a.mask + x.b * p.a.mask_stride + key) != 0);
+                        const uint32_t w = __ballot_sync(0xffffffffu, seen);
+                        if (lane == 0) words[(tile_no & 3) * 4 + q] = w;
+                        info[(tile_no & 3) * 128 + q * 32 + lane] = seen ? INFINITY : -INFINITY;
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(kv_full + 8 * slot, L::kTile);
+#pragma unroll
+                    for (int box = 0; box < DP / 64; ++box)
+                        tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
+                                    kv_full + 8 * slot);
+                }
+                __syncwarp();
+                ++kv_no;
+            };
+            load_kv(0, 0);      // before Q, whose place is free only when the last product of the item before has read it
+            for (int t = 0; t < tiles && ok; ++t) {
                 if (!wait(q_empty + 8 * t, (q_no[t] & 1) ^ 1)) break;
                 ++q_no[t];
                 if (lane == 0) {
@@ -383,32 +444,104 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 }
                 __syncwarp();
             }
-            for (int j = 0; j < x.n && ok; ++j, ++tile_no)
-                for (int which = 0; which < 2; ++which, ++kv_no) {
-                    const uint32_t slot = kv_no & 3;
-                    if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
-                    if (which == 0) {
+            if (ok) load_kv(0, 1);
+            ++tile_no;
+            if (lane == 0 && i + gridDim.x < p.items) {      // the next item's queries to L2
+                const Item y = item_at<KV8>(p, i + gridDim.x);
+                for (int t = 0; t < 2 && t * 128 < y.rows; ++t)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int key = j * kTileKeys + q * 32 + lane;
-                            const bool seen = key < x.seen && (!p.a.mask || gload(p.a.mask + x.b * p.a.mask_stride + key) != 0);
-                            const uint32_t w = __ballot_sync(0xffffffffu, seen);
-                            if (lane == 0) words[(tile_no & 3) * 4 + q] = w;
-                        }
-                    }
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(kv_full + 8 * slot, L::kTile);
-#pragma unroll
-                        for (int box = 0; box < DP / 64; ++box)
-                            tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
-                                        kv_full + 8 * slot);
-                    }
-                    __syncwarp();
+                    for (int box = 0; box < DP / 64; ++box) tma_prefetch_4d(&tmap_q, box * 64, y.row0 + t * 128, y.h * p.q_head, y.b * p.q_batch);
+            }
+            __syncwarp();
+            for (int j = 1; j < x.n && ok; ++j, ++tile_no) {
+                load_kv(j, 0);
+                if (ok) load_kv(j, 1);
+            }
+        }
+      } else if (!KV8) {
+        // ---- rows of V behind keys that are not seen: zeros. Two warps, 16 lanes (8 with 64 columns) to a row.
+        uint32_t kv_no = 1, tile_no = 0;
+        bool ok = true;
+        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            const Item x = item_at<KV8>(p, i);
+            for (int j = 0; j < x.n; ++j, ++tile_no, kv_no += 2) {
+                const uint32_t slot = kv_no & 3;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * slot, kv_no >> 2 & 1, abort_s, ST_TIMEOUT_FULL)))) break;
+                const uint32_t* w = words + (tile_no & 3) * 4;
+                if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
+                    constexpr int kLanes = DP / 8;
+                    const int piece = lane % kLanes, there = min(kTileKeys, p.a.Lkv - j * kTileKeys);      // the rest is zeros already
+                    uint8_t* tile = sm + L::kRing + slot * L::kTile + (piece >> 3) * kBox + (piece & 7) * 16;
+                    for (int key = ((warp - 10) * 32 + lane) / kLanes; key < there; key += 64 / kLanes)
+                        if (!(w[key >> 5] >> (key & 31) & 1)) *reinterpret_cast<uint4*>(tile + key * 128) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_ready + 8 * (slot >> 1));
+            }
         }
       }
+    } else if (!KV8) {
+        // ---- the rows' way out: 64 columns at a time through this warp's staging, so that a row's pieces are stored together
+        fewer_registers<L::kLastRegs>();
+        const int quarter = warp & 3;
+        uint8_t* stage = sm + L::kStaging + quarter * 4096;
+        uint32_t phase[2] = {}, item_no = 0;
+        bool ok = true;
+        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            const Item x = item_at<KV8>(p, i);
+            for (int t = 0; t < 2 && t * 128 < x.rows; ++t) {
+                float inv = 0.f;
+                if (x.n > 0) {
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, phase[t], abort_s, ST_TIMEOUT_TMEM_FULL)))) break;
+                    phase[t] ^= 1;
+                    tc_fence_after();
+                    inv = row_info[(item_no & 1) * 256 + t * 128 + quarter * 32 + lane];
+                }
+                const int left = min(32, x.rows - t * 128 - quarter * 32);      // rows of this warp; none: nothing is stored
+                QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + (x.row0 + t * 128 + quarter * 32) * p.a.os[1] + x.h * p.a.os[2];
+#pragma unroll
+                for (int q = 0; q < DP / 64; ++q) {
+                    uint32_t r[2][32];
+                    if (x.n > 0) {
+                        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 64, r[0]);
+                        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 64 + 32, r[1]);
+                        tmem_ld_wait();
+                        if (q == DP / 64 - 1) {      // the next item's products may have O
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(o_empty + 8 * t);
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, inv == 0.f)) {      // no key seen: the columns may hold anything
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) r[e >> 5][e & 31] = inv == 0.f ? 0u : r[e >> 5][e & 31];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint4 v;
+                        uint32_t* o = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            o[f] = pack2<QT>(__uint_as_float(r[e >> 2][(e & 3) * 8 + 2 * f]) * inv, __uint_as_float(r[e >> 2][(e & 3) * 8 + 2 * f + 1]) * inv);
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = v;
+                    }
+                    __syncwarp();
+                    const int e = lane & 7, d = q * 64 + e * 8;
+                    uint4 row[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) row[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + (lane >> 3)) * 128 + ((e ^ (k * 4 + (lane >> 3))) & 7) * 16);
+                    QT* out = dst + (lane >> 3) * p.a.os[1] + d;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k, out += 4 * p.a.os[1])
+                        if (k * 4 + (lane >> 3) < left && d < D) *reinterpret_cast<uint4*>(out) = row[k];
+                    __syncwarp();
+                }
+            }
+            if (x.n > 0) ++item_no;
+        }
     } else {
-        fewer_registers<L::kCodeRegs>();
+        fewer_registers<L::kLastRegs>();
         // ---- codes to halves: four warps of 32 keys (or query rows) each
         const int w = warp - 12;
         uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0, item_no = 0;
@@ -447,7 +580,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         const int e2 = row_exponent(top);
                         const float mult = __uint_as_float((uint32_t)(127 + e2) << 23);
-                        if (piece == 0) factors[(item_no & 1) * 256 + t * 128 + row] = __uint_as_float((uint32_t)(127 - e2) << 23);
+                        if (piece == 0) row_info[(item_no & 1) * 256 + t * 128 + row] = __uint_as_float((uint32_t)(127 - e2) << 23);
                         uint4 z;
                         uint32_t* o = reinterpret_cast<uint32_t*>(&z);
 #pragma unroll
