@@ -12,12 +12,6 @@ namespace {
 
 using namespace b200q;
 
-__device__ __forceinline__ float dsmem_f32(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, rank)) : "memory");
-    return v;
-}
-
 // 64 query rows (a kv head's queries: row r is query r / ratio, head r % ratio of its group), 64 keys a step, four warps of 16 rows.
 constexpr int kRows = 64, kKeys = 64, kThreads = 128;
 

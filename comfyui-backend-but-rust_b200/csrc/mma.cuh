@@ -25,6 +25,30 @@ template <> __device__ __forceinline__ void mma16816<bf16>(float (&c)[4], uint32
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// c = a b: the first of a sum
+template <typename T> __device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816_first<half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <> __device__ __forceinline__ void mma16816_first<bf16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// (a & mask) | bits in one instruction: with both as literals it is two
+template <uint32_t kMask> __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "n"(kMask), "r"(bits));
+    return r;
+}
+// A literal that stays in a register
+template <uint32_t kValue> __device__ __forceinline__ uint32_t held() {
+    uint32_t r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "n"(kValue));
+    return r;
+}
+
 // 16 bytes from global to shared memory without a register between; `valid` false writes zeros and reads nothing.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -40,4 +64,11 @@ template <> __device__ __forceinline__ uint32_t pack2<half>(float lo, float hi) 
 template <> __device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A value of the shared memory of CTA `rank` of the cluster, at this CTA's address of it
+__device__ __forceinline__ float dsmem_f32(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, rank)) : "memory");
+    return v;
 }

@@ -18,6 +18,12 @@ __device__ __forceinline__ float scale_at(const void* s, int dt, int64_t i) {
 
 // ---- the linear -------------------------------------------------------------------------------------------------------------------
 
+// What a CTA of the kernel for few columns has in shared memory.
+struct RowsShare {
+    int kw, kw_log, rows, rows_log, splits_log;      // warps along K, rows, CTAs along K: powers of two
+    int blocks, stages, x_pitch;                     // blocks of 128 of K to a CTA, stages of a warp, bytes to a column of x
+    int scale_words, zero_words, scales, smem;       // words to a row of scales and of zero points, where they begin, all of it
+};
 struct W4Params {
     const void* x;
     int64_t x_stride;
@@ -29,16 +35,32 @@ struct W4Params {
     int64_t out_stride;
     int M, N, K, G, scale_dt, out_dt, groups;
     float beta;
-    int splits;      // warps that share a tile's K
+    int group_shift; // log2(G / 32)
+    int splits;      // CTAs that share a tile's K
+    RowsShare share;
 };
 
 // Codes in registers: a word holds columns 8t..8t+7 of a row, a pair of neighbours in each byte. The pair's byte goes to both halves of a
 // register, the exponent of 1024 (f16) or 128 (bf16) around its nibble, and one instruction takes away the offset and the zero point: the
 // code minus its zero point is a small integer, exact in either type, and so are its products with x in the f32 sums.
+// `expand` gives neighbouring columns (2i, 2i + 1); `expand4` columns (i, i + 4), which takes fewer instructions but needs x in that order.
 template <typename T> struct Nibbles;
 template <> struct Nibbles<half> {
     uint32_t sub;       // (-1024 - z, -64 - z): the high half's nibble sits four bits up, its scale of 1/16 is in the same instruction
-    __device__ __forceinline__ explicit Nibbles(uint32_t z) : sub((0xE400u + z) | (0xD400u + (z << 4)) << 16) {}
+    uint32_t lo, hi;    // the same for both halves of a register alike
+    __device__ __forceinline__ explicit Nibbles(uint32_t z)
+        : sub((0xE400u + z) | (0xD400u + (z << 4)) << 16), lo((0xE400u + z) * 0x00010001u), hi((0xD400u + (z << 4)) * 0x00010001u) {}
+    static constexpr uint32_t kBits = 0x64006400u;
+    __device__ __forceinline__ void expand4(uint32_t w, uint32_t (&r)[4], uint32_t bits) const {      // bits: kBits, held
+        const uint32_t one_16th = 0x2C002C00u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i, w >>= 8) {
+            const uint32_t a = and_or<0x000F000Fu>(w, bits), b = and_or<0x00F000F0u>(w, bits);
+            const half2 x = __hadd2(*reinterpret_cast<const half2*>(&a), *reinterpret_cast<const half2*>(&lo));
+            const half2 y = __hfma2(*reinterpret_cast<const half2*>(&b), *reinterpret_cast<const half2*>(&one_16th), *reinterpret_cast<const half2*>(&hi));
+            r[2 * i] = *reinterpret_cast<const uint32_t*>(&x), r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+    }
     __device__ __forceinline__ void expand(uint32_t w, uint32_t (&r)[4]) const {
         const uint32_t one_16th = 0x2C003C00u;      // (1, 1/16)
 #pragma unroll
@@ -52,6 +74,15 @@ template <> struct Nibbles<half> {
 template <> struct Nibbles<bf16> {
     uint32_t sub;       // 128 + z in both halves
     __device__ __forceinline__ explicit Nibbles(uint32_t z) : sub((0x4300u + z) * 0x00010001u) {}
+    static constexpr uint32_t kBits = 0x43004300u;
+    __device__ __forceinline__ void expand4(uint32_t w, uint32_t (&r)[4], uint32_t bits) const {      // bits: kBits, held
+#pragma unroll
+        for (int i = 0; i < 4; ++i, w >>= 4) {
+            const uint32_t b = and_or<0x000F000Fu>(w, bits);
+            const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&sub));
+            r[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
     __device__ __forceinline__ void expand(uint32_t w, uint32_t (&r)[4]) const {
         const uint32_t up = w >> 4;
 #pragma unroll
@@ -63,15 +94,22 @@ template <> struct Nibbles<bf16> {
     }
 };
 
-// One row's f32 value as three bf16 numbers whose sum it is: eight leading bits each, cut off, so that every remainder is exact.
+// Two f32 values as three bf16 numbers each, whose sum they are: eight leading bits each, cut off, so that every remainder is exact.
 // Infinities and NaN stay in the first.
-__device__ __forceinline__ uint32_t bf16_part(float v, int part) {
-    if (!(fabsf(v) <= FLT_MAX)) return part == 0 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)) : 0u;
-    uint32_t hi = __float_as_uint(v) & 0xFFFF0000u;
+__device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
+    if (!(fabsf(v) <= FLT_MAX)) {
+        part[0] = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)) << 16, part[1] = part[2] = 0u;
+        return;
+    }
+    part[0] = __float_as_uint(v) & 0xFFFF0000u;
+    v -= __uint_as_float(part[0]), part[1] = __float_as_uint(v) & 0xFFFF0000u;
+    v -= __uint_as_float(part[1]), part[2] = __float_as_uint(v);
+}
+template <int P> __device__ __forceinline__ void split2(float a, float b, uint4 (&r)[P], int at) {
+    uint32_t pa[3], pb[3];
+    split3(a, pa), split3(b, pb);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (i < part) v -= __uint_as_float(hi), hi = __float_as_uint(v) & 0xFFFF0000u;
-    return hi >> 16;
+    for (int q = 0; q < P; ++q) reinterpret_cast<uint32_t*>(&r[q])[at] = __byte_perm(pa[q], pb[q], 0x7632);
 }
 
 template <int XT> struct XType { using Mma = bf16; };
@@ -80,19 +118,18 @@ template <> struct XType<DT_F16> { using Mma = half; };
 // Columns of the product: a token's values, or the three parts of an f32 token's.
 template <int XT> __host__ __device__ constexpr int parts_of() { return XT == DT_F32 ? 3 : 1; }
 
-// Eight values of column `col` from k on, as the four registers that two steps of the product take; zeros outside.
-template <int XT> __device__ __forceinline__ uint4 x_words(const W4Params& p, int col, int k) {
-    constexpr int P = parts_of<XT>();
-    const int m = col / P;
-    if (m >= p.M || k >= p.K) return make_uint4(0, 0, 0, 0);
-    if (XT != DT_F32) return gload(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + m * p.x_stride + k));
-    const float* src = reinterpret_cast<const float*>(p.x) + m * p.x_stride + k;
-    const float4 a = gload(reinterpret_cast<const float4*>(src)), b = gload(reinterpret_cast<const float4*>(src) + 1);
-    const int part = col % P;
-    uint4 r;
-    r.x = bf16_part(a.x, part) | bf16_part(a.y, part) << 16, r.y = bf16_part(a.z, part) | bf16_part(a.w, part) << 16;
-    r.z = bf16_part(b.x, part) | bf16_part(b.y, part) << 16, r.w = bf16_part(b.z, part) | bf16_part(b.w, part) << 16;
-    return r;
+// Eight values of token m from k on, for each of its columns the four registers that two steps of the product take; zeros outside.
+template <int XT> __device__ __forceinline__ void x_words(const W4Params& p, int m, int k, uint4 (&r)[parts_of<XT>()]) {
+    if (m >= p.M || k >= p.K) {
+#pragma unroll
+        for (int q = 0; q < parts_of<XT>(); ++q) r[q] = make_uint4(0, 0, 0, 0);
+    } else if (XT != DT_F32) {
+        r[0] = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + m * p.x_stride + k));
+    } else {
+        const float* src = reinterpret_cast<const float*>(p.x) + m * p.x_stride + k;
+        const float4 a = gload(reinterpret_cast<const float4*>(src)), b = gload(reinterpret_cast<const float4*>(src) + 1);
+        split2(a.x, a.y, r, 0), split2(a.z, a.w, r, 1), split2(b.x, b.y, r, 2), split2(b.z, b.w, r, 3);
+    }
 }
 
 template <typename T> __device__ __forceinline__ float out_value(const W4Params& p, float y, int n, T* o) {
@@ -148,91 +185,218 @@ template <int GB> struct Groups {        // GB groups a block: 4, 2 or 1
     }
 };
 
-// Few columns (at most 8 NT): bound by the weight's bytes. A warp owns 16 rows and a share of K, keeps ST - 1 stages of its own in flight
-// (nothing is shared, so nothing waits for another warp) and multiplies in f32 sums of a group, which its scale then adds to the total.
-// The warps of a tile meet once, at its end, in shared memory, in a fixed order.
-constexpr int kRowsStages = 8;
-constexpr int kRowsWarps = 8;
+// The 4-byte words that `bytes` bytes at src lie in, every step-th from word j on. (A word with one byte of an array in it is in memory.)
+__device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* src, int bytes, int j, int step) {
+    const int before = (int)(reinterpret_cast<uintptr_t>(src) & 3);
+    for (; j * 4 < before + bytes; j += step) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + j * 4), "l"(src - before + j * 4) : "memory");
+}
+// cp.async.wait_group for a number known at run time (0 to 3)
+__device__ __forceinline__ void cp_async_wait_all_but(int n) {
+    if (n >= 3) cp_async_wait<3>();
+    else if (n == 2) cp_async_wait<2>();
+    else if (n == 1) cp_async_wait<1>();
+    else cp_async_wait<0>();
+}
 
-template <int XT, int NT, int GB> __global__ void __launch_bounds__(kRowsWarps * 32) w4_rows_kernel(const W4Params p) {
+// Few columns (at most 8 NT): bound by the weight's bytes. A CTA of eight warps has 256 / kw rows, 32 to a warp, and a share of K, which kw
+// warps divide among them; the CTAs of a cluster share a row tile, and all sums of a row meet at the end in one another's shared memory, in a
+// fixed order. A warp keeps ST - 1 stages of its own rows in flight (nothing is shared, so nothing waits for another warp). x, the scales
+// and the zero points of the CTA's share of K are brought into shared memory once, x in the order in which codes come out of a word. Each
+// group's sum is in f32 and added to the total times its scale.
+constexpr int kRowsStages = 4, kRowsWarps = 8, kRowsStage = 2 * kStageBytes;
+
+inline int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v >> 1); }
+inline RowsShare rows_share(int K, int G, int splits, int kw, int cols, bool zeros) {
+    RowsShare r;
+    r.kw = kw, r.kw_log = log2_of(kw), r.rows = kRowsWarps * 32 / kw, r.rows_log = 8 - r.kw_log, r.splits_log = log2_of(splits);
+    static_assert(kRowsWarps * 32 == 256, "rows_log");
+    r.blocks = ((K + 127) / 128 + splits - 1) / splits;
+    const int per_warp = (r.blocks + kw - 1) / kw;
+    r.stages = per_warp < 2 ? 2 : per_warp < kRowsStages ? per_warp : kRowsStages;
+    r.x_pitch = r.blocks * 256 + 64;         // two columns side by side lie in different halves of the banks
+    const int groups = (r.blocks * 128 + G - 1) / G + 1;
+    r.scale_words = (groups * 2 + 5) / 4 | 1, r.zero_words = (groups + 6) / 4 | 1;      // odd: rows start in different banks
+    r.scales = kRowsWarps * r.stages * kRowsStage + cols * r.x_pitch;
+    r.smem = r.scales + r.rows * (r.scale_words + (zeros ? r.zero_words : 0)) * 4;
+    const int sums = kRowsWarps * 32 * cols * 4;
+    if (r.smem < sums) r.smem = sums;
+    return r;
+}
+
+template <int XT, int NT, int GB, bool ZP> __global__ void __launch_bounds__(kRowsWarps * 32, NT == 1 ? 4 : 2) w4_rows_kernel(const W4Params p) {
     using T = typename XType<XT>::Mma;
+    constexpr int P = parts_of<XT>(), kThreads = kRowsWarps * 32;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int S = p.splits, tile = blockIdx.x * (kRowsWarps / S) + warp / S, split = warp % S;
-    const int n0 = tile * 16, blocks = (p.K + 127) / 128;
-    const int first = (int)((int64_t)split * blocks / S), last = n0 < p.N ? (int)((int64_t)(split + 1) * blocks / S) : first;
-    const uint32_t ring = smem_u32(smem) + warp * kRowsStages * kStageBytes;
-    pdl_wait();
+    const RowsShare sh = p.share;
+    const int kw = sh.kw, wk = warp & (kw - 1), row0 = (warp >> sh.kw_log) * 32;
+    const int S = p.splits, split = blockIdx.x & (S - 1), tile0 = (int)(blockIdx.x >> sh.splits_log) << sh.rows_log, n0 = tile0 + row0;
+    const int used = p.M * P;
+    const int all_blocks = (p.K + 127) >> 7, cta_first = min(split * sh.blocks, all_blocks), cta_n = min(sh.blocks, all_blocks - cta_first);
+    const int per = (cta_n + kw - 1) >> sh.kw_log, mine = min(wk * per, cta_n), first = cta_first + mine, n = min(per, cta_n - mine);
+    const uint32_t ring = smem_u32(smem) + warp * sh.stages * kRowsStage;
+    uint8_t* xs = smem + kRowsWarps * sh.stages * kRowsStage;
+    const int shift = p.group_shift, group0 = cta_first * 4 >> shift, here = min((cta_n * 4 >> shift) + 1, p.groups - group0);
+    const uint8_t* scales = smem + sh.scales;
+    const uint8_t* zeros = scales + sh.rows * sh.scale_words * 4;
+    // This lane's pieces of a stage: 16 bytes (32 columns) of rows lane / 4 + 8 i. Rows that there are not repeat the last one; nothing of
+    // them is stored. Columns behind K are zeros.
+    const uint8_t* src[4];
+    uint32_t dst[4];
 #pragma unroll
-    for (int i = 0; i < kRowsStages - 1; ++i) {
-        if (first + i < last) load_stage(p, ring + i * kStageBytes, n0, first + i, lane);
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2);
+        src[i] = p.W + (int64_t)min(n0 + row, p.N - 1) * (p.K >> 1) + first * 64 + (lane & 3) * 16;
+        dst[i] = ring + (row >> 4) * kStageBytes + stage_at(row & 15, lane & 3);
+    }
+    const int tail = p.K - first * 128 - (lane & 3) * 32;      // columns from this lane's piece of block 0 on
+    auto load = [&](int b, int slot) {
+        const bool valid = b * 128 < tail;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cp_async16(dst[i] + slot * kRowsStage, valid ? src[i] + b * 64 : p.W, valid);
+    };
+    pdl_wait();
+    {   // scales and zero points of a row as the words that they lie in; kw threads to a row
+        const int row = threadIdx.x >> sh.kw_log, j0 = threadIdx.x & (kw - 1);
+        const int64_t at = (int64_t)min(tile0 + row, p.N - 1) * p.groups + group0;
+        copy_words(smem_u32(scales) + row * sh.scale_words * 4, reinterpret_cast<const uint8_t*>(p.scales) + at * 2, here * 2, j0, kw);
+        if (ZP) copy_words(smem_u32(zeros) + row * sh.zero_words * 4, p.zeros + at, here, j0, kw);
+    }
+    const int pieces = cta_n * 16, all_pieces = p.M * pieces;      // eight columns of a token each
+    const float per_piece = 1.f / (float)max(pieces, 1);
+    if (XT != DT_F32)
+        for (int i = threadIdx.x; i < all_pieces; i += kThreads) {
+            const int m = (int)(((float)i + 0.5f) * per_piece), c = i - m * pieces, k = cta_first * 128 + c * 8;      // exact: i < 2^22
+            const bool valid = k < p.K;
+            cp_async16(smem_u32(xs) + m * sh.x_pitch + c * 16, valid ? reinterpret_cast<const uint16_t*>(p.x) + m * p.x_stride + k : p.x, valid);
+        }
+    cp_async_commit();
+    const int stages = sh.stages;
+    for (int i = 0; i < stages - 1; ++i) {
+        if (i < n) load(i, i);
         cp_async_commit();
     }
-    float total[NT][4] = {};
-    Groups<GB> gr;
-    uint4 xw[4][NT];
-    auto fetch = [&](int b) {
-        gr.load(p, n0, b, lane);
+    if (XT == DT_F32) {      // three terms each, four pieces requested at a time
+        constexpr int kBatch = 4;
+        for (int i0 = threadIdx.x; i0 < all_pieces; i0 += kBatch * kThreads) {
+            uint4 v[kBatch][P];
+            int m[kBatch];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) xw[c][j] = x_words<XT>(p, j * 8 + g, b * 128 + c * 32 + t * 8);
-    };
-    if (first < last) fetch(first);
-    int slot = 0;
-    for (int b = first; b < last; ++b) {
-        cp_async_wait<kRowsStages - 2>();
-        __syncwarp();
-        const uint32_t at = ring + slot * kStageBytes;
-        uint32_t w[2][4];      // [columns 0..63, 64..127][row half, column quarter]
-#pragma unroll
-        for (int c = 0; c < 2; ++c) ldmatrix4(w[c], at + stage_at((lane & 7) + (lane & 8), 2 * c + (lane >> 4)));
-        float sum[NT][4] = {};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int grp = c * GB / 4;
-            uint32_t lo[4], hi[4];
-            Nibbles<T>(gr.z[grp][0]).expand(w[c >> 1][(c & 1) * 2], lo);
-            Nibbles<T>(gr.z[grp][1]).expand(w[c >> 1][(c & 1) * 2 + 1], hi);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                mma16816<T>(sum[j], lo[0], hi[0], lo[1], hi[1], xw[c][j].x, xw[c][j].y);
-                mma16816<T>(sum[j], lo[2], hi[2], lo[3], hi[3], xw[c][j].z, xw[c][j].w);
+            for (int u = 0; u < kBatch; ++u) {
+                const int i = i0 + u * kThreads;
+                m[u] = i < all_pieces ? (int)(((float)i + 0.5f) * per_piece) : p.M;
+                x_words<XT>(p, m[u], cta_first * 128 + (i - m[u] * pieces) * 8, v[u]);
             }
-            if ((c + 1) * GB % 4 == 0) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+            for (int u = 0; u < kBatch; ++u)
+                if (m[u] < p.M)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) total[j][i] = __fmaf_rn(gr.s[grp][i >> 1], sum[j][i], total[j][i]), sum[j][i] = 0.f;
+                    for (int q = 0; q < P; ++q) *reinterpret_cast<uint4*>(xs + (m[u] * P + q) * sh.x_pitch + (i0 + u * kThreads - m[u] * pieces) * 16) = v[u][q];
+        }
+    }
+    cp_async_wait_all_but(stages - 1);
+    __syncthreads();
+    float total[2][NT][4] = {};
+    const uint8_t* x_col[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x_col[j] = xs + min(j * 8 + g, used - 1) * sh.x_pitch + mine * 256 + t * 16;
+    // where the scales (and zero points) of this lane's four rows begin; a group of a row is so many values on
+    const uint8_t *s_row[4], *z_row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = row0 + i * 8 + g;
+        const int64_t at = (int64_t)min(tile0 + row, p.N - 1) * p.groups + group0;
+        s_row[i] = scales + row * sh.scale_words * 4 + ((int)reinterpret_cast<uintptr_t>(reinterpret_cast<const uint8_t*>(p.scales) + at * 2) & 3);
+        if (ZP) z_row[i] = zeros + row * sh.zero_words * 4 + ((int)reinterpret_cast<uintptr_t>(p.zeros + at) & 3);
+    }
+    auto scale = [&](int i, int grp) {
+        const uint16_t b = *reinterpret_cast<const uint16_t*>(s_row[i] + grp * 2);
+        return p.scale_dt == DT_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+    };
+    const uint32_t frag = stage_at(lane & 15, lane >> 4), frag2 = stage_at(lane & 15, 2 + (lane >> 4));
+    const uint32_t bits = held<Nibbles<T>::kBits>();
+    int slot = 0;
+    for (int b = 0; b < n; ++b) {
+        cp_async_wait_all_but(stages - 2);
+        __syncwarp();
+        const uint32_t at = ring + slot * kRowsStage;
+        constexpr int kChains = NT <= 2 && GB < 4 ? 2 : 1;      // sums of a group side by side: a product waits for the one before it
+        float sum[2][NT][kChains][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {      // 64 columns
+            uint32_t w[2][4];              // [16 rows][row half, column quarter]
+#pragma unroll
+            for (int r = 0; r < 2; ++r) ldmatrix4(w[r], at + r * kStageBytes + (h ? frag2 : frag));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int grp = min(((first + b) * 4 + h * 2 + c >> shift) - group0, here - 1);      // columns behind K: x is zeros
+                uint4 x[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {      // columns 0..7 -> 0, 4, 1, 5, 2, 6, 3, 7
+                    const uint4 v = *reinterpret_cast<const uint4*>(x_col[j] + b * 256 + (h * 2 + c) * 64);
+                    x[j] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    uint32_t lo[4], hi[4];
+                    Nibbles<T>(ZP ? z_row[r * 2][grp] & 15u : 8u).expand4(w[r][c * 2], lo, bits);
+                    Nibbles<T>(ZP ? z_row[r * 2 + 1][grp] & 15u : 8u).expand4(w[r][c * 2 + 1], hi, bits);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const bool begins = (h * 2 + c) * GB % 4 == 0;
+                        if (begins) mma16816_first<T>(sum[r][j][0], lo[0], hi[0], lo[1], hi[1], x[j].x, x[j].y);
+                        else mma16816<T>(sum[r][j][0], lo[0], hi[0], lo[1], hi[1], x[j].x, x[j].y);
+                        if (begins && kChains > 1) mma16816_first<T>(sum[r][j][kChains - 1], lo[2], hi[2], lo[3], hi[3], x[j].z, x[j].w);
+                        else mma16816<T>(sum[r][j][kChains - 1], lo[2], hi[2], lo[3], hi[3], x[j].z, x[j].w);
+                    }
+                    if ((h * 2 + c + 1) * GB % 4 == 0) {
+                        const float s[2] = {scale(r * 2, grp), scale(r * 2 + 1, grp)};
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                total[r][j][i] = __fmaf_rn(s[i >> 1], kChains > 1 ? sum[r][j][0][i] + sum[r][j][kChains - 1][i] : sum[r][j][0][i], total[r][j][i]);
+                    }
+                }
             }
         }
-        if (b + 1 < last) fetch(b + 1);
         __syncwarp();
-        const int ahead = b + kRowsStages - 1;
-        if (ahead < last) load_stage(p, ring + (slot == 0 ? kRowsStages - 1 : slot - 1) * kStageBytes, n0, ahead, lane);
+        if (b + stages - 1 < n) load(b + stages - 1, slot == 0 ? stages - 1 : slot - 1);
         cp_async_commit();
-        slot = slot + 1 == kRowsStages ? 0 : slot + 1;
+        slot = slot + 1 == stages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
-    // sums of the tile's warps: [warp][column][row], behind the rings
-    float* red = reinterpret_cast<float*>(smem + kRowsWarps * kRowsStages * kStageBytes);
-    constexpr int kCols = NT * 8;
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[(warp * kCols + j * 8 + t * 2 + (i & 1)) * 16 + g + (i >> 1) * 8] = total[j][i];
+    pdl_trigger();                                     // all that is left are the sums' way to the result
     __syncthreads();
-    constexpr int P = parts_of<XT>();
-    const int tiles = kRowsWarps / S;
-    for (int i = threadIdx.x; i < tiles * 16 * p.M; i += kRowsWarps * 32) {
-        const int r = i & 15, tl = (i >> 4) % tiles, m = (i >> 4) / tiles, n = (blockIdx.x * tiles + tl) * 16 + r;
-        if (n >= p.N) continue;
-        float y = 0.f;
-        for (int s = 0; s < S; ++s)
+    float* red = reinterpret_cast<float*>(smem);       // [warp along K][column][row], over the rings
 #pragma unroll
-            for (int q = 0; q < P; ++q) y += red[((tl * S + s) * kCols + m * P + q) * 16 + r];
-        store_out(p, y, m, n);
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (j * 8 + t * 2 + (i & 1) < used) red[(wk * used + j * 8 + t * 2 + (i & 1)) * sh.rows + row0 + r * 16 + g + (i >> 1) * 8] = total[r][j][i];
+    if (S > 1) cluster_sync_all();
+    else __syncthreads();
+    const uint32_t red_at = smem_u32(red);
+    const int rows = sh.rows >> sh.splits_log, rows_log = sh.rows_log - sh.splits_log;      // each CTA of the cluster finishes its share of the rows
+    for (int i = threadIdx.x; i < rows * p.M; i += kThreads) {
+        const int r = split * rows + (i & (rows - 1)), m = i >> rows_log;
+        float y = 0.f;
+        if (S == 1) {
+#pragma unroll 4
+            for (int w = 0; w < kw; ++w)
+#pragma unroll
+                for (int q = 0; q < P; ++q) y += red[((w * used + m * P + q) << sh.rows_log) + r];
+        } else
+            for (int s = 0; s < S; ++s)
+#pragma unroll 4
+                for (int w = 0; w < kw; ++w)
+#pragma unroll
+                    for (int q = 0; q < P; ++q) y += dsmem_f32(red_at + (((w * used + m * P + q) << sh.rows_log) + r) * 4, s);
+        if (tile0 + r < p.N) store_out(p, y, m, tile0 + r);
     }
+    if (S > 1) cluster_sync_all();                     // nobody leaves while its sums are read
 }
 
 // Many columns: 128 rows of the weight by 64 columns a CTA. Each warp has 16 rows, expanded once for all 64 columns; the columns come in
@@ -255,15 +419,21 @@ template <int XT, int GB> __global__ void __launch_bounds__(256) w4_tile_kernel(
     // 16 bytes of a column (8 values): column `col`, piece `c` of 16
     auto x_at = [](int col, int c) { return (uint32_t)(col * 256 + (c ^ ((col & 1) << 2)) * 16); };
     auto load = [&](int b, int slot) {
-        for (int i = threadIdx.x; i < kTileCols * 16; i += 256) {
-            const int col = i >> 4, c = i & 15, k = b * 128 + c * 8, m = m0 + col / P;
-            if (XT == DT_F32)
-                *reinterpret_cast<uint4*>(xs_ptr + slot * kTileXBytes + x_at(col, c)) = col < kTokens * P ? x_words<XT>(p, m0 * P + col, k) : make_uint4(0, 0, 0, 0);
-            else {
+        if (XT == DT_F32) {
+            for (int i = threadIdx.x; i < (kTokens + 1) * 16; i += 256) {      // the last column of 64 is nobody's: zeros
+                const int c = i & 15, m = i >> 4;
+                uint4 v[P];
+                x_words<XT>(p, m < kTokens ? m0 + m : p.M, b * 128 + c * 8, v);
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                    if (m * P + q < kTileCols) *reinterpret_cast<uint4*>(xs_ptr + slot * kTileXBytes + x_at(m * P + q, c)) = v[q];
+            }
+        } else
+            for (int i = threadIdx.x; i < kTileCols * 16; i += 256) {
+                const int col = i >> 4, c = i & 15, k = b * 128 + c * 8, m = m0 + col;
                 const bool valid = m < p.M && k < p.K;
                 cp_async16(xs + slot * kTileXBytes + x_at(col, c), valid ? reinterpret_cast<const uint16_t*>(p.x) + m * p.x_stride + k : p.x, valid);
             }
-        }
         load_stage(p, ring + slot * kStageBytes, n0, b, lane);
     };
 #pragma unroll
@@ -328,25 +498,37 @@ template <int XT, int GB> __global__ void __launch_bounds__(256) w4_tile_kernel(
 
 template <int XT, int GB> int launch_w4(W4Params& p, cudaStream_t st) {
     const int cols = p.M * parts_of<XT>();
-    if (cols > 16) {
-        const size_t smem = kTileStages * (kTileXBytes + 8 * kStageBytes);
-        auto kern = w4_tile_kernel<XT, GB>;
-        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-        const int tokens = kTileCols / parts_of<XT>();
-        const int64_t grid = (int64_t)((p.N + 127) / 128) * ((p.M + tokens - 1) / tokens);
-        if (grid > INT32_MAX) return -1;
-        return launch_pdl(kern, dim3((unsigned)grid), 256, smem, st, p);
-    }
-    // the fewest warps to a tile that still give the device eight warps an SM
-    const int tiles = (p.N + 15) / 16;
+    // CTAs along K (a cluster): as few as leave a CTA's share of x and its rings in shared memory. Warps along K in all: four to an SM as long
+    // as each has two blocks of K, and up to 32 where each keeps as many blocks as there are columns, so that bringing x in costs less than
+    // the weight. Warps along K in a CTA x CTAs, us:
+    //   1 x 2560 -> 19456 bf16      1x4 14.4   2x2 13.8   4x1 13.0   8x1 12.0
+    //   8 x 9728 -> 2560 bf16       1x4 25.3   1x8 16.1   2x4 14.9   4x2 14.2   8x2 18.7   4x4 19.0
+    //   5 x 9728 -> 2563 f32        1x8 21.8   2x4 20.7   4x4 30.5
+    //   16 x 5120 -> 13824 f16      1x2 25.8   2x2 31.3   1x4 33.0   2x4 30.6
+    const int all = (p.K + 127) / 128, slices = (p.N + 31) / 32;
+    auto smem_of = [&](int splits, int kw) { return rows_share(p.K, p.G, splits, kw, cols, p.zeros != nullptr).smem; };
+    int ksplit = 1;
+    while (ksplit < 64 && ((slices * ksplit < 148 * 4 && all >= ksplit * 4) || (slices * ksplit < 148 * 32 && all >= ksplit * 2 * max(2, cols)))) ksplit *= 2;
     p.splits = 1;
-    while (p.splits < kRowsWarps && tiles * p.splits < 148 * 8) p.splits *= 2;
-    const int per = kRowsWarps / p.splits;
-    const int NT = cols > 8 ? 2 : 1;
-    const size_t smem = kRowsWarps * (kRowsStages * kStageBytes + NT * 8 * 16 * 4);
-    auto kern = NT == 1 ? w4_rows_kernel<XT, 1, GB> : w4_rows_kernel<XT, 2, GB>;
+    while (p.splits < 8 && (ksplit > p.splits * 8 || smem_of(p.splits, max(1, ksplit / p.splits)) > 200 * 1024)) p.splits *= 2;
+    const int kw = max(1, ksplit / p.splits);
+    const int tiles = (p.N + 256 / kw - 1) / (256 / kw);
+    const RowsShare sh = p.share = rows_share(p.K, p.G, p.splits, kw, cols, p.zeros != nullptr);
+    if (cols <= 32 && sh.smem <= 224 * 1024) {
+        auto kern = p.zeros ? (cols <= 8 ? w4_rows_kernel<XT, 1, GB, true> : cols <= 16 ? w4_rows_kernel<XT, 2, GB, true> : cols <= 24 ? w4_rows_kernel<XT, 3, GB, true>
+                                                                                                                         : w4_rows_kernel<XT, 4, GB, true>)
+                            : (cols <= 8 ? w4_rows_kernel<XT, 1, GB, false> : cols <= 16 ? w4_rows_kernel<XT, 2, GB, false> : cols <= 24 ? w4_rows_kernel<XT, 3, GB, false>
+                                                                                                                           : w4_rows_kernel<XT, 4, GB, false>);
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem)) return (int)e;
+        return launch_pdl_cluster(kern, dim3((unsigned)(tiles * p.splits)), kRowsWarps * 32, sh.smem, st, p.splits, p);
+    }
+    const size_t smem = kTileStages * (kTileXBytes + 8 * kStageBytes);
+    auto kern = w4_tile_kernel<XT, GB>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-    return launch_pdl(kern, dim3((tiles + per - 1) / per), kRowsWarps * 32, smem, st, p);
+    const int tokens = kTileCols / parts_of<XT>();
+    const int64_t grid = (int64_t)((p.N + 127) / 128) * ((p.M + tokens - 1) / tokens);
+    if (grid > INT32_MAX) return -1;
+    return launch_pdl(kern, dim3((unsigned)grid), 256, smem, st, p);
 }
 template <int XT> int launch_w4_groups(W4Params& p, cudaStream_t st) {
     return p.G == 32 ? launch_w4<XT, 4>(p, st) : p.G == 64 ? launch_w4<XT, 2>(p, st) : launch_w4<XT, 1>(p, st);
@@ -466,7 +648,7 @@ GPU_API int gpu_w4_linear(int dtype, const void* x, int64_t x_stride, const void
     if (M == 0 || N == 0) return 0;
     const int item = dtype == DT_F32 ? 4 : 2;
     if (!x || !Wq4 || !scales || !out || !aligned16(x) || !aligned16(Wq4) || x_stride * item % 16 != 0 || (M > 1 && (x_stride < K || out_stride < N))) return -5;
-    W4Params p{x, x_stride, (const uint8_t*)Wq4, scales, (const uint8_t*)zeros, bias, out, out_stride, M, N, K, G, scale_dt, out_dt, K / G, beta, 1};
+    W4Params p{x, x_stride, (const uint8_t*)Wq4, scales, (const uint8_t*)zeros, bias, out, out_stride, M, N, K, G, scale_dt, out_dt, K / G, beta, G == 32 ? 0 : G == 64 ? 1 : G == 128 ? 2 : 3, 1, {}};
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == DT_F32) return launch_w4_groups<DT_F32>(p, st);
     if (dtype == DT_F16) return launch_w4_groups<DT_F16>(p, st);
