@@ -13,11 +13,8 @@
 // Keys that are not seen get p = 0; what V holds there (16-bit V comes as it lies in memory, NaN perhaps) is overwritten with zeros in shared
 // memory before the product.
 // Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds.
-#include <cuda.h>
-
-#include <atomic>
-
 #include "attention.cuh"
+#include "umma16.cuh"
 
 namespace {
 
@@ -49,39 +46,10 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int 
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
-template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
-}
-// Two f32 operations in one instruction
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {      // (x, y) = (a, b) * m + c
-    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
-        : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(m), "f"(c));
-}
-__device__ __forceinline__ void fma2_into(float (&s)[2], float a, float b, float m) {                  // s += (a, b) * m
-    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%0, %1};\n\tfma.rn.f32x2 w, u, v, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b), "f"(m));
-}
-__device__ __forceinline__ void add2_into(float (&s)[2], float a, float b) {
-    asm("{\n\t.reg .b64 u, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 w, {%0, %1};\n\tadd.rn.f32x2 w, u, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b));
-}
-// kind::f16: D f32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1), B's rows along N when `n_major` (bit 16)
-__host__ __device__ constexpr uint32_t umma_idesc_16(bool is_bf16, bool n_major, int m, int n) {
-    return (1u << 4) | ((is_bf16 ? 1u : 0u) << 7) | ((is_bf16 ? 1u : 0u) << 10) | ((n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-// Both operands from shared memory, K-major boxes
-__device__ __forceinline__ void umma_16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "mov.b64 da, {%1, %5};\n\t"
-        "mov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
-        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128) : "memory");
 }
 // A from tensor memory, B from shared memory
 __device__ __forceinline__ void umma_16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
@@ -669,20 +637,6 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-    static std::atomic<EncodeTiledFn> fn{nullptr};
-    EncodeTiledFn f = fn.load(std::memory_order_acquire);
-    if (f) return f;
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess || !sym)
-        return nullptr;
-    f = reinterpret_cast<EncodeTiledFn>(sym);
-    fn.store(f, std::memory_order_release);
-    return f;
-}
 // Rows [B, L, H, D] of 16-bit values as boxes of 64 columns by 128 rows; columns and rows outside read as zeros. A dimension without a
 // stride is one entry.
 bool make_rows_map(CUtensorMap* tm, const void* ptr, const int64_t (&s)[3], int B, int L, int H, int D) {
@@ -694,12 +648,6 @@ bool make_rows_map(CUtensorMap* tm, const void* ptr, const int64_t (&s)[3], int 
     const cuuint32_t box[4] = {64, 128, 1, 1}, estr[4] = {1, 1, 1, 1};
     return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    return n;
 }
 
 template <typename QT, int DP, bool KV8> int launch_tc(const CUtensorMap (&tm)[3], const TcParams& p, cudaStream_t st) {

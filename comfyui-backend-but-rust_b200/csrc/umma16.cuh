@@ -1,0 +1,64 @@
+// What the kernels on tcgen05 kind::f16 share: products of 16-bit operands with f32 sums in tensor memory, and the host's tensor maps.
+#pragma once
+
+#include <cuda.h>
+
+#include <atomic>
+
+#include "common.cuh"
+
+namespace b200q {
+
+// Registers of a warpgroup (all four warps execute it); the shares of all may not add up to more than the launch has
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Two f32 operations in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {      // (x, y) = (a, b) * m + c
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(m), "f"(c));
+}
+__device__ __forceinline__ void fma2_into(float (&s)[2], float a, float b, float m) {                  // s += (a, b) * m
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%0, %1};\n\tfma.rn.f32x2 w, u, v, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b), "f"(m));
+}
+__device__ __forceinline__ void add2_into(float (&s)[2], float a, float b) {
+    asm("{\n\t.reg .b64 u, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 w, {%0, %1};\n\tadd.rn.f32x2 w, u, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b));
+}
+// kind::f16: D f32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1), B's rows along N when `n_major` (bit 16)
+__host__ __device__ constexpr uint32_t umma_idesc_16(bool is_bf16, bool n_major, int m, int n) {
+    return (1u << 4) | ((is_bf16 ? 1u : 0u) << 7) | ((is_bf16 ? 1u : 0u) << 10) | ((n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Both operands from shared memory, K-major boxes
+__device__ __forceinline__ void umma_16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128) : "memory");
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiledFn encode_fn() {
+    static std::atomic<EncodeTiledFn> fn{nullptr};
+    EncodeTiledFn f = fn.load(std::memory_order_acquire);
+    if (f) return f;
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess || !sym)
+        return nullptr;
+    f = reinterpret_cast<EncodeTiledFn>(sym);
+    fn.store(f, std::memory_order_release);
+    return f;
+}
+inline int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return n;
+}
+
+
+}  // namespace b200q

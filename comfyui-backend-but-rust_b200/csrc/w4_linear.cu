@@ -7,183 +7,18 @@
 //
 // W[n, k] = (c[n, k] - z[n, k/G]) * s[n, k/G] with c and z in 0..15 (z = 8 without zero points). Codes [N, K/2]: column 2i in the low
 // nibble of byte i, 2i + 1 in the high one (the order of the W6 format's nibble plane).
-#include "common.cuh"
-#include "mma.cuh"
+#include "w4.cuh"
 
 namespace {
 
-__device__ __forceinline__ float scale_at(const void* s, int dt, int64_t i) {
-    return dt == DT_F16 ? __half2float(gload(reinterpret_cast<const half*>(s) + i)) : __bfloat162float(gload(reinterpret_cast<const bf16*>(s) + i));
-}
+using namespace b200q;
 
 // ---- the linear -------------------------------------------------------------------------------------------------------------------
-
-// What a CTA of the kernel for few columns has in shared memory.
-struct RowsShare {
-    int kw, kw_log, rows, rows_log, splits_log;      // warps along K, rows, CTAs along K: powers of two
-    int blocks, stages, x_pitch;                     // blocks of 128 of K to a CTA, stages of a warp, bytes to a column of x
-    int scale_words, zero_words, scales, smem;       // words to a row of scales and of zero points, where they begin, all of it
-};
-struct W4Params {
-    const void* x;
-    int64_t x_stride;
-    const uint8_t* W;
-    const void* scales;
-    const uint8_t* zeros;
-    const void* bias;
-    void* out;
-    int64_t out_stride;
-    int M, N, K, G, scale_dt, out_dt, groups;
-    float beta;
-    int group_shift; // log2(G / 32)
-    int splits;      // CTAs that share a tile's K
-    RowsShare share;
-};
-
-// Codes in registers: a word holds columns 8t..8t+7 of a row, a pair of neighbours in each byte. The pair's byte goes to both halves of a
-// register, the exponent of 1024 (f16) or 128 (bf16) around its nibble, and one instruction takes away the offset and the zero point: the
-// code minus its zero point is a small integer, exact in either type, and so are its products with x in the f32 sums.
-// `expand` gives neighbouring columns (2i, 2i + 1); `expand4` columns (i, i + 4), which takes fewer instructions but needs x in that order.
-template <typename T> struct Nibbles;
-template <> struct Nibbles<half> {
-    uint32_t sub;       // (-1024 - z, -64 - z): the high half's nibble sits four bits up, its scale of 1/16 is in the same instruction
-    uint32_t lo, hi;    // the same for both halves of a register alike
-    __device__ __forceinline__ explicit Nibbles(uint32_t z)
-        : sub((0xE400u + z) | (0xD400u + (z << 4)) << 16), lo((0xE400u + z) * 0x00010001u), hi((0xD400u + (z << 4)) * 0x00010001u) {}
-    static constexpr uint32_t kBits = 0x64006400u;
-    __device__ __forceinline__ void expand4(uint32_t w, uint32_t (&r)[4], uint32_t bits) const {      // bits: kBits, held
-        const uint32_t one_16th = 0x2C002C00u;
-#pragma unroll
-        for (int i = 0; i < 2; ++i, w >>= 8) {
-            const uint32_t a = and_or<0x000F000Fu>(w, bits), b = and_or<0x00F000F0u>(w, bits);
-            const half2 x = __hadd2(*reinterpret_cast<const half2*>(&a), *reinterpret_cast<const half2*>(&lo));
-            const half2 y = __hfma2(*reinterpret_cast<const half2*>(&b), *reinterpret_cast<const half2*>(&one_16th), *reinterpret_cast<const half2*>(&hi));
-            r[2 * i] = *reinterpret_cast<const uint32_t*>(&x), r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-    }
-    __device__ __forceinline__ void expand(uint32_t w, uint32_t (&r)[4]) const {
-        const uint32_t one_16th = 0x2C003C00u;      // (1, 1/16)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t b = (__byte_perm(w, 0, 0x4040 + 0x0101 * i) & 0x00F0000Fu) | 0x64006400u;
-            const half2 v = __hfma2(*reinterpret_cast<const half2*>(&b), *reinterpret_cast<const half2*>(&one_16th), *reinterpret_cast<const half2*>(&sub));
-            r[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-    }
-};
-template <> struct Nibbles<bf16> {
-    uint32_t sub;       // 128 + z in both halves
-    __device__ __forceinline__ explicit Nibbles(uint32_t z) : sub((0x4300u + z) * 0x00010001u) {}
-    static constexpr uint32_t kBits = 0x43004300u;
-    __device__ __forceinline__ void expand4(uint32_t w, uint32_t (&r)[4], uint32_t bits) const {      // bits: kBits, held
-#pragma unroll
-        for (int i = 0; i < 4; ++i, w >>= 4) {
-            const uint32_t b = and_or<0x000F000Fu>(w, bits);
-            const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&sub));
-            r[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-    }
-    __device__ __forceinline__ void expand(uint32_t w, uint32_t (&r)[4]) const {
-        const uint32_t up = w >> 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t b = (__byte_perm(w, up, 0x4040 + 0x0101 * i + 0x0400) & 0x000F000Fu) | 0x43004300u;
-            const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&sub));
-            r[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-    }
-};
-
-// Two f32 values as three bf16 numbers each, whose sum they are: eight leading bits each, cut off, so that every remainder is exact.
-// Infinities and NaN stay in the first.
-__device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
-    if (!(fabsf(v) <= FLT_MAX)) {
-        part[0] = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)) << 16, part[1] = part[2] = 0u;
-        return;
-    }
-    part[0] = __float_as_uint(v) & 0xFFFF0000u;
-    v -= __uint_as_float(part[0]), part[1] = __float_as_uint(v) & 0xFFFF0000u;
-    v -= __uint_as_float(part[1]), part[2] = __float_as_uint(v);
-}
-template <int P> __device__ __forceinline__ void split2(float a, float b, uint4 (&r)[P], int at) {
-    uint32_t pa[3], pb[3];
-    split3(a, pa), split3(b, pb);
-#pragma unroll
-    for (int q = 0; q < P; ++q) reinterpret_cast<uint32_t*>(&r[q])[at] = __byte_perm(pa[q], pb[q], 0x7632);
-}
-
-template <int XT> struct XType { using Mma = bf16; };
-template <> struct XType<DT_F16> { using Mma = half; };
-
-// Columns of the product: a token's values, or the three parts of an f32 token's.
-template <int XT> __host__ __device__ constexpr int parts_of() { return XT == DT_F32 ? 3 : 1; }
-
-// Eight values of token m from k on, for each of its columns the four registers that two steps of the product take; zeros outside.
-template <int XT> __device__ __forceinline__ void x_words(const W4Params& p, int m, int k, uint4 (&r)[parts_of<XT>()]) {
-    if (m >= p.M || k >= p.K) {
-#pragma unroll
-        for (int q = 0; q < parts_of<XT>(); ++q) r[q] = make_uint4(0, 0, 0, 0);
-    } else if (XT != DT_F32) {
-        r[0] = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + m * p.x_stride + k));
-    } else {
-        const float* src = reinterpret_cast<const float*>(p.x) + m * p.x_stride + k;
-        const float4 a = gload(reinterpret_cast<const float4*>(src)), b = gload(reinterpret_cast<const float4*>(src) + 1);
-        split2(a.x, a.y, r, 0), split2(a.z, a.w, r, 1), split2(b.x, b.y, r, 2), split2(b.z, b.w, r, 3);
-    }
-}
-
-template <typename T> __device__ __forceinline__ float out_value(const W4Params& p, float y, int n, T* o) {
-    if (p.bias) y += to_f<T>(gload(reinterpret_cast<const T*>(p.bias) + n));
-    if (p.beta != 0.f) y = __fmaf_rn(p.beta, to_f<T>(gload(o)), y);
-    return y;
-}
-__device__ __forceinline__ void store_out(const W4Params& p, float y, int m, int n) {
-    const int64_t at = m * p.out_stride + n;
-    if (p.out_dt == DT_F32) {
-        float* o = reinterpret_cast<float*>(p.out) + at;
-        *o = out_value<float>(p, y, n, o);
-    } else if (p.out_dt == DT_F16) {
-        half* o = reinterpret_cast<half*>(p.out) + at;
-        *o = __float2half_rn(out_value<half>(p, y, n, o));
-    } else {
-        bf16* o = reinterpret_cast<bf16*>(p.out) + at;
-        *o = __float2bfloat16_rn(out_value<bf16>(p, y, n, o));
-    }
-}
 
 // A stage: 128 columns of 16 rows, 64 bytes a row. Eight rows read at the same column have to lie in eight different 16-byte banks: two
 // rows fill a line of 128 bytes, and the pair's number turns the column's.
 constexpr int kStageBytes = 16 * 64;
 __device__ __forceinline__ uint32_t stage_at(int row, int c) { return (uint32_t)(row * 64 + ((c ^ (row >> 1)) & 3) * 16); }
-
-// One warp's copy of columns 128 * block .. of rows n0..n0+15.
-__device__ __forceinline__ void load_stage(const W4Params& p, uint32_t dst, int n0, int block, int lane) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = i * 8 + (lane >> 2), c = lane & 3, k = block * 128 + c * 32;
-        const bool valid = n0 + row < p.N && k < p.K;
-        cp_async16(dst + stage_at(row, c), valid ? p.W + (int64_t)(n0 + row) * (p.K >> 1) + (k >> 1) : p.W, valid);
-    }
-}
-
-// Group scales and zero points of the rows that a lane's sums belong to (g and g + 8 of the tile), for one block of 128 columns.
-template <int GB> struct Groups {        // GB groups a block: 4, 2 or 1
-    float s[GB][2];
-    uint32_t z[GB][2];
-    __device__ __forceinline__ void load(const W4Params& p, int n0, int block, int lane) {
-#pragma unroll
-        for (int j = 0; j < GB; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int n = n0 + (lane >> 2) + 8 * h;
-                const int grp = (block * 128 + j * (128 / GB)) / p.G;
-                const bool valid = n < p.N && grp < p.groups;
-                const int64_t at = (int64_t)n * p.groups + grp;
-                s[j][h] = valid ? scale_at(p.scales, p.scale_dt, at) : 0.f;
-                z[j][h] = valid && p.zeros ? gload(p.zeros + at) & 15u : 8u;
-            }
-    }
-};
 
 // The 4-byte words that `bytes` bytes at src lie in, every step-th from word j on. (A word with one byte of an array in it is in memory.)
 __device__ __forceinline__ void copy_words(uint32_t dst, const uint8_t* src, int bytes, int j, int step) {
@@ -366,7 +201,6 @@ template <int XT, int NT, int GB, bool ZP> __global__ void __launch_bounds__(kRo
         slot = slot + 1 == stages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
-    pdl_trigger();                                     // all that is left are the sums' way to the result
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);       // [warp along K][column][row], over the rings
 #pragma unroll
@@ -399,103 +233,6 @@ template <int XT, int NT, int GB, bool ZP> __global__ void __launch_bounds__(kRo
     if (S > 1) cluster_sync_all();                     // nobody leaves while its sums are read
 }
 
-// Many columns: 128 rows of the weight by 64 columns a CTA. Each warp has 16 rows, expanded once for all 64 columns; the columns come in
-// blocks of 128 of K that the CTA shares.
-constexpr int kTileCols = 64;
-constexpr int kTileStages = 3;
-constexpr int kTileXBytes = kTileCols * 256;
-
-template <int XT, int GB> __global__ void __launch_bounds__(256) w4_tile_kernel(const W4Params p) {
-    using T = typename XType<XT>::Mma;
-    extern __shared__ __align__(128) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr int P = parts_of<XT>(), kTokens = kTileCols / P;
-    const int ntiles = (p.N + 127) / 128, nt = blockIdx.x % ntiles;
-    const int n0 = nt * 128 + warp * 16, m0 = blockIdx.x / ntiles * kTokens;
-    const int blocks = (p.K + 127) / 128;
-    const uint32_t xs = smem_u32(smem), ring = xs + kTileStages * kTileXBytes + warp * kTileStages * kStageBytes;
-    uint8_t* xs_ptr = smem;
-    pdl_wait();
-    // 16 bytes of a column (8 values): column `col`, piece `c` of 16
-    auto x_at = [](int col, int c) { return (uint32_t)(col * 256 + (c ^ ((col & 1) << 2)) * 16); };
-    auto load = [&](int b, int slot) {
-        if (XT == DT_F32) {
-            for (int i = threadIdx.x; i < (kTokens + 1) * 16; i += 256) {      // the last column of 64 is nobody's: zeros
-                const int c = i & 15, m = i >> 4;
-                uint4 v[P];
-                x_words<XT>(p, m < kTokens ? m0 + m : p.M, b * 128 + c * 8, v);
-#pragma unroll
-                for (int q = 0; q < P; ++q)
-                    if (m * P + q < kTileCols) *reinterpret_cast<uint4*>(xs_ptr + slot * kTileXBytes + x_at(m * P + q, c)) = v[q];
-            }
-        } else
-            for (int i = threadIdx.x; i < kTileCols * 16; i += 256) {
-                const int col = i >> 4, c = i & 15, k = b * 128 + c * 8, m = m0 + col;
-                const bool valid = m < p.M && k < p.K;
-                cp_async16(xs + slot * kTileXBytes + x_at(col, c), valid ? reinterpret_cast<const uint16_t*>(p.x) + m * p.x_stride + k : p.x, valid);
-            }
-        load_stage(p, ring + slot * kStageBytes, n0, b, lane);
-    };
-#pragma unroll
-    for (int i = 0; i < kTileStages - 1; ++i) {
-        if (i < blocks) load(i, i);
-        cp_async_commit();
-    }
-    float total[8][4] = {};
-    Groups<GB> gr;
-    gr.load(p, n0, 0, lane);
-    int slot = 0;
-    for (int b = 0; b < blocks; ++b) {
-        cp_async_wait<kTileStages - 2>();
-        __syncthreads();
-        if (b + kTileStages - 1 < blocks) load(b + kTileStages - 1, slot == 0 ? kTileStages - 1 : slot - 1);
-        cp_async_commit();
-        const uint32_t at = ring + slot * kStageBytes;
-        uint32_t w[2][4];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) ldmatrix4(w[c], at + stage_at((lane & 7) + (lane & 8), 2 * c + (lane >> 4)));
-        float sum[8][4] = {};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int grp = c * GB / 4;
-            uint32_t lo[4], hi[4];
-            Nibbles<T>(gr.z[grp][0]).expand(w[c >> 1][(c & 1) * 2], lo);
-            Nibbles<T>(gr.z[grp][1]).expand(w[c >> 1][(c & 1) * 2 + 1], hi);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint4 x = *reinterpret_cast<const uint4*>(xs_ptr + slot * kTileXBytes + x_at(j * 8 + g, c * 4 + t));
-                mma16816<T>(sum[j], lo[0], hi[0], lo[1], hi[1], x.x, x.y);
-                mma16816<T>(sum[j], lo[2], hi[2], lo[3], hi[3], x.z, x.w);
-            }
-            if ((c + 1) * GB % 4 == 0) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) total[j][i] = __fmaf_rn(gr.s[grp][i >> 1], sum[j][i], total[j][i]), sum[j][i] = 0.f;
-            }
-        }
-        if (b + 1 < blocks) gr.load(p, n0, b + 1, lane);
-        slot = slot + 1 == kTileStages ? 0 : slot + 1;
-    }
-    cp_async_wait<0>();
-    __syncthreads();
-    // [column][row] of the tile, a row of 132 floats
-    float* red = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) red[(j * 8 + t * 2 + (i & 1)) * 132 + warp * 16 + g + (i >> 1) * 8] = total[j][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTokens * 128; i += 256) {
-        const int r = i & 127, m = i >> 7, n = nt * 128 + r;
-        if (n >= p.N || m0 + m >= p.M) continue;
-        float y = 0.f;
-#pragma unroll
-        for (int q = 0; q < P; ++q) y += red[(m * P + q) * 132 + r];
-        store_out(p, y, m0 + m, n);
-    }
-}
-
 template <int XT, int GB> int launch_w4(W4Params& p, cudaStream_t st) {
     const int cols = p.M * parts_of<XT>();
     // CTAs along K (a cluster): as few as leave a CTA's share of x and its rings in shared memory. Warps along K in all: four to an SM as long
@@ -522,13 +259,7 @@ template <int XT, int GB> int launch_w4(W4Params& p, cudaStream_t st) {
         if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem)) return (int)e;
         return launch_pdl_cluster(kern, dim3((unsigned)(tiles * p.splits)), kRowsWarps * 32, sh.smem, st, p.splits, p);
     }
-    const size_t smem = kTileStages * (kTileXBytes + 8 * kStageBytes);
-    auto kern = w4_tile_kernel<XT, GB>;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-    const int tokens = kTileCols / parts_of<XT>();
-    const int64_t grid = (int64_t)((p.N + 127) / 128) * ((p.M + tokens - 1) / tokens);
-    if (grid > INT32_MAX) return -1;
-    return launch_pdl(kern, dim3((unsigned)grid), 256, smem, st, p);
+    return w4_tile(XT, p, st);
 }
 template <int XT> int launch_w4_groups(W4Params& p, cudaStream_t st) {
     return p.G == 32 ? launch_w4<XT, 4>(p, st) : p.G == 64 ? launch_w4<XT, 2>(p, st) : launch_w4<XT, 1>(p, st);
