@@ -169,9 +169,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (KV8) {
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
-                        const float mul = in[q] * factor, add = in[8 + q];
+                        const uint64_t mul = pack_f32(in[q] * factor, in[q] * factor), add = pack_f32(in[8 + q], in[8 + q]);
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) fma2(v[q * 16 + e], v[q * 16 + e + 1], v[q * 16 + e], v[q * 16 + e + 1], mul, add);
+                        for (int e = 0; e < 16; e += 2)
+                            unpack_f32(fma_f32x2(pack_f32(v[q * 16 + e], v[q * 16 + e + 1]), mul, add), v[q * 16 + e], v[q * 16 + e + 1]);
                     }
                 }
                 if (!all) {
@@ -216,17 +217,19 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     }
                 }
                 const float shift = m == -INFINITY ? 0.f : m;
-                float sum[2][2] = {};
+                const uint64_t minus = pack_f32(-shift, -shift), by = pack_f32(c, c);
+                uint64_t sum[2] = {};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     uint32_t out[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         float a, b;
-                        fma2(a, b, v[q * 32 + e], v[q * 32 + e + 1], KV8 ? 1.f : c, -shift);
+                        const uint64_t x = pack_f32(v[q * 32 + e], v[q * 32 + e + 1]);
+                        unpack_f32(KV8 ? add_f32x2(x, minus) : fma_f32x2(x, by, minus), a, b);
                         a = exp2_fast(a), b = exp2_fast(b);
-                        if (KV8) fma2_into(sum[e >> 1 & 1], a, b, in[16 + q * 2 + (e >> 4)]);
-                        else add2_into(sum[e >> 1 & 1], a, b);
+                        const float wt = KV8 ? in[16 + q * 2 + (e >> 4)] : 0.f;
+                        sum[e >> 1 & 1] = KV8 ? fma_f32x2(pack_f32(a, b), pack_f32(wt, wt), sum[e >> 1 & 1]) : add_f32x2(pack_f32(a, b), sum[e >> 1 & 1]);
                         out[e >> 1] = pack2<T>(a, b);
                     }
                     tmem_st16(s_at + q * 16, out);
@@ -237,7 +240,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         if (lane == 0) mbar_arrive((q == 1 ? p_half : p_full) + 8 * t);
                     }
                 }
-                l += (sum[0][0] + sum[0][1]) + (sum[1][0] + sum[1][1]);
+                float even, odd;
+                unpack_f32(add_f32x2(sum[0], sum[1]), even, odd);
+                l += even + odd;
             }
             if (!ok) break;
             if (!KV8) {      // 1 / l for the rows' way out; 0: zeros, whatever the sums hold

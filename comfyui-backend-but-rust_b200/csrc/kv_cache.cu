@@ -6,6 +6,7 @@
 // k8, v8 int8 [pages, Hkv, T, D], one f32 scale for each page and head: a value is code * scale. Sequence b's token i is row i % T of page
 // table[b, i / T]. The T rows of a page and head are contiguous: what attention reads for one head is whole runs of T * D bytes.
 #include "common.cuh"
+#include "mma.cuh"
 
 namespace {
 
@@ -34,10 +35,13 @@ template <> __device__ __forceinline__ void load8<float>(const float* src, float
 __device__ __forceinline__ uint32_t pack4(const float* c) {
     return ((uint32_t)(int)c[0] & 255u) | ((uint32_t)(int)c[1] & 255u) << 8 | ((uint32_t)(int)c[2] & 255u) << 16 | (uint32_t)(int)c[3] << 24;
 }
-// code = rint(value / scale), NaN -> 0
-__device__ __forceinline__ float code_of(float v, float s) {
-    const float c = rintf(__fdiv_rn(v, s));
-    return c == c ? fminf(127.f, fmaxf(-127.f, c)) : 0.f;
+// codes rint(value / scale), NaN -> 0
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s) {
+    float c[8];
+    rint_quotients<8>(v, s, c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = c[e] == c[e] ? fminf(127.f, fmaxf(-127.f, c[e])) : 0.f;
+    return make_uint2(pack4(c), pack4(c + 4));
 }
 
 // One CTA for each of K and V, page and head. Twice over the new rows (at most T * D values, so the second time from L1 or L2): their
@@ -84,17 +88,15 @@ template <typename XT> __global__ void __launch_bounds__(256) kv8_append_kernel(
                 const uint2 w = gload(reinterpret_cast<const uint2*>(dst) + i);
                 float c[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) c[e] = code_of(__fmul_rn((float)(int8_t)((e < 4 ? w.x : w.y) >> 8 * (e & 3)), r), 1.f);
-                reinterpret_cast<uint2*>(dst)[i] = make_uint2(pack4(c), pack4(c + 4));
+                for (int e = 0; e < 8; ++e) c[e] = __fmul_rn((float)(int8_t)((e < 4 ? w.x : w.y) >> 8 * (e & 3)), r);
+                reinterpret_cast<uint2*>(dst)[i] = codes_of(c, 1.f);
             }
         }
     }
     for (int i = threadIdx.x; i < n; i += 256) {
         float v[8];
         load8(src + (int64_t)(i / pieces) * xs[1] + i % pieces * 8, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = code_of(v[e], s);
-        reinterpret_cast<uint2*>(dst)[from * pieces + i] = make_uint2(pack4(v), pack4(v + 4));
+        reinterpret_cast<uint2*>(dst)[from * pieces + i] = codes_of(v, s);
     }
     __syncthreads();             // everybody has read the old scale
     if (threadIdx.x == 0) *scale = s;
@@ -106,37 +108,57 @@ struct DequantParams {
     const int32_t *table, *lengths;
     void *k, *v;
     int64_t table_stride, pages, rows;      // rows to a sequence of the result
-    int B, Hkv, D, T, max_pages;
+    int B, Hkv, D, T, max_pages, page_log, seq_blocks;
 };
 
-// 16 codes a thread; rows behind a sequence's last token, or on a page that there is not, are zeros.
+// A thread has the same 32 bytes of the result in eight rows, which lie on one page; rows behind a sequence's last token, or on a page that
+// there is not, are zeros. Threads side by side have neighbouring pieces of a row, of K or of V.
 template <typename XT> __global__ void __launch_bounds__(256) kv8_dequant_kernel(const DequantParams p) {
+    constexpr int kCodes = 32 / sizeof(XT), kRows = 8;
     pdl_wait();
-    const int pieces = p.D / 16;
-    const int64_t all = (int64_t)p.B * p.rows * p.Hkv * pieces;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= all) return;
-    const int c = (int)(i % pieces), h = (int)(i / pieces % p.Hkv);
-    const int64_t row = i / pieces / p.Hkv % p.rows, b = i / pieces / p.Hkv / p.rows;
+    const int which = blockIdx.x & 1, b = (int)(blockIdx.x >> 1) / p.seq_blocks;
+    const int i = ((int)(blockIdx.x >> 1) - b * p.seq_blocks) * 256 + threadIdx.x, pieces = p.D / kCodes, across = pieces * p.Hkv;
+    const int row0 = i / across * kRows, at = i % across, h = at / pieces, c = at % pieces;
+    if (row0 >= p.rows) return;
+    const int length = gload(p.lengths + b), slot = row0 >> p.page_log;
     int64_t page = -1;
-    if (row < gload(p.lengths + b) && row / p.T < p.max_pages) page = gload(p.table + b * p.table_stride + row / p.T);
+    if (row0 < length && slot < p.max_pages) page = gload(p.table + b * p.table_stride + slot);
     const bool there = page >= 0 && page < p.pages;
+    uint32_t w[kRows][kCodes / 4];
+    float s = 0.f;
+    if (there) {
+        const int8_t* src = (which ? p.v8 : p.k8) + ((page * p.Hkv + h) * p.T + (row0 & (p.T - 1))) * p.D + c * kCodes;
+        s = gload((which ? p.v_scale : p.k_scale) + page * p.Hkv + h);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        float s = 0.f;
-        if (there) {
-            w = gload(reinterpret_cast<const uint4*>((which ? p.v8 : p.k8) + ((page * p.Hkv + h) * p.T + row % p.T) * p.D) + c);
-            s = gload((which ? p.v_scale : p.k_scale) + page * p.Hkv + h);
-        }
-        const int8_t* q = reinterpret_cast<const int8_t*>(&w);
-        __align__(16) XT v[16];
+        for (int r = 0; r < kRows; ++r)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = from_f<XT>(__fmul_rn((float)q[e], s));
-        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<XT*>(which ? p.v : p.k) + i * 16);
-#pragma unroll
-        for (int e = 0; e < (int)sizeof(XT); ++e) out[e] = reinterpret_cast<const uint4*>(v)[e];
+            for (int e = 0; e < kCodes / 4; e += 2) {
+                const uint2 x = gload(reinterpret_cast<const uint2*>(src + r * p.D) + e / 2);
+                w[r][e] = x.x, w[r][e + 1] = x.y;
+            }
     }
+    XT* out = reinterpret_cast<XT*>(which ? p.v : p.k) + (((int64_t)b * p.rows + row0) * p.Hkv + h) * p.D + c * kCodes;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        if (row0 + r >= p.rows) return;
+        const bool seen = there && row0 + r < length;
+        uint32_t o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (sizeof(XT) == 4) o[e] = seen ? __float_as_uint(__fmul_rn((float)(int8_t)(w[r][e >> 2] >> 8 * (e & 3)), s)) : 0u;
+            else o[e] = seen ? pack2<XT>(__fmul_rn((float)(int8_t)(w[r][e >> 1] >> 16 * (e & 1)), s), __fmul_rn((float)(int8_t)(w[r][e >> 1] >> (16 * (e & 1) + 8)), s)) : 0u;
+        }
+        store32(out + (int64_t)r * p.Hkv * p.D, o);
+    }
+}
+template <typename XT> int launch_dequant(DequantParams& p, cudaStream_t st) {
+    const int64_t threads = (p.rows + 7) / 8 * p.Hkv * (p.D / (32 / (int)sizeof(XT)));
+    if (threads > INT32_MAX - 256) return -1;
+    p.seq_blocks = (int)((threads + 255) / 256);
+    const int64_t grid = (int64_t)2 * p.B * p.seq_blocks;
+    if (grid > INT32_MAX) return -1;
+    auto kern = kv8_dequant_kernel<XT>;
+    return launch_pdl(kern, dim3((unsigned)grid), 256, 0, st, p);
 }
 
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -174,14 +196,11 @@ GPU_API int gpu_kv8_dequant(int dtype, const int8_t* k8, const int8_t* v8, const
     if (B < 0 || rows < 0) return -1;
     if (dtype < DT_F32 || dtype > DT_BF16) return -4;
     if (B == 0 || rows == 0) return 0;
-    if (!k || !v || !lengths || off16(k) || off16(v) || off16(k8) || off16(v8)) return -5;
+    if (!k || !v || !lengths || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31) || off16(k8) || off16(v8)) return -5;
     if (max_pages > 0 && pages > 0 && (!k8 || !v8 || !k_scale || !v_scale || !table)) return -5;
-    const DequantParams p = {k8, v8, k_scale, v_scale, table, lengths, k, v, table_stride, pages, rows, B, Hkv, D, T, pages > 0 ? max_pages : 0};
-    if (rows > INT64_MAX / 4096 / B / Hkv) return -1;
-    const int64_t grid = (B * rows * Hkv * (D / 16) + 255) / 256;
-    if (grid > INT32_MAX) return -1;
+    DequantParams p = {k8, v8, k_scale, v_scale, table, lengths, k, v, table_stride, pages, rows, B, Hkv, D, T, pages > 0 ? max_pages : 0, 0, 0};
+    while (1 << p.page_log < T) ++p.page_log;
+    if (rows > INT32_MAX / Hkv) return -1;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == DT_F32) return launch_pdl(kv8_dequant_kernel<float>, dim3((unsigned)grid), 256, 0, st, p);
-    if (dtype == DT_F16) return launch_pdl(kv8_dequant_kernel<half>, dim3((unsigned)grid), 256, 0, st, p);
-    return launch_pdl(kv8_dequant_kernel<bf16>, dim3((unsigned)grid), 256, 0, st, p);
+    return dtype == DT_F32 ? launch_dequant<float>(p, st) : dtype == DT_F16 ? launch_dequant<half>(p, st) : launch_dequant<bf16>(p, st);
 }

@@ -12,18 +12,22 @@ namespace b200q {
 // Registers of a warpgroup (all four warps execute it); the shares of all may not add up to more than the launch has
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// Two f32 operations in one instruction
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float m, float c) {      // (x, y) = (a, b) * m + c
-    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%5, %5};\n\tfma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
-        : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(m), "f"(c));
+// Two f32 numbers in a 64-bit register, and two operations on them in one instruction
+__device__ __forceinline__ uint64_t pack_f32(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ void fma2_into(float (&s)[2], float a, float b, float m) {                  // s += (a, b) * m
-    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %4};\n\tmov.b64 w, {%0, %1};\n\tfma.rn.f32x2 w, u, v, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b), "f"(m));
+__device__ __forceinline__ void unpack_f32(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
-__device__ __forceinline__ void add2_into(float (&s)[2], float a, float b) {
-    asm("{\n\t.reg .b64 u, w;\n\tmov.b64 u, {%2, %3};\n\tmov.b64 w, {%0, %1};\n\tadd.rn.f32x2 w, u, w;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "+f"(s[0]), "+f"(s[1]) : "f"(a), "f"(b));
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 // kind::f16: D f32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1), B's rows along N when `n_major` (bit 16)
 __host__ __device__ constexpr uint32_t umma_idesc_16(bool is_bf16, bool n_major, int m, int n) {

@@ -279,58 +279,94 @@ template <> __device__ __forceinline__ void load8<float>(const float* src, float
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-// A thread packs 16 values (8 bytes of codes); a group's 2 to 16 threads are neighbours in a warp. Bound by the weight's bytes: one read,
-// a quarter (bf16) written.
+// Word e of values side by side
+__device__ __forceinline__ uint32_t bits32(const float* v, int e) { return __float_as_uint(v[e]); }
+__device__ __forceinline__ uint32_t bits32(const half* v, int e) { return (uint32_t)__half_as_ushort(v[2 * e]) | (uint32_t)__half_as_ushort(v[2 * e + 1]) << 16; }
+__device__ __forceinline__ uint32_t bits32(const bf16* v, int e) { return (uint32_t)__bfloat16_as_ushort(v[2 * e]) | (uint32_t)__bfloat16_as_ushort(v[2 * e + 1]) << 16; }
+
+// A thread packs 16 values (8 bytes of codes); a group's 2 to 16 threads are neighbours in a warp. Bound by the weight's bytes (one read, a
+// quarter of bf16 written) once the codes are not sixteen divisions: those took 533 instructions a warp and 141 us at 13824 x 5120 bf16.
 template <typename T> __global__ void __launch_bounds__(256) w4_requant_kernel(const T* w, int64_t w_stride, uint8_t* packed, int scale_dt, void* scales,
-                                                                                uint8_t* zeros, int64_t N, int K, int G) {
+                                                                                uint8_t* zeros, uint32_t threads, int K, int group_log) {
     pdl_wait();
-    const int per_row = K / 16, per_group = G / 16, groups = K / G;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const bool live = i < N * per_row;             // K % G == 0 and 256 % per_group == 0: a group's threads are live together
-    const int64_t n = live ? i / per_row : 0;
-    const int at = live ? (int)(i % per_row) : 0;
-    float v[2][8];
-    load8(w + n * w_stride + at * 16, v[0]);
-    load8(w + n * w_stride + at * 16 + 8, v[1]);
+    const uint32_t per_row = K / 16, i = blockIdx.x * 256u + threadIdx.x;
+    const int per_group = 1 << (group_log - 4);
+    const bool live = i < threads;                 // K % G == 0 and 256 % per_group == 0: a group's threads are live together
+    const uint32_t n = live ? i / per_row : 0, at = live ? i - n * per_row : 0;
+    float v[16];
+    load8(w + n * w_stride + at * 16, reinterpret_cast<float(&)[8]>(v[0]));
+    load8(w + n * w_stride + at * 16 + 8, reinterpret_cast<float(&)[8]>(v[8]));
     float lo = 0.f, hi = 0.f;                      // NaN is passed over
 #pragma unroll
-    for (int j = 0; j < 16; ++j) lo = fminf(lo, v[j >> 3][j & 7]), hi = fmaxf(hi, v[j >> 3][j & 7]);
+    for (int j = 0; j < 16; ++j) lo = fminf(lo, v[j]), hi = fmaxf(hi, v[j]);
     for (int o = 1; o < per_group; o <<= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     float s = zeros ? __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f) : __fmul_rn(fmaxf(-lo, hi), 1.f / 7.f);
     // the scale as it is stored, at most the type's largest number; the codes are fitted to that
     s = scale_dt == DT_F16 ? rnd<half>(fminf(s, 65504.f)) : rnd<bf16>(fminf(s, 3.3895313892515355e38f));
     const float z = zeros ? (s > 0.f ? fminf(15.f, fmaxf(0.f, rintf(__fdiv_rn(-lo, s)))) : 0.f) : 8.f;
+    float q[16];
+    rint_quotients<16>(v, s, q);
     uint32_t word[2] = {};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const float c = __fadd_rn(s > 0.f ? rintf(__fdiv_rn(v[j >> 3][j & 7], s)) : 0.f, z);
-        word[j >> 3] |= (uint32_t)fminf(15.f, fmaxf(0.f, c)) << 4 * (j & 7);
+    for (int j = 0; j < 16; ++j) {                 // 2^23 + code: the code in the low bits
+        const float c = __fadd_rn(fminf(15.f, fmaxf(0.f, __fadd_rn(q[j], z))), 8388608.f);
+        word[j >> 3] |= (__float_as_uint(c) & 15u) << 4 * (j & 7);
     }
     if (!live) return;
     reinterpret_cast<uint2*>(packed)[i] = make_uint2(word[0], word[1]);
-    if (at % per_group == 0) {
-        const int64_t gi = n * groups + at / per_group;
+    if ((i & (per_group - 1)) == 0) {              // rows are whole groups: the i-th thread's group, counted through
+        const uint32_t gi = i >> (group_log - 4);
         if (scale_dt == DT_F16) reinterpret_cast<half*>(scales)[gi] = __float2half_rn(s);
         else reinterpret_cast<bf16*>(scales)[gi] = __float2bfloat16_rn(s);
         if (zeros) zeros[gi] = (uint8_t)z;
     }
 }
 
+// 32 bytes of the result a thread and store, four times a CTA's width apart. Rows are whole groups: the index counts through them.
 template <typename T> __global__ void __launch_bounds__(256) w4_dequant_kernel(const uint8_t* packed, int scale_dt, const void* scales, const uint8_t* zeros,
-                                                                                T* out, int64_t N, int K, int G) {
+                                                                                T* out, int64_t values, int group_log) {
+    constexpr int kCodes = 32 / sizeof(T), kTimes = 4;
     pdl_wait();
-    const int per_row = K / 8, groups = K / G;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * per_row) return;
-    const int64_t gi = i / per_row * groups + (i % per_row) * 8 / G;
-    const uint32_t w = gload(reinterpret_cast<const uint32_t*>(packed) + i);
-    const float s = scale_at(scales, scale_dt, gi);
-    const int z = zeros ? gload(zeros + gi) & 15 : 8;
-    __align__(16) T v[8];
+    const int64_t first = ((int64_t)blockIdx.x * (256 * kTimes) + threadIdx.x) * kCodes;
+    uint32_t w[kTimes][kCodes / 8];
+    float s[kTimes];
+    int z[kTimes];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = from_f<T>(__fmul_rn((float)((int)(w >> 4 * j & 15u) - z), s));
+    for (int u = 0; u < kTimes; ++u) {
+        const int64_t k = first + u * 256 * kCodes;
+        if (k < values) {
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(out + i * 8)[j] = reinterpret_cast<const uint4*>(v)[j];
+            for (int e = 0; e < kCodes / 8; ++e) w[u][e] = gload(reinterpret_cast<const uint32_t*>(packed + (k >> 1)) + e);
+            s[u] = scale_at(scales, scale_dt, k >> group_log);
+            z[u] = zeros ? gload(zeros + (k >> group_log)) & 15 : 8;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kTimes; ++u) {
+        const int64_t k = first + u * 256 * kCodes;
+        if (k >= values) break;
+        T v[kCodes];
+#pragma unroll
+        for (int j = 0; j < kCodes; ++j) v[j] = from_f<T>(__fmul_rn((float)((int)(w[u][j >> 3] >> 4 * (j & 7) & 15u) - z[u]), s[u]));
+        uint32_t r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = bits32(v, e);
+        store32(out + k, r);
+    }
+}
+template <typename T> int launch_requant(const void* w, int64_t w_stride, void* packed, int scale_dt, void* scales, void* zeros, int64_t N, int K, int G, cudaStream_t st) {
+    const int64_t threads = N * (K / 16);
+    if (N > INT32_MAX / (K / 16)) return -1;
+    auto kern = w4_requant_kernel<T>;
+    return launch_pdl(kern, dim3((unsigned)((threads + 255) / 256)), 256, 0, st, (const T*)w, w_stride, (uint8_t*)packed, scale_dt, scales, (uint8_t*)zeros,
+                      (uint32_t)threads, K, 5 + log2_of(G / 32));
+}
+template <typename T> int launch_dequant(const void* packed, int scale_dt, const void* scales, const void* zeros, void* out, int64_t N, int K, int G, cudaStream_t st) {
+    const int64_t per_cta = 1024 * (32 / (int)sizeof(T));
+    if (N > (int64_t)INT32_MAX * 16 / K) return -1;
+    auto kern = w4_dequant_kernel<T>;
+    return launch_pdl(kern, dim3((unsigned)((N * K + per_cta - 1) / per_cta)), 256, 0, st, (const uint8_t*)packed, scale_dt, scales, (const uint8_t*)zeros, (T*)out,
+                      N * K, 5 + log2_of(G / 32));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -346,14 +382,10 @@ GPU_API int gpu_w4_requant(int dtype, const void* w, int64_t w_stride, void* pac
     if (N == 0) return 0;
     const int item = dtype == DT_F32 ? 4 : 2;
     if (!w || !packed || !scales || !aligned16(w) || w_stride * item % 16 != 0 || w_stride < K || (reinterpret_cast<uintptr_t>(packed) & 7)) return -5;
-    const int64_t grid = (N * (K / 16) + 255) / 256;
-    if (grid > INT32_MAX) return -1;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == DT_F32)
-        return launch_pdl(w4_requant_kernel<float>, dim3((unsigned)grid), 256, 0, st, (const float*)w, w_stride, (uint8_t*)packed, scale_dt, scales, (uint8_t*)zeros, N, K, G);
-    if (dtype == DT_F16)
-        return launch_pdl(w4_requant_kernel<half>, dim3((unsigned)grid), 256, 0, st, (const half*)w, w_stride, (uint8_t*)packed, scale_dt, scales, (uint8_t*)zeros, N, K, G);
-    return launch_pdl(w4_requant_kernel<bf16>, dim3((unsigned)grid), 256, 0, st, (const bf16*)w, w_stride, (uint8_t*)packed, scale_dt, scales, (uint8_t*)zeros, N, K, G);
+    if (dtype == DT_F32) return launch_requant<float>(w, w_stride, packed, scale_dt, scales, zeros, N, K, G, st);
+    if (dtype == DT_F16) return launch_requant<half>(w, w_stride, packed, scale_dt, scales, zeros, N, K, G, st);
+    return launch_requant<bf16>(w, w_stride, packed, scale_dt, scales, zeros, N, K, G, st);
 }
 
 GPU_API int gpu_w4_dequant(int dtype, const void* packed, int scale_dt, const void* scales, const void* zeros, void* out, int64_t N, int K, int G,
@@ -361,14 +393,11 @@ GPU_API int gpu_w4_dequant(int dtype, const void* packed, int scale_dt, const vo
     if (bad_groups(N, K, G)) return -1;
     if (bad_scales(scale_dt) || dtype < DT_F32 || dtype > DT_BF16) return -4;
     if (N == 0) return 0;
-    if (!packed || !scales || !out || !aligned16(out) || (reinterpret_cast<uintptr_t>(packed) & 3)) return -5;
-    const int64_t grid = (N * (K / 8) + 255) / 256;
-    if (grid > INT32_MAX) return -1;
+    if (!packed || !scales || !out || (reinterpret_cast<uintptr_t>(out) & 31) || (reinterpret_cast<uintptr_t>(packed) & 3)) return -5;
     cudaStream_t st = (cudaStream_t)stream;
-    const uint8_t *q = (const uint8_t*)packed, *z = (const uint8_t*)zeros;
-    if (dtype == DT_F32) return launch_pdl(w4_dequant_kernel<float>, dim3((unsigned)grid), 256, 0, st, q, scale_dt, scales, z, (float*)out, N, K, G);
-    if (dtype == DT_F16) return launch_pdl(w4_dequant_kernel<half>, dim3((unsigned)grid), 256, 0, st, q, scale_dt, scales, z, (half*)out, N, K, G);
-    return launch_pdl(w4_dequant_kernel<bf16>, dim3((unsigned)grid), 256, 0, st, q, scale_dt, scales, z, (bf16*)out, N, K, G);
+    if (dtype == DT_F32) return launch_dequant<float>(packed, scale_dt, scales, zeros, out, N, K, G, st);
+    if (dtype == DT_F16) return launch_dequant<half>(packed, scale_dt, scales, zeros, out, N, K, G, st);
+    return launch_dequant<bf16>(packed, scale_dt, scales, zeros, out, N, K, G, st);
 }
 
 GPU_API int gpu_w4_linear(int dtype, const void* x, int64_t x_stride, const void* Wq4, int scale_dt, const void* scales, const void* zeros, const void* bias,

@@ -1,9 +1,9 @@
-// The 4-bit linear of many tokens, on tcgen05: tiles of 128 rows of the weight by up to 256 columns (tokens; an f32 token is three).
+// The 4-bit linear of many tokens, on tcgen05: tiles of 128 rows of the weight by up to 192 columns (tokens; an f32 token is three).
 //
 // Codes become 16-bit operands in shared memory as they are (code minus zero point: a small integer), so nothing is rounded; the products of
 // one group of K land in tensor memory, and the group's scale, one number to a row and so to a thread, takes them from there into sums in
-// registers. Two accumulators take turns: while a group is multiplied, the one before is read. One thread an output row and half the columns:
-// 128 sums of f32 each at most. A CTA an SM, persistent over its tiles; where there are few tiles a cluster shares one along K and adds up in
+// registers. Two to four accumulators take turns: while a group is multiplied, the one before is read. One thread an output row and half the
+// columns: 96 sums of f32 at most. A CTA an SM, persistent over its tiles; where there are few tiles a cluster shares one along K and adds up in
 // shared memory, in a fixed order.
 //
 // Warps 0-3 and 4-7: sums, for the first and second half of the columns. Warps 8-11: codes from global memory (each its 32 rows, a ring of its
@@ -21,11 +21,12 @@ using namespace b200q;
 
 __device__ int g_w4_status = 0;
 
-constexpr int kRows = 128, kBlock = 64, kStages = 4, kABytes = kRows * 128, kRing = 8, kRingBytes = 32 * 32;
+constexpr int kRows = 128, kBlock = 64, kStages = 4, kBuffers = 4, kABytes = kRows * 128, kRing = 8, kRingBytes = 32 * 32;
 
 struct TileParams {
     W4Params w;
     int tokens, columns, token_tiles, tiles, splits, blocks;      // of a tile; tiles in all; CTAs along K and blocks of 64 of each
+    int buffers;                                                  // accumulators: as many as fit, at most four
 };
 __host__ __device__ inline int stage_bytes(int columns) { return kABytes + columns * 128; }
 __host__ __device__ inline int tail_at(int columns) { return kStages * stage_bytes(columns) + 4 * kRing * kRingBytes; }
@@ -37,20 +38,53 @@ template <int XT> struct Regs {
     static_assert(2 * kSums + kCodes + kIssue == 4 * 128, "register split");
 };
 
-template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const TileParams p) {
+template <int N> __device__ __forceinline__ float sum_at(const uint64_t (&acc)[N], int c) {
+    float v[2];
+    unpack_f32(acc[c >> 1], v[0], v[1]);
+    return v[c & 1];
+}
+// One output row's sums (P to a token) from `token` on: bias once, and where the result is added to, sixteen of its values before the first
+// is written.
+template <typename T, int P, int N> __device__ __forceinline__ void store_column(const W4Params& w, const uint64_t (&acc)[N], int token, int tokens, int n) {
+    T* out = reinterpret_cast<T*>(w.out) + token * w.out_stride + n;
+    const float bias = w.bias ? to_f<T>(gload(reinterpret_cast<const T*>(w.bias) + n)) : 0.f;
+    constexpr int kTokens = 2 * N / P, kBatch = 8;
+#pragma unroll
+    for (int t0 = 0; t0 < kTokens; t0 += kBatch) {
+        if (t0 >= tokens) break;
+        float old[kBatch];
+        if (w.beta != 0.f) {
+#pragma unroll
+            for (int t = 0; t < kBatch; ++t) old[t] = t0 + t < tokens ? to_f<T>(gload(out + t * w.out_stride)) : 0.f;
+        }
+#pragma unroll
+        for (int t = 0; t < kBatch; ++t) {
+            const int c = (t0 + t) * P;
+            float y = sum_at(acc, c);
+#pragma unroll
+            for (int q = 1; q < P; ++q) y += sum_at(acc, c + q);
+            if (w.bias) y += bias;
+            if (w.beta != 0.f) y = __fmaf_rn(w.beta, old[t], y);
+            if (t0 + t < tokens) *out = from_f<T>(y);
+            out += w.out_stride;
+        }
+    }
+}
+
+template <int XT, bool G32, bool WIDE> __global__ void __launch_bounds__(512, 1) w4_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const TileParams p) {
     using T = typename XType<XT>::Mma;
-    constexpr int P = parts_of<XT>(), kMine = XT == DT_F32 ? 96 : 128;      // columns of a sums thread
+    constexpr int P = parts_of<XT>(), kMine = WIDE ? 96 : 64;      // columns of a sums thread
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* sm = smem_raw + (base - raw);
     const W4Params& w = p.w;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stage_size = stage_bytes(p.columns);
-    const uint32_t bars = base + tail_at(p.columns), full = bars, empty = bars + 8 * kStages, d_full = empty + 8 * kStages, d_empty = d_full + 16;
-    uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + tail_at(p.columns) + 16 * kStages + 32);
+    const uint32_t bars = base + tail_at(p.columns), full = bars, empty = bars + 8 * kStages, d_full = empty + 8 * kStages, d_empty = d_full + 8 * kBuffers;
+    uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + tail_at(p.columns) + 16 * kStages + 16 * kBuffers);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, XT == DT_F32 ? 4 : 5), mbar_init(empty + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(d_full + 8 * i, 1), mbar_init(d_empty + 8 * i, 8);
+        for (int i = 0; i < kBuffers; ++i) mbar_init(d_full + 8 * i, 1), mbar_init(d_empty + 8 * i, 8);
         *abort_s = 0;
         fence_mbar_init();
         if (XT != DT_F32) prefetch_tmap(&tmap_x);
@@ -73,58 +107,63 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
     if (warp < 8) {
         // ---- sums
         more_registers<Regs<XT>::kSums>();
-        const int half = warp >> 2, quarter = warp & 3;
+        const int side = warp >> 2, quarter = warp & 3;
         // chunks of 16 columns; all columns of a token (16 of them fill P chunks) on one side
-        const int front = (p.tokens / 16 - p.tokens / 32) * P, mine = half ? p.columns / 16 - front : front, col0 = half ? front * 16 : 0;
+        const int front = (p.tokens / 16 - p.tokens / 32) * P, mine = side ? p.columns / 16 - front : front, col0 = side ? front * 16 : 0;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + col0;
-        uint32_t phase[2] = {}, buf = 0;
+        uint32_t phase = 0;      // flips when the accumulators have been gone through
+        int buf = 0;
         bool ok = true;
         for (int tile = tile_first; tile < p.tiles && ok; tile += tile_step) {
             const int n = tile / p.token_tiles * kRows + quarter * 32 + lane, m0 = tile % p.token_tiles * p.tokens;
             const int64_t scale_row = (int64_t)min(n, w.N - 1) * w.groups + group0;
-            float acc[kMine / 2][2];
+            uint64_t acc[kMine / 2];      // two columns each
 #pragma unroll
-            for (int c = 0; c < kMine / 2; ++c) acc[c][0] = acc[c][1] = 0.f;
-            float next = group_n > 0 ? scale_at(w.scales, w.scale_dt, scale_row) : 0.f;
+            for (int c = 0; c < kMine / 2; ++c) acc[c] = 0;
+            // a group's scale is requested a group ahead, as the bits it is: a conversion here would wait for it
+            const uint16_t* scales = reinterpret_cast<const uint16_t*>(w.scales) + scale_row;
+            uint16_t next = group_n > 0 ? gload(scales) : (uint16_t)0;
             for (int g = 0; g < group_n; ++g) {
-                const float s = next;
-                if (g + 1 < group_n) next = scale_at(w.scales, w.scale_dt, scale_row + g + 1);
-                if (!__all_sync(0xffffffffu, mbar_wait(d_full + 8 * buf, phase[buf], abort_s, ST_TIMEOUT_TMEM_FULL))) { ok = false; break; }
-                phase[buf] ^= 1;
+                const uint16_t bits = next;
+                if (g + 1 < group_n) next = gload(scales + g + 1);
+                if (!__all_sync(0xffffffffu, mbar_wait(d_full + 8 * buf, phase, abort_s, ST_TIMEOUT_TMEM_FULL))) { ok = false; break; }
                 tc_fence_after();
+                const float scale = w.scale_dt == DT_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((uint32_t)bits << 16);
+                const uint64_t s = pack_f32(scale, scale);
+                constexpr int kAtOnce = WIDE ? 3 : 4;      // chunks requested together: as many as there are registers for
 #pragma unroll
-                for (int c = 0; c < kMine / 16; c += 2) {
-                    if (c < mine) {
-                        uint32_t r[2][16];
-                        tmem_ld16(at + buf * 256 + c * 16, r[0]);
-                        if (c + 1 < mine) tmem_ld16(at + buf * 256 + c * 16 + 16, r[1]);
+                for (int c0 = 0; c0 < kMine / 16; c0 += kAtOnce) {
+                    uint32_t r[kAtOnce][16];
+                    if (c0 < mine) {
+#pragma unroll
+                        for (int c = 0; c < kAtOnce; ++c)
+                            if (c0 + c < mine) tmem_ld16(at + buf * p.columns + (c0 + c) * 16, r[c]);
                         tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2)
-                            if (e < 16 || c + 1 < mine) fma2_into(acc[(c * 16 + e) / 2], __uint_as_float(r[e >> 4][e & 15]), __uint_as_float(r[e >> 4][(e & 15) + 1]), s);
                     }
+                    if (c0 + kAtOnce >= kMine / 16) {      // all are in registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(d_empty + 8 * buf);
+                    }
+#pragma unroll
+                    for (int c = 0; c < kAtOnce; ++c)
+                        if (c0 + c < mine)
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) acc[(c0 + c) * 8 + e / 2] = fma_f32x2(pack_f32(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), s, acc[(c0 + c) * 8 + e / 2]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(d_empty + 8 * buf);
-                buf ^= 1;
+                if (++buf == p.buffers) buf = 0, phase ^= 1;
             }
             if (!ok) break;
             if (p.splits > 1) {      // [column][row], over the stages: every product of this CTA's only tile is done
                 float* red = reinterpret_cast<float*>(sm);
 #pragma unroll
                 for (int c = 0; c < kMine; ++c)
-                    if (c / 16 < mine) red[(col0 + c) * kRows + quarter * 32 + lane] = acc[c >> 1][c & 1];
+                    if (c / 16 < mine) red[(col0 + c) * kRows + quarter * 32 + lane] = sum_at(acc, c);
             } else if (n < w.N) {
-#pragma unroll
-                for (int c = 0; c < kMine; c += P)
-                    if (c / 16 < mine) {
-                        float y = acc[c >> 1][c & 1];
-#pragma unroll
-                        for (int q = 1; q < P; ++q) y += acc[(c + q) >> 1][(c + q) & 1];
-                        const int m = m0 + (col0 + c) / P;
-                        if ((col0 + c) / P < p.tokens && m < w.M) store_out(w, y, m, n);
-                    }
+                const int first_token = m0 + col0 / P, tokens = min(mine * 16 / P, w.M - first_token);
+                if (w.out_dt == DT_F32) store_column<float, P>(w, acc, first_token, tokens, n);
+                else if (w.out_dt == DT_F16) store_column<half, P>(w, acc, first_token, tokens, n);
+                else store_column<bf16, P>(w, acc, first_token, tokens, n);
             }
         }
     } else if (warp < 12) {
@@ -155,7 +194,7 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
                 cp_async_commit();
             };
 #pragma unroll
-            for (int b = 0; b < kRing - 1; ++b) request(b);
+            for (int b = 0; b < kRing; ++b) request(b);
             const int64_t zero_row = (int64_t)n * w.groups;
             // f32: four pieces of eight columns a lane, sixteen tokens a warp, requested a block ahead
             float4 raw[XT == DT_F32 ? 8 : 1];
@@ -172,21 +211,30 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
                 }
             };
             request_x(0);
-            uint32_t z[2] = {8u, 8u};
-            for (int b = 0; b < count; ++b, ++step) {
-                const uint32_t stage = step % kStages;
-                cp_async_wait<kRing - 2>();
+            // codes and zero points are in registers a block ahead of their use
+            uint4 code[2], code_next[2];
+            uint32_t z[2] = {8u, 8u}, z_next[2] = {8u, 8u};
+            auto fetch = [&](int b) {
+                cp_async_wait<kRing - 1>();
                 __syncwarp();
-                uint4 code[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(code[c].x), "=r"(code[c].y), "=r"(code[c].z), "=r"(code[c].w)
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(code_next[c].x), "=r"(code_next[c].y), "=r"(code_next[c].z), "=r"(code_next[c].w)
                                  : "r"(ring + (b % kRing) * kRingBytes + lane * 32 + ((c ^ (lane >> 2)) & 1) * 16) : "memory");
                 if (w.zeros) {
                     const int k = (first + b) * 2;      // in halves of a block
-                    z[0] = gload(w.zeros + zero_row + min(k >> w.group_shift, w.groups - 1)) & 15u;
-                    z[1] = G32 ? gload(w.zeros + zero_row + min(k + 1, w.groups - 1)) & 15u : z[0];
+                    z_next[0] = gload(w.zeros + zero_row + min(k >> w.group_shift, w.groups - 1));
+                    z_next[1] = G32 ? gload(w.zeros + zero_row + min(k + 1, w.groups - 1)) : z_next[0];
                 }
+            };
+            fetch(0);
+            for (int b = 0; b < count; ++b, ++step) {
+                const uint32_t stage = step % kStages;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) code[c] = code_next[c], z[c] = z_next[c] & 15u;
+                __syncwarp();                       // everybody has read block b's slot before it is written again
+                request(b + kRing);
+                fetch(b + 1);
                 if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * stage, (step / kStages & 1) ^ 1, abort_s, ST_TIMEOUT_EMPTY))) { ok = false; break; }
                 uint8_t* a = sm + stage * stage_size + row * 128;
 #pragma unroll
@@ -216,7 +264,6 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + 8 * stage);
-                request(b + kRing - 1);
             }
             cp_async_wait<0>();      // the next tile's ring begins anew
             __syncwarp();
@@ -227,7 +274,8 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
         // ---- products
         const uint32_t idesc = umma_idesc_16(std::is_same<T, bf16>::value, false, kRows, p.columns);
         const bool one = elect_one();
-        uint32_t step = 0, buf = 0, phase[2] = {1, 1};
+        uint32_t step = 0, phase = 1;
+        int buf = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity, int code) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, code)); };
         for (int tile = tile_first; tile < p.tiles && ok; tile += tile_step) {
@@ -239,20 +287,19 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
                     if (G32 && b * 2 + part >= w.groups) break;
                     const bool begins = G32 || (b & ((1 << block_shift) - 1)) == 0, ends = G32 || b + 1 == last || ((b + 1) & ((1 << block_shift) - 1)) == 0;
                     if (begins) {
-                        if (!wait(d_empty + 8 * buf, phase[buf], ST_TIMEOUT_TMEM_EMPTY)) break;
-                        phase[buf] ^= 1;
+                        if (!wait(d_empty + 8 * buf, phase, ST_TIMEOUT_TMEM_EMPTY)) break;
                     }
                     tc_fence_after();
                     if (one) {
 #pragma unroll
                         for (int kk = 0; kk < (G32 ? 2 : 4); ++kk) {
                             const uint32_t k = (part * 2 + kk) * 2;
-                            umma_16_ss(tmem + buf * 256, a + k, x + k, idesc, !(begins && kk == 0));
+                            umma_16_ss(tmem + buf * p.columns, a + k, x + k, idesc, !(begins && kk == 0));
                         }
                         if (ends) umma_commit(d_full + 8 * buf);
                     }
                     __syncwarp();
-                    if (ends) buf ^= 1;
+                    if (ends && ++buf == p.buffers) buf = 0, phase ^= 1;
                 }
                 if (!ok) break;
                 if (one) umma_commit(empty + 8 * stage);
@@ -304,9 +351,9 @@ template <int XT, bool G32> __global__ void __launch_bounds__(512, 1) w4_tile_ke
     }
 }
 
-template <int XT, bool G32> int launch_tile(const CUtensorMap& tm, const TileParams& p, int grid, cudaStream_t st) {
+template <int XT, bool G32, bool WIDE> int launch_tile(const CUtensorMap& tm, const TileParams& p, int grid, cudaStream_t st) {
     const int smem = tail_at(p.columns) + 256 + 1024;
-    auto kern = w4_tile_kernel<XT, G32>;
+    auto kern = w4_tile_kernel<XT, G32, WIDE>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return (int)e;
     return launch_pdl_cluster(kern, dim3((unsigned)grid), 512, smem, st, p.splits, tm, p);
 }
@@ -314,20 +361,21 @@ template <int XT, bool G32> int launch_tile(const CUtensorMap& tm, const TilePar
 template <int XT> int launch(const W4Params& w, cudaStream_t st) {
     TileParams p = {};
     p.w = w;
-    constexpr int P = parts_of<XT>(), kMost = XT == DT_F32 ? 64 : 256, kStep = 16;      // tokens of a tile
+    constexpr int P = parts_of<XT>(), kMost = XT == DT_F32 ? 64 : 192, kStep = 16;      // tokens of a tile
     const int sms = sm_count();
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
     const int64_t row_tiles = (w.N + kRows - 1) / kRows;
-    // The number of token tiles that costs least: rounds of tiles over the SMs times a tile's columns (below 96 the operands, not the
-    // products, take the time).
+    // The number of token tiles that costs least: rounds of tiles over the SMs times what a tile takes, which grows with its columns from a
+    // start of some 300 (a block takes 0.67 us with 112 columns and 0.7 with 176: the sums' way out of tensor memory, a group at a time).
     int64_t best = INT64_MAX;
     const int fewest = (w.M + kMost - 1) / kMost;
     for (int t = fewest; t <= fewest + 3; ++t) {
         const int tokens = ((w.M + t - 1) / t + kStep - 1) / kStep * kStep;
-        const int64_t rounds = (row_tiles * t + sms - 1) / sms, cost = rounds * (tokens * P < 96 ? 96 : tokens * P);
+        const int64_t rounds = (row_tiles * t + sms - 1) / sms, cost = rounds * (300 + tokens * P);
         if (cost < best) best = cost, p.token_tiles = t, p.tokens = tokens;
     }
     p.columns = p.tokens * P;
+    p.buffers = 512 / p.columns < kBuffers ? 512 / p.columns : kBuffers;
     const int64_t tiles = row_tiles * p.token_tiles;
     if (tiles > INT32_MAX) return -1;
     p.tiles = (int)tiles;
@@ -346,7 +394,8 @@ template <int XT> int launch(const W4Params& w, cudaStream_t st) {
             return -203;
     }
     const int grid = p.splits > 1 ? p.tiles * p.splits : (int)(tiles < sms ? tiles : sms);
-    return w.G == 32 ? launch_tile<XT, true>(tm, p, grid, st) : launch_tile<XT, false>(tm, p, grid, st);
+    if (p.columns <= 128) return w.G == 32 ? launch_tile<XT, true, false>(tm, p, grid, st) : launch_tile<XT, false, false>(tm, p, grid, st);
+    return w.G == 32 ? launch_tile<XT, true, true>(tm, p, grid, st) : launch_tile<XT, false, true>(tm, p, grid, st);
 }
 
 }  // namespace

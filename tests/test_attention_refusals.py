@@ -17,8 +17,8 @@ def _attention(lib, dtype=2, B=1, Lq=1, H=4, Hkv=2, D=64, T=64, pages=4, max_pag
     return lib.gpu_kv8_attention(dtype, q, 16, strides, 16, 16, 16, 16, 16, 4, 16, 0, 1, B, Lq, H, Hkv, D, T, pages, max_pages, 1.0, 0)
 
 
-def _dequant(lib, dtype=0, B=1, rows=4, Hkv=2, D=64, T=64, pages=4, max_pages=4, k=16):
-    return lib.gpu_kv8_dequant(dtype, 16, 16, 16, 16, 16, 4, 16, k, 16, B, rows, Hkv, D, T, pages, max_pages, 0)
+def _dequant(lib, dtype=0, B=1, rows=4, Hkv=2, D=64, T=64, pages=4, max_pages=4, k=32):
+    return lib.gpu_kv8_dequant(dtype, 16, 16, 16, 16, 16, 4, 16, k, 32, B, rows, Hkv, D, T, pages, max_pages, 0)
 
 
 def _cross(lib, dtype=2, B=1, Lq=1, Lkv=5, H=4, Hkv=2, D=64, q=16, k=16, strides=S):
