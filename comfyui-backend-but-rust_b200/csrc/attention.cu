@@ -272,6 +272,7 @@ template <typename QT, int DP, bool KV8> int launch_tile(AttnParams& p, cudaStre
 // neighbouring values of a key with the same 16 of its query row, and in p . v its column 16 g + j of every key stands for column g of the
 // product's j-th tile. So codes are read from shared memory in 16-byte pieces and nothing is transposed.
 constexpr int kRowsWarps = 8, kRowsStages = 3;
+constexpr float kSlack = 8.f;
 
 template <int DP> struct RowsTile {
     static constexpr int kHalf = 16 * DP, kStage = 2 * kHalf, kRing = kRowsWarps * kRowsStages * kStage;
@@ -302,8 +303,18 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits % p.row_tiles, bh = blockIdx.x / p.splits / p.row_tiles;
-    const int b = bh / p.Hkv, kvh = bh % p.Hkv, ratio = p.H / p.Hkv, D = p.D;
+    const int kvh = bh % p.Hkv, ratio = p.H / p.Hkv, D = p.D;
+    int b = bh / p.Hkv;
     pdl_wait();
+    if (p.B > 1 && p.B <= 32) {      // the longest sequences first: the last CTAs to run then have little to do. Every warp finds the b-th longest.
+        const int mine = lane < p.B ? gload(p.kv_len + lane) : INT32_MIN;
+        int rank = 0;
+        for (int j = 0; j < p.B; ++j) {
+            const int other = __shfl_sync(0xffffffffu, mine, j);
+            rank += other > mine || (other == mine && j < lane);
+        }
+        b = __ffs((int)__ballot_sync(0xffffffffu, lane < p.B && rank == b)) - 1;
+    }
     const int len = min(max(gload(p.kv_len + b), 0), p.Lkv);
     const int ql = p.q_len ? min(max(gload(p.q_len + b), 0), p.Lq) : p.Lq;
     const int r0 = rt * 16, live = min(16, ql * ratio - r0);
@@ -333,18 +344,31 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
         }
     };
     // 16 rows of K, then of V. K's 16-byte pieces are read four to a row by two rows at a time, V's two to a row by four pairs of rows: the
-    // piece's number is turned so that either lies in all 32 banks.
+    // piece's number is turned so that either lies in all 32 banks. A lane has the same piece of every kStep-th row.
+    constexpr int kPieces = DP / 16, kStep = 32 / kPieces;
+    const int piece = lane % kPieces, row0 = lane / kPieces, from = row0 * D + piece * 16;
+    const uint32_t to = ring + row0 * DP;
+    const bool wide = piece * 16 < D;
     auto load = [&](int i, int slot) {
         const int64_t off = __shfl_sync(0xffffffffu, page_off, i & 31);
-        const int key = (first + warp + i * kRowsWarps) * 16;
-        const uint32_t dst = ring + slot * R::kStage;
+        const int left = seen - (first + warp + i * kRowsWarps) * 16;      // rows that are seen
+        const uint32_t dst = to + slot * R::kStage;
+        const int8_t *k = reinterpret_cast<const int8_t*>(p.k) + (off < 0 ? 0 : off + from), *v = reinterpret_cast<const int8_t*>(p.v) + (off < 0 ? 0 : off + from);
+        if (left >= 16 && off >= 0 && D == DP) {
 #pragma unroll
-        for (int j = 0; j < DP / 32; ++j) {
-            const int x = j * 32 + lane, row = x / (DP / 16), c = x % (DP / 16);
-            const bool valid = off >= 0 && c * 16 < D && key + row < seen;
-            const int64_t o = valid ? off + row * D + c * 16 : 0;
-            cp_async16(dst + row * DP + ((c ^ ((row & 1) << 2)) & (DP / 16 - 1)) * 16, reinterpret_cast<const int8_t*>(p.k) + o, valid);
-            cp_async16(dst + R::kHalf + row * DP + ((c ^ (row & 6)) & (DP / 16 - 1)) * 16, reinterpret_cast<const int8_t*>(p.v) + o, valid);
+            for (int j = 0; j < 16 / kStep; ++j) {
+                const int row = j * kStep;
+                cp_async16(dst + row * DP + ((piece ^ (row0 & 1) << 2) & (kPieces - 1)) * 16, k + row * D, true);
+                cp_async16(dst + R::kHalf + row * DP + ((piece ^ ((row + row0) & 6)) & (kPieces - 1)) * 16, v + row * D, true);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16 / kStep; ++j) {
+                const int row = j * kStep;
+                const bool valid = off >= 0 && wide && row + row0 < left;
+                cp_async16(dst + row * DP + ((piece ^ ((row + row0) & 1) << 2) & (kPieces - 1)) * 16, valid ? k + row * D : reinterpret_cast<const int8_t*>(p.k), valid);
+                cp_async16(dst + R::kHalf + row * DP + ((piece ^ ((row + row0) & 6)) & (kPieces - 1)) * 16, valid ? v + row * D : reinterpret_cast<const int8_t*>(p.v), valid);
+            }
         }
         if (lane == (i & 31)) info[slot] = make_float4(mul_l, add_l, wt_l, page_off >= 0 ? 1.f : 0.f);
     };
@@ -431,10 +455,16 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
                 top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                 top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
             }
-            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {      // a larger exponent: the sums follow it
+            // m follows the largest exponent only when that has grown by 2^8: until then p is at most 256, and the sums stay as they are
+            const bool grew[2] = {top[0] > m[0] + kSlack, top[1] > m[1] + kSlack};
+            if (__any_sync(0xffffffffu, grew[0] || grew[1])) {
                 float keep[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) keep[h] = exp2_fast(m[h] - (top[h] == -INFINITY ? 0.f : top[h])), m[h] = top[h], l[h] *= keep[h];
+                for (int h = 0; h < 2; ++h) {
+                    keep[h] = grew[h] ? exp2_fast(m[h] - top[h]) : 1.f;
+                    if (grew[h]) m[h] = top[h];
+                    l[h] *= keep[h];
+                }
 #pragma unroll
                 for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
