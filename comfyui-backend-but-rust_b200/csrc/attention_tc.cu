@@ -31,7 +31,7 @@ template <int DP, bool KV8> struct Tc {
     // barriers and two words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
     // item % 2: 1 / l of every row (16-bit), or bf16 queries' powers of two
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
-    static constexpr int kEnd = kRowInfo + 2048, kSmem = kEnd + 1024;
+    static constexpr int kOrder = kRowInfo + 2048, kEnd = kOrder + 128, kSmem = kEnd + 1024;
     static constexpr int kThreads = 512;
     // Registers of the warpgroups (softmax twice, products and loads, codes or rows out): a softmax thread holds a row of 128 logits. Their
     // sum over the threads is what the launch has, 512 x 128.
@@ -74,14 +74,17 @@ struct TcParams {
 struct Item {
     int b, h, row0, rows, len, ql, seen, n;      // h: query head, or kv head of packed rows; rows from row0 on; n key tiles
 };
-template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, int64_t i) {
+// The item of a CTA's r-th round: the rounds run through the CTAs forwards and backwards in turn, so that where the items get smaller, as the
+// cache's do, the sums of a CTA's items come out alike.
+__device__ __forceinline__ int64_t item_of(int r) { return (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
+template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, int64_t i, const int* order) {
     Item x;
     const int heads = KV8 ? p.a.Hkv : p.a.H;
-    // heads next to one another: together they read and write whole rows of Q and of the result. Cache: long causal tiles first.
-    const int rest = (int)(i / heads);
+    // Heads next to one another: together they read and write whole rows of Q and of the result. Cache: long sequences first, of each the
+    // tiles with most keys.
+    const int rest = (int)(i / heads), b = rest / p.q_tiles, qt = rest - b * p.q_tiles;
     x.h = (int)(i - (int64_t)rest * heads);
-    const int qt = KV8 ? p.q_tiles - 1 - rest / p.a.B : rest % p.q_tiles;
-    x.b = KV8 ? rest % p.a.B : rest / p.q_tiles, x.row0 = qt * 256;
+    x.b = KV8 && p.a.B <= 32 ? order[b] : b, x.row0 = (KV8 ? p.q_tiles - 1 - qt : qt) * 256;
     x.len = p.a.kv_len ? min(max(gload(p.a.kv_len + x.b), 0), p.a.Lkv) : p.a.Lkv;
     x.ql = p.a.Lq;
     x.seen = x.len;
@@ -132,6 +135,19 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const uint32_t tmem = *tmem_s;
     pdl_wait();
     const int D = p.a.D;
+    int* order = reinterpret_cast<int*>(sm + L::kOrder);      // sequences by length, the longest first
+    if (KV8 && p.a.B <= 32) {
+        if (warp == 0) {
+            const int mine = lane < p.a.B ? gload(p.a.kv_len + lane) : INT32_MIN;
+            int rank = 0;
+            for (int j = 0; j < p.a.B; ++j) {
+                const int other = __shfl_sync(0xffffffffu, mine, j);
+                rank += other > mine || (other == mine && j < lane);
+            }
+            if (lane < p.a.B) order[rank] = lane;
+        }
+        __syncthreads();
+    }
 
     if (warp < 8) {
         more_registers<L::kSoftmaxRegs>();
@@ -142,8 +158,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint8_t* stage = sm + L::kStaging + warp * 2048;
         uint32_t s_phase = 0, tile_no = 0, item_no = 0;
         bool ok = true;
-        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item x = item_at<KV8>(p, i);
+        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+            const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n > 0 && t * 128 >= x.rows) {
                 tile_no += x.n, ++item_no;
                 continue;
@@ -309,8 +325,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             umma_commit(s_full + 8 * t);
             mbar_arrive(s_full + 8 * t);
         };
-        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item x = item_at<KV8>(p, i);
+        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+            const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
             uint32_t ks = kv_no & 3, k_phase = kv_no >> 2 & 1;
@@ -377,8 +393,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
-        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item x = item_at<KV8>(p, i);
+        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+            const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1, kvh = x.h / (p.a.H / p.a.Hkv);
             auto load_kv = [&](int j, int which) {
@@ -419,8 +435,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             if (ok) load_kv(0, 1);
             ++tile_no;
-            if (lane == 0 && i + gridDim.x < p.items) {      // the next item's queries to L2
-                const Item y = item_at<KV8>(p, i + gridDim.x);
+            if (lane == 0 && item_of(r + 1) < p.items) {      // the next item's queries to L2
+                const Item y = item_at<KV8>(p, item_of(r + 1), order);
                 for (int t = 0; t < 2 && t * 128 < y.rows; ++t)
 #pragma unroll
                     for (int box = 0; box < DP / 64; ++box) tma_prefetch_4d(&tmap_q, box * 64, y.row0 + t * 128, y.h * p.q_head, y.b * p.q_batch);
@@ -435,8 +451,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         // ---- rows of V behind keys that are not seen: zeros. Two warps, 16 lanes (8 with 64 columns) to a row.
         uint32_t kv_no = 1, tile_no = 0;
         bool ok = true;
-        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item x = item_at<KV8>(p, i);
+        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+            const Item x = item_at<KV8>(p, item_of(r), order);
             for (int j = 0; j < x.n; ++j, ++tile_no, kv_no += 2) {
                 const uint32_t slot = kv_no & 3;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * slot, kv_no >> 2 & 1, abort_s, ST_TIMEOUT_FULL)))) break;
@@ -461,8 +477,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint8_t* stage = sm + L::kStaging + quarter * 4096;
         uint32_t phase[2] = {}, item_no = 0;
         bool ok = true;
-        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item x = item_at<KV8>(p, i);
+        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+            const Item x = item_at<KV8>(p, item_of(r), order);
             for (int t = 0; t < 2 && t * 128 < x.rows; ++t) {
                 float inv = 0.f;
                 if (x.n > 0) {
@@ -529,8 +545,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             *reinterpret_cast<uint4*>(tile + (piece >> 3) * kBox + row * 128 + ((piece ^ row) & 7) * 16) = v;
         };
         const int ratio = p.a.H / p.a.Hkv;
-        for (int64_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item x = item_at<KV8>(p, i);
+        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+            const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
             for (int t = 0; t < tiles; ++t) {
@@ -565,19 +581,20 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 done(q_full + 8 * t);
             }
             ++item_no;
-            // Pages are looked up a tile ahead, codes requested a step (K or V of a tile) ahead of their conversion.
+            // Nothing is waited for when it is requested: a tile's page indices two tiles ahead, its scales one, its codes (K and V) as soon as the
+            // tile before has been converted.
             constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
-            int64_t off = -1, off_next = -1;
-            float mul = 0.f, add = 0.f, wt = 0.f, mul_next = 0.f, add_next = 0.f, wt_next = 0.f;
-            auto look_up = [&](int j) {      // this warp's 32 keys of a tile: one to a lane
+            auto page_of = [&](int j) {      // this warp's 32 keys of a tile: one to a lane
                 const int key = j * kTileKeys + w * 32 + lane;
-                const int64_t page = key < x.seen ? gload(p.a.table + x.b * p.a.table_stride + key / p.a.T) : -1;
-                off_next = -1, mul_next = 0.f, add_next = 0.f, wt_next = 0.f;
-                if (page >= 0 && page < p.a.pages) {
-                    off_next = ((page * p.a.Hkv + x.h) * p.a.T + key % p.a.T) * D;
-                    const float s = fmaxf(gload(p.a.v_scale + page * p.a.Hkv + x.h), kTiny);
-                    mul_next = gload(p.a.k_scale + page * p.a.Hkv + x.h) * (p.a.scale * kLog2e), add_next = log2f(s), wt_next = 1.f / s;
-                }
+                return key < x.seen ? gload(p.a.table + x.b * p.a.table_stride + key / p.a.T) : -1;
+            };
+            auto offset_of = [&](int j, int page) {
+                const int key = j * kTileKeys + w * 32 + lane;
+                return page >= 0 && page < p.a.pages ? (((int64_t)page * p.a.Hkv + x.h) * p.a.T + key % p.a.T) * D : (int64_t)-1;
+            };
+            auto scales_of = [&](int page, float& k, float& v) {
+                const bool there = page >= 0 && page < p.a.pages;
+                k = there ? gload(p.a.k_scale + (int64_t)page * p.a.Hkv + x.h) : 0.f, v = there ? gload(p.a.v_scale + (int64_t)page * p.a.Hkv + x.h) : 1.f;
             };
             auto request = [&](uint4 (&code)[32 / kAtOnce], int64_t offs, int which) {
                 const int8_t* src = reinterpret_cast<const int8_t*>(which ? p.a.v : p.a.k);
@@ -601,12 +618,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 done(kv_full + 8 * slot);
             };
             uint4 kc[32 / kAtOnce], vc[32 / kAtOnce];
-            look_up(0);
-            off = off_next, mul = mul_next, add = add_next, wt = wt_next;
+            float k_scale, v_scale;
+            int page = page_of(0), page_next = page_of(1);
+            int64_t off = offset_of(0, page);
             request(kc, off, 0);
+            request(vc, off, 1);
+            scales_of(page, k_scale, v_scale);
             for (int j = 0; j < x.n && ok; ++j, ++tile_no) {
-                request(vc, off, 1);
-                if (j + 1 < x.n) look_up(j + 1);
                 uint32_t slot = kv_no & 3;
                 if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
                 ++kv_no;
@@ -614,15 +632,19 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (lane == 0) words[(tile_no & 3) * 4 + w] = seen;
                 if ((lane & 15) == 0) {
                     float* in = info + (tile_no & 3) * 24 + w * 2 + (lane >> 4);
-                    in[0] = mul, in[8] = add, in[16] = wt;
+                    const float s = fmaxf(v_scale, kTiny);
+                    in[0] = k_scale * (p.a.scale * kLog2e), in[8] = log2f(s), in[16] = 1.f / s;
                 }
                 convert(kc, slot);
-                off = off_next, mul = mul_next, add = add_next, wt = wt_next;
-                if (j + 1 < x.n) request(kc, off, 0);
+                page = page_next, off = offset_of(j + 1, page);      // past the last tile: no key is seen, nothing is requested
+                request(kc, off, 0);
+                scales_of(page, k_scale, v_scale);
+                page_next = page_of(j + 2);
                 slot = kv_no & 3;
                 if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) break;
                 ++kv_no;
                 convert(vc, slot);
+                request(vc, off, 1);
             }
         }
     }
