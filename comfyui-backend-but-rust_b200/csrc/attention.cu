@@ -15,141 +15,63 @@ using namespace b200q;
 // 64 query rows (a kv head's queries: row r is query r / ratio, head r % ratio of its group), 64 keys a step, four warps of 16 rows.
 constexpr int kRows = 64, kKeys = 64, kThreads = 128;
 
-template <typename QT, int DP, bool KV8> struct Tile {
-    using T = typename std::conditional<KV8, half, QT>::type;      // of the products
+template <int DP> struct Tile {
     static constexpr int kRowBytes = DP * 2, kBytes = kKeys * DP * 2;
-    static constexpr int kStage = KV8 ? kKeys * DP : kBytes;       // K or V of a step as it is loaded
-    // Q | loaded K, V x 2 | (int8: K, V as halves) | per key: factor, offset, weight x 2 | m, l of every row
-    static constexpr int kLoaded = kRows * kRowBytes, kHalves = kLoaded + 4 * kStage, kKeyInfo = kHalves + (KV8 ? 2 * kBytes : 0);
-    static constexpr int kStats = kKeyInfo + 2 * 3 * kKeys * 4, kSmem = kStats + 2 * kRows * 4;
+    // Q | K, V x 2 | 0 or -inf per key x 2 | m, l of every row; the sums of the rows, f32, over K and V at the end
+    static constexpr int kLoaded = kRows * kRowBytes, kKeyInfo = kLoaded + 4 * kBytes, kStats = kKeyInfo + 2 * kKeys * 4, kSmem = kStats + 2 * kRows * 4;
     static __device__ __forceinline__ uint32_t at(int row, int c) { return (uint32_t)(row * kRowBytes + ((c ^ (row & 7)) * 16)); }
 };
 
-template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThreads) attention_tile_kernel(const AttnParams p) {
-    using L = Tile<QT, DP, KV8>;
-    using T = typename L::T;
+template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attention_tile_kernel(const AttnParams p) {
+    using L = Tile<DP>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits % p.row_tiles, bh = blockIdx.x / p.splits / p.row_tiles;
     const int b = bh / p.Hkv, kvh = bh % p.Hkv, ratio = p.H / p.Hkv;
     const int D = p.D, chunks = DP / 8;
     pdl_wait();
-    const int limit = p.Lkv;
-    const int len = p.kv_len ? min(max(gload(p.kv_len + b), 0), limit) : limit;
-    const int ql = p.q_len ? min(max(gload(p.q_len + b), 0), p.Lq) : p.Lq;
-    const int r0 = rt * kRows, live = min(kRows, ql * ratio - r0);      // rows of this tile that exist
-    if (live <= 0) return;                                              // the same for every CTA of the cluster
-    // keys that the tile's last row sees
-    const int seen = p.causal ? max(0, min(len, len - ql + (r0 + live - 1) / ratio + 1)) : len;
-    const int steps = (seen + kKeys - 1) / kKeys, per = (steps + p.splits - 1) / p.splits;
+    const int len = p.kv_len ? min(max(gload(p.kv_len + b), 0), p.Lkv) : p.Lkv;
+    const int r0 = rt * kRows, live = min(kRows, p.Lq * ratio - r0);    // rows of this tile that exist
+    const int steps = (len + kKeys - 1) / kKeys, per = (steps + p.splits - 1) / p.splits;
     const int first = min(split * per, steps), last = min(first + per, steps);
 
     const uint32_t base = smem_u32(smem);
-    float* key_mul = reinterpret_cast<float*>(smem + L::kKeyInfo);      // [stage][factor, offset, weight][key]
-    // ---- queries: into shared memory, for int8 keys as halves times a power of two per row (so that bf16's range does no harm)
-    float row_factor[2] = {1.f, 1.f};
+    float* key_info = reinterpret_cast<float*>(smem + L::kKeyInfo);     // [stage][key]
+    // ---- queries into shared memory
     {
         const int row = tid >> 1, i = (r0 + row) / ratio, h = kvh * ratio + (r0 + row) % ratio;
-        const QT* src = reinterpret_cast<const QT*>(p.q) + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
-        float mult = 1.f;
-        if constexpr (KV8 && std::is_same<QT, bf16>::value) {
-            float top = 0.f;
-            if (row < live)
-                for (int c = tid & 1; c < D / 8; c += 2) {
-                    const uint4 w = gload(reinterpret_cast<const uint4*>(src) + c);
-                    const QT* x = reinterpret_cast<const QT*>(&w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f<QT>(x[e])));
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            const int e = row_exponent(top);
-            mult = __uint_as_float((uint32_t)(127 + e) << 23);
-            if ((tid & 1) == 0) reinterpret_cast<float*>(smem + L::kStats)[row] = __uint_as_float((uint32_t)(127 - e) << 23);
-        }
-        for (int c = tid & 1; c < chunks; c += 2) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (row < live && c * 8 < D) {
-                w = gload(reinterpret_cast<const uint4*>(src) + c);
-                if constexpr (KV8 && std::is_same<QT, bf16>::value) {
-                    const QT* x = reinterpret_cast<const QT*>(&w);
-                    uint4 y;
-                    uint32_t* o = reinterpret_cast<uint32_t*>(&y);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = pack2<half>(to_f<QT>(x[2 * e]) * mult, to_f<QT>(x[2 * e + 1]) * mult);
-                    w = y;
-                }
-            }
-            *reinterpret_cast<uint4*>(smem + L::at(row, c)) = w;
-        }
+        const T* src = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
+        for (int c = tid & 1; c < chunks; c += 2)
+            *reinterpret_cast<uint4*>(smem + L::at(row, c)) =
+                row < live && c * 8 < D ? gload(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
     }
-    // ---- one step's keys and values on their way
+    // ---- one step's keys and values on their way; what is not seen is zeros, whatever lies there
     auto load = [&](int step, int stage) {
-        const uint32_t ks = base + L::kLoaded + stage * 2 * L::kStage, vs = ks + L::kStage;
-        if constexpr (KV8) {
-            for (int i = tid; i < kKeys * DP / 16; i += kThreads) {
-                const int key = i / (DP / 16), c = i % (DP / 16), at = step * kKeys + key;
-                int64_t page = at < seen ? gload(p.table + b * p.table_stride + at / p.T) : -1;
-                const bool valid = page >= 0 && page < p.pages && c * 16 < D;
-                const int64_t off = valid ? ((page * p.Hkv + kvh) * p.T + at % p.T) * D + c * 16 : 0;
-                cp_async16(ks + i * 16, reinterpret_cast<const int8_t*>(p.k) + off, valid);
-                cp_async16(vs + i * 16, reinterpret_cast<const int8_t*>(p.v) + off, valid);
-            }
-        } else {
-            for (int i = tid; i < kKeys * chunks; i += kThreads) {
-                const int key = i / chunks, c = i % chunks, at = step * kKeys + key;
-                const bool valid = at < seen && c * 8 < D && (!p.mask || gload(p.mask + b * p.mask_stride + at));
-                const QT* k = reinterpret_cast<const QT*>(p.k) + (valid ? b * p.ks[0] + at * p.ks[1] + kvh * p.ks[2] + c * 8 : 0);
-                const QT* v = reinterpret_cast<const QT*>(p.v) + (valid ? b * p.vs[0] + at * p.vs[1] + kvh * p.vs[2] + c * 8 : 0);
-                cp_async16(ks + L::at(key, c), k, valid);
-                cp_async16(vs + L::at(key, c), v, valid);
-            }
+        const uint32_t ks = base + L::kLoaded + stage * 2 * L::kBytes, vs = ks + L::kBytes;
+        for (int i = tid; i < kKeys * chunks; i += kThreads) {
+            const int key = i / chunks, c = i % chunks, at = step * kKeys + key;
+            const bool valid = at < len && c * 8 < D && (!p.mask || gload(p.mask + b * p.mask_stride + at));
+            const T* k = reinterpret_cast<const T*>(p.k) + (valid ? b * p.ks[0] + at * p.ks[1] + kvh * p.ks[2] + c * 8 : 0);
+            const T* v = reinterpret_cast<const T*>(p.v) + (valid ? b * p.vs[0] + at * p.vs[1] + kvh * p.vs[2] + c * 8 : 0);
+            cp_async16(ks + L::at(key, c), k, valid);
+            cp_async16(vs + L::at(key, c), v, valid);
         }
-        // logit (base 2) = product * factor + offset; an offset of -inf is a key that is not seen. With pages the offset is log2 of the
-        // value's scale, so that p carries it and the products take the codes as they are; `weight` takes it out of the sum of p.
         if (tid < kKeys) {
             const int at = step * kKeys + tid;
-            bool valid = at < seen;
-            float mul = p.scale * kLog2e, add = 0.f, wt = 1.f;
-            if constexpr (KV8) {
-                const int64_t page = valid ? gload(p.table + b * p.table_stride + at / p.T) : -1;
-                valid = page >= 0 && page < p.pages;
-                if (valid) {
-                    const float s = fmaxf(gload(p.v_scale + page * p.Hkv + kvh), kTiny);
-                    mul *= gload(p.k_scale + page * p.Hkv + kvh), add = log2f(s), wt = 1.f / s;
-                }
-            } else if (valid && p.mask) valid = gload(p.mask + b * p.mask_stride + at) != 0;
-            float* info = key_mul + stage * 3 * kKeys + tid;
-            info[0] = mul, info[kKeys] = valid ? add : -INFINITY, info[2 * kKeys] = valid ? wt : 0.f;
+            key_info[stage * kKeys + tid] = at < len && (!p.mask || gload(p.mask + b * p.mask_stride + at)) ? 0.f : -INFINITY;
         }
     };
     float o[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
-    int bound[2];      // keys that rows g and g + 8 of this warp see
-#pragma unroll
-    for (int h = 0; h < 2; ++h) bound[h] = p.causal ? len - ql + (r0 + warp * 16 + g + 8 * h) / ratio + 1 : len;
+    const float to_log2 = p.scale * kLog2e;
     if (first < last) load(first, 0);
     cp_async_commit();
-    __syncthreads();
-    if constexpr (KV8 && std::is_same<QT, bf16>::value) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) row_factor[h] = reinterpret_cast<const float*>(smem + L::kStats)[warp * 16 + g + 8 * h];
-    }
     for (int step = first; step < last; ++step) {
         const int stage = (step - first) & 1;
         if (step + 1 < last) load(step + 1, stage ^ 1);
         cp_async_commit();
         cp_async_wait<1>();
         __syncthreads();
-        uint32_t ks = base + L::kLoaded + stage * 2 * L::kStage, vs = ks + L::kStage;
-        if constexpr (KV8) {      // codes -> halves
-            const uint8_t* src = smem + L::kLoaded + stage * 2 * L::kStage;
-            for (int i = tid; i < 2 * kKeys * DP / 8; i += kThreads) {
-                const int which = i / (kKeys * DP / 8), j = i % (kKeys * DP / 8);
-                const uint2 w = *reinterpret_cast<const uint2*>(src + which * L::kStage + j * 8), x = halves_of4(w.x), y = halves_of4(w.y);
-                *reinterpret_cast<uint4*>(smem + L::kHalves + which * L::kBytes + L::at(j / chunks, j % chunks)) = make_uint4(x.x, x.y, y.x, y.y);
-            }
-            __syncthreads();
-            ks = base + L::kHalves, vs = ks + L::kBytes;
-        }
+        const uint32_t ks = base + L::kLoaded + stage * 2 * L::kBytes, vs = ks + L::kBytes;
         float s[8][4] = {};
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
@@ -163,17 +85,14 @@ template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThre
                 mma16816<T>(s[n + 1], a[0], a[1], a[2], a[3], k4[2], k4[3]);
             }
         }
-        const float* info = key_mul + stage * 3 * kKeys;
+        const float* info = key_info + stage * kKeys;
         float top[2] = {m[0], m[1]};
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int key = n * 8 + 2 * t + (i & 1), h = i >> 1;
-                const float add = info[kKeys + key];
-                const bool valid = add != -INFINITY && step * kKeys + key < bound[h];
-                s[n][i] = valid ? __fmaf_rn(s[n][i] * row_factor[h], info[key], add) : -INFINITY;
-                top[h] = fmaxf(top[h], s[n][i]);
+                s[n][i] = info[n * 8 + 2 * t + (i & 1)] == 0.f ? s[n][i] * to_log2 : -INFINITY;
+                top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
             }
         float keep[2], shift[2];
 #pragma unroll
@@ -197,7 +116,7 @@ template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThre
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[n][i] = exp2_fast(s[n][i] - shift[i >> 1]);
-                    l[i >> 1] = __fmaf_rn(s[n][i], KV8 ? info[2 * kKeys + n * 8 + 2 * t + (i & 1)] : 1.f, l[i >> 1]);
+                    l[i >> 1] += s[n][i];
                 }
                 a[2 * j] = pack2<T>(s[n][0], s[n][1]), a[2 * j + 1] = pack2<T>(s[n][2], s[n][3]);
             }
@@ -248,14 +167,14 @@ template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(kThre
                 for (int e = 0; e < 8; ++e) y[e] = __fmaf_rn(dsmem_f32(part_at + (row * kPitch + (n ^ (row & 3)) * 8 + e) * 4, s), w, y[e]);
             }
         }
-        store_row(p, y, total, b, r0 + row, kvh, ratio, n * 8, QT());
+        store_row(p, y, total, b, r0 + row, kvh, ratio, n * 8, T());
     }
     if (p.splits > 1) cluster_sync_all();      // nobody leaves while its shared memory is read
 }
 
-template <typename QT, int DP, bool KV8> int launch_tile(AttnParams& p, cudaStream_t st) {
-    using L = Tile<QT, DP, KV8>;
-    auto kern = attention_tile_kernel<QT, DP, KV8>;
+template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
+    using L = Tile<DP>;
+    auto kern = attention_tile_kernel<T, DP>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
     const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + kRows - 1) / kRows, base = tiles * p.B * p.Hkv;
     p.row_tiles = (int)tiles;
@@ -265,8 +184,8 @@ template <typename QT, int DP, bool KV8> int launch_tile(AttnParams& p, cudaStre
     if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kThreads, L::kSmem, st, p.splits, p);
 }
-// ---- few rows over the cache ---------------------------------------------------------------------------------------------------------
-// Up to 16 rows to a kv head (a token's query heads, or a few tokens'): bound by the cache's bytes. A CTA's eight warps take 16 keys each
+// ---- rows over the cache ---------------------------------------------------------------------------------------------------------
+// Tiles of 16 rows of a kv head (a token's query heads, or a few tokens'): bound by the cache's bytes. A CTA's eight warps take 16 keys each
 // in turn, and every warp is on its own until the end: its ring of stages, its m, l and sums. The operands of the products come out of the
 // codes as they lie in memory, because the order of a product's inner index is free as long as both operands have it: a lane multiplies 16
 // neighbouring values of a key with the same 16 of its query row, and in p . v its column 16 g + j of every key stands for column g of the
@@ -278,7 +197,7 @@ template <int DP> struct RowsTile {
     static constexpr int kHalf = 16 * DP, kStage = 2 * kHalf, kRing = kRowsWarps * kRowsStages * kStage;
     static constexpr int kPitch = DP + 8;                              // floats to a row of sums
     static constexpr int kParts = kRowsWarps * 16 * kPitch * 4, kSmem0 = kParts + 16 * kPitch * 4 > kRing ? kParts + 16 * kPitch * 4 : kRing;
-    static constexpr int kStats = kSmem0, kInfo = kStats + (kRowsWarps + 1) * 32 * 4, kSmem = kInfo + kRowsWarps * kRowsStages * 16;
+    static constexpr int kStats = kSmem0, kInfo = kStats + (kRowsWarps + 1) * 32 * 4, kSmem = kInfo + kRowsWarps * 64 * 16;
 };
 
 // Four int8 codes (sign bits turned) of each of two rows as four registers of halves (row a's value, row b's value)
@@ -325,23 +244,25 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
     const int first = min(split * per, blocks), last = min(first + per, blocks);
     const int mine = (last - first - warp + kRowsWarps - 1) / kRowsWarps;      // blocks first + warp + 8 i, i < mine
     const uint32_t ring = smem_u32(smem) + warp * kRowsStages * R::kStage;
-    float4* info = reinterpret_cast<float4*>(smem + R::kInfo) + warp * kRowsStages;      // factor, offset, weight of a stage's page
+    float4* info = reinterpret_cast<float4*>(smem + R::kInfo) + warp * 64;      // [block % 64]: factor, offset, weight of its page, and whether there is one
 
-    // Pages and scales of the next 32 blocks, one to a lane
+    // Pages of the next 32 blocks, one to a lane. Their scales are requested with the blocks and worked out behind them (note_scales).
     int64_t page_off = -1;
-    float mul_l = 0.f, add_l = -INFINITY, wt_l = 0.f;
+    float k_scale = 0.f, v_scale = 1.f;
     auto look_up = [&](int i0) {
-        page_off = -1, mul_l = 0.f, add_l = -INFINITY, wt_l = 0.f;
-        const int i = i0 + lane;
-        if (i < mine) {
-            const int key = (first + warp + i * kRowsWarps) * 16;
+        page_off = -1;
+        const int key = (first + warp + (i0 + lane) * kRowsWarps) * 16;
+        if (i0 + lane < mine) {
             const int64_t page = gload(p.table + b * p.table_stride + key / p.T);
             if (page >= 0 && page < p.pages) {
-                const float s = fmaxf(gload(p.v_scale + page * p.Hkv + kvh), kTiny);
-                mul_l = gload(p.k_scale + page * p.Hkv + kvh) * (p.scale * kLog2e), add_l = log2f(s), wt_l = 1.f / s;
                 page_off = ((page * p.Hkv + kvh) * p.T + key % p.T) * D;
+                k_scale = gload(p.k_scale + page * p.Hkv + kvh), v_scale = gload(p.v_scale + page * p.Hkv + kvh);
             }
         }
+    };
+    auto note_scales = [&](int i0) {
+        const float s = fmaxf(v_scale, kTiny);
+        info[(i0 + lane) & 63] = page_off >= 0 ? make_float4(k_scale * (p.scale * kLog2e), log2f(s), 1.f / s, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     // 16 rows of K, then of V. K's 16-byte pieces are read four to a row by two rows at a time, V's two to a row by four pairs of rows: the
     // piece's number is turned so that either lies in all 32 banks. A lane has the same piece of every kStep-th row.
@@ -370,7 +291,6 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
                 cp_async16(dst + R::kHalf + row * DP + ((piece ^ ((row + row0) & 6)) & (kPieces - 1)) * 16, valid ? v + row * D : reinterpret_cast<const int8_t*>(p.v), valid);
             }
         }
-        if (lane == (i & 31)) info[slot] = make_float4(mul_l, add_l, wt_l, page_off >= 0 ? 1.f : 0.f);
     };
     float o[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
     uint32_t q[DP / 16][4];
@@ -381,6 +301,7 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
         if (i < mine) load(i, i);
         cp_async_commit();
     }
+    note_scales(0);
     int bound[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -423,7 +344,7 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
         cp_async_wait<kRowsStages - 2>();
         __syncwarp();
         const uint32_t ks = ring + slot * R::kStage, vs = ks + R::kHalf;
-        const float4 in = info[slot];
+        const float4 in = info[i & 63];
         const int key0 = (first + warp + i * kRowsWarps) * 16;
         if (in.w != 0.f) {      // the page exists
             float s[2][4] = {};
@@ -508,7 +429,7 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
         __syncwarp();
         const int ahead = i + kRowsStages - 1;
         if (ahead < mine) {
-            if ((ahead & 31) == 0) look_up(ahead);
+            if ((ahead & 31) == 0) look_up(ahead), note_scales(ahead);
             load(ahead, slot == 0 ? kRowsStages - 1 : slot - 1);
         }
         cp_async_commit();
@@ -584,20 +505,20 @@ template <typename QT, int DP> int launch_rows(AttnParams& p, cudaStream_t st) {
     const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + 15) / 16, base = tiles * p.B * p.Hkv;
     p.row_tiles = (int)tiles;
     p.splits = 1;
-    while (p.splits < 8 && base * p.splits < 148 * 8 && (int64_t)p.Lkv > (int64_t)p.splits * 16 * kRowsWarps) p.splits *= 2;
+    while (p.splits < 8 && base * p.splits < 148 * 2 && (int64_t)p.Lkv > (int64_t)p.splits * 16 * kRowsWarps) p.splits *= 2;
     if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kRowsWarps * 32, R::kSmem, st, p.splits, p);
 }
 
-template <typename QT, bool KV8> int launch_width(AttnParams& p, cudaStream_t st) {
-    if (attention_tc_takes(p, KV8)) return attention_tc(std::is_same<QT, half>::value ? DT_F16 : DT_BF16, KV8, p, st);
-    if constexpr (KV8)
-        if ((int64_t)p.Lq * (p.H / p.Hkv) <= 16)
-            return p.D <= 64 ? launch_rows<QT, 64>(p, st) : p.D <= 128 ? launch_rows<QT, 128>(p, st) : launch_rows<QT, 256>(p, st);
-    if (p.D <= 64) return launch_tile<QT, 64, KV8>(p, st);
-    if (p.D <= 128) return launch_tile<QT, 128, KV8>(p, st);
-    if (p.D <= 192) return launch_tile<QT, 192, KV8>(p, st);
-    return launch_tile<QT, 256, KV8>(p, st);
+template <typename T> int launch_cross(AttnParams& p, cudaStream_t st) {
+    if (attention_tc_takes(p, false)) return attention_tc(std::is_same<T, half>::value ? DT_F16 : DT_BF16, false, p, st);
+    if (p.D <= 64) return launch_tile<T, 64>(p, st);
+    if (p.D <= 128) return launch_tile<T, 128>(p, st);
+    return p.D <= 192 ? launch_tile<T, 192>(p, st) : launch_tile<T, 256>(p, st);
+}
+template <typename QT> int launch_kv8(AttnParams& p, cudaStream_t st) {
+    if (attention_tc_takes(p, true)) return attention_tc(std::is_same<QT, half>::value ? DT_F16 : DT_BF16, true, p, st);
+    return p.D <= 64 ? launch_rows<QT, 64>(p, st) : p.D <= 128 ? launch_rows<QT, 128>(p, st) : launch_rows<QT, 256>(p, st);
 }
 
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -621,7 +542,7 @@ GPU_API int gpu_cross_attention(int dtype, const void* q, const void* k, const v
     for (int i = 0; i < 3; ++i) p.qs[i] = strides[i], p.ks[i] = strides[3 + i], p.vs[i] = strides[6 + i], p.os[i] = strides[9 + i];
     p.B = B, p.Lq = Lq, p.Lkv = Lkv, p.H = H, p.Hkv = Hkv, p.D = D, p.T = 1, p.scale = scale;
     cudaStream_t st = (cudaStream_t)stream;
-    return dtype == DT_F16 ? launch_width<half, false>(p, st) : launch_width<bf16, false>(p, st);
+    return dtype == DT_F16 ? launch_cross<half>(p, st) : launch_cross<bf16>(p, st);
 }
 
 GPU_API int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t* strides, const int8_t* k8, const int8_t* v8, const float* k_scale,
@@ -640,5 +561,5 @@ GPU_API int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t
     p.kv_len = lengths, p.q_len = q_len, p.causal = causal;
     p.B = B, p.Lq = Lq, p.Lkv = pages > 0 ? max_pages * T : 0, p.H = H, p.Hkv = Hkv, p.D = D, p.T = T, p.scale = scale;
     cudaStream_t st = (cudaStream_t)stream;
-    return dtype == DT_F16 ? launch_width<half, true>(p, st) : launch_width<bf16, true>(p, st);
+    return dtype == DT_F16 ? launch_kv8<half>(p, st) : launch_kv8<bf16>(p, st);
 }
