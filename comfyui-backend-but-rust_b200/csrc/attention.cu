@@ -504,8 +504,11 @@ template <typename QT, int DP> int launch_rows(AttnParams& p, cudaStream_t st) {
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kSmem)) return (int)e;
     const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + 15) / 16, base = tiles * p.B * p.Hkv;
     p.row_tiles = (int)tiles;
+    // CTAs along the keys: as long as there are fewer than one to an SM (two where sequences of different lengths leave some idle) and each has
+    // a block for each warp. CTAs begin and end slowly: 16 sequences of up to 32768 tokens, 8 kv heads, 2 | 4 | 8 CTAs 182 | 120 | 156 us; 8 of up to
+    // 8000 with 64 rows a head 94 | 73 | 148; one of 8000 with 120 rows a head 37 | 48 | 53.
     p.splits = 1;
-    while (p.splits < 8 && base * p.splits < 148 * 2 && (int64_t)p.Lkv > (int64_t)p.splits * 16 * kRowsWarps) p.splits *= 2;
+    while (p.splits < 8 && base * p.splits < (p.B > 1 ? 296 : 148) && (int64_t)p.Lkv > (int64_t)p.splits * 16 * kRowsWarps) p.splits *= 2;
     if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kRowsWarps * 32, R::kSmem, st, p.splits, p);
 }

@@ -690,11 +690,11 @@ template <typename QT, int DP, bool KV8> int launch_tc(const CUtensorMap (&tm)[3
 
 bool b200q::attention_tc_takes(const AttnParams& p, bool kv8) {
     if (p.D > 128 || !(p.scale > 0.f) || p.Lkv <= 0) return false;
-    // Half a tile of rows at least, and 64 tiles of 64 rows: with fewer the other kernels, which share a row tile's keys among CTAs, are done
-    // sooner (8 sequences, 1000 to 8000 tokens, 128 rows for each of 8 kv heads: 64 items here 218 us, 16 rows at a time 203; one sequence of
-    // 8000 and 256 rows: 8 items 232 us, 16 rows at a time 110).
+    // Half an item's rows at least, and enough tiles of 64 rows: with fewer the other kernels, which share a row tile's keys among CTAs, are
+    // done sooner. Over the cache, 8 sequences of 1000 to 8000 tokens and 128 rows for each of 8 kv heads (128 tiles): 219 us here, 124 with 16 rows at
+    // a time; one sequence of 8000 and 256 rows: 232 and 63; two of up to 4133 and 4096 rows (1024 tiles): 151 here.
     const int64_t rows = kv8 ? (int64_t)p.Lq * (p.H / p.Hkv) : p.Lq;
-    if (rows < 128 || (rows + 63) / 64 * p.B * (kv8 ? p.Hkv : p.H) < 64) return false;
+    if (rows < 128 || (rows + 63) / 64 * p.B * (kv8 ? p.Hkv : p.H) < (kv8 ? 160 : 64)) return false;
     // rows without a stride between them have no tensor map
     return kv8 || ((p.Lq == 1 || p.qs[1] > 0) && (p.Lkv == 1 || (p.ks[1] > 0 && p.vs[1] > 0)) && p.qs[0] >= 0 && p.qs[2] >= 0 && p.ks[0] >= 0 &&
                    p.ks[2] >= 0 && p.vs[0] >= 0 && p.vs[2] >= 0 && (p.ks[0] == 0) == (p.vs[0] == 0) && (p.ks[2] == 0) == (p.vs[2] == 0));

@@ -58,7 +58,9 @@ def _cross_check(got, q, k, v, seen, scale):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("B,Lq,Lkv,H,Hkv,D", [(1, 1, 1, 1, 1, 8), (2, 64, 77, 2, 2, 64), (1, 65, 64, 3, 1, 40), (2, 100, 154, 4, 2, 80), (1, 333, 333, 2, 2, 128),
                                               (3, 7, 65, 6, 2, 160), (1, 130, 512, 1, 1, 256), (1, 5, 2048, 2, 1, 64), (1, 1, 1500, 1, 1, 200), (2, 129, 63, 5, 5, 96),
-                                              (1, 1000, 257, 2, 1, 128), (1, 384, 128, 8, 8, 64), (2, 257, 129, 3, 3, 128)])
+                                              (1, 1000, 257, 2, 1, 128), (1, 384, 128, 8, 8, 64), (2, 257, 129, 3, 3, 128),
+                                              # two tiles of 128 rows a CTA: one and several key tiles, ragged rows, half a tile, shared heads, more items than SMs
+                                              (2, 300, 77, 8, 8, 64), (1, 1000, 257, 4, 2, 128), (3, 129, 513, 8, 4, 40), (1, 4096, 130, 1, 1, 80), (2, 2500, 1, 16, 16, 16), (1, 9800, 384, 5, 5, 128)])
 def test_cross_attention(pkg, dev, B, Lq, Lkv, H, Hkv, D, dtype):
     g = torch.Generator().manual_seed(B + Lq * 3 + Lkv + D)
     dt = DT[dtype]
@@ -185,7 +187,10 @@ def _kv8_check(got, q, c, table, lens, q_lens, causal, scale):
 @pytest.mark.parametrize("B,L,lens,H,Hkv,D,T", [(1, 1, [1], 1, 1, 64, 16), (1, 1, [1999], 32, 8, 128, 64), (3, 1, [0, 1, 700], 8, 8, 64, 64), (2, 1, [65, 4097], 8, 1, 96, 32),
                                                 (2, 3, [3, 200], 6, 2, 80, 16), (1, 70, [333], 4, 2, 128, 128), (2, 130, [130, 1000], 3, 1, 64, 32), (1, 16, [2000], 16, 1, 256, 128),
                                                 (2, 5, [2, 40], 2, 2, 256, 64), (1, 300, [300], 4, 4, 160, 64), (4, 2, [127, 128, 129, 2], 4, 4, 16, 16), (1, 1, [9000], 4, 4, 128, 64),
-                                                (1, 257, [700], 2, 2, 128, 64), (5, 1, [1, 64, 65, 1023, 5000], 24, 2, 64, 16)])
+                                                (1, 257, [700], 2, 2, 128, 64), (5, 1, [1, 64, 65, 1023, 5000], 24, 2, 64, 16), (1, 9, [1500], 14, 2, 112, 32), (33, 1, list(range(33)), 2, 1, 64, 16),
+                                                # two tiles of 128 rows a CTA
+                                                (2, 300, [300, 700], 16, 16, 128, 64), (1, 260, [1000], 64, 16, 64, 16), (3, 140, [140, 333, 150], 24, 8, 96, 32), (2, 1000, [1000, 1], 12, 12, 80, 128),
+                                                (34, 130, [130 + 7 * i for i in range(34)], 2, 2, 128, 16), (1, 2600, [2600], 8, 8, 128, 32)])
 def test_kv8_attention(pkg, dev, B, L, lens, H, Hkv, D, T, dtype):
     g = torch.Generator().manual_seed(B + L + sum(lens) + D)
     c, table = _cache(pkg, dev, g, B, lens, Hkv, D, T)
