@@ -95,6 +95,25 @@ def _setup_hbm(name, b, torch, dev, wl, I):
         b.tout = torch.empty((M, N), dtype=torch.float32, device=dev)
         b.tscr = (torch.empty(4 * M * K, dtype=torch.uint8, device=dev), torch.empty(2 * N * K, dtype=torch.uint8, device=dev))
         return None
+    if name in ("w4_linear", "w4_linear_prompt"):                # the same linear with 4-bit weights, one token | 333 tokens of bf16
+        M, K, N = 1 if name == "w4_linear" else 333, 2560, 19456
+        b.q = I.w4_requant((rnd(N, K) * 0.03).bfloat16(), 128)
+        b.qx, b.qout = rnd(M, K).bfloat16(), torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        return N * K // 2 + N * (K // 128) * 2 + 2 * M * K + 2 * M * N
+    if name == "kv8_attention":                                  # one token each of 16 sequences of 16384, 32 heads over 8 of the cache
+        B, S, H, Hkv, D, T = 16, 16384, 32, 8, 128, 64
+        b.A = sys.modules[I.__package__ + ".attention"]
+        b.cache = b.A.Kv8Cache.empty(B * S // T, Hkv, D, T, dev)
+        b.table = torch.arange(B * S // T, dtype=torch.int32, device=dev).view(B, S // T)
+        b.start, b.lengths = torch.zeros(B, dtype=torch.int32, device=dev), torch.full((B,), S, dtype=torch.int32, device=dev)
+        b.A.kv8_append(b.cache, rnd(B, S, Hkv, D).half(), rnd(B, S, Hkv, D).half(), b.table, b.start)
+        b.q = rnd(B, 1, H, D).half()
+        return 2 * B * S * Hkv * D + 8 * B * S // T * Hkv + 4 * B * H * D
+    if name == "cross_attention":                                # a DiT's image rows over a prompt: 16384 x 512, 24 heads of 128
+        b.A = sys.modules[I.__package__ + ".attention"]
+        b.q, b.k, b.v = (rnd(1, n, 24, 128).bfloat16() for n in (16384, 512, 512))
+        b.qout = torch.empty_like(b.q)
+        return None
     raise KeyError(name)
 
 
@@ -108,6 +127,10 @@ def _fp32_flow(b, I):
 HBM_KERNELS = {
     "wo8_linear": lambda b, I: I.wo8_linear(b.tx, b.tw[0], b.tw[1], out=b.tout, scratch=b.tscr),
     "wo8_fp32_flow": _fp32_flow,
+    "w4_linear": lambda b, I: I.w4_linear(b.qx, *b.q, out=b.qout),
+    "w4_linear_prompt": lambda b, I: I.w4_linear(b.qx, *b.q, out=b.qout),
+    "kv8_attention": lambda b, I: b.A.kv8_attention(b.q, b.cache, b.table, b.lengths),
+    "cross_attention": lambda b, I: b.A.cross_attention(b.q, b.k, b.v, out=b.qout),
     "pack_f32": lambda b, I: I.convrot_requant(b.hw, 0),
     "pack_bf16": lambda b, I: I.convrot_requant(b.hw, 0),
     "sd_quant": lambda b, I: I.sd_quant_rows(b.hx, 256),

@@ -11,8 +11,11 @@ from typing import Optional
 
 import torch
 
-from .ffi import ok
-from .linear import _DT, _h, _lib, _one_device, _ptr, _stream
+from .linear import _h
+
+
+def _scale(q: torch.Tensor, scale: Optional[float]) -> float:
+    return scale if scale is not None else max(q.shape[-1], 1) ** -0.5
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len: Optional[torch.Tensor] = None,
@@ -21,7 +24,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     16-byte pieces; D a multiple of 8 up to 256; H a multiple of Hkv (head h reads kv head h // (H // Hkv)). Keys from kv_len[b]
     (int32 [B]) on, and those whose key_mask (bool [B, Lkv]) is False, are not seen, whatever they hold; a query that sees none gets
     zeros. `scale` defaults to D ** -0.5."""
-    return _h.cross_attention(q, k, v, kv_len, key_mask, q.shape[-1] ** -0.5 if scale is None else scale, out)
+    return _h.cross_attention(q, k, v, kv_len, key_mask, _scale(q, scale), out)
 
 
 @dataclass
@@ -52,18 +55,7 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, table: torch.T
 
 def kv8_dequant(cache: Kv8Cache, table: torch.Tensor, lengths: torch.Tensor, rows: int, *, dtype=torch.float32):
     """gpu_kv8_dequant: (k, v) [B, rows, Hkv, D] of the sequences' first `rows` tokens; zeros from lengths[b] on."""
-    _one_device(cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths)
-    pages, Hkv, T, D = cache.k.shape
-    B = table.shape[0]
-    for t, dt, shape in ((cache.k, torch.int8, cache.k.shape), (cache.v, torch.int8, cache.k.shape), (cache.k_scale, torch.float32, (pages, Hkv)),
-                         (cache.v_scale, torch.float32, (pages, Hkv)), (table, torch.int32, table.shape), (lengths, torch.int32, (B,))):
-        if t.dtype != dt or t.shape != shape or not t.is_contiguous():
-            raise ValueError("expected int8 [pages, Hkv, T, D], f32 [pages, Hkv], an int32 table [B, pages to a sequence] and int32 lengths [B]")
-    with torch.cuda.device(cache.k.device):
-        k, v = (torch.empty((B, rows, Hkv, D), dtype=dtype, device=cache.k.device) for _ in range(2))
-        ok(_lib().gpu_kv8_dequant(_DT[dtype], _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(table), table.shape[1],
-                                  _ptr(lengths), _ptr(k), _ptr(v), B, rows, Hkv, D, T, pages, table.shape[1], _stream()), "gpu_kv8_dequant")
-    return k, v
+    return _h.kv8_dequant(cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths, rows, dtype)
 
 
 def kv8_attention(q: torch.Tensor, cache: Kv8Cache, table: torch.Tensor, lengths: torch.Tensor, *, q_len: Optional[torch.Tensor] = None,
@@ -72,4 +64,4 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, table: torch.Tensor, lengths
     multiple of the cache's heads. The first q_len[b] (all L without) rows of q are the sequence's last tokens: causal, row i sees
     tokens up to lengths[b] - q_len[b] + i. Rows from q_len[b] on are not written; a row that sees no token gets zeros."""
     return _h.kv8_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, lengths, q_len, 1 if causal else 0,
-                            q.shape[-1] ** -0.5 if scale is None else scale, out)
+                            _scale(q, scale), out)

@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t umma_desc_lo_n_major(uint32_t addr) { return
 struct TcParams {
     AttnParams a;
     int q_tiles;             // pairs of tiles: 256 rows
-    int64_t items;
+    uint32_t items;
     int kv_batch, kv_head;   // 0: the batch's (the heads') keys and values are one
     int q_batch, q_head;
 };
@@ -76,15 +76,15 @@ struct Item {
 };
 // The item of a CTA's r-th round: the rounds run through the CTAs forwards and backwards in turn, so that where the items get smaller, as the
 // cache's do, the sums of a CTA's items come out alike.
-__device__ __forceinline__ int64_t item_of(int r) { return (int64_t)r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
-template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, int64_t i, const int* order) {
+__device__ __forceinline__ uint32_t item_of(uint32_t r) { return r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
+template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, uint32_t i, const int* order) {
     Item x;
-    const int heads = KV8 ? p.a.Hkv : p.a.H;
+    const uint32_t heads = KV8 ? p.a.Hkv : p.a.H;
     // Heads next to one another: together they read and write whole rows of Q and of the result. Cache: long sequences first, of each the
     // tiles with most keys.
-    const int rest = (int)(i / heads), b = rest / p.q_tiles, qt = rest - b * p.q_tiles;
-    x.h = (int)(i - (int64_t)rest * heads);
-    x.b = KV8 && p.a.B <= 32 ? order[b] : b, x.row0 = (KV8 ? p.q_tiles - 1 - qt : qt) * 256;
+    const uint32_t rest = i / heads, b = rest / (uint32_t)p.q_tiles, qt = rest - b * p.q_tiles;
+    x.h = (int)(i - rest * heads);
+    x.b = KV8 && p.a.B <= 32 ? order[b] : (int)b, x.row0 = (int)(KV8 ? p.q_tiles - 1 - qt : qt) * 256;
     x.len = p.a.kv_len ? min(max(gload(p.a.kv_len + x.b), 0), p.a.Lkv) : p.a.Lkv;
     x.ql = p.a.Lq;
     x.seen = x.len;
@@ -158,7 +158,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint8_t* stage = sm + L::kStaging + warp * 2048;
         uint32_t s_phase = 0, tile_no = 0, item_no = 0;
         bool ok = true;
-        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+        for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n > 0 && t * 128 >= x.rows) {
                 tile_no += x.n, ++item_no;
@@ -325,7 +325,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             umma_commit(s_full + 8 * t);
             mbar_arrive(s_full + 8 * t);
         };
-        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+        for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
@@ -393,7 +393,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
-        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+        for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1, kvh = x.h / (p.a.H / p.a.Hkv);
@@ -451,7 +451,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         // ---- rows of V behind keys that are not seen: zeros. Two warps, 16 lanes (8 with 64 columns) to a row.
         uint32_t kv_no = 1, tile_no = 0;
         bool ok = true;
-        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+        for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             for (int j = 0; j < x.n; ++j, ++tile_no, kv_no += 2) {
                 const uint32_t slot = kv_no & 3;
@@ -477,7 +477,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint8_t* stage = sm + L::kStaging + quarter * 4096;
         uint32_t phase[2] = {}, item_no = 0;
         bool ok = true;
-        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+        for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             for (int t = 0; t < 2 && t * 128 < x.rows; ++t) {
                 float inv = 0.f;
@@ -545,7 +545,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             *reinterpret_cast<uint4*>(tile + (piece >> 3) * kBox + row * 128 + ((piece ^ row) & 7) * 16) = v;
         };
         const int ratio = p.a.H / p.a.Hkv;
-        for (int r = 0; item_of(r) < p.items && ok; ++r) {
+        for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
@@ -683,13 +683,14 @@ template <typename QT, int DP, bool KV8> int launch_tc(const CUtensorMap (&tm)[3
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
     const int sms = sm_count();
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
-    return launch_pdl(kern, dim3((unsigned)(p.items < sms ? p.items : sms)), L::kThreads, L::kSmem, st, tm[0], tm[1], tm[2], p);
+    return launch_pdl(kern, dim3(p.items < (uint32_t)sms ? p.items : (uint32_t)sms), L::kThreads, L::kSmem, st, tm[0], tm[1], tm[2], p);
 }
 
 }  // namespace
 
 bool b200q::attention_tc_takes(const AttnParams& p, bool kv8) {
-    if (p.D > 128 || !(p.scale > 0.f) || p.Lkv <= 0) return false;
+    // (the rows' way out waits for a whole item: at 2^26 keys that is half of a wait's limit)
+    if (p.D > 128 || !(p.scale > 0.f) || p.Lkv <= 0 || p.Lkv > 1 << 26) return false;
     // Half an item's rows at least, and enough tiles of 64 rows: with fewer the other kernels, which share a row tile's keys among CTAs, are
     // done sooner. Over the cache, 8 sequences of 1000 to 8000 tokens and 128 rows for each of 8 kv heads (128 tiles): 219 us here, 124 with 16 rows at
     // a time; one sequence of 8000 and 256 rows: 232 and 63; two of up to 4133 and 4096 rows (1024 tiles): 151 here.
@@ -704,8 +705,9 @@ int b200q::attention_tc(int dtype, bool kv8, AttnParams& a, cudaStream_t st) {
     TcParams p = {};
     p.a = a;
     const int64_t rows = kv8 ? (int64_t)a.Lq * (a.H / a.Hkv) : a.Lq, tiles = (rows + 255) / 256;
-    if (rows > INT32_MAX - 512) return -1;
-    p.q_tiles = (int)tiles, p.items = tiles * a.B * (kv8 ? a.Hkv : a.H);
+    const int heads = kv8 ? a.Hkv : a.H;
+    if (rows > INT32_MAX - 512 || tiles > INT32_MAX / 2 / a.B / heads) return -1;
+    p.q_tiles = (int)tiles, p.items = (uint32_t)(tiles * a.B * heads);
     p.q_batch = a.qs[0] != 0, p.q_head = a.qs[2] != 0, p.kv_batch = a.ks[0] != 0, p.kv_head = a.ks[2] != 0;
     CUtensorMap tm[3] = {};
     if (!kv8 && (!make_rows_map(&tm[0], a.q, a.qs, a.B, a.Lq, a.H, a.D) || !make_rows_map(&tm[1], a.k, a.ks, a.B, a.Lkv, a.Hkv, a.D) ||

@@ -354,6 +354,21 @@ FAST(kv8_append, 9)
                          small(table.size(1)), stream());
     Py_RETURN_NONE;
 END
+// cache (4), table, lengths, rows, dtype
+FAST(kv8_dequant, 8)
+    const Cache c(a);
+    const at::Tensor &table = ten(a[4]), &len = ten(a[5]);
+    const On on(c.k);
+    on.same({&c.v, &c.ks, &c.vs, &table, &len});
+    const int64_t B = table.size(0), rows = integer(a[6]);
+    check_table(table, B);
+    check(plain(len, at::kInt, {B}) && rows >= 0, "lengths is int32 [B], rows at least 0");
+    const auto opts = at::TensorOptions().dtype(out_dtype(a[7])).device(c.k.device());
+    at::Tensor k = at::empty({B, rows, c.Hkv, c.D}, opts), v = at::empty({B, rows, c.Hkv, c.D}, opts);
+    CALL(gpu_kv8_dequant, dtype_code(k), ptr<int8_t>(c.k), ptr<int8_t>(c.v), ptr<float>(c.ks), ptr<float>(c.vs), ptr<int32_t>(table), table_stride(table),
+                          ptr<int32_t>(len), ptr(k), ptr(v), small(B), rows, small(c.Hkv), small(c.D), small(c.T), c.pages, small(table.size(1)), stream());
+    return pair(nullptr, k, nullptr, v);
+END
 // cache (4), q, table, lengths, q_len, causal, scale, out
 FAST(kv8_attention, 11)
     const Cache c(a);
@@ -380,7 +395,7 @@ END
 #define M(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {M(quant_rows), M(sd_quant_rows), M(sd_ln_quant_rows), M(sd_geglu_quant_rows), M(sd_group_norm_quant_rows),
                          M(sd_unpad_quant_rows), M(int8_gemm), M(int8_gemm_act_rot), M(quant_rows_rotated), M(w6a8_gemm),
-                         M(w4_linear), M(cross_attention), M(kv8_append), M(kv8_attention),
+                         M(w4_linear), M(cross_attention), M(kv8_append), M(kv8_dequant), M(kv8_attention),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
