@@ -196,14 +196,15 @@ template <int XT, bool G32, bool WIDE> __global__ void __launch_bounds__(512, 1)
 #pragma unroll
             for (int b = 0; b < kRing; ++b) request(b);
             const int64_t zero_row = (int64_t)n * w.groups;
-            // f32: four pieces of eight columns a lane, sixteen tokens a warp, requested a block ahead
+            // f32: a piece of eight columns of every sixteen tokens a lane, requested a block ahead
             float4 raw[XT == DT_F32 ? 8 : 1];
             auto request_x = [&](int b) {
                 if constexpr (XT == DT_F32) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int t = mw * 16 + u * 4 + (lane >> 3), k = (first + b) * kBlock + (lane & 7) * 8;
-                        const bool valid = b < count && t < p.tokens && m0 + t < w.M && k < w.K;
+                        if (u * 16 >= p.tokens) break;      // tokens of a tile come in sixteens
+                        const int t = u * 16 + mw * 4 + (lane >> 3), k = (first + b) * kBlock + (lane & 7) * 8;
+                        const bool valid = b < count && m0 + t < w.M && k < w.K;
                         const float* x = reinterpret_cast<const float*>(w.x) + (int64_t)(m0 + t) * w.x_stride + k;
                         raw[2 * u] = valid ? gload(reinterpret_cast<const float4*>(x)) : make_float4(0.f, 0.f, 0.f, 0.f);
                         raw[2 * u + 1] = valid ? gload(reinterpret_cast<const float4*>(x) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -251,13 +252,13 @@ template <int XT, bool G32, bool WIDE> __global__ void __launch_bounds__(512, 1)
                     uint8_t* xs = sm + stage * stage_size + kABytes;
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int t = mw * 16 + u * 4 + (lane >> 3);
+                        if (u * 16 >= p.tokens) break;
+                        const int t = u * 16 + mw * 4 + (lane >> 3);
                         uint4 v[3];
                         split2(raw[2 * u].x, raw[2 * u].y, v, 0), split2(raw[2 * u].z, raw[2 * u].w, v, 1);
                         split2(raw[2 * u + 1].x, raw[2 * u + 1].y, v, 2), split2(raw[2 * u + 1].z, raw[2 * u + 1].w, v, 3);
-                        if (t < p.tokens)
 #pragma unroll
-                            for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(xs + (t * 3 + q) * 128 + ((lane ^ (t * 3 + q)) & 7) * 16) = v[q];
+                        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(xs + (t * 3 + q) * 128 + ((lane ^ (t * 3 + q)) & 7) * 16) = v[q];
                     }
                     request_x(b + 1);
                 }
