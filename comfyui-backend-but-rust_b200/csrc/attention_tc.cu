@@ -5,13 +5,18 @@
 // operand from tensor memory. While the softmax warps of one query tile work, the tensor cores multiply for the other. Tensor memory: S of
 // both tiles in columns 0..255, O in 256..511.
 //
-// Warps 0-3 and 4-7: softmax and the rows' way out, for the two tiles. Warp 8 issues the products (one thread), in the order S0 S1 | O0 S0'
-// O1 S1' | ..., in which the tensor cores execute them: S' of the next key tile overwrites p only behind the product that read it. Warp 9
-// loads 16-bit Q, K and V by TMA; for the int8 cache warps 12-15 load codes, turn them into halves and write them as TMA would.
+// Warps 0-3 and 4-7: softmax of the two tiles, over the cache also their rows' way out. Warp 8 issues the products (one thread), in the order
+// S0 S1 | O0 S0' O1 S1' | ..., in which the tensor cores execute them: S' of the next key tile overwrites p only behind the product that read
+// it; the product of the first half of the keys starts when half of p is there. 16-bit keys: warp 9 loads Q, K and V by TMA, warps 10 and 11
+// clear hidden rows of V, warps 12-15 carry the rows out (by the softmax warps that took 181 us instead of 131 at 16384 x 512 x 24 heads of
+// 128). Cache: warps 12-15 load codes, turn them into halves and write them as TMA would; what they request they take up a step later.
 // m follows the running maximum only when that has grown by 2^8: until then p is at most 256 and the sums need no rescaling; O is then scaled
 // in tensor memory by the row's own thread, which nothing else touches between the two products of its tile.
 // Keys that are not seen get p = 0; what V holds there (16-bit V comes as it lies in memory, NaN perhaps) is overwritten with zeros in shared
 // memory before the product.
+// Measured: 1.83 us a step of 256 rows, 128 keys and 128 columns (the products 1.1 at the tensor rate, the exponentials as much: 16 a cycle);
+// 2048 keys 1210 TFLOP/s, 512 keys 920 (787 with a mask, new inputs each time), 128 keys at the pace of the rows' way in and out. Over the
+// cache, chunks of 1024 tokens 465 TFLOP/s.
 // Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds.
 #include "attention.cuh"
 #include "umma16.cuh"

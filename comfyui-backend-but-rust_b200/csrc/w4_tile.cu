@@ -9,6 +9,9 @@
 // Warps 0-3 and 4-7: sums, for the first and second half of the columns. Warps 8-11: codes from global memory (each its 32 rows, a ring of its
 // own) to operands, K-major with the 128-byte swizzle, a row to a lane; for f32 x also its three terms. Warp 12 issues the products, warp 13
 // loads 16-bit x by TMA.
+// Measured: 333 x 5120 -> 13824 fp16, groups of 64, 142 us (332 TFLOP/s); 64 x 5120 -> 13824 bf16, groups of 128, 39; 512 x 2560 -> 19456 f32 379. A block of 64
+// of K takes 0.6 to 0.7 us whatever the columns: a group's way from the end of its product to the next one's start, through a warp's wait, its
+// reads of tensor memory and its arrival, is what bounds it.
 // Every wait is bounded; one that runs out is recorded in g_w4_status and the CTA unwinds.
 #include "umma16.cuh"
 #include "w4.cuh"

@@ -392,6 +392,78 @@ def test_replayed_from_a_graph_with_longer_sequences(pkg, dev):
     assert all(torch.equal(A.kv8_attention(q, c, table, lens), out) for _ in range(3))
 
 
+def test_pages_beyond_32_bits(pkg, dev):
+    """A cache of more than 2^31 bytes of keys, with sequences on its last pages: written, read back, attended to by few rows and by many."""
+    A = pkg.attention
+    g = torch.Generator().manual_seed(13)
+    pages, Hkv, D, T = 17000, 8, 128, 128
+    c = A.Kv8Cache.empty(pages, Hkv, D, T, dev)
+    table = torch.tensor([[pages - 1, 0, pages - 2], [pages - 5, pages - 3, 1]], dtype=torch.int32, device=dev)
+    k, v = (torch.randn(2, 300, Hkv, D, generator=g).half().to(dev) for _ in range(2))
+    start = torch.zeros(2, dtype=torch.int32, device=dev)
+    n = torch.tensor([300, 290], dtype=torch.int32, device=dev)
+    A.kv8_append(c, k, v, table, start, n)
+    back, _ = A.kv8_dequant(c, table, n, 300)
+    for b, m in enumerate(n.tolist()):
+        step = c.k_scale[table[b].long()].repeat_interleave(T, 0)[:m, :, None]
+        assert bool(((back[b, :m] - k[b, :m].float()).abs() <= step * 0.5001).all())
+    for L, H in ((1, 32), (200, 16), (260, 32)):
+        q = torch.randn(2, L, H, D, generator=g).half().to(dev)
+        _kv8_check(A.kv8_attention(q, c, table, n), q, c, table, [300, 290], [L, L], True, D ** -0.5)
+
+
+@pytest.mark.parametrize("Lq", [1, 40, 600])
+def test_two_streams_at_once_and_ordinary_launches(pkg, dev, Lq):
+    """Nothing is shared between calls: two at a time give what one gives. Beside a collective's kernels launches are ordinary ones."""
+    A, L = pkg.attention, pkg.linear
+    g = torch.Generator().manual_seed(Lq)
+    c, table = _cache(pkg, dev, g, 2, [900, 700], 8, 64, 32)
+    n = torch.tensor([900, 700], dtype=torch.int32, device=dev)
+    q = torch.randn(2, Lq, 16, 64, generator=g).half().to(dev)
+    kv = torch.randn(2, 150, 8, 64, generator=g).half().to(dev)
+    calls = (lambda out: A.kv8_attention(q, c, table, n, out=out), lambda out: A.cross_attention(q, kv, kv, out=out))
+    want = [call(torch.zeros_like(q)) for call in calls]
+    outs, streams = [torch.zeros_like(q) for _ in range(8)], [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        with torch.cuda.stream(streams[i % 2]):
+            calls[i // 2 % 2](out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i // 2 % 2]) for i, out in enumerate(outs))
+    was = L.set_gemm_cluster_limit(4)
+    try:
+        assert all(torch.equal(call(torch.zeros_like(q)), w) for call, w in zip(calls, want))
+    finally:
+        L.set_gemm_cluster_limit(was)
+    assert L.kernel_status() == 0
+
+
+@pytest.mark.parametrize("Lq", [2, 300])
+def test_pages_shared_by_sequences(pkg, dev, Lq):
+    """Two sequences with the same first pages (a prefix), and one with a page twice: attention only reads them."""
+    g = torch.Generator().manual_seed(Lq)
+    c, table = _cache(pkg, dev, g, 3, [400], 12, 64, 32)
+    table[1, :5], table[2, 3] = table[0, :5], table[2, 0]
+    q = torch.randn(3, Lq, 24, 64, generator=g).bfloat16().to(dev)
+    lens = [400, 390, 333]
+    _kv8_check(pkg.attention.kv8_attention(q, c, table, torch.tensor(lens, dtype=torch.int32, device=dev)), q, c, table, lens, [Lq] * 3, True, 64 ** -0.5)
+
+
+def test_rows_beyond_the_last_and_zero_sizes(pkg, dev):
+    """No pages at all, no tokens, a negative length: zeros, or nothing written."""
+    A = pkg.attention
+    c = A.Kv8Cache.empty(0, 2, 64, 16, dev)
+    table, n = torch.zeros(2, 0, dtype=torch.int32, device=dev), torch.tensor([5, -3], dtype=torch.int32, device=dev)
+    for Lq in (1, 300):
+        q = torch.randn(2, Lq, 32, 64, device=dev).half()
+        assert bool((A.kv8_attention(q, c, table, n) == 0).all())
+    kv = torch.randn(2, 4, 2, 64, device=dev).half()
+    A.kv8_append(c, kv, kv, table, n)
+    k, v = A.kv8_dequant(c, table, n, 7, dtype=torch.bfloat16)
+    assert k.shape == (2, 7, 2, 64) and bool((k == 0).all()) and bool((v == 0).all())
+    assert A.kv8_dequant(c, table, n, 0)[0].shape == (2, 0, 2, 64)
+
+
 def test_refusals(pkg, dev):
     A = pkg.attention
     q = torch.zeros(2, 3, 4, 64, device=dev).half()

@@ -45,7 +45,9 @@ def _check(got, x, w, bias, base):
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("M,N,K,G", [(1, 1, 32, 32), (1, 16, 128, 128), (1, 2563, 2560, 128), (2, 40, 96, 32), (3, 1000, 9728, 32), (4, 17, 64, 64),
                                      (5, 513, 4096 + 64, 64), (7, 130, 1024, 256), (8, 19456, 256, 64), (9, 33, 160, 32), (16, 257, 768, 128),
-                                     (17, 129, 192, 64), (63, 127, 288, 32), (65, 640, 1280, 128), (129, 300, 512, 256), (333, 1030, 1024, 64)])
+                                     (17, 129, 192, 64), (63, 127, 288, 32), (65, 640, 1280, 128), (129, 300, 512, 256), (333, 1030, 1024, 64),
+                                     # several tiles to a CTA; a tile to a cluster; columns that make tiles wide and narrow
+                                     (333, 13829, 320, 64), (300, 9000, 288, 32), (70, 200, 8192, 256), (40, 100, 4160, 64), (193, 2050, 640, 128), (12, 3000, 96, 32)])
 def test_linear(pkg, dev, M, N, K, G, dtype):
     g = torch.Generator().manual_seed(M * 7 + N + K)
     dt = DT[dtype]
@@ -217,6 +219,43 @@ def test_replayed_from_a_graph_and_on_another_stream(pkg, dev):
             side.synchronize()
         assert torch.equal(out, eager)
         assert all(torch.equal(pkg.linear.w4_linear(x, packed, scales, z), eager) for _ in range(3))      # the same bits every time
+
+
+@pytest.mark.parametrize("M", [1, 11, 40, 200])
+def test_two_streams_at_once_and_ordinary_launches(pkg, dev, M):
+    """Nothing is shared between calls: two at a time give what one gives. Beside a collective's kernels launches are ordinary ones."""
+    g = torch.Generator().manual_seed(M)
+    L = pkg.linear
+    packed, scales, z = _weight(g, dev, 1500, 2048, 64)
+    for dt in DT.values():
+        x = torch.randn(M, 2048, generator=g).to(dt).to(dev)
+        want = L.w4_linear(x, packed, scales, z)
+        outs, streams = [torch.empty_like(want) for _ in range(8)], [torch.cuda.Stream(dev) for _ in range(2)]
+        torch.cuda.synchronize()
+        for i, out in enumerate(outs):
+            with torch.cuda.stream(streams[i % 2]):
+                L.w4_linear(x, packed, scales, z, out=out)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out in outs)
+        was = L.set_gemm_cluster_limit(4)
+        try:
+            assert torch.equal(L.w4_linear(x, packed, scales, z), want)
+        finally:
+            L.set_gemm_cluster_limit(was)
+    assert L.kernel_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_offsets_beyond_32_bits(pkg, dev, M):
+    """A packed weight of more than 2^31 bytes: rows at its beginning and its end."""
+    N, K, G = 66000, 65536, 256
+    gen = torch.Generator(device=dev).manual_seed(M)
+    packed = torch.empty((N, K // 2), dtype=torch.uint8, device=dev).random_(0, 256, generator=gen)
+    scales = (torch.rand(N, K // G, generator=gen, device=dev) * 0.01 + 1e-3).half()
+    x = torch.randn(M, K, generator=gen, device=dev).bfloat16()
+    y = pkg.linear.w4_linear(x, packed, scales, out_dtype=torch.float32)
+    rows = torch.cat([torch.arange(3), torch.arange(N - 200, N, 7)]).to(dev)
+    _check(y[:, rows], x, _unpack(packed[rows], scales[rows], None), None, None)
 
 
 def test_refusals(pkg, dev):
