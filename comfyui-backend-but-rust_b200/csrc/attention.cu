@@ -177,6 +177,7 @@ template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
     auto kern = attention_tile_kernel<T, DP>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
     const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + kRows - 1) / kRows, base = tiles * p.B * p.Hkv;
+    if (rows > INT32_MAX - kRows) return -1;
     p.row_tiles = (int)tiles;
     // CTAs to a row tile: as long as the device has room for twice as many and each keeps 256 keys
     p.splits = 1;
@@ -504,6 +505,7 @@ template <typename QT, int DP> int launch_rows(AttnParams& p, cudaStream_t st) {
     auto kern = kv8_rows_kernel<QT, DP>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kSmem)) return (int)e;
     const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + 15) / 16, base = tiles * p.B * p.Hkv;
+    if (rows > INT32_MAX - 16) return -1;
     p.row_tiles = (int)tiles;
     // CTAs along the keys: as long as there are fewer than one to an SM (two where sequences of different lengths leave some idle) and each has
     // a block for each warp. CTAs begin and end slowly: 16 sequences of up to 32768 tokens, 8 kv heads, 2 | 4 | 8 CTAs 182 | 120 | 156 us; 8 of up to

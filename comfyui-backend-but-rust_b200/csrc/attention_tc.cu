@@ -40,7 +40,7 @@ template <int DP, bool KV8> struct Tc {
     static constexpr int kThreads = 512;
     // Registers of the warpgroups (softmax twice, products and loads, codes or rows out): a softmax thread holds a row of 128 logits. Their
     // sum over the threads is what the launch has, 512 x 128.
-    static constexpr int kSoftmaxRegs = KV8 ? 176 : 184, kIssueRegs = KV8 ? 48 : 56, kLastRegs = KV8 ? 112 : 88;
+    static constexpr int kSoftmaxRegs = 184, kIssueRegs = KV8 ? 40 : 56, kLastRegs = KV8 ? 104 : 88;
     static_assert(2 * kSoftmaxRegs + kIssueRegs + kLastRegs == 4 * 128, "register split");
 };
 
@@ -698,7 +698,7 @@ bool b200q::attention_tc_takes(const AttnParams& p, bool kv8) {
     if (p.D > 128 || !(p.scale > 0.f) || p.Lkv <= 0 || p.Lkv > 1 << 26) return false;
     // Half an item's rows at least, and enough tiles of 64 rows: with fewer the other kernels, which share a row tile's keys among CTAs, are
     // done sooner. Over the cache, 8 sequences of 1000 to 8000 tokens and 128 rows for each of 8 kv heads (128 tiles): 219 us here, 124 with 16 rows at
-    // a time; one sequence of 8000 and 256 rows: 232 and 63; two of up to 4133 and 4096 rows (1024 tiles): 151 here.
+    // a time; one sequence of 8000 and 256 rows: 232 and 63; two of up to 4133 and 4096 rows (1024 tiles): 148 here.
     const int64_t rows = kv8 ? (int64_t)p.Lq * (p.H / p.Hkv) : p.Lq;
     if (rows < 128 || (rows + 63) / 64 * p.B * (kv8 ? p.Hkv : p.H) < (kv8 ? 160 : 64)) return false;
     // rows without a stride between them have no tensor map

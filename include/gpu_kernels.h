@@ -226,7 +226,8 @@ int gpu_embed_dequant(const int8_t* q, const float* s, float* out, int M, int K,
  * gpu_w4_linear    out[m,n] = beta * out[m,n] + sum_k x[m,k] W[n,k] + bias[n], beta 0 or 1 (-207). x [M, K] f32, f16 or bf16, out [M, N]
  *                  in x's type or f32, bias [N] in out's type or NULL. Codes and x enter the products exactly (an f32 x as three
  *                  bf16 terms), sums are f32, one rounding to out's type. M from one token up; out must not overlap x.
- * Errors: -4 types, -5 a NULL, a row of x or w, or Wq4 off a 16-byte boundary, packed of the packer off 8, out of gpu_w4_dequant off 32 bytes. */
+ * Errors: -4 types, -5 a NULL, a row of x or w, or Wq4 off a 16-byte boundary, packed of the packer off 8, out of gpu_w4_dequant off 32 bytes,
+ * -203 descriptor (x of many tokens). */
 int gpu_w4_requant(int dtype, const void* w, int64_t w_stride, void* packed, int scale_dt, void* scales, void* zeros, int64_t N,
                    int K, int G, void* stream);
 int gpu_w4_dequant(int dtype, const void* packed, int scale_dt, const void* scales, const void* zeros, void* out, int64_t N, int K,
@@ -250,7 +251,7 @@ int gpu_w4_linear(int dtype, const void* x, int64_t x_stride, const void* Wq4, i
  *                    tokens < lengths[b]. Rows i < q_len[b] (NULL: Lq) are the sequence's last tokens: with causal != 0 row i sees
  *                    tokens <= lengths[b] - q_len[b] + i. Rows from q_len[b] on are not written; a row that sees no token is zeros.
  *                    Needs no workspace. bf16 queries are taken as fp16 times a power of two per row (values below 2^-29 of their row's largest lose bits).
- * Errors: -1 sizes, -4 types, -5 a NULL or rows off a 16-byte boundary (strides in whole 16 bytes; gpu_kv8_dequant's k and v: 32). */
+ * Errors: -1 sizes, -4 types, -5 a NULL or rows off a 16-byte boundary (strides in whole 16 bytes; gpu_kv8_dequant's k and v: 32), -203 descriptor. */
 int gpu_kv8_append(int dtype, const void* k, const void* v, const int64_t* strides, int8_t* k8, int8_t* v8, float* k_scale,
                    float* v_scale, const int32_t* table, int64_t table_stride, const int32_t* start, const int32_t* count, int B, int L,
                    int Hkv, int D, int T, int64_t pages, int max_pages, void* stream);
