@@ -7,7 +7,7 @@
 //
 // Warps 0-3 and 4-7: softmax of the two tiles, over the cache also their rows' way out. Warp 8 issues the products (one thread), in the order
 // S0 S1 | O0 S0' O1 S1' | ..., in which the tensor cores execute them: S' of the next key tile overwrites p only behind the product that read
-// it; the product of the first half of the keys starts when half of p is there. 16-bit keys: warp 9 loads Q, K and V by TMA, warps 10 and 11
+// it; the product of the first three quarters of the keys (half, with 64 columns) starts when their p is there. 16-bit keys: warp 9 loads Q, K and V by TMA, warps 10 and 11
 // clear hidden rows of V, warps 12-15 carry the rows out (by the softmax warps that took 181 us instead of 131 at 16384 x 512 x 24 heads of
 // 128). Cache: warps 12-15 load codes, turn them into halves and write them as TMA would; what they request they take up a step later.
 // m follows the running maximum only when that has grown by 2^8: until then p is at most 256 and the sums need no rescaling; O is then scaled
@@ -15,8 +15,8 @@
 // Keys that are not seen get p = 0; what V holds there (16-bit V comes as it lies in memory, NaN perhaps) is overwritten with zeros in shared
 // memory before the product.
 // Measured: 1.83 us a step of 256 rows, 128 keys and 128 columns (the products 1.1 at the tensor rate, the exponentials as much: 16 a cycle);
-// 2048 keys 1210 TFLOP/s, 512 keys 920 (787 with a mask, new inputs each time), 128 keys at the pace of the rows' way in and out. Over the
-// cache, chunks of 1024 tokens 465 TFLOP/s.
+// 2048 keys 1210 TFLOP/s, 512 keys 955 (806 with a mask, new inputs each time), 128 keys at the pace of the rows' way in and out. Over the
+// cache, chunks of 1024 tokens 478 TFLOP/s.
 // Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds.
 #include "attention.cuh"
 #include "umma16.cuh"
@@ -38,6 +38,9 @@ template <int DP, bool KV8> struct Tc {
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
     static constexpr int kOrder = kRowInfo + 2048, kEnd = kOrder + 128, kSmem = kEnd + 1024;
     static constexpr int kThreads = 512;
+    // Quarters of a key tile whose products with V start before the softmax has the rest: what is left of them stands between it and the next
+    // logits, which take p's place. 16384 rows, 2048 keys, 128 columns, two | three: 357 | 349 us; 4096 x 4096, 64 columns: 165 | 166.
+    static constexpr int kEarly = DP > 64 ? 3 : 2;
     // Registers of the warpgroups (softmax twice, products and loads, codes or rows out): a softmax thread holds a row of 128 logits. Their
     // sum over the threads is what the launch has, 512 x 128.
     static constexpr int kSoftmaxRegs = 184, kIssueRegs = KV8 ? 40 : 56, kLastRegs = KV8 ? 104 : 88;
@@ -115,7 +118,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t bars = base + L::kTail;
     const uint32_t kv_full = bars, kv_empty = bars + 32, q_full = bars + 64, q_empty = bars + 80, s_full = bars + 96, p_full = bars + 112,
-                   o_full = bars + 128, o_empty = bars + 144, p_half = bars + 160, v_ready = bars + 176;
+                   o_full = bars + 128, o_empty = bars + 144, p_early = bars + 160, v_ready = bars + 176;
     uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
     uint32_t* words = reinterpret_cast<uint32_t*>(sm + L::kWords);            // [key tile % 4][4]: bit = key is seen
@@ -125,7 +128,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
         for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
-            mbar_init(o_full + 8 * t, 5), mbar_init(o_empty + 8 * t, 4), mbar_init(p_half + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
+            mbar_init(o_full + 8 * t, 5), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
         *abort_s = 0;
         fence_mbar_init();
         if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
@@ -254,11 +257,11 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         out[e >> 1] = pack2<T>(a, b);
                     }
                     tmem_st16(s_at + q * 16, out);
-                    if (q & 1) {      // the products of half the keys start while the other half is on its way
+                    if (q == L::kEarly - 1 || q == 3) {
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive((q == 1 ? p_half : p_full) + 8 * t);
+                        if (lane == 0) mbar_arrive((q < 3 ? p_early : p_full) + 8 * t);
                     }
                 }
                 float even, odd;
@@ -356,7 +359,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (!KV8 && !wait(v_ready + 8 * (vs >> 1), v_no >> 2 & 1, ST_TIMEOUT_UNPACK)) break;
                 ks = (kv_no + 2) & 3, k_phase = (kv_no + 2) >> 2 & 1;
                 for (int t = 0; t < tiles; ++t) {
-                    if (!wait(p_half + 8 * t, p_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
+                    if (!wait(p_early + 8 * t, p_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
                     if (!KV8 && j == 0) {      // the rows before have left O
                         if (!wait(o_empty + 8 * t, o_phase[t], ST_TIMEOUT_TMEM_EMPTY)) break;
                         o_phase[t] ^= 1;
@@ -365,7 +368,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     tc_fence_after();
                     if (one) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)      // 16 keys: 8 columns of p, two swizzle atoms of V
+                        for (int kk = 0; kk < 2 * L::kEarly; ++kk)      // 16 keys: 8 columns of p, two swizzle atoms of V
                             umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, j > 0 || kk > 0);
                     }
                     __syncwarp();
@@ -375,7 +378,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     tc_fence_after();
                     if (one) {
 #pragma unroll
-                        for (int kk = 4; kk < 8; ++kk) umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, 1);
+                        for (int kk = 2 * L::kEarly; kk < 8; ++kk) umma_16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * (2048 >> 4), idesc_o, 1);
                         if (more) {
                             issue_s(t, ks);
                             if (j + 2 == x.n) umma_commit(q_empty + 8 * t);
