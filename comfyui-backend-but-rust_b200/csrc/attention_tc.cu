@@ -14,6 +14,10 @@
 // in tensor memory by the row's own thread, which nothing else touches between the two products of its tile.
 // Keys that are not seen get p = 0; what V holds there (16-bit V comes as it lies in memory, NaN perhaps) is overwritten with zeros in shared
 // memory before the product.
+// Waits are by parity, so no barrier may complete twice before everybody who waits for the first completion has seen it, nor get an arrival meant
+// for the next. s_full is the tight one: an item's first logits are issued without a wait for the softmax warps, so "O is done" has a barrier of
+// its own (o_full). Between two completions of s_full there is the p_full that answers the first, between two of o_full an item's p_full.
+// tests/test_attention_order.py goes through the roles' orders.
 // Measured: 1.83 us a step of 256 rows, 128 keys and 128 columns (the products 1.1 at the tensor rate, the exponentials as much: 16 a cycle);
 // 2048 keys 1210 TFLOP/s, 512 keys 955 (806 with a mask, new inputs each time), 128 keys at the pace of the rows' way in and out. Over the
 // cache, chunks of 1024 tokens 478 TFLOP/s.
@@ -128,7 +132,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
         for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
-            mbar_init(o_full + 8 * t, 5), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
+            mbar_init(o_full + 8 * t, KV8 ? 1 : 5), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
         *abort_s = 0;
         fence_mbar_init();
         if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
@@ -164,7 +168,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
         const float c = p.a.scale * kLog2e;
         uint8_t* stage = sm + L::kStaging + warp * 2048;
-        uint32_t s_phase = 0, tile_no = 0, item_no = 0;
+        uint32_t s_phase = 0, o_phase = 0, tile_no = 0, item_no = 0;
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
@@ -277,8 +281,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             // ---- the rows out: 32 columns at a time through this warp's staging, so that a row's pieces are stored together
             if (x.n > 0) {
-                if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
-                s_phase ^= 1, ++item_no;
+                if (!__all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, o_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
+                o_phase ^= 1, ++item_no;
                 tc_fence_after();
             }
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -383,7 +387,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                             issue_s(t, ks);
                             if (j + 2 == x.n) umma_commit(q_empty + 8 * t);
                         }
-                        if (KV8 || more) ready(t);
+                        if (more) ready(t);
                         else umma_commit(o_full + 8 * t);
                     }
                     __syncwarp();

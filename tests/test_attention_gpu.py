@@ -210,6 +210,24 @@ def test_kv8_attention(pkg, dev, B, L, lens, H, Hkv, D, T, dtype):
     _kv8_check(got[:, L - min(q_lens):], q[:, L - min(q_lens):], c, table, lens, [min(q_lens)] * B, True, D ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("B,L,ratio,Hkv,D,T", [(20, 300, 1, 24, 64, 16), (23, 64, 2, 20, 128, 32), (40, 65, 2, 12, 96, 64), (12, 385, 1, 20, 16, 128)])
+def test_kv8_attention_with_several_items_to_a_cta(pkg, dev, B, L, ratio, Hkv, D, T, dtype):
+    """Three items and more to each SM's CTA, of one row tile, of two, and of both in turn: what one item leaves is not taken for the next one's."""
+    g = torch.Generator().manual_seed(B + L)
+    lens = [L + (37 * b) % 200 for b in range(B)]
+    lens[3] = 0
+    c, table = _cache(pkg, dev, g, B, lens, Hkv, D, T)
+    q = (torch.randn(B, L, Hkv * ratio, D, generator=g) * 1.5).to(DT[dtype]).to(dev)
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    assert -(-L * ratio // 256) * B * Hkv > 3 * torch.cuda.get_device_properties(dev).multi_processor_count
+    for causal in (True, False):
+        got = pkg.attention.kv8_attention(q, c, table, n, causal=causal)
+        _kv8_check(got, q, c, table, lens, [min(L, m) for m in lens], causal, D ** -0.5)
+        assert bool((got[3] == 0).all()) and all(torch.equal(pkg.attention.kv8_attention(q, c, table, n, causal=causal), got) for _ in range(3))
+    assert pkg.linear.kernel_status() == 0
+
+
 @pytest.mark.parametrize("size", [1e-20, 1e-4, 1.0, 3e4, 1e20])
 def test_bf16_queries_of_any_size(pkg, dev, size):
     """A row of queries is taken times a power of two: large and small ones are as good as others."""
