@@ -38,7 +38,7 @@ template <int DP, bool KV8> struct Tc {
     static constexpr int kTile = DP / 64 * kBox;                   // 128 rows of Q, K or V
     static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + (KV8 ? 8 * 2048 : 4 * 4096);
     // barriers and two words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
-    // item % 2: 1 / l of every row (16-bit), or bf16 queries' powers of two
+    // item of the tile % 2: 1 / l of every row (16-bit), or bf16 queries' powers of two
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
     static constexpr int kOrder = kRowInfo + 2048, kEnd = kOrder + 128, kSmem = kEnd + 1024;
     static constexpr int kThreads = 512;
@@ -128,7 +128,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     uint32_t* words = reinterpret_cast<uint32_t*>(sm + L::kWords);            // [key tile % 4][4]: bit = key is seen
     // [key tile % 4]: 16-bit: [key] +inf, or -inf where a key is not seen; cache: [factor, offset, weight][16 keys]
     float* info = reinterpret_cast<float*>(sm + L::kInfo);
-    float* row_info = reinterpret_cast<float*>(sm + L::kRowInfo);             // [item % 2][tile][row]
+    // [n % 2][tile][row]: of a tile's n-th item, counted by each tile for itself, since an item of at most 128 rows has no second tile. Written again
+    // for item n + 2 only behind what waited for item n's reader: 1 / l behind the logits of n + 2, which are issued behind the sums of n + 1, and those
+    // wait for o_empty of n, which the rows' way out gives when it has read; powers behind q_empty of n + 1, whose logits are issued behind p of n.
+    float* row_info = reinterpret_cast<float*>(sm + L::kRowInfo);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
         for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
@@ -173,7 +176,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
             if (x.n > 0 && t * 128 >= x.rows) {
-                tile_no += x.n, ++item_no;
+                tile_no += x.n;
                 continue;
             }
             if (x.rows <= 0 || (!KV8 && x.n == 0)) continue;
@@ -487,7 +490,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         fewer_registers<L::kLastRegs>();
         const int quarter = warp & 3;
         uint8_t* stage = sm + L::kStaging + quarter * 4096;
-        uint32_t phase[2] = {}, item_no = 0;
+        uint32_t phase[2] = {}, item_no[2] = {};
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
@@ -497,7 +500,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, phase[t], abort_s, ST_TIMEOUT_TMEM_FULL)))) break;
                     phase[t] ^= 1;
                     tc_fence_after();
-                    inv = row_info[(item_no & 1) * 256 + t * 128 + quarter * 32 + lane];
+                    inv = row_info[(item_no[t]++ & 1) * 256 + t * 128 + quarter * 32 + lane];
                 }
                 const int left = min(32, x.rows - t * 128 - quarter * 32);      // rows of this warp; none: nothing is stored
                 QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + (x.row0 + t * 128 + quarter * 32) * p.a.os[1] + x.h * p.a.os[2];
@@ -539,13 +542,12 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     __syncwarp();
                 }
             }
-            if (x.n > 0) ++item_no;
         }
     } else {
         fewer_registers<L::kLastRegs>();
         // ---- codes to halves: four warps of 32 keys (or query rows) each
         const int w = warp - 12;
-        uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0, item_no = 0;
+        uint32_t kv_no = 0, q_no[2] = {}, tile_no = 0;
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
         auto done = [&](uint32_t bar) {
@@ -563,7 +565,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             const int tiles = x.rows > 128 ? 2 : 1;
             for (int t = 0; t < tiles; ++t) {
                 if (!wait(q_empty + 8 * t, (q_no[t] & 1) ^ 1)) break;
-                ++q_no[t];
+                const uint32_t item_no = q_no[t]++;
                 constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes;        // lanes to a row, rows to an instruction
 #pragma unroll 4
                 for (int k = 0; k < 32 / kAtOnce; ++k) {
@@ -592,7 +594,6 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 }
                 done(q_full + 8 * t);
             }
-            ++item_no;
             // Nothing is waited for when it is requested: a tile's page indices two tiles ahead, its scales one, its codes (K and V) as soon as the
             // tile before has been converted.
             constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;

@@ -84,6 +84,23 @@ def test_cross_attention(pkg, dev, B, Lq, Lkv, H, Hkv, D, dtype):
             assert bool((got[1] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("B,Lq,Lkv,H,D", [(4, 1100, 77, 40, 64), (8, 300, 128, 40, 128), (16, 128, 33, 30, 80), (15, 385, 130, 16, 64)])
+def test_cross_attention_with_several_items_to_a_cta(pkg, dev, B, Lq, Lkv, H, D, dtype):
+    """Three items and more to each SM's CTA, among them items without a second tile of 128 rows, over one key tile and over two."""
+    g = torch.Generator().manual_seed(B + Lq)
+    q, k, v = (torch.randn(B, n, H, D, generator=g).to(DT[dtype]).to(dev) for n in (Lq, Lkv, Lkv))
+    assert -(-Lq // 256) * B * H > 3 * torch.cuda.get_device_properties(dev).multi_processor_count
+    kv_len = torch.randint(1, Lkv + 1, (B,), generator=g, dtype=torch.int32)
+    kv_len[1] = 0
+    kv_len = kv_len.to(dev)
+    for kw, seen in (({}, torch.ones(B, Lkv, dtype=torch.bool, device=dev)), ({"kv_len": kv_len}, torch.arange(Lkv, device=dev) < kv_len[:, None])):
+        got = pkg.attention.cross_attention(q, k, v, **kw)
+        _cross_check(got, q, k, v, seen, D ** -0.5)
+        assert all(torch.equal(pkg.attention.cross_attention(q, k, v, **kw), got) for _ in range(3))
+    assert pkg.linear.kernel_status() == 0
+
+
 @pytest.mark.parametrize("Lq", [3, 300])
 def test_strides_of_fused_projections(pkg, dev, Lq):
     """q, k and v as slices of wider projections, the result into one, heads before rows, one k and v for the whole batch."""

@@ -114,7 +114,6 @@ def _cache_form(items, own_o_full=True):
             for i, (tiles, n) in enumerate(items):
                 if t >= tiles:
                     tile_no += n
-                    mine += 1
                     continue
                 for j in range(n):
                     seen["s_full"] += 1
@@ -187,7 +186,7 @@ def _cache_form(items, own_o_full=True):
             for t in range(tiles):
                 ops.append(("wait", ("q_empty", t), q_no[t]))
                 q_no[t] += 1
-                ops += [mem.put(("power", i % 2, t, w), i), mem.put(("q", t), i), ("arrive", ("q_full", t))]
+                ops += [mem.put(("power", (q_no[t] - 1) % 2, t, w), i), mem.put(("q", t), i), ("arrive", ("q_full", t))]
             for j in range(n):
                 for kind in "kv":
                     ops.append(("wait", ("kv_empty", kv_no % 4), kv_no // 4))
@@ -197,6 +196,139 @@ def _cache_form(items, own_o_full=True):
                     kv_no += 1
                 tile_no += 1
         actors[f"operands {w}"] = ops
+    return actors, counts
+
+
+def _rows_form(items, slot_by_tile=True, with_p=False):
+    """Warps 0-7 softmax, 8 products, 9 loads, 10 and 11 hidden rows of V, 12-15 rows out."""
+    mem, queue = Memory(), []
+    counts = {**{("kv_full", s): 1 for s in range(4)}, **{("kv_empty", s): 1 for s in range(4)}}
+    for t in (0, 1):
+        counts.update({("q_full", t): 1, ("q_empty", t): 1, ("s_full", t): 2, ("p_early", t): WARPS, ("p_full", t): WARPS, ("o_full", t): 2 if with_p else WARPS + 1,
+                       ("o_empty", t): WARPS, ("v_ready", t): WARPS})
+    actors = {}
+    # ---- softmax, and 1 / l of its rows
+    for t in (0, 1):
+        for w in range(WARPS):
+            ops, s_seen, tile_no, mine = [], 0, 0, 0
+            for i, (tiles, n) in enumerate(items):
+                if t >= tiles:
+                    tile_no += n
+                    mine += not slot_by_tile
+                    continue
+                for j in range(n):
+                    s_seen += 1
+                    ops += [("wait", ("s_full", t), s_seen), mem.get(("info", tile_no % 4), tile_no), mem.get(("s", t), (i, j))]
+                    if j > 0:
+                        ops.append(mem.get(("o", t), (i, j - 1)))
+                    ops += [mem.put(("p early", t, w), (i, j)), ("arrive", ("p_early", t)), mem.put(("p", t, w), (i, j))]
+                    if with_p and j + 1 == n:
+                        ops.append(mem.put(("1 / l", mine % 2, t, w), i))
+                    ops.append(("arrive", ("p_full", t)))
+                    tile_no += 1
+                if not with_p:
+                    ops += [mem.put(("1 / l", mine % 2, t, w), i), ("arrive", ("o_full", t))]
+                mine += 1
+            actors[f"softmax {t}.{w}"] = ops
+    # ---- products
+    issue, seen = [], {}
+
+    def wait(bar):
+        seen[bar] = seen.get(bar, 0) + 1
+        issue.append(("wait", bar, seen[bar]))
+
+    def push(*ops):
+        for op in ops:
+            issue.append(("arrive", f"issued{len(queue)}"))
+            queue.append(op)
+
+    def issue_s(t, i, j, slot, tile):
+        push(mem.get(("q", t), i), mem.get(("ring", slot), ("k", tile)), mem.put(("s", t), (i, j)))
+
+    def ready(t):
+        push(("arrive", ("s_full", t)))
+        issue.append(("arrive", ("s_full", t)))
+    kv_no, tile_no, o_no = 0, 0, [0, 0]
+    for i, (tiles, n) in enumerate(items):
+        wait(("kv_full", kv_no % 4))
+        for t in range(tiles):
+            wait(("q_full", t))
+            issue_s(t, i, 0, kv_no % 4, tile_no)
+            if n == 1:
+                push(("arrive", ("q_empty", t)))
+            ready(t)
+        push(("arrive", ("kv_empty", kv_no % 4)))
+        for j in range(n):
+            vs, ks, more = (kv_no + 1) % 4, (kv_no + 2) % 4, j + 1 < n
+            wait(("kv_full", vs))
+            wait(("v_ready", vs // 2))
+            for t in range(tiles):
+                wait(("p_early", t))
+                if j == 0:
+                    issue.append(("wait", ("o_empty", t), o_no[t]))
+                    o_no[t] += 1
+                push(mem.get(("ring", vs), ("v", tile_no)), *(mem.get(("p early", t, w), (i, j)) for w in range(WARPS)), mem.put(("o", t), "being added to"))
+                wait(("p_full", t))
+                if more and t == 0:
+                    wait(("kv_full", ks))
+                push(*(mem.get(("p", t, w), (i, j)) for w in range(WARPS)), mem.put(("o", t), (i, j)))
+                if more:
+                    issue_s(t, i, j + 1, ks, tile_no + 1)
+                    if j + 2 == n:
+                        push(("arrive", ("q_empty", t)))
+                    ready(t)
+                else:
+                    push(("arrive", ("o_full", t)))
+                    if with_p:
+                        issue.append(("arrive", ("o_full", t)))
+            push(("arrive", ("kv_empty", vs)))
+            if more:
+                push(("arrive", ("kv_empty", ks)))
+            kv_no, tile_no = kv_no + 2, tile_no + 1
+    actors["products"] = issue
+    actors["tensor cores"] = _tensor_core(queue, counts)
+    # ---- loads
+    ops, q_no, state = [], [0, 0], {"kv": 0, "tile": 0}
+
+    def load(kind):
+        slot = state["kv"] % 4
+        ops.append(("wait", ("kv_empty", slot), state["kv"] // 4))
+        if kind == "k":
+            ops.append(mem.put(("info", state["tile"] % 4), state["tile"]))
+        ops.extend([mem.put(("ring", slot), (kind, state["tile"])), ("arrive", ("kv_full", slot))])
+        state["kv"] += 1
+    for i, (tiles, n) in enumerate(items):
+        load("k")
+        for t in range(tiles):
+            ops += [("wait", ("q_empty", t), q_no[t]), mem.put(("q", t), i), ("arrive", ("q_full", t))]
+            q_no[t] += 1
+        load("v")
+        state["tile"] += 1
+        for j in range(1, n):
+            load("k")
+            load("v")
+            state["tile"] += 1
+    actors["loads"] = ops
+    # ---- hidden rows of V
+    for w in range(WARPS):
+        ops, v_no, tile_no = [], {1: 0, 3: 0}, 0
+        for i, (tiles, n) in enumerate(items):
+            for j in range(n):
+                slot = (2 * tile_no + 1) % 4
+                v_no[slot] += 1
+                ops += [("wait", ("kv_full", slot), v_no[slot]), mem.get(("info", tile_no % 4), tile_no), mem.get(("ring", slot), ("v", tile_no)), ("arrive", ("v_ready", slot // 2))]
+                tile_no += 1
+        actors[f"hidden rows {w}"] = ops
+    # ---- rows out
+    for w in range(WARPS):
+        ops, o_seen, mine = [], [0, 0], [0, 0]
+        for i, (tiles, n) in enumerate(items):
+            for t in range(tiles):
+                o_seen[t] += 1
+                at = mine[t] if slot_by_tile else i
+                ops += [("wait", ("o_full", t), o_seen[t]), mem.get(("1 / l", at % 2, t, w), i), mem.get(("o", t), (i, n - 1)), ("arrive", ("o_empty", t))]
+                mine[t] += 1
+        actors[f"rows out {w}"] = ops
     return actors, counts
 
 
@@ -222,6 +354,13 @@ def _go_through(build, items, **kw):
 @pytest.mark.parametrize("items", RUNS)
 def test_cache_form(items):
     _go_through(_cache_form, items)
+
+
+def test_a_slot_by_items_of_the_cta_is_found_out():
+    """1 / l of a second tile, its slot taken by the number of the CTA's item: an item without a second tile lets the next but one overwrite it."""
+    with pytest.raises(Hazard, match="1 / l"):
+        _go_through(_rows_form, RUNS[1], slot_by_tile=False, with_p=True)
+    _go_through(_rows_form, RUNS[1], slot_by_tile=True, with_p=True)
 
 
 @pytest.mark.parametrize("items", RUNS[:3])
