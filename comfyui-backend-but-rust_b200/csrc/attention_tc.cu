@@ -38,7 +38,7 @@ template <int DP, bool KV8> struct Tc {
     static constexpr int kTile = DP / 64 * kBox;                   // 128 rows of Q, K or V
     static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + (KV8 ? 8 * 2048 : 4 * 4096);
     // barriers and two words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
-    // item of the tile % 2: 1 / l of every row (16-bit), or bf16 queries' powers of two
+    // item of the tile % 2: l of every row (16-bit), or bf16 queries' powers of two
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
     static constexpr int kOrder = kRowInfo + 2048, kEnd = kOrder + 128, kSmem = kEnd + 1024;
     static constexpr int kThreads = 512;
@@ -129,13 +129,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     // [key tile % 4]: 16-bit: [key] +inf, or -inf where a key is not seen; cache: [factor, offset, weight][16 keys]
     float* info = reinterpret_cast<float*>(sm + L::kInfo);
     // [n % 2][tile][row]: of a tile's n-th item, counted by each tile for itself, since an item of at most 128 rows has no second tile. Written again
-    // for item n + 2 only behind what waited for item n's reader: 1 / l behind the logits of n + 2, which are issued behind the sums of n + 1, and those
+    // for item n + 2 only behind what waited for item n's reader: l behind the logits of n + 2, which are issued behind the sums of n + 1, and those
     // wait for o_empty of n, which the rows' way out gives when it has read; powers behind q_empty of n + 1, whose logits are issued behind p of n.
     float* row_info = reinterpret_cast<float*>(sm + L::kRowInfo);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
         for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
-            mbar_init(o_full + 8 * t, KV8 ? 1 : 5), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
+            mbar_init(o_full + 8 * t, 2), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
         *abort_s = 0;
         fence_mbar_init();
         if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
@@ -264,6 +264,14 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         out[e >> 1] = pack2<T>(a, b);
                     }
                     tmem_st16(s_at + q * 16, out);
+                    if (q == 3) {
+                        float even, odd;
+                        unpack_f32(add_f32x2(sum[0], sum[1]), even, odd);
+                        l += even + odd;
+                        // l for the rows' way out, announced with p: an arrival of its own behind p could be that of a warp which is an item ahead, in
+                        // place of one that is late (2 x 4096 x 77 15.5 us instead of 15.2, 16384 x 512 130.6 instead of 130.1)
+                        if (!KV8 && j + 1 == x.n) row_info[(item_no++ & 1) * 256 + t * 128 + row] = l;
+                    }
                     if (q == L::kEarly - 1 || q == 3) {
                         tmem_st_wait();
                         tc_fence_before();
@@ -271,17 +279,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         if (lane == 0) mbar_arrive((q < 3 ? p_early : p_full) + 8 * t);
                     }
                 }
-                float even, odd;
-                unpack_f32(add_f32x2(sum[0], sum[1]), even, odd);
-                l += even + odd;
             }
             if (!ok) break;
-            if (!KV8) {      // 1 / l for the rows' way out; 0: zeros, whatever the sums hold
-                row_info[(item_no++ & 1) * 256 + t * 128 + row] = l > 0.f || l != l ? 1.f / l : 0.f;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(o_full + 8 * t);
-                continue;
-            }
+            if (!KV8) continue;
             // ---- the rows out: 32 columns at a time through this warp's staging, so that a row's pieces are stored together
             if (x.n > 0) {
                 if (!__all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, o_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
@@ -336,9 +336,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 umma_16_ss(tmem + t * 128, q + step, k + step, idesc_s, kk > 0);
             }
         };
-        auto ready = [&](int t) {      // one arrival when the products are done, one that orders what this warp has seen in shared memory
-            umma_commit(s_full + 8 * t);
-            mbar_arrive(s_full + 8 * t);
+        auto announce = [&](uint32_t bar) {      // one arrival when the products are done, one that orders what this warp has seen in shared memory
+            umma_commit(bar);
+            mbar_arrive(bar);
         };
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
@@ -353,7 +353,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (one) {
                     issue_s(t, ks);
                     if (x.n == 1) umma_commit(q_empty + 8 * t);
-                    ready(t);
+                    announce(s_full + 8 * t);
                 }
                 __syncwarp();
             }
@@ -390,8 +390,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                             issue_s(t, ks);
                             if (j + 2 == x.n) umma_commit(q_empty + 8 * t);
                         }
-                        if (more) ready(t);
-                        else umma_commit(o_full + 8 * t);
+                        announce((more ? s_full : o_full) + 8 * t);
                     }
                     __syncwarp();
                 }
@@ -500,7 +499,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, phase[t], abort_s, ST_TIMEOUT_TMEM_FULL)))) break;
                     phase[t] ^= 1;
                     tc_fence_after();
-                    inv = row_info[(item_no[t]++ & 1) * 256 + t * 128 + quarter * 32 + lane];
+                    const float l = row_info[(item_no[t]++ & 1) * 256 + t * 128 + quarter * 32 + lane];
+                    inv = l > 0.f || l != l ? 1.f / l : 0.f;      // 0: zeros, whatever the sums hold
                 }
                 const int left = min(32, x.rows - t * 128 - quarter * 32);      // rows of this warp; none: nothing is stored
                 QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + (x.row0 + t * 128 + quarter * 32) * p.a.os[1] + x.h * p.a.os[2];

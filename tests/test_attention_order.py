@@ -104,7 +104,7 @@ def _cache_form(items, own_o_full=True):
     mem, queue = Memory(), []
     counts = {**{("kv_full", s): WARPS for s in range(4)}, **{("kv_empty", s): 1 for s in range(4)}}
     for t in (0, 1):
-        counts.update({("q_full", t): WARPS, ("q_empty", t): 1, ("s_full", t): 2, ("p_early", t): WARPS, ("p_full", t): WARPS, ("o_full", t): 1})
+        counts.update({("q_full", t): WARPS, ("q_empty", t): 1, ("s_full", t): 2, ("p_early", t): WARPS, ("p_full", t): WARPS, ("o_full", t): 2})
     o_bar = "o_full" if own_o_full else "s_full"
     actors = {f"softmax {t}.{w}": [] for t in (0, 1) for w in range(WARPS)}
     # ---- softmax
@@ -173,6 +173,7 @@ def _cache_form(items, own_o_full=True):
                     ready(t)
                 else:
                     push(("arrive", ("o_full", t)))
+                    issue.append(("arrive", ("o_full", t)))
             push(("arrive", ("kv_empty", vs)))
             if more:
                 push(("arrive", ("kv_empty", ks)))
@@ -199,7 +200,7 @@ def _cache_form(items, own_o_full=True):
     return actors, counts
 
 
-def _rows_form(items, slot_by_tile=True, with_p=False):
+def _rows_form(items, slot_by_tile=True, with_p=True):
     """Warps 0-7 softmax, 8 products, 9 loads, 10 and 11 hidden rows of V, 12-15 rows out."""
     mem, queue = Memory(), []
     counts = {**{("kv_full", s): 1 for s in range(4)}, **{("kv_empty", s): 1 for s in range(4)}}
@@ -207,7 +208,7 @@ def _rows_form(items, slot_by_tile=True, with_p=False):
         counts.update({("q_full", t): 1, ("q_empty", t): 1, ("s_full", t): 2, ("p_early", t): WARPS, ("p_full", t): WARPS, ("o_full", t): 2 if with_p else WARPS + 1,
                        ("o_empty", t): WARPS, ("v_ready", t): WARPS})
     actors = {}
-    # ---- softmax, and 1 / l of its rows
+    # ---- softmax, and l of its rows
     for t in (0, 1):
         for w in range(WARPS):
             ops, s_seen, tile_no, mine = [], 0, 0, 0
@@ -223,11 +224,11 @@ def _rows_form(items, slot_by_tile=True, with_p=False):
                         ops.append(mem.get(("o", t), (i, j - 1)))
                     ops += [mem.put(("p early", t, w), (i, j)), ("arrive", ("p_early", t)), mem.put(("p", t, w), (i, j))]
                     if with_p and j + 1 == n:
-                        ops.append(mem.put(("1 / l", mine % 2, t, w), i))
+                        ops.append(mem.put(("l", mine % 2, t, w), i))
                     ops.append(("arrive", ("p_full", t)))
                     tile_no += 1
                 if not with_p:
-                    ops += [mem.put(("1 / l", mine % 2, t, w), i), ("arrive", ("o_full", t))]
+                    ops += [mem.put(("l", mine % 2, t, w), i), ("arrive", ("o_full", t))]
                 mine += 1
             actors[f"softmax {t}.{w}"] = ops
     # ---- products
@@ -326,7 +327,7 @@ def _rows_form(items, slot_by_tile=True, with_p=False):
             for t in range(tiles):
                 o_seen[t] += 1
                 at = mine[t] if slot_by_tile else i
-                ops += [("wait", ("o_full", t), o_seen[t]), mem.get(("1 / l", at % 2, t, w), i), mem.get(("o", t), (i, n - 1)), ("arrive", ("o_empty", t))]
+                ops += [("wait", ("o_full", t), o_seen[t]), mem.get(("l", at % 2, t, w), i), mem.get(("o", t), (i, n - 1)), ("arrive", ("o_empty", t))]
                 mine[t] += 1
         actors[f"rows out {w}"] = ops
     return actors, counts
@@ -356,11 +357,21 @@ def test_cache_form(items):
     _go_through(_cache_form, items)
 
 
+@pytest.mark.parametrize("items", RUNS)
+def test_rows_form(items):
+    _go_through(_rows_form, items)
+
+
 def test_a_slot_by_items_of_the_cta_is_found_out():
-    """1 / l of a second tile, its slot taken by the number of the CTA's item: an item without a second tile lets the next but one overwrite it."""
-    with pytest.raises(Hazard, match="1 / l"):
-        _go_through(_rows_form, RUNS[1], slot_by_tile=False, with_p=True)
-    _go_through(_rows_form, RUNS[1], slot_by_tile=True, with_p=True)
+    """l of a second tile, its slot taken by the number of the CTA's item: an item without a second tile lets the next but one overwrite it."""
+    with pytest.raises(Hazard, match="l"):
+        _go_through(_rows_form, RUNS[1], slot_by_tile=False)
+
+
+def test_an_arrival_of_its_own_for_the_sums_is_found_out():
+    """l announced by its writers' arrivals behind p: a warp of one item later arrives in place of one that is late."""
+    with pytest.raises(Hazard, match="l"):
+        _go_through(_rows_form, RUNS[0], with_p=False)
 
 
 @pytest.mark.parametrize("items", RUNS[:3])
