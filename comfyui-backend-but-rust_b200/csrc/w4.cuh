@@ -143,6 +143,10 @@ __device__ __forceinline__ void store_out(const W4Params& p, float y, int m, int
     }
 }
 
+// What a kernel may have of shared memory is one setting for all threads of the program: always the most a CTA can have, never a call's own need,
+// which another thread's smaller one could replace before the launch.
+constexpr int kMostSmem = 227 * 1024;
+
 // The kernel for many tokens (w4_tile.cu)
 int w4_tile(int dtype, const W4Params& p, cudaStream_t st);
 int w4_status_read_clear(int* out);

@@ -257,7 +257,7 @@ template <int XT, int GB> int launch_w4(W4Params& p, cudaStream_t st) {
                                                                                                                          : w4_rows_kernel<XT, 4, GB, true>)
                             : (cols <= 8 ? w4_rows_kernel<XT, 1, GB, false> : cols <= 16 ? w4_rows_kernel<XT, 2, GB, false> : cols <= 24 ? w4_rows_kernel<XT, 3, GB, false>
                                                                                                                            : w4_rows_kernel<XT, 4, GB, false>);
-        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem)) return (int)e;
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) return (int)e;
         return launch_pdl_cluster(kern, dim3((unsigned)(tiles * p.splits)), kRowsWarps * 32, sh.smem, st, p.splits, p);
     }
     return w4_tile(XT, p, st);

@@ -358,7 +358,7 @@ template <int XT, bool G32, bool WIDE> __global__ void __launch_bounds__(512, 1)
 template <int XT, bool G32, bool WIDE> int launch_tile(const CUtensorMap& tm, const TileParams& p, int grid, cudaStream_t st) {
     const int smem = tail_at(p.columns) + 256 + 1024;
     auto kern = w4_tile_kernel<XT, G32, WIDE>;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return (int)e;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) return (int)e;
     return launch_pdl_cluster(kern, dim3((unsigned)grid), 512, smem, st, p.splits, tm, p);
 }
 

@@ -6,6 +6,8 @@ Linear: codes and activations enter exactly, so an output is off by the rounding
 sums, at most 2^-23 of the absolute terms for each of the K additions (the products' own sums may cut off instead of rounding)."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -243,6 +245,40 @@ def test_two_streams_at_once_and_ordinary_launches(pkg, dev, M):
         finally:
             L.set_gemm_cluster_limit(was)
     assert L.kernel_status() == 0
+
+
+@pytest.mark.parametrize("M", [(1, 8), (34, 160)])
+def test_two_host_threads_with_different_sizes(pkg, dev, M):
+    """The same kernel with little and with much shared memory, launched by two threads at once: neither takes the other's limit."""
+    g = torch.Generator().manual_seed(M[0])
+    L, errors = pkg.linear, []
+    work = []
+    for m, K in zip(M, (256, 9728)):
+        packed, scales, _ = _weight(g, dev, 64, K, 128, zeros=False)
+        x = torch.randn(m, K, generator=g).bfloat16().to(dev)
+        want = L.w4_linear(x, packed, scales)
+        _check(want, x, _unpack(packed, scales, None), None, None)
+        work.append((x, packed, scales, want))
+    torch.cuda.synchronize()
+    start = threading.Barrier(2)
+
+    def loop(x, packed, scales, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                out = torch.empty_like(want)
+                start.wait()
+                for _ in range(3000):
+                    L.w4_linear(x, packed, scales, out=out)
+                torch.cuda.current_stream(dev).synchronize()
+                assert torch.equal(out, want)
+        except BaseException as e:
+            errors.append(e)
+    threads = [threading.Thread(target=loop, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
 
 
 @pytest.mark.parametrize("M", [1, 40])
