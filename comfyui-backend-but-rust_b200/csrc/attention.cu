@@ -364,12 +364,14 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
                 }
             float top[2] = {m[0], m[1]};
             const bool all = key0 + 16 <= lowest;
+            // the row's power with the page's factor: with the product, of up to 2^30, it may leave f32's range where the logit does not
+            const float times[2] = {in.x * factor[0], in.x * factor[1]};
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const int h = x >> 1;
-                    s[n][x] = __fmaf_rn(s[n][x] * factor[h], in.x, in.y);
+                    s[n][x] = __fmaf_rn(s[n][x], times[h], in.y);
                     if (!all && key0 + n * 8 + 2 * t + (x & 1) >= bound[h]) s[n][x] = -INFINITY;
                     top[h] = fmaxf(top[h], s[n][x]);
                 }

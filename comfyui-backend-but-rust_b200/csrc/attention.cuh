@@ -40,10 +40,11 @@ __device__ __forceinline__ uint2 halves_of4(uint32_t w) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-// bf16 queries over int8 keys are taken as halves times a power of two: 2^e brings a row's largest magnitude to [2^14, 2^15). 2^e and 2^-e are
-// f32 numbers.
+// bf16 queries over int8 keys are taken as halves times a power of two: 2^e brings a row's largest magnitude to [2^14, 2^15). e is -113 for the
+// type's largest numbers and at most 126, so that 2^e and 2^-e are normal f32 numbers; rows below 2^-112 stay smaller, but times 2^126 every
+// bf16 number of at most that size is a half exactly (the smallest, 2^-133, is 2^-7).
 __device__ __forceinline__ int row_exponent(float top) {
-    return top > 0.f && top <= FLT_MAX ? min(100, max(-100, 14 - ((int)(__float_as_uint(top) >> 23) - 127))) : 0;
+    return top > 0.f && top <= FLT_MAX ? min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)) : 0;
 }
 
 // Eight columns of a finished row; one that saw no key is zeros, NaN stays.

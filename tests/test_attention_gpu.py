@@ -256,6 +256,24 @@ def test_bf16_queries_of_any_size(pkg, dev, size):
     _kv8_check(got, q, c, table, [200], [3], True, 0.1 / size)
 
 
+@pytest.mark.parametrize("L,H,lens", [(3, 4, [200]), (300, 16, [300, 333, 400, 310])])
+@pytest.mark.parametrize("power", [118, 128, -100, -122, -131])
+def test_bf16_queries_at_the_ends_of_the_range(pkg, dev, L, H, lens, power):
+    """Rows up to the type's largest numbers and down to its subnormal ones, by few rows and by many. Logits of some units, and of some
+    thousands for the largest: scale * k_scale is kept to f32's normal numbers."""
+    g = torch.Generator().manual_seed(power + 200)
+    B, Hkv, D, T = len(lens), 2 if L < 100 else 16, 64, 32
+    c, table = _cache(pkg, dev, g, B, lens, Hkv, D, T)
+    shift = -8 if power > 0 else 6
+    c.k_scale.mul_(2.0 ** shift)
+    q = torch.randn(B, L, H, D, generator=g).clamp(-3.9, 3.9).mul(2.0 ** (power - 2)).bfloat16().to(dev)
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    scale = 2.0 ** (max(-power, -118) - shift)
+    assert bool(torch.isfinite(q).all()) and float(q.float().abs().max()) > 2.0 ** (power - 1)
+    got = pkg.attention.kv8_attention(q, c, table, n, scale=scale)
+    _kv8_check(got, q, c, table, lens, [L] * B, True, scale)
+
+
 def test_scales_far_apart(pkg, dev):
     """Pages whose values differ by many orders of magnitude: p carries the value's scale, so the largest contribution keeps fp16's bits
     whatever the others' size; a page of zeros (scale 1e-30, or 0 where nothing was ever written) only weighs in the sum of p."""
