@@ -263,8 +263,8 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
         }
     };
     auto note_scales = [&](int i0) {
-        const float s = fmaxf(v_scale, kTiny);
-        info[(i0 + lane) & 63] = page_off >= 0 ? make_float4(k_scale * (p.scale * kLog2e), log2f(s), 1.f / s, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+        info[(i0 + lane) & 63] =
+            page_off >= 0 ? make_float4(k_scale * (p.scale * kLog2e), v_scale_log2(v_scale), v_scale_weight(v_scale), 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     // 16 rows of K, then of V. K's 16-byte pieces are read four to a row by two rows at a time, V's two to a row by four pairs of rows: the
     // piece's number is turned so that either lies in all 32 banks. A lane has the same piece of every kStep-th row.

@@ -47,6 +47,11 @@ __device__ __forceinline__ int row_exponent(float top) {
     return top > 0.f && top <= FLT_MAX ? min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)) : 0;
 }
 
+// A page's scale of V in the logits (its power of two, which p then carries) and out of the sum of p again. A scale below kTiny is taken for it. NaN
+// makes p NaN where a key is seen; its weight is a number, so that a key which is not seen adds nothing.
+__device__ __forceinline__ float v_scale_log2(float s) { return log2f(s < kTiny ? kTiny : s); }
+__device__ __forceinline__ float v_scale_weight(float s) { return s != s ? 1.f : 1.f / fmaxf(s, kTiny); }
+
 // Eight columns of a finished row; one that saw no key is zeros, NaN stays.
 template <typename QT> __device__ __forceinline__ void store_row(const AttnParams& p, const float (&y)[8], float total, int b, int row, int kvh, int ratio, int d, QT) {
     const float inv = total > 0.f || total != total ? 1.f / total : 0.f;

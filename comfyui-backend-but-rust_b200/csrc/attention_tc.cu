@@ -645,8 +645,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (lane == 0) words[(tile_no & 3) * 4 + w] = seen;
                 if ((lane & 15) == 0) {
                     float* in = info + (tile_no & 3) * 24 + w * 2 + (lane >> 4);
-                    const float s = fmaxf(v_scale, kTiny);
-                    in[0] = k_scale * (p.a.scale * kLog2e), in[8] = log2f(s), in[16] = 1.f / s;
+                    in[0] = k_scale * (p.a.scale * kLog2e), in[8] = v_scale_log2(v_scale), in[16] = v_scale_weight(v_scale);
                 }
                 convert(kc, slot);
                 page = page_next, off = offset_of(j + 1, page);      // past the last tile: no key is seen, nothing is requested

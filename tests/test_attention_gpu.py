@@ -295,6 +295,27 @@ def test_scales_far_apart(pkg, dev):
             _kv8_check(pkg.attention.kv8_attention(q, c, table, length), q, c, table, [n], [2], True, D ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("L,H,Hkv,lens", [(40, 2, 2, [100, 90]), (300, 16, 16, [400, 350, 300, 310, 320, 330])])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_a_scale_that_is_no_number(pkg, dev, L, H, Hkv, lens, dtype, which):
+    """A page whose scale of K or of V is NaN: rows that see one of its keys are NaN, as what it stands for is; rows before it are not touched."""
+    g = torch.Generator().manual_seed(L)
+    B, D, T = len(lens), 64, 16
+    c, table = _cache(pkg, dev, g, B, lens, Hkv, D, T)
+    q = torch.randn(B, L, H, D, generator=g).to(DT[dtype]).to(dev)
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    want = pkg.attention.kv8_attention(q, c, table, n)
+    slot = (lens[1] - 20) // T
+    getattr(c, which)[table[1, slot].long(), 0] = float("nan")
+    got = pkg.attention.kv8_attention(q, c, table, n)
+    sees = torch.arange(lens[1] - L, lens[1], device=dev) >= slot * T
+    hit = torch.zeros(B, L, H, dtype=torch.bool, device=dev)
+    hit[1, sees, :H // Hkv] = True
+    assert 0 < int(sees.sum()) < L
+    assert bool(torch.isnan(got[hit]).all()) and torch.equal(got[~hit], want[~hit])
+
+
 def test_what_is_never_seen_may_hold_anything(pkg, dev):
     """Behind a sequence's last token: codes and scales of unused pages (NaN), table entries that are no pages at all."""
     g = torch.Generator().manual_seed(9)
