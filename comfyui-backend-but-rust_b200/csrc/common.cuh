@@ -103,9 +103,14 @@ __device__ __forceinline__ float gelu_tanh_f(float x) {
     return 0.5f * x * (1.f + tanhf(k0 * (x + k1 * x * x * x)));
 }
 
-// rint(v / s) for N values and one scale, as the division and the rounding would give it (|v / s| < 128, s >= 0; s = 0 gives 0): the product with
-// the reciprocal is less than 2^-15 from the quotient, so it rounds to the same integer unless it lies that close to a half, and then the
-// thread divides. Scales whose reciprocal is no normal number are divided by, too.
+__device__ __forceinline__ float max_or_nan(float a, float b) {      // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// rint(v / s) for N values and one scale, as the division and the rounding would give it (|v / s| < 128 or taken for more, s >= 0; s = 0 and what
+// is no number give 0): the product with the reciprocal is less than 2^-15 from the quotient, so it rounds to the same integer unless it lies that
+// close to a half, and then the thread divides, as it does for infinities and NaN. Scales whose reciprocal is no normal number are divided by, too.
 template <int N> __device__ __forceinline__ void rint_quotients(const float (&v)[N], float s, float (&q)[N]) {
     const bool normal = s > 1e-30f && s < 1e30f;
     const float inv = normal ? __frcp_rn(s) : 0.f;
@@ -114,11 +119,14 @@ template <int N> __device__ __forceinline__ void rint_quotients(const float (&v)
     for (int i = 0; i < N; ++i) {
         const float x = __fmul_rn(v[i], inv);
         q[i] = __fsub_rn(__fadd_rn(x, 12582912.f), 12582912.f);      // 1.5 x 2^23: rounds to the nearest integer, ties to even
-        near = fmaxf(near, fabsf(__fsub_rn(x, q[i])));
+        near = max_or_nan(near, fabsf(__fsub_rn(x, q[i])));
     }
-    if (near > 0.4999f) {
+    if (!(near <= 0.4999f)) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q[i] = s > 0.f ? rintf(__fdiv_rn(v[i], s)) : 0.f;
+        for (int i = 0; i < N; ++i) {
+            const float x = __fdiv_rn(v[i], s);
+            q[i] = s > 0.f && x == x ? rintf(x) : 0.f;
+        }
     }
 }
 // 32 bytes in one store

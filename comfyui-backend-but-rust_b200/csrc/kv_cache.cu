@@ -40,7 +40,7 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s) {
     float c[8];
     rint_quotients<8>(v, s, c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = c[e] == c[e] ? fminf(127.f, fmaxf(-127.f, c[e])) : 0.f;
+    for (int e = 0; e < 8; ++e) c[e] = fminf(127.f, fmaxf(-127.f, c[e]));
     return make_uint2(pack4(c), pack4(c + 4));
 }
 

@@ -220,8 +220,9 @@ int gpu_embed_dequant(const int8_t* q, const float* s, float* out, int M, int K,
  *
  * gpu_w4_requant   w [N, K] (f32, f16 or bf16, rows w_stride apart) -> codes and scales, nearest even. Without zeros: s = amax * (1/7)
  *                  rounded to its type, c = clamp(rint(w / s), -8, 7) + 8. With: s = (max(w, 0) - min(w, 0)) * (1/15),
- *                  z = clamp(rint(-min / s), 0, 15), c = clamp(rint(w / s) + z, 0, 15). A group of zeros has s = 0. Weights in another
- *                  basis: gpu_rotate_rows_f32 first.
+ *                  z = clamp(rint(-min / s), 0, 15), c = clamp(rint(w / s) + z, 0, 15). A group of zeros has s = 0. NaN is passed over in s
+ *                  and z and gets the code of 0, c = z; infinities get the end of the range that they are at, s the type's largest number. Weights
+ *                  in another basis: gpu_rotate_rows_f32 first.
  * gpu_w4_dequant   the way back, out [N, K] in dtype.
  * gpu_w4_linear    out[m,n] = beta * out[m,n] + sum_k x[m,k] W[n,k] + bias[n], beta 0 or 1 (-207). x [M, K] f32, f16 or bf16, out [M, N]
  *                  in x's type or f32, bias [N] in out's type or NULL. Codes and x enter the products exactly (an f32 x as three

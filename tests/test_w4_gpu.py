@@ -170,6 +170,25 @@ def test_packer(pkg, dev, N, K, G, dtype, sdt):
         assert bool((off <= step * (0.5 + 15 * torch.finfo(sdt).eps + (0.5 if zeros else 0)) + 1e-6 * step + (6e-8 if sdt == torch.float16 else 0)).all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_packer_on_nan_and_infinities(pkg, dev, dtype, zeros):
+    """NaN stands for 0 after packing, and the other weights of its group are as without it; an infinity takes the end of the range."""
+    g = torch.Generator().manual_seed(5)
+    N, K, G = 67, 256, 32
+    w = (torch.randn(N, K, generator=g) * 0.02).to(DT[dtype]).to(dev)
+    bad = (torch.rand(N, K, generator=g) < 0.1).to(dev)
+    bad[3, :G] = True                                # a group of nothing else
+    packed, s, z = pkg.linear.w4_requant(torch.where(bad, torch.tensor(float("nan"), dtype=w.dtype, device=dev), w), G, zero_points=zeros)
+    want = pkg.linear.w4_requant(torch.where(bad, torch.zeros_like(w), w), G, zero_points=zeros)
+    assert torch.equal(packed, want[0]) and torch.equal(s, want[1]) and (z is None or torch.equal(z, want[2]))
+    assert bool((pkg.linear.w4_dequant(packed, s, z)[bad] == 0).all())
+    w[1, 5], w[2, 7] = float("inf"), -float("inf")
+    packed, s, z = pkg.linear.w4_requant(w, G, zero_points=zeros)
+    codes = torch.stack((packed & 15, packed >> 4), 2).flatten(1)
+    assert int(codes[1, 5]) == 15 and int(codes[2, 7]) == 0 and float(s[1, 0]) == 65504.0 and bool(torch.isfinite(s).all())
+
+
 def test_a_lora_bake_goes_there_and_back(pkg, dev):
     """Packed, read back, packed again: the same codes (the largest of a group lands on its own scale again)."""
     g = torch.Generator().manual_seed(1)
