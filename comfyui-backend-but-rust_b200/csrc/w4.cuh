@@ -33,11 +33,14 @@ struct W4Params {
 };
 
 // Codes in registers: a word holds columns 8t..8t+7 of a row, a pair of neighbours in each byte. The pair's byte goes to both halves of a
-// register, the exponent of 1024 (f16) or 128 (bf16) around its nibble, and one instruction takes away the offset and the zero point: the
-// code minus its zero point is a small integer, exact in either type, and so are its products with x in the f32 sums.
+// register, the exponent of 1024 (f16) or 1/32 (bf16) around its nibble, and one instruction takes away the offset and the zero point: the
+// code minus its zero point is a small integer (bf16: times 2^-12), exact in either type, and so are its products with x in the f32 sums.
+// The 2^-12 keeps a group's sum, up to 256 terms of 15 |x|, in f32's range for every x that bf16 and f32 have; kUp takes it out of the
+// finished row's value. (|x| below 2^-100 may lose bits to it.)
 // `expand` gives neighbouring columns (2i, 2i + 1); `expand4` columns (i, i + 4), which takes fewer instructions but needs x in that order.
 template <typename T> struct Nibbles;
 template <> struct Nibbles<half> {
+    static constexpr float kUp = 1.f;
     uint32_t sub;       // (-1024 - z, -64 - z): the high half's nibble sits four bits up, its scale of 1/16 is in the same instruction
     uint32_t lo, hi;    // the same for both halves of a register alike
     __device__ __forceinline__ explicit Nibbles(uint32_t z)
@@ -64,9 +67,10 @@ template <> struct Nibbles<half> {
     }
 };
 template <> struct Nibbles<bf16> {
-    uint32_t sub;       // 128 + z in both halves
-    __device__ __forceinline__ explicit Nibbles(uint32_t z) : sub((0x4300u + z) * 0x00010001u) {}
-    static constexpr uint32_t kBits = 0x43004300u;
+    static constexpr float kUp = 4096.f;
+    uint32_t sub;       // 2^-5 + 2^-12 z in both halves
+    __device__ __forceinline__ explicit Nibbles(uint32_t z) : sub((0x3D00u + z) * 0x00010001u) {}
+    static constexpr uint32_t kBits = 0x3D003D00u;
     __device__ __forceinline__ void expand4(uint32_t w, uint32_t (&r)[4], uint32_t bits) const {      // bits: kBits, held
 #pragma unroll
         for (int i = 0; i < 4; ++i, w >>= 4) {
@@ -79,7 +83,7 @@ template <> struct Nibbles<bf16> {
         const uint32_t up = w >> 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t b = (__byte_perm(w, up, 0x4040 + 0x0101 * i + 0x0400) & 0x000F000Fu) | 0x43004300u;
+            const uint32_t b = (__byte_perm(w, up, 0x4040 + 0x0101 * i + 0x0400) & 0x000F000Fu) | kBits;
             const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&sub));
             r[i] = *reinterpret_cast<const uint32_t*>(&v);
         }

@@ -229,7 +229,7 @@ template <int XT, int NT, int GB, bool ZP> __global__ void __launch_bounds__(kRo
                 for (int w = 0; w < kw; ++w)
 #pragma unroll
                     for (int q = 0; q < P; ++q) y += dsmem_f32(red_at + (((w * used + m * P + q) << sh.rows_log) + r) * 4, s);
-        if (tile0 + r < p.N) store_out(p, y, m, tile0 + r);
+        if (tile0 + r < p.N) store_out(p, y * Nibbles<T>::kUp, m, tile0 + r);
     }
     if (S > 1) cluster_sync_all();                     // nobody leaves while its sums are read
 }

@@ -48,7 +48,7 @@ template <int N> __device__ __forceinline__ float sum_at(const uint64_t (&acc)[N
 }
 // One output row's sums (P to a token) from `token` on: bias once, and where the result is added to, sixteen of its values before the first
 // is written.
-template <typename T, int P, int N> __device__ __forceinline__ void store_column(const W4Params& w, const uint64_t (&acc)[N], int token, int tokens, int n) {
+template <typename T, int P, int N> __device__ __forceinline__ void store_column(const W4Params& w, const uint64_t (&acc)[N], float up, int token, int tokens, int n) {
     T* out = reinterpret_cast<T*>(w.out) + token * w.out_stride + n;
     const float bias = w.bias ? to_f<T>(gload(reinterpret_cast<const T*>(w.bias) + n)) : 0.f;
     constexpr int kTokens = 2 * N / P, kBatch = 8;
@@ -66,6 +66,7 @@ template <typename T, int P, int N> __device__ __forceinline__ void store_column
             float y = sum_at(acc, c);
 #pragma unroll
             for (int q = 1; q < P; ++q) y += sum_at(acc, c + q);
+            y *= up;
             if (w.bias) y += bias;
             if (w.beta != 0.f) y = __fmaf_rn(w.beta, old[t], y);
             if (t0 + t < tokens) *out = from_f<T>(y);
@@ -164,9 +165,9 @@ template <int XT, bool G32, bool WIDE> __global__ void __launch_bounds__(512, 1)
                     if (c / 16 < mine) red[(col0 + c) * kRows + quarter * 32 + lane] = sum_at(acc, c);
             } else if (n < w.N) {
                 const int first_token = m0 + col0 / P, tokens = min(mine * 16 / P, w.M - first_token);
-                if (w.out_dt == DT_F32) store_column<float, P>(w, acc, first_token, tokens, n);
-                else if (w.out_dt == DT_F16) store_column<half, P>(w, acc, first_token, tokens, n);
-                else store_column<bf16, P>(w, acc, first_token, tokens, n);
+                if (w.out_dt == DT_F32) store_column<float, P>(w, acc, Nibbles<T>::kUp, first_token, tokens, n);
+                else if (w.out_dt == DT_F16) store_column<half, P>(w, acc, Nibbles<T>::kUp, first_token, tokens, n);
+                else store_column<bf16, P>(w, acc, Nibbles<T>::kUp, first_token, tokens, n);
             }
         }
     } else if (warp < 12) {
@@ -349,7 +350,7 @@ template <int XT, bool G32, bool WIDE> __global__ void __launch_bounds__(512, 1)
             for (int s = 0; s < p.splits; ++s)
 #pragma unroll
                 for (int q = 0; q < P; ++q) y += dsmem_f32(base + ((m * P + q) * kRows + r) * 4, s);
-            if (n0 + r < w.N) store_out(w, y, m0 + m, n0 + r);
+            if (n0 + r < w.N) store_out(w, y * Nibbles<T>::kUp, m0 + m, n0 + r);
         }
         cluster_sync_all();      // nobody leaves while its sums are read
     }

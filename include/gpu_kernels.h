@@ -226,7 +226,8 @@ int gpu_embed_dequant(const int8_t* q, const float* s, float* out, int M, int K,
  * gpu_w4_dequant   the way back, out [N, K] in dtype.
  * gpu_w4_linear    out[m,n] = beta * out[m,n] + sum_k x[m,k] W[n,k] + bias[n], beta 0 or 1 (-207). x [M, K] f32, f16 or bf16, out [M, N]
  *                  in x's type or f32, bias [N] in out's type or NULL. Codes and x enter the products exactly (an f32 x as three
- *                  bf16 terms), sums are f32, one rounding to out's type. M from one token up; out must not overlap x.
+ *                  bf16 terms; magnitudes below 2^-100 may lose bits), sums are f32 and stay in range for every bf16 and f32 x as long
+ *                  as the result does, one rounding to out's type. M from one token up; out must not overlap x.
  * Errors: -4 types, -5 a NULL, a row of x or w, or Wq4 off a 16-byte boundary, packed of the packer off 8, out of gpu_w4_dequant off 32 bytes,
  * -203 descriptor (x of many tokens). */
 int gpu_w4_requant(int dtype, const void* w, int64_t w_stride, void* packed, int scale_dt, void* scales, void* zeros, int64_t N,

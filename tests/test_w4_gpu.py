@@ -104,6 +104,41 @@ def test_f32_rows_keep_24_bits_whatever_their_size(pkg, dev, M):
     assert bool(((y.double() - one.double() @ w.t()).abs() <= 2.0 ** -23 * w[:, 5].abs()).all())
 
 
+@pytest.mark.parametrize("M", [1, 9, 40, 200])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("G", [32, 256])
+def test_rows_up_to_the_largest_numbers(pkg, dev, M, dtype, G):
+    """Activations near the type's largest number: the codes' sums stay in range where the result does. Many columns of one sign and the
+    largest codes, so that a group's sum before its scale is as large as it gets."""
+    g = torch.Generator().manual_seed(M)
+    K, N = 512, 70
+    packed, scales, z = _weight(g, dev, N, K, G)
+    packed[0], z[0] = 0xFF, 0                        # every weight 15 steps
+    packed[1], z[1] = 0x00, 15                       # and every one -15
+    scales.mul_(0.1)                                 # sums of at most (30 + 482 x 0.03) x 15 x 0.0011 x 3.3e38 = 2.5e38
+    x = torch.rand(M, K, generator=g).mul(0.02).add(0.98).mul(torch.where(torch.rand(M, 1, generator=g) < 0.5, -1.0, 1.0)).mul(3.3e38)
+    x[:, 30:] *= 0.03
+    x = x.to(DT[dtype]).to(dev)
+    assert bool(torch.isfinite(x).all())
+    w = _unpack(packed, scales, z)
+    y = pkg.linear.w4_linear(x, packed, scales, z, out_dtype=torch.float32)
+    assert float((x.double() @ w.t()).abs().max()) < 3.3e38
+    _check(y, x, w, None, None)
+
+
+@pytest.mark.parametrize("M", [1, 30])
+def test_small_values_keep_their_bits(pkg, dev, M):
+    """One f32 value of 2^-100 with bits in all three of its bf16 terms: nothing but the scale's product and the terms' sum is rounded."""
+    g = torch.Generator().manual_seed(M)
+    K, N = 256, 64
+    packed, scales, z = _weight(g, dev, N, K, 32)
+    w = _unpack(packed, scales, z)
+    one = torch.zeros(M, K, device=dev)
+    one[:, 5] = (1.0 + 2.0 ** -15 + 2.0 ** -22) * 2.0 ** -100
+    y = pkg.linear.w4_linear(one, packed, scales, z)
+    assert bool(((y.double() - one.double() @ w.t()).abs() <= 2.0 ** -23 * 2.0 ** -100 * w[:, 5].abs()).all())
+
+
 @pytest.mark.parametrize("M", [2, 33])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_infinities_and_nan_stay_in_their_row(pkg, dev, M, dtype):
