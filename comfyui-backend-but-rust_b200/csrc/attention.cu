@@ -175,14 +175,14 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
 template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
     using L = Tile<DP>;
     auto kern = attention_tile_kernel<T, DP>;
+    const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + kRows - 1) / kRows;
+    if (rows > INT32_MAX - kRows || tiles > INT32_MAX / p.B / p.Hkv) return -1;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
-    const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + kRows - 1) / kRows, base = tiles * p.B * p.Hkv;
-    if (rows > INT32_MAX - kRows) return -1;
+    const int64_t base = tiles * p.B * p.Hkv;
     p.row_tiles = (int)tiles;
     // CTAs to a row tile: as long as the device has room for twice as many and each keeps 256 keys
     p.splits = 1;
     while (p.splits < 8 && base * p.splits * 2 <= 296 && (int64_t)p.Lkv >= (int64_t)p.splits * 2 * 256) p.splits *= 2;
-    if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kThreads, L::kSmem, st, p.splits, p);
 }
 // ---- rows over the cache ---------------------------------------------------------------------------------------------------------
@@ -505,16 +505,16 @@ template <typename QT, int DP> __global__ void __launch_bounds__(kRowsWarps * 32
 template <typename QT, int DP> int launch_rows(AttnParams& p, cudaStream_t st) {
     using R = RowsTile<DP>;
     auto kern = kv8_rows_kernel<QT, DP>;
+    const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + 15) / 16;
+    if (rows > INT32_MAX - 16 || tiles > INT32_MAX / p.B / p.Hkv) return -1;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kSmem)) return (int)e;
-    const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + 15) / 16, base = tiles * p.B * p.Hkv;
-    if (rows > INT32_MAX - 16) return -1;
+    const int64_t base = tiles * p.B * p.Hkv;
     p.row_tiles = (int)tiles;
     // CTAs along the keys: as long as there are fewer than one to an SM (two where sequences of different lengths leave some idle) and each has
     // a block for each warp. CTAs begin and end slowly: 16 sequences of up to 32768 tokens, 8 kv heads, 2 | 4 | 8 CTAs 182 | 120 | 156 us; 8 of up to
     // 8000 with 64 rows a head 94 | 73 | 148; one of 8000 with 120 rows a head 37 | 48 | 53.
     p.splits = 1;
     while (p.splits < 8 && base * p.splits < (p.B > 1 ? 296 : 148) && (int64_t)p.Lkv > (int64_t)p.splits * 16 * kRowsWarps) p.splits *= 2;
-    if (tiles * p.splits > INT32_MAX / p.B / p.Hkv) return -1;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kRowsWarps * 32, R::kSmem, st, p.splits, p);
 }
 
@@ -541,7 +541,7 @@ bool ragged(const int64_t* s, int n) {
 
 GPU_API int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides, const int32_t* kv_len,
                                 const uint8_t* key_mask, int64_t mask_stride, int B, int Lq, int Lkv, int H, int Hkv, int D, float scale, void* stream) {
-    if (B < 0 || Lq < 0 || Lkv < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || D % 8 != 0 || D > 256) return -1;
+    if (B < 0 || Lq < 0 || Lkv < 0 || Lkv > INT32_MAX - 256 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || D % 8 != 0 || D > 256) return -1;
     if (dtype != DT_F16 && dtype != DT_BF16) return -4;
     if (B == 0 || Lq == 0) return 0;
     if (!q || !out || !strides || (Lkv > 0 && (!k || !v)) || off16(q) || off16(k) || off16(v) || off16(out) || ragged(strides, 12)) return -5;

@@ -707,7 +707,8 @@ bool b200q::attention_tc_takes(const AttnParams& p, bool kv8) {
     // done sooner. Over the cache, 8 sequences of 1000 to 8000 tokens and 128 rows for each of 8 kv heads (128 tiles): 219 us here, 124 with 16 rows at
     // a time; one sequence of 8000 and 256 rows: 232 and 63; two of up to 4133 and 4096 rows (1024 tiles): 148 here.
     const int64_t rows = kv8 ? (int64_t)p.Lq * (p.H / p.Hkv) : p.Lq;
-    if (rows < 128 || (rows + 63) / 64 * p.B * (kv8 ? p.Hkv : p.H) < (kv8 ? 160 : 64)) return false;
+    const int64_t few = (kv8 ? 160 : 64) - 1;
+    if (rows < 128 || (rows + 63) / 64 <= few / p.B / (kv8 ? p.Hkv : p.H)) return false;
     // rows without a stride between them have no tensor map
     return kv8 || ((p.Lq == 1 || p.qs[1] > 0) && (p.Lkv == 1 || (p.ks[1] > 0 && p.vs[1] > 0)) && p.qs[0] >= 0 && p.qs[2] >= 0 && p.ks[0] >= 0 &&
                    p.ks[2] >= 0 && p.vs[0] >= 0 && p.vs[2] >= 0 && (p.ks[0] == 0) == (p.vs[0] == 0) && (p.ks[2] == 0) == (p.vs[2] == 0));

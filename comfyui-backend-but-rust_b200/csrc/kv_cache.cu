@@ -181,8 +181,8 @@ GPU_API int gpu_kv8_append(int dtype, const void* k, const void* v, const int64_
         if (strides[i] % (dtype == DT_F32 ? 4 : 8) != 0) return -5;
     AppendParams p = {k, v, {strides[0], strides[1], strides[2]}, {strides[3], strides[4], strides[5]}, k8, v8, k_scale, v_scale, table, start, count,
                       table_stride, pages, B, L, Hkv, D, T, max_pages, (L - 1) / T + 2};
+    if (p.touched > INT32_MAX / 2 / Hkv / B) return -1;
     const int64_t grid = (int64_t)2 * Hkv * p.touched * B;
-    if (grid > INT32_MAX) return -1;
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == DT_F32) return launch_pdl(kv8_append_kernel<float>, dim3((unsigned)grid), 256, 0, st, p);
     if (dtype == DT_F16) return launch_pdl(kv8_append_kernel<half>, dim3((unsigned)grid), 256, 0, st, p);

@@ -235,6 +235,7 @@ template <int XT, int NT, int GB, bool ZP> __global__ void __launch_bounds__(kRo
 }
 
 template <int XT, int GB> int launch_w4(W4Params& p, cudaStream_t st) {
+    if (p.M > 32 / parts_of<XT>()) return w4_tile(XT, p, st);      // before what is counted in 32 bits for few columns
     const int cols = p.M * parts_of<XT>();
     // CTAs along K (a cluster): as few as leave a CTA's share of x and its rings in shared memory. Warps along K in all: four to an SM as long
     // as each has two blocks of K, and up to 32 where each keeps as many blocks as there are columns, so that bringing x in costs less than
@@ -252,7 +253,7 @@ template <int XT, int GB> int launch_w4(W4Params& p, cudaStream_t st) {
     const int kw = max(1, ksplit / p.splits);
     const int tiles = (p.N + 256 / kw - 1) / (256 / kw);
     const RowsShare sh = p.share = rows_share(p.K, p.G, p.splits, kw, cols, p.zeros != nullptr);
-    if (cols <= 32 && sh.smem <= 224 * 1024) {
+    if (sh.smem <= 224 * 1024) {
         auto kern = p.zeros ? (cols <= 8 ? w4_rows_kernel<XT, 1, GB, true> : cols <= 16 ? w4_rows_kernel<XT, 2, GB, true> : cols <= 24 ? w4_rows_kernel<XT, 3, GB, true>
                                                                                                                          : w4_rows_kernel<XT, 4, GB, true>)
                             : (cols <= 8 ? w4_rows_kernel<XT, 1, GB, false> : cols <= 16 ? w4_rows_kernel<XT, 2, GB, false> : cols <= 24 ? w4_rows_kernel<XT, 3, GB, false>
@@ -370,6 +371,7 @@ template <typename T> int launch_dequant(const void* packed, int scale_dt, const
                       N * K, 5 + log2_of(G / 32));
 }
 
+constexpr int kMostRows = INT32_MAX - 1024;      // of x and of the weight: a tile's number and its last row fit 32 bits
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool bad_groups(int64_t N, int K, int G) { return N < 0 || K <= 0 || (G != 32 && G != 64 && G != 128 && G != 256) || K % G != 0; }
 bool bad_scales(int dt) { return dt != DT_F16 && dt != DT_BF16; }
@@ -403,7 +405,7 @@ GPU_API int gpu_w4_dequant(int dtype, const void* packed, int scale_dt, const vo
 
 GPU_API int gpu_w4_linear(int dtype, const void* x, int64_t x_stride, const void* Wq4, int scale_dt, const void* scales, const void* zeros, const void* bias,
                           int out_dt, void* out, int64_t out_stride, float beta, int M, int N, int K, int G, void* stream) {
-    if (bad_groups(N, K, G) || M < 0) return -1;
+    if (bad_groups(N, K, G) || M < 0 || M > kMostRows || N > kMostRows) return -1;
     if (bad_scales(scale_dt) || dtype < DT_F32 || dtype > DT_BF16 || (out_dt != dtype && out_dt != DT_F32)) return -4;
     if (beta != 0.f && beta != 1.f) return -207;
     if (M == 0 || N == 0) return 0;

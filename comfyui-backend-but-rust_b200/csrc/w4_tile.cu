@@ -375,14 +375,14 @@ template <int XT> int launch(const W4Params& w, cudaStream_t st) {
     int64_t best = INT64_MAX;
     const int fewest = (w.M + kMost - 1) / kMost;
     for (int t = fewest; t <= fewest + 3; ++t) {
-        const int tokens = ((w.M + t - 1) / t + kStep - 1) / kStep * kStep;
+        const int tokens = (int)(((int64_t)w.M + t - 1) / t + kStep - 1) / kStep * kStep;
         const int64_t rounds = (row_tiles * t + sms - 1) / sms, cost = rounds * (300 + tokens * P);
         if (cost < best) best = cost, p.token_tiles = t, p.tokens = tokens;
     }
     p.columns = p.tokens * P;
     p.buffers = 512 / p.columns < kBuffers ? 512 / p.columns : kBuffers;
     const int64_t tiles = row_tiles * p.token_tiles;
-    if (tiles > INT32_MAX) return -1;
+    if (tiles > INT32_MAX / 2) return -1;      // and so does a tile a round further on
     p.tiles = (int)tiles;
     // few tiles: a cluster of CTAs to each, every one with whole groups and at least four blocks
     const int all = (w.K + kBlock - 1) / kBlock, unit = w.G > kBlock ? w.G / kBlock : 1;

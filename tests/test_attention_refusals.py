@@ -70,3 +70,12 @@ def test_host_tensors_are_refused(pkg):
                  lambda: L.w4_dequant(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2).half())):
         with pytest.raises(ValueError, match="CUDA tensors only"):
             call()
+
+
+@pytest.mark.parametrize("call,kw", [
+    (_cross, dict(Lkv=2 ** 31 - 64)), (_cross, dict(Lkv=2 ** 31 - 1)), (_cross, dict(Lq=2 ** 31 - 1, H=4, Hkv=1, D=136)), (_cross, dict(Lq=1, B=2 ** 31 - 1, H=2 ** 30, Hkv=2 ** 30)),
+    (_attention, dict(Lq=2 ** 31 - 1, H=2 ** 20, Hkv=1)), (_attention, dict(Lq=1, B=2 ** 31 - 1, H=2 ** 30, Hkv=2 ** 30)),
+    (_append, dict(B=2 ** 31 - 1, L=2 ** 31 - 1, Hkv=2 ** 31 - 1)),
+    (_w4, dict(M=2 ** 31 - 1, x_stride=64)), (_w4, dict(M=2 ** 31 - 100, dtype=0, odt=0)), (_w4, dict(N=2 ** 31 - 1))])
+def test_sizes_that_32_bits_do_not_count(pkg, call, kw):
+    assert call(pkg.lib, **kw) == -1
