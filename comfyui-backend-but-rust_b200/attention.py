@@ -23,7 +23,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     """gpu_cross_attention: softmax(scale q k^T) v. q [B, Lq, H, D], k and v [B, Lkv, Hkv, D], fp16 or bf16, any strides of whole
     16-byte pieces; D a multiple of 8 up to 256; H a multiple of Hkv (head h reads kv head h // (H // Hkv)). Keys from kv_len[b]
     (int32 [B]) on, and those whose key_mask (bool [B, Lkv]) is False, are not seen, whatever they hold; a query that sees none gets
-    zeros. `scale` defaults to D ** -0.5."""
+    zeros. `scale` defaults to D ** -0.5. `out` may be q itself."""
     return _h.cross_attention(q, k, v, kv_len, key_mask, _scale(q, scale), out)
 
 
@@ -48,7 +48,8 @@ class Kv8Cache:
 def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
                count: Optional[torch.Tensor] = None) -> Kv8Cache:
     """gpu_kv8_append: rows k[b, i], v[b, i] ([B, L, Hkv, D], f32 / f16 / bf16) become tokens start[b] + i of sequence b, for i < count[b]
-    (int32 [B]; all L without). A page that a sequence writes belongs to it alone. Rows that fall on no page are dropped."""
+    (int32 [B]; all L without). A page that a sequence writes belongs to it alone, and to one
+    entry of its table. Rows that fall on no page are dropped."""
     _h.kv8_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, table, start, count)
     return cache
 
@@ -62,6 +63,7 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, table: torch.Tensor, lengths
                   causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """gpu_kv8_attention: softmax(scale q k^T) v over the first lengths[b] tokens of each sequence. q [B, L, H, D] fp16 or bf16, H a
     multiple of the cache's heads. The first q_len[b] (all L without) rows of q are the sequence's last tokens: causal, row i sees
-    tokens up to lengths[b] - q_len[b] + i. Rows from q_len[b] on are not written; a row that sees no token gets zeros."""
+    tokens up to lengths[b] - q_len[b] + i. Rows from q_len[b] on are not written; a row that sees no token gets zeros. `out`
+    may be q itself."""
     return _h.kv8_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, lengths, q_len, 1 if causal else 0,
                             _scale(q, scale), out)

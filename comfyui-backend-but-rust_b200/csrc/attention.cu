@@ -537,6 +537,9 @@ bool ragged(const int64_t* s, int n) {
     return false;
 }
 
+// Rows of the result in the same place
+bool shared_rows(const int64_t* s, int B, int Lq, int H) { return (B > 1 && s[0] == 0) || (Lq > 1 && s[1] == 0) || (H > 1 && s[2] == 0); }
+
 }  // namespace
 
 GPU_API int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides, const int32_t* kv_len,
@@ -544,7 +547,8 @@ GPU_API int gpu_cross_attention(int dtype, const void* q, const void* k, const v
     if (B < 0 || Lq < 0 || Lkv < 0 || Lkv > INT32_MAX - 256 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || D % 8 != 0 || D > 256) return -1;
     if (dtype != DT_F16 && dtype != DT_BF16) return -4;
     if (B == 0 || Lq == 0) return 0;
-    if (!q || !out || !strides || (Lkv > 0 && (!k || !v)) || off16(q) || off16(k) || off16(v) || off16(out) || ragged(strides, 12)) return -5;
+    if (!q || !out || !strides || (Lkv > 0 && (!k || !v)) || off16(q) || off16(k) || off16(v) || off16(out) || ragged(strides, 12) || shared_rows(strides + 9, B, Lq, H))
+        return -5;
     AttnParams p = {};
     p.q = q, p.k = k, p.v = v, p.out = out, p.kv_len = kv_len, p.mask = key_mask, p.mask_stride = mask_stride;
     for (int i = 0; i < 3; ++i) p.qs[i] = strides[i], p.ks[i] = strides[3 + i], p.vs[i] = strides[6 + i], p.os[i] = strides[9 + i];
@@ -561,7 +565,7 @@ GPU_API int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t
     if (dtype != DT_F16 && dtype != DT_BF16) return -4;
     if ((int64_t)max_pages * T > INT32_MAX - 256) return -1;
     if (B == 0 || Lq == 0) return 0;
-    if (!q || !out || !strides || !lengths || off16(q) || off16(out) || off16(k8) || off16(v8) || ragged(strides, 6)) return -5;
+    if (!q || !out || !strides || !lengths || off16(q) || off16(out) || off16(k8) || off16(v8) || ragged(strides, 6) || shared_rows(strides + 3, B, Lq, H)) return -5;
     if (max_pages > 0 && pages > 0 && (!k8 || !v8 || !k_scale || !v_scale || !table)) return -5;
     AttnParams p = {};
     p.q = q, p.k = k8, p.v = v8, p.out = out, p.k_scale = k_scale, p.v_scale = v_scale, p.table = table, p.table_stride = table_stride, p.pages = pages;

@@ -523,6 +523,24 @@ def test_pages_shared_by_sequences(pkg, dev, Lq):
     _kv8_check(pkg.attention.kv8_attention(q, c, table, torch.tensor(lens, dtype=torch.int32, device=dev)), q, c, table, lens, [Lq] * 3, True, 64 ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("Lq", [1, 70, 700])
+def test_in_place_of_the_queries(pkg, dev, Lq, dtype):
+    A = pkg.attention
+    g = torch.Generator().manual_seed(Lq)
+    B, H, Hkv, D = 2, 24, 8, 64
+    c, table = _cache(pkg, dev, g, B, [1500, 900], Hkv, D, 32)
+    n = torch.tensor([1500, 900], dtype=torch.int32, device=dev)
+    q = torch.randn(B, Lq, H, D, generator=g).to(DT[dtype]).to(dev)
+    kv = torch.randn(B, 600, Hkv, D, generator=g).to(DT[dtype]).to(dev)
+    for call in (lambda q, out: A.kv8_attention(q, c, table, n, out=out), lambda q, out: A.cross_attention(q, kv, kv, out=out)):
+        want = call(q, None)
+        for _ in range(3):
+            x = q.clone()
+            call(x, x)
+            assert torch.equal(x, want)
+
+
 def test_rows_beyond_the_last_and_zero_sizes(pkg, dev):
     """No pages at all, no tokens, a negative length: zeros, or nothing written."""
     A = pkg.attention

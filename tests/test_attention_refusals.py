@@ -79,3 +79,11 @@ def test_host_tensors_are_refused(pkg):
     (_w4, dict(M=2 ** 31 - 1, x_stride=64)), (_w4, dict(M=2 ** 31 - 100, dtype=0, odt=0)), (_w4, dict(N=2 ** 31 - 1))])
 def test_sizes_that_32_bits_do_not_count(pkg, call, kw):
     assert call(pkg.lib, **kw) == -1
+
+
+@pytest.mark.parametrize("call,at,kw", [(_cross, 9, dict(B=2)), (_cross, 10, dict(Lq=2)), (_cross, 11, dict(H=4)), (_attention, 3, dict(B=2)), (_attention, 4, dict(Lq=2)),
+                                        (_attention, 5, dict(H=4))])
+def test_rows_of_the_result_in_one_place(pkg, call, at, kw):
+    strides = (C.c_int64 * 12)(*S)
+    strides[at] = 0
+    assert call(pkg.lib, strides=strides, **kw) == -5
