@@ -9,7 +9,7 @@
 namespace b200q {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kTiny = 1e-30f;          // the smallest scale of a page; smaller ones are taken for it
+constexpr float kTiny = 1e-30f;          // the smallest scale of a page that the cache's writer gives; attention takes smaller ones for it
 
 struct AttnParams {
     const void *q, *k, *v;

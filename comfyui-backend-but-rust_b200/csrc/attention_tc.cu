@@ -325,7 +325,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         // ---- products
         const uint32_t idesc_s = umma_idesc_16(kBf16Mma, false, 128, kTileKeys), idesc_o = umma_idesc_16(kBf16Mma, true, 128, DP);
         const bool one = elect_one();
-        uint32_t kv_no = 0, q_no[2] = {}, p_phase[2] = {}, tile_no = 0, o_phase[2] = {1, 1};
+        uint32_t kv_no = 0, q_no[2] = {}, p_phase[2] = {}, o_phase[2] = {1, 1};
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity, int code) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, code)); };
         auto issue_s = [&](int t, uint32_t slot) {
@@ -359,7 +359,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             }
             if (!ok) break;
             if (one) umma_commit(kv_empty + 8 * ks);
-            for (int j = 0; j < x.n; ++j, ++tile_no) {
+            for (int j = 0; j < x.n; ++j) {
                 const uint32_t v_no = kv_no + 1, vs = v_no & 3;
                 const bool more = j + 1 < x.n;
                 if (!wait(kv_full + 8 * vs, v_no >> 2 & 1, ST_TIMEOUT_FULL)) break;

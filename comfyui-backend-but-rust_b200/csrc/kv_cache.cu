@@ -5,12 +5,11 @@
 //
 // k8, v8 int8 [pages, Hkv, T, D], one f32 scale for each page and head: a value is code * scale. Sequence b's token i is row i % T of page
 // table[b, i / T]. The T rows of a page and head are contiguous: what attention reads for one head is whole runs of T * D bytes.
-#include "common.cuh"
-#include "mma.cuh"
+#include "attention.cuh"
 
 namespace {
 
-constexpr float kTiny = 1e-30f;      // the smallest scale that is written
+using namespace b200q;
 
 struct AppendParams {
     const void *k, *v;
@@ -22,16 +21,6 @@ struct AppendParams {
     int B, L, Hkv, D, T, max_pages, touched;      // touched: pages that L rows can reach
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
-    const uint4 r = gload(reinterpret_cast<const uint4*>(src));
-    const T* h = reinterpret_cast<const T*>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f<T>(h[i]);
-}
-template <> __device__ __forceinline__ void load8<float>(const float* src, float (&v)[8]) {
-    const float4 a = gload(reinterpret_cast<const float4*>(src)), b = gload(reinterpret_cast<const float4*>(src) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
 __device__ __forceinline__ uint32_t pack4(const float* c) {
     return ((uint32_t)(int)c[0] & 255u) | ((uint32_t)(int)c[1] & 255u) << 8 | ((uint32_t)(int)c[2] & 255u) << 16 | (uint32_t)(int)c[3] << 24;
 }

@@ -56,6 +56,18 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Eight neighbouring values in f32
+template <typename T> __device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
+    const uint4 r = gload(reinterpret_cast<const uint4*>(src));
+    const T* h = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f<T>(h[i]);
+}
+template <> __device__ __forceinline__ void load8<float>(const float* src, float (&v)[8]) {
+    const float4 a = gload(reinterpret_cast<const float4*>(src)), b = gload(reinterpret_cast<const float4*>(src) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<half>(float lo, float hi) {
     const half2 h = __floats2half2_rn(lo, hi);

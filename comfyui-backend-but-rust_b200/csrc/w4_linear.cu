@@ -269,18 +269,6 @@ template <int XT> int launch_w4_groups(W4Params& p, cudaStream_t st) {
 
 // ---- the packer and its inverse -----------------------------------------------------------------------------------------------------
 
-// Eight neighbouring values in f32
-template <typename T> __device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
-    const uint4 r = gload(reinterpret_cast<const uint4*>(src));
-    const T* h = reinterpret_cast<const T*>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f<T>(h[i]);
-}
-template <> __device__ __forceinline__ void load8<float>(const float* src, float (&v)[8]) {
-    const float4 a = gload(reinterpret_cast<const float4*>(src)), b = gload(reinterpret_cast<const float4*>(src) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-
 // Word e of values side by side
 __device__ __forceinline__ uint32_t bits32(const float* v, int e) { return __float_as_uint(v[e]); }
 __device__ __forceinline__ uint32_t bits32(const half* v, int e) { return (uint32_t)__half_as_ushort(v[2 * e]) | (uint32_t)__half_as_ushort(v[2 * e + 1]) << 16; }
