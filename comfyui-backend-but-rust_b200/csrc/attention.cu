@@ -5,7 +5,9 @@
 //
 // o[i] = sum_t p[i, t] v[t] / sum_t p[i, t],  p[i, t] = exp(scale q[i] . k[t] - m[i]), m[i] the largest exponent seen so far; a row that sees
 // no key is zeros. One pass over the keys: the sums are scaled when m grows. Exponents, m and both sums are f32; p is rounded to the type
-// of the matrix product (as its operands have to be) after it entered the sum of p, so that the rounding is at most half a step of each term.
+// of the matrix product (as its operands have to be: q's for 16-bit keys, fp16 over the cache) after it entered the sum of p. That is at most
+// half a step of each term, and below fp16's normal numbers at most 2^-25 of the largest p: keys far below the maximum may count in the sum of
+// p and not in the result.
 #include "attention.cuh"
 
 namespace {
@@ -191,7 +193,9 @@ template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
 // codes as they lie in memory, because the order of a product's inner index is free as long as both operands have it: a lane multiplies 16
 // neighbouring values of a key with the same 16 of its query row, and in p . v its column 16 g + j of every key stands for column g of the
 // product's j-th tile. So codes are read from shared memory in 16-byte pieces and nothing is transposed. Measured (32 heads over 8 of 128): a
-// token over 1999 keys 8.4 us, 16 tokens over up to 32768 keys 120 us (4.5 TB/s; about 500 instructions to 4 KB of codes).
+// token over 1999 keys 8.6 us; 16 tokens over up to 32768 keys 121 us on the same buffers again and again, 124 to 130 on new ones (4.1 to 4.3
+// TB/s). 475 warp instructions to 4 KB of codes take half of the issue slots: with four warps to a scheduler 6.9 cycles pass between two of a
+// warp's instructions, 2.0 of them fixed latencies, 0.8 the integer pipe (44 % busy), 0.8 the other warps' turns.
 constexpr int kRowsWarps = 8, kRowsStages = 3;
 constexpr float kSlack = 8.f;
 

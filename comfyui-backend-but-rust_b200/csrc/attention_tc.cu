@@ -19,8 +19,9 @@
 // its own (o_full). Between two completions of s_full there is the p_full that answers the first, between two of o_full an item's p_full.
 // tests/test_attention_order.py goes through the roles' orders.
 // Measured: 1.83 us a step of 256 rows, 128 keys and 128 columns (the products 1.1 at the tensor rate, the exponentials as much: 16 a cycle);
-// 2048 keys 1210 TFLOP/s, 512 keys 955 (806 with a mask, new inputs each time), 128 keys at the pace of the rows' way in and out. Over the
-// cache, chunks of 1024 tokens 478 TFLOP/s.
+// 16384 rows, 24 heads of 128: 2048 keys 1214 TFLOP/s, 512 keys 924, 785 with a mask (727 one call at a time on new inputs). At most 128 keys:
+// a chain of two products, softmax and the rows' way for each item. Over the cache, chunks of 1024 tokens 470 TFLOP/s: a step of 128 keys waits
+// for the softmax, whose exponentials and products each take a quarter of the time, issue slots 31 %.
 // Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds.
 #include "attention.cuh"
 #include "umma16.cuh"
@@ -171,7 +172,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
         const float c = p.a.scale * kLog2e;
         uint8_t* stage = sm + L::kStaging + warp * 2048;
-        uint32_t s_phase = 0, o_phase = 0, tile_no = 0, item_no = 0;
+        uint32_t s_phase = 0, tile_no = 0, item_no = 0;
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
             const Item x = item_at<KV8>(p, item_of(r), order);
@@ -284,8 +285,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (!KV8) continue;
             // ---- the rows out: 32 columns at a time through this warp's staging, so that a row's pieces are stored together
             if (x.n > 0) {
-                if (!__all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, o_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
-                o_phase ^= 1, ++item_no;
+                if (!__all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, item_no & 1, abort_s, ST_TIMEOUT_TMEM_FULL))) break;
+                ++item_no;
                 tc_fence_after();
             }
             const float inv = l > 0.f || l != l ? 1.f / l : 0.f;

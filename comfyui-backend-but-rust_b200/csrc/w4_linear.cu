@@ -38,7 +38,7 @@ __device__ __forceinline__ void cp_async_wait_all_but(int n) {
 // fixed order. A warp keeps ST - 1 stages of its own rows in flight (nothing is shared, so nothing waits for another warp). x, the scales
 // and the zero points of the CTA's share of K are brought into shared memory once, x in the order in which codes come out of a word. Each
 // group's sum is in f32 and added to the total times its scale. Measured: 1 x 2560 -> 19456 bf16 10.8 us (25.7 MB: 3.9 at the DRAM's rate; some 4
-// are the loop, the rest its beginning and end), 8 x 9728 -> 2560 14.3, 16 x 5120 -> 13824 fp16 26.8, 5 x 9728 -> 2563 f32 18.
+// are the loop, the rest its beginning and end), 8 x 9728 -> 2560 13.5, 16 x 5120 -> 13824 fp16 27, 5 x 9728 -> 2563 f32 18.
 constexpr int kRowsStages = 4, kRowsWarps = 8, kRowsStage = 2 * kStageBytes;
 
 inline int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v >> 1); }

@@ -9,9 +9,11 @@
 // Warps 0-3 and 4-7: sums, for the first and second half of the columns. Warps 8-11: codes from global memory (each its 32 rows, a ring of its
 // own) to operands, K-major with the 128-byte swizzle, a row to a lane; for f32 x also its three terms. Warp 12 issues the products, warp 13
 // loads 16-bit x by TMA.
-// Measured: 333 x 5120 -> 13824 fp16, groups of 64, 142 us (332 TFLOP/s); 64 x 5120 -> 13824 bf16, groups of 128, 39; 512 x 2560 -> 19456 f32 379. A block of 64
-// of K takes 0.6 to 0.7 us whatever the columns: a group's way from the end of its product to the next one's start, through a warp's wait, its
-// reads of tensor memory and its arrival, is what bounds it.
+// Measured, 5120 -> 13824 fp16, us for groups of 32 | 64 | 128 | 256: 112 tokens 99 | 58 | 38 | 36 (a tile an SM), 333 tokens 231 | 143 | 86 | 81 (two tiles of 176
+// columns; 330 and 545 TFLOP/s at 64 and 128). So there are two bounds. A block of 64 of K takes 0.45 us with 112 columns and 0.5 with 176 where groups are long:
+// its codes' way through four warps. A group takes 0.6 to 0.7 us with 112 columns and 0.7 to 0.9 with 176: its way from tensor memory into the sums, which
+// spill there (384 bytes a thread with fp16, 224 with bf16, 530 with f32 x). Issue slots 42 %, tensor pipe 14 % at 333 tokens, groups of 64.
+// f32 x: 32 | 77 | 512 x 2560 -> 19456, groups of 128, 80 | 126 | 382 us: x's three terms are made again by every row tile, codes by every 64 tokens.
 // Every wait is bounded; one that runs out is recorded in g_w4_status and the CTA unwinds.
 #include "umma16.cuh"
 #include "w4.cuh"
@@ -371,7 +373,7 @@ template <int XT> int launch(const W4Params& w, cudaStream_t st) {
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
     const int64_t row_tiles = (w.N + kRows - 1) / kRows;
     // The number of token tiles that costs least: rounds of tiles over the SMs times what a tile takes, which grows with its columns from a
-    // start of some 300 (a block takes 0.67 us with 112 columns and 0.7 with 176: the sums' way out of tensor memory, a group at a time).
+    // start of some 300 (a block takes 0.73 us with 112 columns and 0.91 with 176 at groups of 64, 0.48 and 0.56 at 128).
     int64_t best = INT64_MAX;
     const int fewest = (w.M + kMost - 1) / kMost;
     for (int t = fewest; t <= fewest + 3; ++t) {

@@ -253,7 +253,8 @@ int gpu_w4_linear(int dtype, const void* x, int64_t x_stride, const void* Wq4, i
  * gpu_kv8_attention  q, out [B, Lq, H, D] f16 or bf16 (strides = 6 HOST values: of q, then of out; H % Hkv == 0): out = softmax(scale q k^T) v over
  *                    tokens < lengths[b]. Rows i < q_len[b] (NULL: Lq) are the sequence's last tokens: with causal != 0 row i sees
  *                    tokens <= lengths[b] - q_len[b] + i. Rows from q_len[b] on are not written; a row that sees no token is zeros.
- *                    Needs no workspace. bf16 queries are taken as fp16 times a power of two per row (values below 2^-29 of their row's largest lose bits).
+ *                    Needs no workspace. bf16 queries are taken as fp16 times a power of two per row (values below 2^-29 of their row's largest lose bits). p
+ *                    is rounded to fp16 for its product with v (below 2^-25 of the largest it is 0 there), f32 otherwise.
  *                    out may be q itself and overlaps nothing else that the call reads.
  * Errors: -1 sizes, -4 types, -5 a NULL, rows off a 16-byte boundary (strides in whole 16 bytes; gpu_kv8_dequant's k and v: 32) or rows of out
  * that share their place (a stride of 0), -203 descriptor. */
@@ -270,7 +271,7 @@ int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t* stride
 
 /* New: cross attention to an encoder's states, out = softmax(scale q k^T) v without the scores in memory. q, out [B, Lq, H, D], k, v
  * [B, Lkv, Hkv, D], f16 or bf16 (strides = 12 HOST values, in elements: batch, row, head of q, k, v, out); D a multiple of 8 up to 256; H % Hkv == 0. Keys >= kv_len[b] and keys
- * with key_mask[b * mask_stride + t] == 0 (either may be NULL) are not seen, whatever they hold; a row that sees none is zeros. out may be q itself and overlaps nothing else that the call reads.
+ * with key_mask[b * mask_stride + t] == 0 (either may be NULL) are not seen, whatever they hold; a row that sees none is zeros. p is rounded to q's type for its product with v, f32 otherwise. out may be q itself and overlaps nothing else that the call reads.
  * Errors as above. Stands between gpu_int8_gemm of q, k, v and gpu_sd_quant_rows / gpu_quant_rows of its result. */
 int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides,
                         const int32_t* kv_len, const uint8_t* key_mask, int64_t mask_stride, int B, int Lq, int Lkv, int H, int Hkv,
