@@ -31,9 +31,10 @@ class Barriers:
                     raise Hazard(f"{bar} completed again before {who} saw the completion before")
 
 
-def _run(actors, counts, choose):
-    """actors: name -> generator of ("wait", bar, n-th completion), ("arrive", bar) or a callable. n = 0 passes at once. Everybody who ever waits for
-    a barrier has to see each of its completions that it waits for in turn."""
+def _run(actors, counts, held=None, stop=0, rng=None):
+    """actors: name -> list of ("wait", bar, n-th completion), ("arrive", bar) or ("do", callable). n = 0 passes at once. Everybody who ever waits for
+    a barrier has to see each of its completions that it waits for in turn. `held` stands at its stop-th step until nobody else can go on;
+    with `rng` who goes next, and how far, is drawn."""
     bars = Barriers(counts)
     waits = {}
     for name, ops in actors.items():
@@ -45,27 +46,41 @@ def _run(actors, counts, choose):
     bars.seen = {key: 0 for key in waits}
     at = dict.fromkeys(actors, 0)
 
-    def ready(name):
+    def step(name):
+        """False when it has to wait or is through."""
         if at[name] == len(actors[name]):
             return False
         op = actors[name][at[name]]
-        return op[0] != "wait" or bars.done[op[1]] >= op[2]
-
-    while True:
-        able = [name for name in actors if ready(name)]
-        if not able:
-            break
-        name = choose(able, at)
-        op = actors[name][at[name]]
-        at[name] += 1
-        if op[0] == "wait" and op[2] > 0:
-            bars.seen[op[1], name] = op[2]
-            if op[2] == len(waits[op[1], name]):
-                del bars.seen[op[1], name]                 # it waits for this barrier no more
+        if op[0] == "wait":
+            if bars.done[op[1]] < op[2]:
+                return False
+            if op[2] > 0:
+                bars.seen[op[1], name] = op[2]
+                if op[2] == len(waits[op[1], name]):
+                    del bars.seen[op[1], name]             # it waits for this barrier no more
         elif op[0] == "arrive":
             bars.arrive(op[1])
-        elif op[0] == "do":
+        else:
             op[1]()
+        at[name] += 1
+        return True
+
+    if rng is not None:
+        names = list(actors)
+        for _ in range(300):
+            rng.shuffle(names)
+            for name in names:
+                for _ in range(rng.choice((0, 0, 1, 3, 40))):
+                    if not step(name):
+                        break
+    going = True
+    while going:
+        going = False
+        for name in actors:
+            while not (name == held and at[name] == stop) and step(name):
+                going = True
+        if not going and held is not None:
+            held, going = None, True
     stuck = [name for name in actors if at[name] < len(actors[name])]
     if stuck:
         raise Hazard(f"nobody can go on: {stuck}")
@@ -334,22 +349,13 @@ def _rows_form(items, slot_by_tile=True, with_p=True):
 
 
 def _go_through(build, items, **kw):
-    actors, _ = build(items, **kw)
-    for held in actors:
+    for held, ops in build(items, **kw)[0].items():
         if held != "tensor cores":
-            for stop in range(len(actors[held])):
-                a, c = build(items, **kw)
-
-                def choose(able, at):
-                    # the one held back stands at its stop-th step until nobody else can go on
-                    others = [x for x in able if x != held or at[x] != stop]
-                    return (others or able)[0]
-                _run(a, c, choose)
+            for stop in range(len(ops)):
+                _run(*build(items, **kw), held, stop)
     rng = random.Random(0)
-    for _ in range(30):
-        a, c = build(items, **kw)
-        slow = {x: rng.random() ** 3 for x in a}
-        _run(a, c, lambda able, at: rng.choices(able, [slow[x] + 1e-9 for x in able])[0])
+    for _ in range(20):
+        _run(*build(items, **kw), rng=rng)
 
 
 @pytest.mark.parametrize("items", RUNS)
