@@ -22,7 +22,8 @@
 // 16384 rows, 24 heads of 128: 2048 keys 1214 TFLOP/s, 512 keys 924, 785 with a mask (727 one call at a time on new inputs). At most 128 keys:
 // a chain of two products, softmax and the rows' way for each item. Over the cache, chunks of 1024 tokens 470 TFLOP/s: a step of 128 keys waits
 // for the softmax, whose exponentials and products each take a quarter of the time, issue slots 31 %.
-// Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds.
+// Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds. Two kinds of wait can be as long as whole items:
+// for sums, and for the logits of a second row tile behind items that have none. Their limit counts from the last key tile that was multiplied.
 #include "attention.cuh"
 #include "umma16.cuh"
 
@@ -38,7 +39,7 @@ constexpr float kSlack = 8.f;                                      // by how muc
 template <int DP, bool KV8> struct Tc {
     static constexpr int kTile = DP / 64 * kBox;                   // 128 rows of Q, K or V
     static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + (KV8 ? 8 * 2048 : 4 * 4096);
-    // barriers and two words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
+    // barriers and three words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
     // item of the tile % 2: l of every row (16-bit), or bf16 queries' powers of two
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
     static constexpr int kOrder = kRowInfo + 2048, kEnd = kOrder + 128, kSmem = kEnd + 1024;
@@ -76,6 +77,26 @@ __device__ __forceinline__ void umma_16_ts(uint32_t d, uint32_t a, uint32_t b_lo
 // V lies with its columns side by side: rows of 64 columns, 8 keys to a swizzle atom (1024 bytes apart, the stride offset); the next 64
 // columns are a box further on (the leading offset).
 __device__ __forceinline__ uint32_t umma_desc_lo_n_major(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | ((uint32_t)(kBox >> 4) << 16); }
+
+// mbar_wait whose limit begins anew whenever *moving has changed
+__device__ __forceinline__ bool mbar_wait_moving(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code, const volatile uint32_t* moving) {
+    if (mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    uint32_t last = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 63u) == 0u) {
+            if (*abort_flag) return false;
+            const uint64_t now = globaltimer_ns();
+            const uint32_t at = *moving;
+            if (t0 == 0 || at != last) t0 = now, last = at;
+            else if (now - t0 > kWaitLimitNs) {
+                *abort_flag = code;
+                return false;
+            }
+        }
+    }
+}
 
 struct TcParams {
     AttnParams a;
@@ -126,6 +147,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                    o_full = bars + 128, o_empty = bars + 144, p_early = bars + 160, v_ready = bars + 176;
     uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 192);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
+    volatile uint32_t* moving = tmem_s + 2;                                   // key tiles multiplied
     uint32_t* words = reinterpret_cast<uint32_t*>(sm + L::kWords);            // [key tile % 4][4]: bit = key is seen
     // [key tile % 4]: 16-bit: [key] +inf, or -inf where a key is not seen; cache: [factor, offset, weight][16 keys]
     float* info = reinterpret_cast<float*>(sm + L::kInfo);
@@ -137,7 +159,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
         for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
             mbar_init(o_full + 8 * t, 2), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
-        *abort_s = 0;
+        *abort_s = 0, *moving = 0;
         fence_mbar_init();
         if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
     }
@@ -185,7 +207,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             // keys that this row sees
             const int bound = KV8 && p.a.causal ? x.len - x.ql + (x.row0 + t * 128 + row) / ratio + 1 : x.seen;
             for (int j = 0; j < x.n; ++j, ++tile_no) {
-                if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, mbar_wait_moving(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL, moving))) { ok = false; break; }
                 s_phase ^= 1;
                 tc_fence_after();
                 const uint32_t* w = words + (tile_no & 3) * 4;
@@ -401,6 +423,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     if (more) umma_commit(kv_empty + 8 * ks);
                 }
                 kv_no += 2;
+                if (one) *moving = kv_no;
             }
         }
       } else if (!KV8 && warp == 9) {
@@ -497,7 +520,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             for (int t = 0; t < 2 && t * 128 < x.rows; ++t) {
                 float inv = 0.f;
                 if (x.n > 0) {
-                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, phase[t], abort_s, ST_TIMEOUT_TMEM_FULL)))) break;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait_moving(o_full + 8 * t, phase[t], abort_s, ST_TIMEOUT_TMEM_FULL, moving)))) break;
                     phase[t] ^= 1;
                     tc_fence_after();
                     const float l = row_info[(item_no[t]++ & 1) * 256 + t * 128 + quarter * 32 + lane];
@@ -702,7 +725,6 @@ template <typename QT, int DP, bool KV8> int launch_tc(const CUtensorMap (&tm)[3
 }  // namespace
 
 bool b200q::attention_tc_takes(const AttnParams& p, bool kv8) {
-    // (the rows' way out waits for a whole item: at 2^26 keys that is half of a wait's limit)
     if (p.D > 128 || !(p.scale > 0.f) || p.Lkv <= 0 || p.Lkv > 1 << 26) return false;
     // Half an item's rows at least, and enough tiles of 64 rows: with fewer the other kernels, which share a row tile's keys among CTAs, are
     // done sooner. Over the cache, 8 sequences of 1000 to 8000 tokens and 128 rows for each of 8 kv heads (128 tiles): 219 us here, 124 with 16 rows at

@@ -486,6 +486,48 @@ def test_pages_beyond_32_bits(pkg, dev):
         _kv8_check(A.kv8_attention(q, c, table, n), q, c, table, [300, 290], [L, L], True, D ** -0.5)
 
 
+@pytest.mark.parametrize("Lq,Lkv,H", [(128, 2 ** 26, 64), (128, 2 ** 26 + 77, 64), (2, 2 ** 25 + 5, 8)])
+def test_very_many_keys(pkg, dev, Lq, Lkv, H):
+    """A few keys spread over the whole length have logits of about 60, all others 0: together less than 2^27 e^-60 = 1.2e-18 of the sums, so that the rows
+    are those of the few keys alone."""
+    g = torch.Generator().manual_seed(Lq + Lkv)
+    D = 64
+    k, v = (torch.zeros(1, Lkv, 1, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    at = torch.tensor([0, 1, 127, 128, Lkv // 3, Lkv // 2, 2 ** 23 + 1, Lkv - 129, Lkv - 1], device=dev)
+    k[0, at, 0] = (1 + 0.05 * torch.randn(len(at), D, generator=g)).bfloat16().to(dev)
+    v[0, at, 0] = torch.randn(len(at), D, generator=g).bfloat16().to(dev)
+    q = (7.5 + 0.1 * torch.randn(1, Lq, H, D, generator=g)).bfloat16().to(dev)
+    got = pkg.attention.cross_attention(q, k, v)
+    few = torch.ones(1, len(at), dtype=torch.bool, device=dev)
+    _cross_check(got, q, k[:, at], v[:, at], few, D ** -0.5)
+    assert pkg.linear.kernel_status() == 0
+
+
+@pytest.mark.parametrize("Lq,Hkv,pages", [(1, 8, 2 ** 14), (256, 96, 2 ** 11)])
+def test_very_many_tokens_of_the_cache(pkg, dev, Lq, Hkv, pages):
+    """The same over the cache: two million tokens for single rows, a quarter of a million for many."""
+    g = torch.Generator().manual_seed(pages)
+    D, T = 64, 128
+    n = pages * T - 5
+    c = pkg.attention.Kv8Cache.empty(pages, Hkv, D, T, dev)
+    c.k_scale.fill_(0.01), c.v_scale.fill_(0.02)
+    table = torch.randperm(pages, generator=g).to(torch.int32).to(dev)[None]
+    at = torch.tensor([0, 1, 127, 128, n // 3, n // 2, n - 300, n - 257], device=dev)
+    page, row = table[0, at // T].long(), at % T
+    k8 = torch.randint(90, 110, (len(at), Hkv, D), generator=g, dtype=torch.int32).to(torch.int8).to(dev)
+    v8 = torch.randint(-127, 128, (len(at), Hkv, D), generator=g, dtype=torch.int32).to(torch.int8).to(dev)
+    for i in range(len(at)):
+        c.k[page[i], :, row[i]], c.v[page[i], :, row[i]] = k8[i], v8[i]
+    q = (7.5 + 0.1 * torch.randn(1, Lq, Hkv, D, generator=g)).half().to(dev)
+    got = pkg.attention.kv8_attention(q, c, table, torch.tensor([n], dtype=torch.int32, device=dev))
+    few = torch.ones(Lq, len(at), dtype=torch.bool, device=dev)
+    step = [float(c.k_scale[0, 0]), float(c.v_scale[0, 0])]
+    for h in range(Hkv):
+        want, a, rest = _reference(q[0, :, h].double(), k8[:, h].double() * step[0], v8[:, h].double() * step[1], few, D ** -0.5)
+        _check(got[0, :, h], want, a, rest, 2.0 ** -11)
+    assert pkg.linear.kernel_status() == 0
+
+
 @pytest.mark.parametrize("Lq", [1, 40, 600])
 def test_two_streams_at_once_and_ordinary_launches(pkg, dev, Lq):
     """Nothing is shared between calls: two at a time give what one gives. Beside a collective's kernels launches are ordinary ones."""
