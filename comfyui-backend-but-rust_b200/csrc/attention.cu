@@ -193,7 +193,7 @@ template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
 // codes as they lie in memory, because the order of a product's inner index is free as long as both operands have it: a lane multiplies 16
 // neighbouring values of a key with the same 16 of its query row, and in p . v its column 16 g + j of every key stands for column g of the
 // product's j-th tile. So codes are read from shared memory in 16-byte pieces and nothing is transposed. Measured (32 heads over 8 of 128): a
-// token over 1999 keys 8.6 us; 16 tokens over up to 32768 keys 121 us on the same buffers again and again, 124 to 130 on new ones (4.1 to 4.3
+// token over 1999 keys 8.6 us; 16 tokens over up to 32768 keys 121 us on the same buffers again and again, 124 to 131 on new ones (4.1 to 4.3
 // TB/s). 475 warp instructions to 4 KB of codes take half of the issue slots: with four warps to a scheduler 6.9 cycles pass between two of a
 // warp's instructions, 2.0 of them fixed latencies, 0.8 the integer pipe (44 % busy), 0.8 the other warps' turns.
 constexpr int kRowsWarps = 8, kRowsStages = 3;

@@ -19,7 +19,7 @@
 // its own (o_full). Between two completions of s_full there is the p_full that answers the first, between two of o_full an item's p_full.
 // tests/test_attention_order.py goes through the roles' orders.
 // Measured: 1.83 us a step of 256 rows, 128 keys and 128 columns (the products 1.1 at the tensor rate, the exponentials as much: 16 a cycle);
-// 16384 rows, 24 heads of 128: 2048 keys 1214 TFLOP/s, 512 keys 924, 785 with a mask (727 one call at a time on new inputs). At most 128 keys:
+// 16384 rows, 24 heads of 128: 2048 keys 1214 TFLOP/s, 512 keys 924, 785 with a mask (720 one call at a time on new inputs). At most 128 keys:
 // a chain of two products, softmax and the rows' way for each item. Over the cache, chunks of 1024 tokens 470 TFLOP/s: a step of 128 keys waits
 // for the softmax, whose exponentials and products each take a quarter of the time, issue slots 31 %.
 // Every wait is bounded; one that runs out is recorded in g_attention_status and the CTA unwinds. Two kinds of wait can be as long as whole items:
