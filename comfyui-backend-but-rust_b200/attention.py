@@ -1,11 +1,13 @@
 """Host side of the attention that stands between the quantized linears, over torch CUDA tensors: cross attention to an encoder's
-states (a U-Net's or DiT's image rows over a prompt's), and the cache of int8 keys and values that a text encoder's or a video
-model's steps fill and attend to. torch supplies device memory and the stream only.
+states (a U-Net's or DiT's image rows over a prompt's), attention of packed sequences to themselves (whole prompts), the cache of int8 keys
+and values that a text encoder's or a video model's steps fill and attend to, and the rotary positions of queries and keys before
+either. torch supplies device memory and the stream only.
 
 Every call runs on the device of its tensors, on that device's current stream.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -67,3 +69,43 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, table: torch.Tensor, lengths
     may be q itself."""
     return _h.kv8_attention(cache.k, cache.v, cache.k_scale, cache.v_scale, q, table, lengths, q_len, 1 if causal else 0,
                             _scale(q, scale), out)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, *, causal: bool = True, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gpu_packed_attention: sequences one behind the other, each over itself. q [rows, H, D], k and v [rows, Hkv, D], fp16 or bf16, any
+    strides of whole 16-byte pieces; D a multiple of 8 up to 256; H a multiple of Hkv (head h reads kv head h // (H // Hkv)). Sequence b is
+    rows offsets[b] to offsets[b + 1] (int32 [B + 1] on the device, ascending). Causal, a row sees the rows of its sequence up to itself.
+    Rows outside every sequence are not written (zeros in a new result). `scale` defaults to D ** -0.5. `out` may be q itself."""
+    return _h.packed_attention(q, k, v, offsets, 1 if causal else 0, _scale(q, scale), out)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freq: torch.Tensor, *, interleaved: bool = False,
+           axis: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+           scale: float = 1.0, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """gpu_rotary: (q, k) turned by their positions. q [B, L, H, D], k [B, L, Hkv, D] or None, f32 / f16 / bf16. The pairs of the first
+    2 * len(freq) values of a head -- the first half with the second, or neighbours if `interleaved` -- turn by positions * freq radians (f64,
+    rope_frequencies) and grow by `scale`. positions int32 [B, L]; or [axes, B, L] with `axis` (uint8 [len(freq)]) saying whose position turns which
+    pair. With q_norm, k_norm (f32 [D]) heads are RMS-normalised first. The outs may be q and k themselves."""
+    return _h.rotary(q, k, positions, freq, 1 if interleaved else 0, axis, q_norm, k_norm, eps, scale, q_out, k_out)
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0, trained: int = 4096, slow: float = 1.0,
+                     fast: float = 32.0, device="cuda"):
+    """(freq, scale) for `rotary`: freq f64 [rot / 2], base^(-2 i / rot) radians a position, stretched for contexts `factor` times as long as the
+    `trained` ones: "linear" divides all of them; "base" takes a base under which the slowest turns 1 / factor as fast and the fastest as
+    before; "bands" divides those that turn less than `slow` times in `trained` positions, keeps those that turn more than `fast` times, goes over
+    from one to the other in proportion (Peng et al., 2023), and has scale = 0.1 ln(factor) + 1 on queries and keys."""
+    if rot < 0 or rot % 2 or factor < 1.0 or scaling not in (None, "linear", "base", "bands"):
+        raise ValueError("rot is even, factor at least 1, scaling None, \"linear\", \"base\" or \"bands\"")
+    if scaling == "base" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    freq = torch.tensor([base ** (-2.0 * i / rot) for i in range(rot // 2)], dtype=torch.float64)
+    scale = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "bands":
+        kept = ((trained * freq / (2.0 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        freq = freq / factor * (1.0 - kept) + freq * kept
+        scale = 0.1 * math.log(factor) + 1.0
+    return freq.to(device), scale

@@ -21,7 +21,8 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libb200_qlinear.so")
 ARCHIVE = os.path.join(HERE, "libb200_qlinear.a")
 HOST_OPS = os.path.join(HERE, "_host_ops.so")      # linear.py's hot calls (csrc/host_ops.cpp), linked against LIB and torch
-UNITS = ["quant_rows", "gemm_i8", "gemm_skinny", "weight_pack", "w4_linear", "w4_tile", "kv_cache", "attention", "attention_tc"]
+UNITS = ["quant_rows", "gemm_i8", "gemm_skinny", "weight_pack", "w4_linear", "w4_tile", "kv_cache", "attention", "attention_tc", "norm_rows",
+         "rotary", "f8_linear"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
          "-Xcompiler", "-fPIC,-fvisibility=hidden", "-I" + CSRC, "-I" + os.path.join(os.path.dirname(HERE), "include")]

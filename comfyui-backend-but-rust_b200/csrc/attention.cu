@@ -2,6 +2,7 @@
 //
 //   gpu_cross_attention   q rows of one sequence, k and v rows of another, 16-bit
 //   gpu_kv8_attention     q rows over pages of int8 keys and values, one f32 scale for each page and head
+//   gpu_packed_attention  rows of several sequences one after the other, each over its own, 16-bit
 //
 // o[i] = sum_t p[i, t] v[t] / sum_t p[i, t],  p[i, t] = exp(scale q[i] . k[t] - m[i]), m[i] the largest exponent seen so far; a row that sees
 // no key is zeros. One pass over the keys: the sums are scaled when m grows. Exponents, m and both sums are f32; p is rounded to the type
@@ -21,19 +22,25 @@ template <int DP> struct Tile {
     static constexpr int kRowBytes = DP * 2, kBytes = kKeys * DP * 2;
     // Q | K, V x 2 | 0 or -inf per key x 2 | m, l of every row; the sums of the rows, f32, over K and V at the end
     static constexpr int kLoaded = kRows * kRowBytes, kKeyInfo = kLoaded + 4 * kBytes, kStats = kKeyInfo + 2 * kKeys * 4, kSmem = kStats + 2 * kRows * 4;
+    static constexpr int kFrom = kSmem, kSmemPacked = kFrom + DP * 4;      // packed: for each column the first token whose row is NaN there
     static __device__ __forceinline__ uint32_t at(int row, int c) { return (uint32_t)(row * kRowBytes + ((c ^ (row & 7)) * 16)); }
 };
 
-template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attention_tile_kernel(const AttnParams p) {
+template <typename T, int DP, bool PACKED> __global__ void __launch_bounds__(kThreads) attention_tile_kernel(const AttnParams p) {
     using L = Tile<DP>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x % p.splits, rt = blockIdx.x / p.splits % p.row_tiles, bh = blockIdx.x / p.splits / p.row_tiles;
-    const int b = bh / p.Hkv, kvh = bh % p.Hkv, ratio = p.H / p.Hkv;
     const int D = p.D, chunks = DP / 8;
     pdl_wait();
-    const int len = p.kv_len ? min(max(gload(p.kv_len + b), 0), p.Lkv) : p.Lkv;
-    const int r0 = rt * kRows, live = min(kRows, p.Lq * ratio - r0);    // rows of this tile that exist
+    // packed: the last tiles of a sequence, which have most keys, first
+    const PackedTile x = PACKED ? packed_tile(p, p.row_tiles - 1 - rt) : PackedTile();
+    if (PACKED && x.tokens == 0) return;
+    const int b = PACKED ? 0 : bh / p.Hkv, ratio = PACKED ? p.pack : p.H / p.Hkv, group = PACKED ? bh : bh % p.Hkv;      // group: of `ratio` heads
+    const int kvh = PACKED ? group * ratio / (p.H / p.Hkv) : group;
+    const int len = PACKED ? (p.causal ? x.token0 + x.tokens : x.len) : p.kv_len ? min(max(gload(p.kv_len + b), 0), p.Lkv) : p.Lkv;
+    const int r0 = PACKED ? x.token0 * ratio : rt * kRows, live = PACKED ? x.tokens * ratio : min(kRows, p.Lq * ratio - r0);    // rows of this tile that exist
+    const int64_t q_at = PACKED ? x.start * p.qs[1] : b * p.qs[0], k_at = PACKED ? x.start * p.ks[1] : b * p.ks[0], v_at = PACKED ? x.start * p.vs[1] : b * p.vs[0];
     const int steps = (len + kKeys - 1) / kKeys, per = (steps + p.splits - 1) / p.splits;
     const int first = min(split * per, steps), last = min(first + per, steps);
 
@@ -41,8 +48,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
     float* key_info = reinterpret_cast<float*>(smem + L::kKeyInfo);     // [stage][key]
     // ---- queries into shared memory
     {
-        const int row = tid >> 1, i = (r0 + row) / ratio, h = kvh * ratio + (r0 + row) % ratio;
-        const T* src = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + (int64_t)i * p.qs[1] + h * p.qs[2];
+        const int row = tid >> 1, i = (r0 + row) / ratio, h = group * ratio + (r0 + row) % ratio;
+        const T* src = reinterpret_cast<const T*>(p.q) + q_at + (int64_t)i * p.qs[1] + h * p.qs[2];
         for (int c = tid & 1; c < chunks; c += 2)
             *reinterpret_cast<uint4*>(smem + L::at(row, c)) =
                 row < live && c * 8 < D ? gload(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
@@ -53,8 +60,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
         for (int i = tid; i < kKeys * chunks; i += kThreads) {
             const int key = i / chunks, c = i % chunks, at = step * kKeys + key;
             const bool valid = at < len && c * 8 < D && (!p.mask || gload(p.mask + b * p.mask_stride + at));
-            const T* k = reinterpret_cast<const T*>(p.k) + (valid ? b * p.ks[0] + at * p.ks[1] + kvh * p.ks[2] + c * 8 : 0);
-            const T* v = reinterpret_cast<const T*>(p.v) + (valid ? b * p.vs[0] + at * p.vs[1] + kvh * p.vs[2] + c * 8 : 0);
+            const T* k = reinterpret_cast<const T*>(p.k) + (valid ? k_at + at * p.ks[1] + kvh * p.ks[2] + c * 8 : 0);
+            const T* v = reinterpret_cast<const T*>(p.v) + (valid ? v_at + at * p.vs[1] + kvh * p.vs[2] + c * 8 : 0);
             cp_async16(ks + L::at(key, c), k, valid);
             cp_async16(vs + L::at(key, c), v, valid);
         }
@@ -65,6 +72,13 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
     };
     float o[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
     const float to_log2 = p.scale * kLog2e;
+    int* from = reinterpret_cast<int*>(smem + L::kFrom);
+    int bound[2] = {};          // keys that this thread's rows see
+    if constexpr (PACKED) {
+        for (int i = tid; i < DP; i += kThreads) from[i] = INT32_MAX;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bound[h] = p.causal ? (r0 + warp * 16 + g + 8 * h) / ratio + 1 : len;
+    }
     if (first < last) load(first, 0);
     cp_async_commit();
     for (int step = first; step < last; ++step) {
@@ -74,6 +88,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
         cp_async_wait<1>();
         __syncthreads();
         const uint32_t ks = base + L::kLoaded + stage * 2 * L::kBytes, vs = ks + L::kBytes;
+        const bool mixed = PACKED && p.causal && step * kKeys + kKeys > x.token0 + 1;      // some rows see keys here that others do not
+        if (mixed) {
+            for (int i = tid; i < kKeys * (DP / 8); i += kThreads) {
+                const int key = i / (DP / 8), c = i % (DP / 8);
+                uint4* at = reinterpret_cast<uint4*>(smem + (vs - base) + L::at(key, c));
+                if (any_infinite<T>(*at)) *at = without_infinite<T>(*at, step * kKeys + key, from + c * 8);
+            }
+            __syncthreads();
+        }
         float s[8][4] = {};
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
@@ -94,6 +117,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[n][i] = info[n * 8 + 2 * t + (i & 1)] == 0.f ? s[n][i] * to_log2 : -INFINITY;
+                if (mixed && step * kKeys + n * 8 + 2 * t + (i & 1) >= bound[i >> 1]) s[n][i] = -INFINITY;
                 top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
             }
         float keep[2], shift[2];
@@ -169,14 +193,20 @@ template <typename T, int DP> __global__ void __launch_bounds__(kThreads) attent
                 for (int e = 0; e < 8; ++e) y[e] = __fmaf_rn(dsmem_f32(part_at + (row * kPitch + (n ^ (row & 3)) * 8 + e) * 4, s), w, y[e]);
             }
         }
-        store_row(p, y, total, b, r0 + row, kvh, ratio, n * 8, T());
+        if constexpr (PACKED) {
+            const int token = (r0 + row) / ratio;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (token >= from[n * 8 + e]) y[e] = NAN;
+            store_piece(reinterpret_cast<T*>(p.out) + (x.start + token) * p.os[1] + (group * ratio + (r0 + row) % ratio) * p.os[2] + n * 8, y, total);
+        } else store_row(p, y, total, b, r0 + row, kvh, ratio, n * 8, T());
     }
     if (p.splits > 1) cluster_sync_all();      // nobody leaves while its shared memory is read
 }
 
 template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
     using L = Tile<DP>;
-    auto kern = attention_tile_kernel<T, DP>;
+    auto kern = attention_tile_kernel<T, DP, false>;
     const int64_t rows = (int64_t)p.Lq * (p.H / p.Hkv), tiles = (rows + kRows - 1) / kRows;
     if (rows > INT32_MAX - kRows || tiles > INT32_MAX / p.B / p.Hkv) return -1;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
@@ -186,6 +216,16 @@ template <typename T, int DP> int launch_tile(AttnParams& p, cudaStream_t st) {
     p.splits = 1;
     while (p.splits < 8 && base * p.splits * 2 <= 296 && (int64_t)p.Lkv >= (int64_t)p.splits * 2 * 256) p.splits *= 2;
     return launch_pdl_cluster(kern, dim3((unsigned)(base * p.splits)), kThreads, L::kSmem, st, p.splits, p);
+}
+template <typename T, int DP> int launch_packed(AttnParams& p, cudaStream_t st) {
+    using L = Tile<DP>;
+    auto kern = attention_tile_kernel<T, DP, true>;
+    p.tile_tokens = kRows / p.pack, p.splits = 1;
+    const int64_t tiles = (int64_t)p.rows / p.tile_tokens + p.B;
+    if (tiles > INT32_MAX / (p.H / p.pack)) return -1;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemPacked)) return (int)e;
+    p.row_tiles = (int)tiles;
+    return launch_pdl(kern, dim3((unsigned)(tiles * (p.H / p.pack))), kThreads, L::kSmemPacked, st, p);
 }
 // ---- rows over the cache ---------------------------------------------------------------------------------------------------------
 // Tiles of 16 rows of a kv head (a token's query heads, or a few tokens'): bound by the cache's bytes. A CTA's eight warps take 16 keys each
@@ -528,6 +568,11 @@ template <typename T> int launch_cross(AttnParams& p, cudaStream_t st) {
     if (p.D <= 128) return launch_tile<T, 128>(p, st);
     return p.D <= 192 ? launch_tile<T, 192>(p, st) : launch_tile<T, 256>(p, st);
 }
+template <typename T> int launch_packed(AttnParams& p, cudaStream_t st) {
+    if (p.D <= 64) return launch_packed<T, 64>(p, st);
+    if (p.D <= 128) return launch_packed<T, 128>(p, st);
+    return p.D <= 192 ? launch_packed<T, 192>(p, st) : launch_packed<T, 256>(p, st);
+}
 template <typename QT> int launch_kv8(AttnParams& p, cudaStream_t st) {
     if (attention_tc_takes(p, true)) return attention_tc(std::is_same<QT, half>::value ? DT_F16 : DT_BF16, true, p, st);
     return p.D <= 64 ? launch_rows<QT, 64>(p, st) : p.D <= 128 ? launch_rows<QT, 128>(p, st) : launch_rows<QT, 256>(p, st);
@@ -578,4 +623,22 @@ GPU_API int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t
     p.B = B, p.Lq = Lq, p.Lkv = pages > 0 ? max_pages * T : 0, p.H = H, p.Hkv = Hkv, p.D = D, p.T = T, p.scale = scale;
     cudaStream_t st = (cudaStream_t)stream;
     return dtype == DT_F16 ? launch_kv8<half>(p, st) : launch_kv8<bf16>(p, st);
+}
+
+GPU_API int gpu_packed_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides, const int32_t* offsets, int causal, int B,
+                                 int rows, int H, int Hkv, int D, float scale, void* stream) {
+    if (B < 0 || rows < 0 || rows > INT32_MAX - 512 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || D <= 0 || D % 8 != 0 || D > 256) return -1;
+    if (dtype != DT_F16 && dtype != DT_BF16) return -4;
+    if (B == 0 || rows == 0) return 0;
+    if (!q || !k || !v || !out || !strides || !offsets || off16(q) || off16(k) || off16(v) || off16(out) || ragged(strides, 8)) return -5;
+    if ((rows > 1 && strides[6] == 0) || (H > 1 && strides[7] == 0)) return -5;      // rows of the result in the same place
+    AttnParams p = {};
+    p.q = q, p.k = k, p.v = v, p.out = out, p.offsets = offsets, p.rows = rows, p.causal = causal != 0;
+    for (int i = 0; i < 2; ++i) p.qs[1 + i] = strides[i], p.ks[1 + i] = strides[2 + i], p.vs[1 + i] = strides[4 + i], p.os[1 + i] = strides[6 + i];
+    p.B = B, p.H = H, p.Hkv = Hkv, p.D = D, p.scale = scale;
+    // Heads of a token that share a tile: all that read one head of k and v, or as many as divide them and leave a tile several tokens
+    const int ratio = H / Hkv;
+    for (p.pack = ratio < 16 ? ratio : 16; ratio % p.pack != 0;) --p.pack;
+    cudaStream_t st = (cudaStream_t)stream;
+    return dtype == DT_F16 ? launch_packed<half>(p, st) : launch_packed<bf16>(p, st);
 }

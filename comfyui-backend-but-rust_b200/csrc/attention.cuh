@@ -24,7 +24,55 @@ struct AttnParams {
     int64_t mask_stride;
     int B, Lq, Lkv, H, Hkv, D, T, causal, splits, row_tiles;
     float scale;
+    // packed sequences: rows offsets[b] to offsets[b + 1] of `rows` are sequence b; a tile has tile_tokens of its tokens and `pack` heads of each,
+    // which read one head of k and v
+    const int32_t* offsets;
+    int rows, pack, tile_tokens;
 };
+
+// ---- packed sequences
+// Their tiles are numbered without a table: sequence b has those from offsets[b] / tile_tokens + b on, at least as many as it fills and at most one
+// more than it needs. Offsets outside the rows, or falling ones, give tiles inside the rows all the same.
+struct PackedTile {
+    int64_t start;             // row of the sequence's first token
+    int len, token0, tokens;   // its tokens, and those of the tile; none: a tile that nobody needs
+};
+__device__ __forceinline__ int offset_at(const AttnParams& p, int b) { return min(max(gload(p.offsets + b), 0), p.rows); }
+// A whole warp finds the tile, 32 sequences at a look
+__device__ __forceinline__ PackedTile packed_tile(const AttnParams& p, int tile) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, b = lo + (lane + 1) * step;
+        const bool before = b < hi && offset_at(p, b) / p.tile_tokens + b <= tile;
+        lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+        hi = min(hi, lo + step);
+    }
+    PackedTile x;
+    const int start = offset_at(p, lo), end = offset_at(p, lo + 1);
+    x.start = start, x.len = max(0, end - start);
+    const int64_t at = (int64_t)(tile - (start / p.tile_tokens + lo)) * p.tile_tokens;
+    x.tokens = at >= 0 && at < x.len ? min(p.tile_tokens, x.len - (int)at) : 0;
+    x.token0 = (int)min(max(at, (int64_t)0), (int64_t)x.len);
+    return x;
+}
+// Numbers beyond the type's range, and what is none, among eight neighbouring values
+template <typename T> __device__ __forceinline__ bool any_infinite(uint4 w) {
+    const uint32_t top = std::is_same<T, half>::value ? 0x7C007C00u : 0x7F807F80u;
+    return (__vcmpeq2(w.x & top, top) | __vcmpeq2(w.y & top, top) | __vcmpeq2(w.z & top, top) | __vcmpeq2(w.w & top, top)) != 0;
+}
+// Takes them out of values of V that some rows of a tile see and others do not (a weight of 0 does not hide them in a product) and notes for each
+// of the eight columns the first key that had one: rows from that token on get NaN there.
+template <typename T> __device__ __forceinline__ uint4 without_infinite(uint4 w, int key, int* from) {
+    T* v = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (!(fabsf(to_f<T>(v[e])) <= FLT_MAX)) {
+            v[e] = from_f<T>(0.f);
+            atomicMin(from + e, key);
+        }
+    return w;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -53,14 +101,16 @@ __device__ __forceinline__ float v_scale_log2(float s) { return log2f(s < kTiny 
 __device__ __forceinline__ float v_scale_weight(float s) { return s != s ? 1.f : 1.f / fmaxf(s, kTiny); }
 
 // Eight columns of a finished row; one that saw no key is zeros, NaN stays.
-template <typename QT> __device__ __forceinline__ void store_row(const AttnParams& p, const float (&y)[8], float total, int b, int row, int kvh, int ratio, int d, QT) {
+template <typename QT> __device__ __forceinline__ void store_piece(QT* dst, const float (&y)[8], float total) {
     const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
     uint4 w;
     uint32_t* ow = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
     for (int e = 0; e < 4; ++e) ow[e] = pack2<QT>(y[2 * e] * inv, y[2 * e + 1] * inv);
-    QT* dst = reinterpret_cast<QT*>(p.out) + b * p.os[0] + (int64_t)(row / ratio) * p.os[1] + (kvh * ratio + row % ratio) * p.os[2] + d;
     *reinterpret_cast<uint4*>(dst) = w;
+}
+template <typename QT> __device__ __forceinline__ void store_row(const AttnParams& p, const float (&y)[8], float total, int b, int row, int kvh, int ratio, int d, QT) {
+    store_piece(reinterpret_cast<QT*>(p.out) + b * p.os[0] + (int64_t)(row / ratio) * p.os[1] + (kvh * ratio + row % ratio) * p.os[2] + d, y, total);
 }
 
 // The kernel for many query rows (attention_tc.cu): takes rows of at most 128 values and positive scales.

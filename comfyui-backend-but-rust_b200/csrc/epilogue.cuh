@@ -57,6 +57,7 @@ int act_lut_ptr(int act, cudaStream_t st, const uint16_t** out);
 int quant_status_read_clear(int* out);
 int attention_status_read_clear(int* out);
 int w4_status_read_clear(int* out);
+int f8_status_read_clear(int* out);
 // quant_rows.cu: gpu_rotate_rows_f32's prologue + rotation with the rows written as three signed 8-bit digits [3][M, K] and a factor
 // per row, negative for a spread row, whose groups of 256 have the factor |f| 2^-shift with shifts [K / 256][M] (written for spread
 // rows only); zeroes nzero words at `zero`

@@ -2099,10 +2099,11 @@ GPU_API int gpu_kernels_status(int* status) {
     if (e != cudaSuccess) return (int)e;
     int qv = 0;
     if (int rc = quant_status_read_clear(&qv)) return rc;
-    int av = 0, wv = 0;
+    int av = 0, wv = 0, fv = 0;
     if (int rc = attention_status_read_clear(&av)) return rc;
     if (int rc = w4_status_read_clear(&wv)) return rc;
+    if (int rc = f8_status_read_clear(&fv)) return rc;
     if (v) g_workspace_epoch.fetch_add(1, std::memory_order_acq_rel);   // scratch may hold partial sums: clear before reuse
-    if (status) *status = v ? v : qv ? qv : av ? av : wv;
+    if (status) *status = v ? v : qv ? qv : av ? av : wv ? wv : fv;
     return 0;
 }

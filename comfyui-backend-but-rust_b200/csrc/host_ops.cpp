@@ -391,11 +391,137 @@ FAST(kv8_attention, 11)
                             small(c.T), c.pages, small(table.size(1)), real(a[9]), stream());
     return wrap(a[10], out);
 END
+// Strides of rows and heads of [rows, heads, D]
+void put_row_strides(const at::Tensor& t, int64_t* s) {
+    check(t.dim() == 3 && (t.size(2) <= 1 || t.stride(2) == 1), "expected [rows, heads, D] with the values of a head side by side");
+    for (int i = 0; i < 2; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+// q, k, v, offsets, causal, scale, out
+FAST(packed_attention, 7)
+    const at::Tensor &q = on_gpu(a[0]), &k = ten(a[1]), &v = ten(a[2]), &offsets = ten(a[3]);
+    const at::Tensor* given = opt(a[6]);
+    const On on(q);
+    on.same({&k, &v, &offsets, given});
+    const int dt = attention_dtype(q);
+    int64_t st[8];
+    put_row_strides(q, st), put_row_strides(k, st + 2), put_row_strides(v, st + 4);
+    const int64_t rows = q.size(0), H = q.size(1), D = q.size(2), Hkv = k.size(1);
+    check(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v have one type");
+    check(shaped(k, {rows, Hkv, D}) && shaped(v, {rows, Hkv, D}) && Hkv > 0 && H % Hkv == 0, "expected k and v [rows, Hkv, D], H a multiple of Hkv");
+    check(offsets.dim() == 1 && offsets.size(0) >= 1 && plain(offsets, at::kInt, {offsets.size(0)}), "offsets is int32 [sequences + 1]");
+    at::Tensor out = given ? *given : at::zeros(q.sizes(), q.options());
+    check(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out has the shape and type of q");
+    put_row_strides(out, st + 6);
+    CALL(gpu_packed_attention, dt, ptr(q), ptr(k), ptr(v), ptr(out), st, ptr<int32_t>(offsets), integer32(a[4]), small(offsets.size(0) - 1), small(rows),
+                               small(H), small(Hkv), small(D), real(a[5]), stream());
+    return wrap(a[6], out);
+END
+// q, k, pos, freq, interleaved, axis, q_norm, k_norm, eps, scale, q_out, k_out
+FAST(rotary, 12)
+    const at::Tensor &q = on_gpu(a[0]), &pos = ten(a[2]), &freq = ten(a[3]);
+    const at::Tensor *k = opt(a[1]), *axis = opt(a[5]), *qn = opt(a[6]), *kn = opt(a[7]), *gq = opt(a[10]), *gk = opt(a[11]);
+    const On on(q);
+    on.same({k, &pos, &freq, axis, qn, kn, gq, gk});
+    const int dt = dtype_code(q);
+    int64_t st[12] = {};
+    put_strides(q, st);
+    const int64_t B = q.size(0), L = q.size(1), D = q.size(3), half = freq.numel();
+    if (k) {
+        put_strides(*k, st + 3);
+        check(k->scalar_type() == q.scalar_type() && k->size(0) == B && k->size(1) == L && k->size(3) == D, "expected q [B, L, H, D] and k [B, L, Hkv, D] of one type");
+    }
+    check(plain(freq, at::kDouble, {half}) && 2 * half <= D, "freq is f64 [rot / 2], rot at most D");
+    const bool many = pos.dim() == 3;
+    check(pos.scalar_type() == at::kInt && (many || pos.dim() == 2) && pos.size(-1) == L && pos.size(-2) == B && (L <= 1 || pos.stride(-1) == 1),
+          "positions are int32 [B, L] or [axes, B, L]");
+    const int64_t axes = many ? pos.size(0) : 1;
+    check(axes >= 1 && (axes == 1 || axis), "positions of several axes need the axis of each frequency");
+    check(!axis || plain(*axis, at::kByte, {half}), "axis is uint8 [rot / 2]");
+    check((!qn || plain(*qn, at::kFloat, {D})) && (!kn || plain(*kn, at::kFloat, {D})), "q_norm and k_norm are f32 [D]");
+    at::Tensor qo = gq ? *gq : at::empty(q.sizes(), q.options()), ko;
+    check(qo.sizes() == q.sizes() && qo.scalar_type() == q.scalar_type(), "q_out has the shape and type of q");
+    put_strides(qo, st + 6);
+    check(k || !gk, "k_out needs k");
+    if (k) {
+        ko = gk ? *gk : at::empty(k->sizes(), k->options());
+        check(ko.sizes() == k->sizes() && ko.scalar_type() == k->scalar_type(), "k_out has the shape and type of k");
+        put_strides(ko, st + 9);
+    }
+    CALL(gpu_rotary, dt, ptr(q), ptr(k), ptr(qo), k ? ptr(ko) : nullptr, st, ptr<int32_t>(pos), many ? pos.stride(0) : 0, B > 1 ? pos.stride(-2) : 0, small(axes),
+                     ptr<uint8_t>(axis), ptr<double>(freq), small(2 * half), integer32(a[4]), real(a[9]), ptr<float>(qn), ptr<float>(kn), real(a[8]), small(B),
+                     small(L), small(q.size(2)), k ? small(k->size(2)) : 0, small(D), stream());
+    if (!k) {
+        PyObject* r = wrap(a[10], qo);
+        PyObject* both = r ? PyTuple_Pack(2, r, Py_None) : nullptr;
+        Py_XDECREF(r);
+        return both;
+    }
+    return pair(a[10], qo, a[11], ko);
+END
+
+bool side_by_side(const at::Tensor& t) { return t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1); }
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+int64_t blocks_of(int64_t K) { return (K + 127) / 128; }
+
+// x, prologue, K, up_offset, norm_w, eps, resid, resid_out, out, scales, out_dtype
+FAST(norm_rows, 11)
+    const at::Tensor& x = on_gpu(a[0]);
+    const at::Tensor *w = opt(a[4]), *resid = opt(a[6]), *resid_out = opt(a[7]), *given = opt(a[8]), *given_s = opt(a[9]);
+    const On on(x);
+    on.same({w, resid, resid_out, given, given_s});
+    check(side_by_side(x), "x is a matrix, the values of a row side by side");
+    const int64_t M = x.size(0), K = a[2] == Py_None ? x.size(1) : integer(a[2]), up = integer(a[3]);
+    const int prologue = integer32(a[1]);
+    check(K >= 0 && K <= x.size(1) && (prologue != 3 || (up >= 0 && up + K <= x.size(1))), "x has fewer columns than the call reads");
+    check(!w || plain(*w, at::kFloat, {K}), "norm_w is f32 [K]");
+    check(resid || !resid_out, "resid_out needs resid");
+    if (resid && !resid_out) resid_out = resid;
+    for (const at::Tensor* t : {resid, resid_out})
+        check(!t || (shaped(*t, {M, K}) && side_by_side(*t) && t->scalar_type() == x.scalar_type()), "resid and resid_out are [M, K] in x's type");
+    const at::ScalarType dt = given ? given->scalar_type() : a[10] == Py_None ? x.scalar_type() : out_dtype(a[10]);
+    const bool f8 = dt == at::kFloat8_e4m3fn;
+    at::Tensor out = given ? *given : matrix(x, M, K, dt), s;
+    check(shaped(out, {M, K}) && side_by_side(out), "out is [M, K], the values of a row side by side");
+    check(f8 || !given_s, "scales are for e4m3");
+    if (f8) {
+        s = given_s ? *given_s : matrix(x, M, blocks_of(K), at::kFloat);
+        check(plain(s, at::kFloat, {M, blocks_of(K)}), "scales are f32 [M, ceil(K / 128)]");
+    }
+    CALL(gpu_norm_rows, dtype_code(x), prologue, ptr(x), row_stride(x), up, ptr(resid), resid ? row_stride(*resid) : 0, ptr(resid_out),
+                        resid_out ? row_stride(*resid_out) : 0, ptr<float>(w), real(a[5]), f8 ? 3 : dtype_code(out), ptr(out), row_stride(out),
+                        f8 ? ptr<float>(s) : nullptr, small(M), small(K), stream());
+    if (!f8) return wrap(a[8], out);
+    return pair(a[8], out, a[9], s);
+END
+// x, xs, W, ws, bias, out, beta, out_dtype
+FAST(f8_linear, 8)
+    const at::Tensor &x = on_gpu(a[0]), &xs = ten(a[1]), &W = ten(a[2]), &ws = ten(a[3]);
+    const at::Tensor *bias = opt(a[4]), *given = opt(a[5]);
+    const On on(x);
+    on.same({&xs, &W, &ws, bias, given});
+    int64_t M, K;
+    rows_cols(x, M, K);
+    check(x.scalar_type() == at::kFloat8_e4m3fn && side_by_side(x), "x is e4m3, the values of a row side by side");
+    check(W.dim() == 2, "the weight is e4m3 [N, K], contiguous");
+    const int64_t N = W.size(0);
+    check(plain(W, at::kFloat8_e4m3fn, {N, K}), "the weight is e4m3 [N, K], contiguous");
+    check(plain(xs, at::kFloat, {M, blocks_of(K)}) && plain(ws, at::kFloat, {blocks_of(N), blocks_of(K)}),
+          "scales are f32, contiguous: [M, ceil(K / 128)] of x, [ceil(N / 128), ceil(K / 128)] of the weight");
+    const float beta = real(a[6]);
+    check(beta == 0.f || given, "beta needs the out that it scales");
+    at::Tensor D = given ? *given : matrix(x, M, N, out_dtype(a[7]));
+    check(shaped(D, {M, N}) && side_by_side(D), "out is [M, N], the values of a row side by side");
+    check(!bias || plain(*bias, D.scalar_type(), {N}), "bias is [N] in the type of out");
+    CALL(gpu_f8_linear, ptr(x), row_stride(x), ptr<float>(xs), ptr(W), ptr<float>(ws), ptr(bias), dtype_code(D), ptr(D), row_stride(D), beta, small(M), small(N),
+                        small(K), stream());
+    return wrap(a[5], D);
+END
 
 #define M(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {M(quant_rows), M(sd_quant_rows), M(sd_ln_quant_rows), M(sd_geglu_quant_rows), M(sd_group_norm_quant_rows),
                          M(sd_unpad_quant_rows), M(int8_gemm), M(int8_gemm_act_rot), M(quant_rows_rotated), M(w6a8_gemm),
                          M(w4_linear), M(cross_attention), M(kv8_append), M(kv8_dequant), M(kv8_attention),
+                         M(packed_attention), M(rotary), M(norm_rows), M(f8_linear),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,182 @@
+// gpu_rotary: queries and keys turned by their positions, one launch for both, the norm of each head before it where the model has one.
+//
+//   y = x, or x / sqrt(mean(x^2) + eps) w over a head's D values
+//   (a, b) -> scale (a cos t - b sin t, a sin t + b cos t) for the pairs of the first rot values, t = pos freq; the others stay as y
+//   pairs: (i, i + rot / 2), or neighbours (2 i, 2 i + 1)
+//
+// Angles: freq and pos freq in 64 bits (position 10^6 times 1 radian leaves an f32 angle 0.06 off), as turns, of which the whole ones are
+// dropped; the rest's sine and cosine in f32. A token's angles are worked out once, by as many threads, and serve all of its heads from shared
+// memory; the rotation is f32, one rounding to the rows' type. Bound by the rows' bytes.
+#include "common.cuh"
+
+namespace {
+
+struct RotaryParams {
+    const void* x[2];            // q, k
+    void* y[2];
+    const float* norm[2];
+    int64_t xs[2][3], ys[2][3];  // strides of batch, row, head
+    const int32_t* pos;          // [axes, B, L]
+    const uint8_t* axis;         // [rot / 2], or null: 0
+    const double* freq;          // [rot / 2]
+    int64_t pos_axis, pos_batch;
+    float scale, eps;
+    int B, L, H, heads, D, half, interleaved, axes, tokens;      // heads: of q and k together; tokens: to a CTA
+};
+
+template <typename T, int V> struct Values;
+template <typename T, int V> __device__ __forceinline__ void load_values(const T* p, float (&v)[V]) {
+    constexpr int kBytes = V * sizeof(T);
+    T e[V];
+    if (kBytes % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(e)[i] = gload(reinterpret_cast<const uint4*>(p) + i);
+    } else if (kBytes == 8) {
+        *reinterpret_cast<uint2*>(e) = gload(reinterpret_cast<const uint2*>(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] = gload(p + i);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f<T>(e[i]);
+}
+template <typename T, int V> __device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
+    constexpr int kBytes = V * sizeof(T);
+    T e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = from_f<T>(v[i]);
+    if (kBytes % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<uint4*>(e)[i];
+    } else if (kBytes == 8) {
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = e[i];
+    }
+}
+
+constexpr int kThreads = 256, kMaxHalf = 128;
+
+// A group of `lanes` threads has a head, a thread of it one slot (more with V = 1): V values and the V that they are paired with, or next to.
+template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, const int lanes) {
+    extern __shared__ float2 turn[];      // [token][half]: cos, sin
+    const int64_t tokens = (int64_t)p.B * p.L, first = (int64_t)blockIdx.x * p.tokens;
+    const int here = (int)min((int64_t)p.tokens, tokens - first);
+    pdl_wait();
+    for (int i = threadIdx.x; i < here * p.half; i += kThreads) {
+        const int t = i / p.half, f = i - t * p.half;
+        const int64_t at = first + t, b = at / p.L;
+        const int axis = p.axis ? min((int)gload(p.axis + f), p.axes - 1) : 0;
+        const int pos = gload(p.pos + axis * p.pos_axis + b * p.pos_batch + (at - b * p.L));
+        // turns: two products of 64 bits; less than half a turn is left, which f32 holds to 2^-25
+        const double turns = (double)pos * gload(p.freq + f) * 0.15915494309189533577;
+        float s, c;
+        sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+        turn[i] = make_float2(c * p.scale, s * p.scale);
+    }
+    __syncthreads();
+    const int lane = threadIdx.x % lanes, slots = p.D / (2 * V), rotated = p.half / V;
+    for (int64_t i = threadIdx.x / lanes; i < (int64_t)here * p.heads; i += kThreads / lanes) {
+        const int t = (int)(i / p.heads), head = (int)(i - (int64_t)t * p.heads), which = head >= p.H, h = which ? head - p.H : head;
+        const int64_t at = first + t, b = at / p.L, l = at - b * p.L;
+        const T* x = reinterpret_cast<const T*>(p.x[which]) + b * p.xs[which][0] + l * p.xs[which][1] + h * p.xs[which][2];
+        T* y = reinterpret_cast<T*>(p.y[which]) + b * p.ys[which][0] + l * p.ys[which][1] + h * p.ys[which][2];
+        const float* w = p.norm[which];
+        // where slot s has its two vectors: with V = 1 and neighbours as pairs, next to one another as well
+        auto places = [&](int s, int& a, int& b2) {
+            if (p.interleaved || s >= rotated) a = 2 * V * s, b2 = a + V;
+            else a = V * s, b2 = a + p.half;
+        };
+        float u[V], v[V], sum = 0.f, r = 1.f;
+        if (w) {
+            for (int s = lane; s < slots; s += lanes) {
+                int a, b2;
+                places(s, a, b2);
+                load_values<T, V>(x + a, u), load_values<T, V>(x + b2, v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum = __fmaf_rn(u[e], u[e], __fmaf_rn(v[e], v[e], sum));
+            }
+            const unsigned mask = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
+            for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+            r = rsqrtf(sum / (float)p.D + p.eps);
+        }
+        for (int s = lane; s < slots; s += lanes) {
+            int a, b2;
+            places(s, a, b2);
+            load_values<T, V>(x + a, u), load_values<T, V>(x + b2, v);
+            if (w) {
+                float wu[V], wv[V];
+                load_values<float, V>(w + a, wu), load_values<float, V>(w + b2, wv);
+#pragma unroll
+                for (int e = 0; e < V; ++e) u[e] = u[e] * r * wu[e], v[e] = v[e] * r * wv[e];
+            }
+            if (s < rotated) {
+                const float2* cs = turn + t * p.half + s * V;
+                if (p.interleaved && V > 1) {
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 c = cs[e / 2], d = cs[(V + e) / 2];
+                        const float u0 = u[e], u1 = u[(e + 1) % V], v0 = v[e], v1 = v[(e + 1) % V];
+                        u[e] = u0 * c.x - u1 * c.y, u[(e + 1) % V] = u0 * c.y + u1 * c.x;
+                        v[e] = v0 * d.x - v1 * d.y, v[(e + 1) % V] = v0 * d.y + v1 * d.x;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float2 c = cs[e];
+                        const float u0 = u[e], v0 = v[e];
+                        u[e] = u0 * c.x - v0 * c.y, v[e] = u0 * c.y + v0 * c.x;
+                    }
+                }
+            }
+            store_values<T, V>(y + a, u), store_values<T, V>(y + b2, v);
+        }
+    }
+}
+
+template <typename T> int launch_rotary(RotaryParams& p, cudaStream_t st) {
+    // Values side by side to a thread: what pairs, the rest and whole vectors allow
+    const int rest = (p.D - 2 * p.half) / 2;
+    const int V = p.half % 8 == 0 && rest % 8 == 0 ? 8 : p.half % 4 == 0 && rest % 4 == 0 ? 4 : 1;
+    const int slots = p.D / (2 * V);
+    int lanes = 1;
+    while (lanes < 32 && lanes < slots) lanes *= 2;
+    const int64_t tokens = (int64_t)p.B * p.L;
+    p.tokens = 1;
+    while (p.tokens < 4 && tokens >= (int64_t)p.tokens * 2 * 592) p.tokens *= 2;
+    const int64_t ctas = (tokens + p.tokens - 1) / p.tokens;
+    if (ctas > INT32_MAX) return -1;
+    auto kern = V == 8 ? rotary_kernel<T, 8> : V == 4 ? rotary_kernel<T, 4> : rotary_kernel<T, 1>;
+    return launch_pdl(kern, dim3((unsigned)ctas), kThreads, p.tokens * p.half * sizeof(float2), st, p, lanes);
+}
+
+bool off(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+}  // namespace
+
+GPU_API int gpu_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const int32_t* pos, int64_t pos_axis,
+                       int64_t pos_batch, int axes, const uint8_t* axis, const double* freq, int rot, int interleaved, float scale, const float* q_norm,
+                       const float* k_norm, float eps, int B, int L, int H, int Hkv, int D, void* stream) {
+    if (dtype < DT_F32 || dtype > DT_BF16) return -4;
+    if (B < 0 || L < 0 || H < 0 || Hkv < 0 || H > 65536 || Hkv > 65536 || D <= 0 || D % 8 != 0 || D > 2 * kMaxHalf || rot < 0 || rot % 2 != 0 || rot > D || axes < 1) return -1;
+    if (B == 0 || L == 0 || H + Hkv == 0) return 0;
+    if (!strides || (H > 0 && (!q || !q_out)) || (Hkv > 0 && (!k || !k_out)) || (rot > 0 && (!pos || !freq || (axes > 1 && !axis)))) return -5;
+    const int e = dtype == DT_F32 ? 4 : 2;
+    if (off(q, 16) || off(k, 16) || off(q_out, 16) || off(k_out, 16) || (q_norm && off(q_norm, 16)) || (k_norm && off(k_norm, 16))) return -5;
+    RotaryParams p = {};
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < 4; ++j)
+            if (strides[3 * j + i] * e % 16 != 0) return -5;
+        p.xs[0][i] = strides[i], p.xs[1][i] = strides[3 + i], p.ys[0][i] = strides[6 + i], p.ys[1][i] = strides[9 + i];
+    }
+    const int sizes[3] = {B, L, 0};
+    for (int w = 0; w < 2; ++w)
+        for (int i = 0; i < 3; ++i)
+            if ((i < 2 ? sizes[i] : w ? Hkv : H) > 1 && (w ? Hkv : H) > 0 && p.ys[w][i] == 0) return -5;
+    p.x[0] = q, p.x[1] = k, p.y[0] = q_out, p.y[1] = k_out, p.norm[0] = q_norm, p.norm[1] = k_norm;
+    p.pos = pos, p.pos_axis = pos_axis, p.pos_batch = pos_batch, p.axis = axis, p.axes = axes, p.freq = freq, p.scale = scale, p.eps = eps;
+    p.B = B, p.L = L, p.H = H, p.heads = H + Hkv, p.D = D, p.half = rot / 2, p.interleaved = interleaved != 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    return dtype == DT_F32 ? launch_rotary<float>(p, st) : dtype == DT_F16 ? launch_rotary<half>(p, st) : launch_rotary<bf16>(p, st);
+}

@@ -13,7 +13,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200_qlinear.so")
 
-DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+DT_F32, DT_F16, DT_BF16, DT_E4M3 = 0, 1, 2, 3
 (PRO_PLAIN, PRO_RMS, PRO_GATE, PRO_SWIGLU, PRO_LAYERNORM, PRO_SILU, PRO_GELU, PRO_ADALN, PRO_SITU, PRO_LN_MOD,
  PRO_LN_AFFINE, PRO_GELU_TANH, PRO_LN_AFFINE_SILU, PRO_SITU_FAST) = range(14)
 ACT_NONE, ACT_GELU_TANH, ACT_SILU, ACT_GELU_ERF = range(4)
@@ -61,6 +61,12 @@ SIGNATURES = {
     "gpu_kv8_dequant": [i32, P, P, P, P, P, i64, P, P, P, i32, i64, i32, i32, i32, i64, i32, P],
     "gpu_kv8_attention": [i32, P, P, C.POINTER(i64), P, P, P, P, P, i64, P, P, i32, i32, i32, i32, i32, i32, i32, i64, i32, f32, P],
     "gpu_cross_attention": [i32, P, P, P, P, C.POINTER(i64), P, P, i64, i32, i32, i32, i32, i32, i32, f32, P],
+    "gpu_packed_attention": [i32, P, P, P, P, C.POINTER(i64), P, i32, i32, i32, i32, i32, i32, f32, P],
+    "gpu_rotary": [i32, P, P, P, P, C.POINTER(i64), P, i64, i64, i32, P, P, i32, i32, f32, P, P, f32, i32, i32, i32, i32, i32, P],
+    "gpu_norm_rows": [i32, i32, P, i64, i64, P, i64, P, i64, P, f32, i32, P, i64, P, i32, i32, P],
+    "gpu_f8_requant": [i32, P, i64, P, P, i64, i32, P],
+    "gpu_f8_dequant": [i32, P, P, i32, P, i64, i32, P],
+    "gpu_f8_linear": [P, i64, P, P, P, P, i32, P, i64, f32, i32, i32, i32, P],
     "gpu_wddm_budget": [C.POINTER(u64), C.POINTER(u64)],
     "gpu_kernels_status": [C.POINTER(i32)],
 }

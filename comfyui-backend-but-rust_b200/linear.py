@@ -254,6 +254,49 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     return _h.w4_linear(x, packed, scales, zeros, bias, out, beta, out_dtype)
 
 
+def norm_rows(x: torch.Tensor, prologue: int = ffi.PRO_RMS, *, K: Optional[int] = None, up_offset: int = 0, norm_w: Optional[torch.Tensor] = None,
+              eps: float = 0.0, resid: Optional[torch.Tensor] = None, resid_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+              scales: Optional[torch.Tensor] = None, out_dtype=None):
+    """gpu_norm_rows: rows on their way to the next linear. PRO_RMS: the RMS norm (norm_w f32 [K]) of x, or of the residual stream x + resid, which goes
+    to resid_out (resid itself when not given) in x's type. PRO_PLAIN: x. PRO_SWIGLU: silu(x[:, :K]) * x[:, up_offset:up_offset + K]. As
+    rows of `out_dtype` (x's type by default), or with float8_e4m3fn as (codes [M, K], scales f32 [M, ceil(K / 128)])."""
+    return _h.norm_rows(x, prologue, K, up_offset, norm_w, eps, resid, resid_out, out, scales, out_dtype)
+
+
+def f8_requant(w: torch.Tensor):
+    """gpu_f8_requant: f32 / f16 / bf16 [N, K] -> (e4m3 [N, K], scales f32 [ceil(N / 128), ceil(K / 128)]), one scale for each block of 128 x 128."""
+    _one_device(w)
+    if w.dim() != 2 or w.stride(1) != 1:
+        raise ValueError("expected a matrix whose rows' values lie side by side")
+    N, K = w.shape
+    with torch.cuda.device(w.device):
+        codes = torch.empty((N, K), dtype=torch.float8_e4m3fn, device=w.device)
+        scales = torch.empty((-(-N // 128), -(-K // 128)), dtype=torch.float32, device=w.device)
+        ok(_lib().gpu_f8_requant(_DT[w.dtype], _ptr(w), w.stride(0) if N > 1 else K, _ptr(codes), _ptr(scales), N, K, _stream()), "gpu_f8_requant")
+    return codes, scales
+
+
+def f8_dequant(codes: torch.Tensor, scales: torch.Tensor, *, rows: int = 128, dtype=torch.float32) -> torch.Tensor:
+    """gpu_f8_dequant: what e4m3 codes [N, K] and their scales stand for: a weight's (a scale for each 128 x 128), or with rows=1 those of norm_rows."""
+    _one_device(codes, scales)
+    N, K = codes.shape
+    if codes.dtype != torch.float8_e4m3fn or not codes.is_contiguous() or rows not in (1, 128):
+        raise ValueError("expected contiguous e4m3 codes [N, K], rows 1 or 128")
+    if scales.dtype != torch.float32 or scales.shape != (-(-N // rows), -(-K // 128)) or not scales.is_contiguous():
+        raise ValueError("expected contiguous f32 scales [ceil(N / rows), ceil(K / 128)]")
+    with torch.cuda.device(codes.device):
+        out = torch.empty((N, K), dtype=dtype, device=codes.device)
+        ok(_lib().gpu_f8_dequant(_DT[dtype], _ptr(codes), _ptr(scales), rows, _ptr(out), N, K, _stream()), "gpu_f8_dequant")
+    return out
+
+
+def f8_linear(x: torch.Tensor, xs: torch.Tensor, weight: torch.Tensor, ws: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+              out: Optional[torch.Tensor] = None, beta: float = 0.0, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """gpu_f8_linear: out = beta * out + x @ W^T + bias from norm_rows' codes and scales and f8_requant's. out [M, N] f32 / f16 / bf16 (`out_dtype`, or the
+    type of the `out` given); bias [N] in out's type; beta 0 or 1."""
+    return _h.f8_linear(x, xs, weight, ws, bias, out, beta, out_dtype)
+
+
 def int8_gemm(A, W, xs, ws, bias=None, *, out_dtype=torch.bfloat16, act: int = 0, rscale=None, resid=None, out=None):
     """gpu_int8_gemm / gpu_int8_gemm_act / gpu_int8_gemm_residual, chosen by the arguments given."""
     return _h.int8_gemm(A, W, xs, ws, bias, out_dtype, act, rscale, resid, out)
@@ -330,3 +373,22 @@ class QuantLinear:
             a8, xs = quant_rows(x, prologue, 1 if self.rotate else 0)
         return int8_gemm(a8, self.weight, xs, self.scale, self.bias, out_dtype=x.dtype, act=act, rscale=rscale,
                          resid=resid, out=out)
+
+
+@dataclass
+class F8Linear:
+    """A linear over e4m3 blocks: weight e4m3 [N, K], scale f32 [ceil(N / 128), ceil(K / 128)], optional bias in the type of its results."""
+    weight: torch.Tensor
+    scale: torch.Tensor
+    bias: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def from_float(w: torch.Tensor, bias=None) -> "F8Linear":
+        """Quantize-at-load of f32 / f16 / bf16 weights."""
+        return F8Linear(*f8_requant(w), bias)
+
+    def forward(self, x: torch.Tensor, *, prologue: int = ffi.PRO_PLAIN, K: Optional[int] = None, up_offset: int = 0, norm_w=None, eps: float = 0.0,
+                resid=None, out=None, beta: float = 0.0) -> torch.Tensor:
+        """norm_rows of x, then the linear; the result is in x's type. `resid` is the residual stream that x is added to before the norm."""
+        a8, xs = norm_rows(x, prologue, K=K, up_offset=up_offset, norm_w=norm_w, eps=eps, resid=resid, out_dtype=torch.float8_e4m3fn)
+        return f8_linear(a8, xs, self.weight, self.scale, self.bias, out=out, beta=beta, out_dtype=x.dtype)

@@ -21,6 +21,7 @@ extern "C" {
 #endif
 
 enum { GPU_DT_F32 = 0, GPU_DT_F16 = 1, GPU_DT_BF16 = 2 }; /* src/ffi.rs:11-13 */
+enum { GPU_DT_E4M3 = 3 };                                 /* where a call says so */
 
 /* quantizer prologues, src/ffi.rs:15-29 */
 enum {
@@ -276,6 +277,50 @@ int gpu_kv8_attention(int dtype, const void* q, void* out, const int64_t* stride
 int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides,
                         const int32_t* kv_len, const uint8_t* key_mask, int64_t mask_stride, int B, int Lq, int Lkv, int H, int Hkv,
                         int D, float scale, void* stream);
+
+/* New: attention of packed sequences to themselves (whole prompts of different lengths, no padding), out = softmax(scale q k^T) v. q, out
+ * [rows, H, D], k, v [rows, Hkv, D], f16 or bf16 (strides = 8 HOST values, in elements: row, head of q, k, v, out); H % Hkv == 0, D a multiple of
+ * 8 up to 256. Sequence b is rows offsets[b] to offsets[b + 1] - 1 (int32 [B + 1], ascending; may be empty); with causal != 0 a row sees
+ * itself and the rows of its sequence before it, otherwise all of them. Rows outside every sequence are not written. What a row does not see does not reach it,
+ * NaN and infinities included; with causal != 0 an infinity in v that it sees may show as NaN. p is rounded to q's type for its product with v, f32 otherwise. Needs no workspace.
+ * out may be q itself and overlaps nothing else that the call reads. Errors as above. */
+int gpu_packed_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides, const int32_t* offsets,
+                         int causal, int B, int rows, int H, int Hkv, int D, float scale, void* stream);
+
+/* New: rotary positions of q [B, L, H, D] and k [B, L, Hkv, D] in one launch (f32, f16 or bf16; strides = 12 HOST values, in elements: batch, row,
+ * head of q, k, q_out, k_out; outs may be q and k themselves; H or Hkv may be 0). A head is first divided by sqrt(mean of its squares + eps) and multiplied by q_norm or k_norm
+ * (f32 [D]) where that is given. Then pair i < rot / 2 of its first rot values -- (i, i + rot / 2), or (2i, 2i + 1) with interleaved != 0 -- is turned by
+ * pos * freq[i] and multiplied by scale; the others stay. pos int32: element [axis[i] * pos_axis + b * pos_batch + row], axis u8 [rot / 2]
+ * with values below axes, or NULL: 0; freq f64 [rot / 2], radians a position. Angles are 64-bit, the rest f32, one rounding to the type.
+ * D a multiple of 8 up to 256, rot even. Errors: -1 sizes, -4 types, -5 a NULL, rows off a 16-byte boundary or rows of an out that share their place. */
+int gpu_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const int32_t* pos, int64_t pos_axis,
+               int64_t pos_batch, int axes, const uint8_t* axis, const double* freq, int rot, int interleaved, float scale, const float* q_norm,
+               const float* k_norm, float eps, int B, int L, int H, int Hkv, int D, void* stream);
+
+/* ---- e4m3 in blocks of 128 -------------------------------------------------------------------------------------- */
+
+/* New: linears whose weight and activations are e4m3 with f32 scales: one for each 128 x 128 of the weight (ws [ceil(N/128), ceil(K/128)]), one for each
+ * 128 columns of a row of x (xs [M, ceil(K/128)]); a value is code * scale. K a multiple of 16 (-1), at most 32768 (-2; packer and way back: any).
+ * A writer's scale is max(largest magnitude of the block, 1e-30) * (1/448), its codes are value * (1/scale), both f32 products, rounded to nearest even.
+ * NaN is passed over in the scale and stays NaN; a block with an infinity has that as its scale and NaN in its place.
+ *
+ * gpu_norm_rows    rows [M, K] of dtype (f32, f16, bf16) on their way to the next linear: prologue PLAIN y = x; RMS, with a residual stream where resid is
+ *                  given: s = x + resid in dtype, written to resid_out (may be resid or x itself), y = s / sqrt(mean(s^2) + eps) * norm_w (f32 [K], or NULL: 1);
+ *                  SWIGLU y = silu(x[:, :K]) * x[:, up_offset : up_offset + K]. y, f32 until then, becomes out [M, K]: out_dt f32, f16, bf16
+ *                  (K a multiple of 8), or GPU_DT_E4M3 with scales [M, ceil(K/128)]. K <= 32768 (-2); -3 prologue, or resid and norm_w without RMS; -4 types; -5 a
+ *                  NULL, a row or norm_w off a 16-byte boundary.
+ * gpu_f8_requant   w [N, K] (rows w_stride apart) -> codes [N, K] and ws.
+ * gpu_f8_dequant   codes [N, K] with a scale for every block_rows (1 or 128) rows and 128 columns -> out [N, K] in dtype.
+ * gpu_f8_linear    out[m,n] = beta * out[m,n] + sum_g xs[m,g] ws[n/128,g] (sum over the block's k of x[m,k] W[n,k]) + bias[n], beta 0 or 1 (-207); out f32, f16 or bf16,
+ *                  bias [N] in out's type or NULL. Codes enter exactly, sums of a block on the tensor cores and over the blocks are f32, one rounding to out's type. M from
+ *                  one token up. out must not overlap x. -4 types, -5 a NULL, x or W off a 16-byte boundary, -203 descriptor. */
+int gpu_norm_rows(int dtype, int prologue, const void* x, int64_t x_stride, int64_t up_offset, const void* resid, int64_t resid_stride, void* resid_out,
+                  int64_t resid_out_stride, const float* norm_w, float eps, int out_dt, void* out, int64_t out_stride, float* scales, int M, int K,
+                  void* stream);
+int gpu_f8_requant(int dtype, const void* w, int64_t w_stride, void* codes, float* scales, int64_t N, int K, void* stream);
+int gpu_f8_dequant(int dtype, const void* codes, const float* scales, int block_rows, void* out, int64_t N, int K, void* stream);
+int gpu_f8_linear(const void* x, int64_t x_stride, const float* xs, const void* W, const float* ws, const void* bias, int out_dt, void* out,
+                  int64_t out_stride, float beta, int M, int N, int K, void* stream);
 
 /* Windows video-memory budget query the Rust side imports unconditionally (src/cuda.rs:136-153; the reference
  * defines it in csrc/wddm.cu). HOST pointers. Always returns non-zero here: no budget is known. */
