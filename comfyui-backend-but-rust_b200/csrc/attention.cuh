@@ -49,11 +49,11 @@ __device__ __forceinline__ PackedTile packed_tile(const AttnParams& p, int tile)
         hi = min(hi, lo + step);
     }
     PackedTile x;
-    const int start = offset_at(p, lo), end = offset_at(p, lo + 1);
-    x.start = start, x.len = max(0, end - start);
-    const int64_t at = (int64_t)(tile - (start / p.tile_tokens + lo)) * p.tile_tokens;
-    x.tokens = at >= 0 && at < x.len ? min(p.tile_tokens, x.len - (int)at) : 0;
-    x.token0 = (int)min(max(at, (int64_t)0), (int64_t)x.len);
+    const int start = offset_at(p, lo), ahead = tile - (start / p.tile_tokens + lo);
+    x.start = start;
+    x.len = ahead < 0 ? 0 : max(0, offset_at(p, lo + 1) - start);
+    x.token0 = ahead < 0 || ahead > x.len / p.tile_tokens ? x.len : ahead * p.tile_tokens;
+    x.tokens = min(p.tile_tokens, x.len - x.token0);
     return x;
 }
 // Numbers beyond the type's range, and what is none, among eight neighbouring values
@@ -116,6 +116,8 @@ template <typename QT> __device__ __forceinline__ void store_row(const AttnParam
 // The kernel for many query rows (attention_tc.cu): takes rows of at most 128 values and positive scales.
 bool attention_tc_takes(const AttnParams& p, bool kv8);
 int attention_tc(int dtype, bool kv8, AttnParams& p, cudaStream_t st);
+bool attention_tc_takes_packed(const AttnParams& p);
+int attention_tc_packed(int dtype, AttnParams& p, cudaStream_t st);
 int attention_status_read_clear(int* v);
 
 }  // namespace b200q

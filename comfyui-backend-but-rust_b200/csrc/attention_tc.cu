@@ -1,4 +1,5 @@
-// Attention with many query rows, on tcgen05: the kernel behind gpu_cross_attention and gpu_kv8_attention where tiles of 128 rows fill.
+// Attention with many query rows, on tcgen05: the kernel behind gpu_cross_attention, gpu_kv8_attention and
+// gpu_packed_attention where tiles of 128 rows fill.
 //
 // A CTA an SM, persistent, two tiles of 128 query rows at a time over tiles of 128 keys. Per key tile and query tile: S = Q K^T into tensor
 // memory (128 columns of f32), p = exp2(S c - m) by one thread a row, p back into the same columns as 16-bit values, O += p V with p as the
@@ -36,13 +37,18 @@ __device__ int g_attention_status = 0;
 constexpr int kTileKeys = 128, kSlots = 4, kBox = 128 * 128;       // a box: 128 rows of 128 bytes, 128-byte swizzle
 constexpr float kSlack = 8.f;                                      // by how much (a power of two) p may exceed 1
 
-template <int DP, bool KV8> struct Tc {
+enum Mode { CROSS, CACHE, PACKED };                               // whose keys: an encoder's, a cache's, the rows' own sequences'
+
+template <int DP, Mode MODE> struct Tc {
+    static constexpr bool KV8 = MODE == CACHE;
     static constexpr int kTile = DP / 64 * kBox;                   // 128 rows of Q, K or V
     static constexpr int kRing = 2 * kTile, kStaging = kRing + kSlots * kTile, kTail = kStaging + (KV8 ? 8 * 2048 : 4 * 4096);
     // barriers and three words | key tile % 4: bits of the keys that are seen | the same as limits of logits (16-bit), or factors of the pages |
     // item of the tile % 2: l of every row (16-bit), or bf16 queries' powers of two
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
-    static constexpr int kOrder = kRowInfo + 2048, kEnd = kOrder + 128, kSmem = kEnd + 1024;
+    static constexpr int kOrder = kRowInfo + 2048, kEnd0 = kOrder + 128;
+    // packed: for each of the two warps that look through V, item % 8: whether it found numbers that are none, and the first key with one for each column
+    static constexpr int kFound = kEnd0, kFrom = kFound + 64, kEnd = MODE == PACKED ? kFrom + 16 * DP * 4 : kEnd0, kSmem = kEnd + 1024;
     static constexpr int kThreads = 512;
     // Quarters of a key tile whose products with V start before the softmax has the rest: what is left of them stands between it and the next
     // logits, which take p's place. 16384 rows, 2048 keys, 128 columns, two | three: 357 | 349 us; 4096 x 4096, 64 columns: 165 | 166.
@@ -106,13 +112,26 @@ struct TcParams {
     int q_batch, q_head;
 };
 struct Item {
-    int b, h, row0, rows, len, ql, seen, n;      // h: query head, or kv head of packed rows; rows from row0 on; n key tiles
+    int b, h, row0, rows, len, ql, seen, n;      // h: query head, kv head, or group of `pack` heads; rows from row0 on; n key tiles
+    int start, token0, live[2];                  // packed: the sequence's row, the item's first token in it, rows of the two tiles
 };
 // The item of a CTA's r-th round: the rounds run through the CTAs forwards and backwards in turn, so that where the items get smaller, as the
 // cache's do, the sums of a CTA's items come out alike.
 __device__ __forceinline__ uint32_t item_of(uint32_t r) { return r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
-template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, uint32_t i, const int* order) {
+template <Mode MODE> __device__ __forceinline__ Item item_at(const TcParams& p, uint32_t i, const int* order) {
+    constexpr bool KV8 = MODE == CACHE;
     Item x;
+    if constexpr (MODE == PACKED) {      // a whole warp asks; the last tiles of a sequence, which see most keys, first
+        const uint32_t groups = p.a.H / p.a.pack, slot = i / groups;
+        const PackedTile y = packed_tile(p.a, p.q_tiles - 1 - (int)slot);
+        x.b = 0, x.h = (int)(i - slot * groups), x.row0 = 0, x.ql = 0, x.len = y.len, x.start = (int)y.start, x.token0 = y.token0;
+        const int half = p.a.tile_tokens >> 1;
+        x.live[0] = min(y.tokens, half) * p.a.pack, x.live[1] = max(0, y.tokens - half) * p.a.pack;
+        x.rows = x.live[1] > 0 ? 128 + x.live[1] : x.live[0];
+        x.seen = p.a.causal ? y.token0 + y.tokens : y.len;
+        x.n = x.rows > 0 ? (x.seen + kTileKeys - 1) / kTileKeys : 0;
+        return x;
+    }
     const uint32_t heads = KV8 ? p.a.Hkv : p.a.H;
     // Heads next to one another: together they read and write whole rows of Q and of the result. Cache: long sequences first, of each the
     // tiles with most keys.
@@ -132,10 +151,11 @@ template <bool KV8> __device__ __forceinline__ Item item_at(const TcParams& p, u
     return x;
 }
 
-template <typename QT, int DP, bool KV8> __global__ void __launch_bounds__(Tc<DP, KV8>::kThreads, 1)
+template <typename QT, int DP, Mode MODE> __global__ void __launch_bounds__(Tc<DP, MODE>::kThreads, 1)
 attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                     const TcParams p) {
-    using L = Tc<DP, KV8>;
+    using L = Tc<DP, MODE>;
+    constexpr bool KV8 = MODE == CACHE;
     constexpr bool kBf16 = std::is_same<QT, bf16>::value, kBf16Mma = kBf16 && !KV8;
     using T = typename std::conditional<KV8, half, QT>::type;
     extern __shared__ uint8_t smem_raw[];
@@ -155,11 +175,17 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     // for item n + 2 only behind what waited for item n's reader: l behind the logits of n + 2, which are issued behind the sums of n + 1, and those
     // wait for o_empty of n, which the rows' way out gives when it has read; powers behind q_empty of n + 1, whose logits are issued behind p of n.
     float* row_info = reinterpret_cast<float*>(sm + L::kRowInfo);
+    // packed: [warp][item % 8], [warp][item % 8][column]. A warp clears an item's flag an item ahead: by then the rows' way out is behind the item that
+    // had the place before, seven items back, for V of item n is loaded behind the sums of n - 2, and those begin when all the warps of the rows' way
+    // out have begun with n - 3.
+    int *found = reinterpret_cast<int*>(sm + L::kFound), *from = reinterpret_cast<int*>(sm + L::kFrom);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
         for (int t = 0; t < 2; ++t) mbar_init(q_full + 8 * t, KV8 ? 4 : 1), mbar_init(q_empty + 8 * t, 1), mbar_init(s_full + 8 * t, 2), mbar_init(p_full + 8 * t, 4),
             mbar_init(o_full + 8 * t, 2), mbar_init(o_empty + 8 * t, 4), mbar_init(p_early + 8 * t, 4), mbar_init(v_ready + 8 * t, 2);
         *abort_s = 0, *moving = 0;
+        if (MODE == PACKED)
+            for (int i = 0; i < 16; ++i) found[i] = 0;
         fence_mbar_init();
         if (!KV8) prefetch_tmap(&tmap_q), prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
     }
@@ -197,7 +223,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t s_phase = 0, tile_no = 0, item_no = 0;
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<KV8>(p, item_of(r), order);
+            const Item x = item_at<MODE>(p, item_of(r), order);
             if (x.n > 0 && t * 128 >= x.rows) {
                 tile_no += x.n;
                 continue;
@@ -205,7 +231,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (x.rows <= 0 || (!KV8 && x.n == 0)) continue;
             float m = -INFINITY, l = 0.f, factor = 1.f;
             // keys that this row sees
-            const int bound = KV8 && p.a.causal ? x.len - x.ql + (x.row0 + t * 128 + row) / ratio + 1 : x.seen;
+            const int bound = KV8 && p.a.causal ? x.len - x.ql + (x.row0 + t * 128 + row) / ratio + 1
+                            : MODE == PACKED && p.a.causal ? min(x.seen, x.token0 + t * (p.a.tile_tokens >> 1) + row / p.a.pack + 1) : x.seen;
             for (int j = 0; j < x.n; ++j, ++tile_no) {
                 if (!__all_sync(0xffffffffu, mbar_wait_moving(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL, moving))) { ok = false; break; }
                 s_phase ^= 1;
@@ -214,7 +241,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 const float* in = info + (tile_no & 3) * (KV8 ? 24 : 128);
                 if (KV8 && kBf16 && j == 0) factor = row_info[(item_no & 1) * 256 + t * 128 + row];
                 const int limit = bound - j * kTileKeys;
-                const bool all = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu && (!KV8 || __all_sync(0xffffffffu, limit >= kTileKeys));
+                const bool all = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu && (MODE == CROSS || __all_sync(0xffffffffu, limit >= kTileKeys));
                 // logits: in powers of two for the cache, without the factor c for 16-bit keys (the exponent's product applies it)
                 float v[128];
 #pragma unroll
@@ -237,6 +264,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
                             for (int e = 0; e < 16; ++e) v[q * 16 + e] = e < end ? v[q * 16 + e] : -INFINITY;
                         }
+                    } else if (MODE == PACKED) {
+#pragma unroll
+                        for (int e = 0; e < 128; ++e) v[e] = e < limit ? v[e] : -INFINITY;
                     } else {        // the smaller of logit and limit: -inf also for what is no number
 #pragma unroll
                         for (int q = 0; q < 32; ++q) {
@@ -364,7 +394,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             mbar_arrive(bar);
         };
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<KV8>(p, item_of(r), order);
+            const Item x = item_at<MODE>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
             uint32_t ks = kv_no & 3, k_phase = kv_no >> 2 & 1;
@@ -432,9 +462,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<KV8>(p, item_of(r), order);
+            const Item x = item_at<MODE>(p, item_of(r), order);
             if (x.n == 0) continue;
-            const int tiles = x.rows > 128 ? 2 : 1, kvh = x.h / (p.a.H / p.a.Hkv);
+            const int tiles = x.rows > 128 ? 2 : 1, kvh = MODE == PACKED ? x.h * p.a.pack / (p.a.H / p.a.Hkv) : x.h / (p.a.H / p.a.Hkv);
+            const uint32_t q_bytes = MODE == PACKED ? DP / 64 * 128 * (p.a.tile_tokens >> 1) * p.a.pack : L::kTile;
             auto load_kv = [&](int j, int which) {
                 const uint32_t slot = kv_no & 3;
                 if (!wait(kv_empty + 8 * slot, (kv_no >> 2 & 1) ^ 1)) return;
@@ -445,7 +476,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         const bool seen = key < x.seen && (!p.a.mask || gload(p.a.mask + x.b * p.a.mask_stride + key) != 0);
                         const uint32_t w = __ballot_sync(0xffffffffu, seen);
                         if (lane == 0) words[(tile_no & 3) * 4 + q] = w;
-                        info[(tile_no & 3) * 128 + q * 32 + lane] = seen ? INFINITY : -INFINITY;
+                        if (MODE == CROSS) info[(tile_no & 3) * 128 + q * 32 + lane] = seen ? INFINITY : -INFINITY;
                     }
                     __syncwarp();
                 }
@@ -453,7 +484,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     mbar_arrive_expect_tx(kv_full + 8 * slot, L::kTile);
 #pragma unroll
                     for (int box = 0; box < DP / 64; ++box)
-                        tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
+                        tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, (MODE == PACKED ? x.start : 0) + j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
                                     kv_full + 8 * slot);
                 }
                 __syncwarp();
@@ -464,17 +495,20 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 if (!wait(q_empty + 8 * t, (q_no[t] & 1) ^ 1)) break;
                 ++q_no[t];
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(q_full + 8 * t, L::kTile);
+                    mbar_arrive_expect_tx(q_full + 8 * t, q_bytes);
 #pragma unroll
-                    for (int box = 0; box < DP / 64; ++box)
-                        tma_load_4d(base + t * L::kTile + box * kBox, &tmap_q, box * 64, x.row0 + t * 128, x.h * p.q_head, x.b * p.q_batch, q_full + 8 * t);
+                    for (int box = 0; box < DP / 64; ++box) {
+                        const uint32_t dst = base + t * L::kTile + box * kBox;
+                        if (MODE == PACKED) tma_load_4d(dst, &tmap_q, box * 64, 0, x.start + x.token0 + t * (p.a.tile_tokens >> 1), x.h, q_full + 8 * t);
+                        else tma_load_4d(dst, &tmap_q, box * 64, x.row0 + t * 128, x.h * p.q_head, x.b * p.q_batch, q_full + 8 * t);
+                    }
                 }
                 __syncwarp();
             }
             if (ok) load_kv(0, 1);
             ++tile_no;
-            if (lane == 0 && item_of(r + 1) < p.items) {      // the next item's queries to L2
-                const Item y = item_at<KV8>(p, item_of(r + 1), order);
+            if (MODE == CROSS && lane == 0 && item_of(r + 1) < p.items) {      // the next item's queries to L2
+                const Item y = item_at<MODE>(p, item_of(r + 1), order);
                 for (int t = 0; t < 2 && t * 128 < y.rows; ++t)
 #pragma unroll
                     for (int box = 0; box < DP / 64; ++box) tma_prefetch_4d(&tmap_q, box * 64, y.row0 + t * 128, y.h * p.q_head, y.b * p.q_batch);
@@ -487,17 +521,41 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         }
       } else if (!KV8) {
         // ---- rows of V behind keys that are not seen: zeros. Two warps, 16 lanes (8 with 64 columns) to a row.
-        uint32_t kv_no = 1, tile_no = 0;
+        uint32_t kv_no = 1, tile_no = 0, item_no = 0;
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<KV8>(p, item_of(r), order);
+            const Item x = item_at<MODE>(p, item_of(r), order);
+            if (x.n == 0) continue;
+            bool noted = false;
+            if (MODE == PACKED && lane == 0) found[(warp - 10) * 8 + (item_no + 1 & 7)] = 0;
             for (int j = 0; j < x.n; ++j, ++tile_no, kv_no += 2) {
                 const uint32_t slot = kv_no & 3;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(kv_full + 8 * slot, kv_no >> 2 & 1, abort_s, ST_TIMEOUT_FULL)))) break;
                 const uint32_t* w = words + (tile_no & 3) * 4;
+                constexpr int kLanes = DP / 8;
+                const int piece = lane % kLanes;
+                if (MODE == PACKED && p.a.causal && (j + 1) * kTileKeys > x.token0 + 1) {
+                    // some of the item's rows see keys here that others do not: what would come through a weight of 0 is taken out and noted
+                    uint8_t* tile = sm + L::kRing + slot * L::kTile + (piece >> 3) * kBox;
+                    const int key0 = ((warp - 10) * 32 + lane) / kLanes, end = min(kTileKeys, x.seen - j * kTileKeys);
+                    auto at = [&](int key) { return reinterpret_cast<uint4*>(tile + key * 128 + ((piece ^ key) & 7) * 16); };
+                    bool bad = false;
+                    for (int key = key0; key < end; key += 64 / kLanes) bad |= any_infinite<QT>(*at(key));
+                    if (__any_sync(0xffffffffu, bad)) {
+                        int* first = from + ((warp - 10) * 8 + (item_no & 7)) * DP;
+                        if (!noted) {
+                            for (int c = lane; c < DP; c += 32) first[c] = INT32_MAX;
+                            noted = true;
+                            if (lane == 0) found[(warp - 10) * 8 + (item_no & 7)] = 1;
+                            __syncwarp();
+                        }
+                        for (int key = key0; key < end; key += 64 / kLanes)
+                            if (any_infinite<QT>(*at(key))) *at(key) = without_infinite<QT>(*at(key), j * kTileKeys + key, first + piece * 8);
+                        fence_proxy_async_smem();
+                    }
+                }
                 if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-                    constexpr int kLanes = DP / 8;
-                    const int piece = lane % kLanes, there = min(kTileKeys, p.a.Lkv - j * kTileKeys);      // the rest is zeros already
+                    const int there = MODE == PACKED ? kTileKeys : min(kTileKeys, p.a.Lkv - j * kTileKeys);      // the rest is zeros already
                     uint8_t* tile = sm + L::kRing + slot * L::kTile + (piece >> 3) * kBox + (piece & 7) * 16;
                     for (int key = ((warp - 10) * 32 + lane) / kLanes; key < there; key += 64 / kLanes)
                         if (!(w[key >> 5] >> (key & 31) & 1)) *reinterpret_cast<uint4*>(tile + key * 128) = make_uint4(0, 0, 0, 0);
@@ -506,17 +564,18 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(v_ready + 8 * (slot >> 1));
             }
+            ++item_no;
         }
       }
     } else if (!KV8) {
         // ---- the rows' way out: 64 columns at a time through this warp's staging, so that a row's pieces are stored together
         fewer_registers<L::kLastRegs>();
-        const int quarter = warp & 3;
+        const int quarter = warp & 3, by_pack = MODE == PACKED ? 65536 / p.a.pack + 1 : 0;      // row / pack of rows below 128, pack at most 16: (row * by_pack) >> 16
         uint8_t* stage = sm + L::kStaging + quarter * 4096;
-        uint32_t phase[2] = {}, item_no[2] = {};
+        uint32_t phase[2] = {}, item_no[2] = {}, done = 0;      // done: items of PACKED, none of which is without keys
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<KV8>(p, item_of(r), order);
+            const Item x = item_at<MODE>(p, item_of(r), order);
             for (int t = 0; t < 2 && t * 128 < x.rows; ++t) {
                 float inv = 0.f;
                 if (x.n > 0) {
@@ -526,7 +585,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     const float l = row_info[(item_no[t]++ & 1) * 256 + t * 128 + quarter * 32 + lane];
                     inv = l > 0.f || l != l ? 1.f / l : 0.f;      // 0: zeros, whatever the sums hold
                 }
-                const int left = min(32, x.rows - t * 128 - quarter * 32);      // rows of this warp; none: nothing is stored
+                // rows of this warp; none: nothing is stored
+                const int left = MODE == PACKED ? min(32, x.live[t] - quarter * 32) : min(32, x.rows - t * 128 - quarter * 32);
+                const int token0 = x.token0 + t * (p.a.tile_tokens >> 1);
+                const bool none = MODE == PACKED && p.a.causal && (found[done & 7] | found[8 + (done & 7)]) != 0;
                 QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + (x.row0 + t * 128 + quarter * 32) * p.a.os[1] + x.h * p.a.os[2];
 #pragma unroll
                 for (int q = 0; q < DP / 64; ++q) {
@@ -540,6 +602,14 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                             __syncwarp();
                             if (lane == 0) mbar_arrive(o_empty + 8 * t);
                         }
+                    }
+                    if (none) {      // columns of V with numbers that are none, from the row on that sees the first of them
+                        const int token = token0 + ((quarter * 32 + lane) * by_pack >> 16);
+                        for (int w = 0; w < 2; ++w)
+                            if (found[w * 8 + (done & 7)])
+#pragma unroll
+                                for (int e = 0; e < 64; ++e)
+                                    if (token >= from[(w * 8 + (done & 7)) * DP + q * 64 + e]) r[e >> 5][e & 31] = 0x7FC00000u;
                     }
                     if (__any_sync(0xffffffffu, inv == 0.f)) {      // no key seen: the columns may hold anything
 #pragma unroll
@@ -556,16 +626,28 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     }
                     __syncwarp();
                     const int e = lane & 7, d = q * 64 + e * 8;
-                    uint4 row[8];
+                    if constexpr (MODE == PACKED) {      // places worked out as they are needed: eight at a time would not fit beside the columns
+                        QT* out = reinterpret_cast<QT*>(p.a.out) + ((int64_t)x.start + token0) * p.a.os[1] + x.h * p.a.pack * p.a.os[2] + d;
+#pragma unroll 2
+                        for (int k = 0; k < 8; ++k) {
+                            const int r2 = k * 4 + (lane >> 3), at = quarter * 32 + r2, token = at * by_pack >> 16;
+                            if (r2 < left && d < D)
+                                *reinterpret_cast<uint4*>(out + token * p.a.os[1] + (at - token * p.a.pack) * p.a.os[2]) =
+                                    *reinterpret_cast<const uint4*>(stage + r2 * 128 + ((e ^ r2) & 7) * 16);
+                        }
+                    } else {
+                        uint4 row[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) row[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + (lane >> 3)) * 128 + ((e ^ (k * 4 + (lane >> 3))) & 7) * 16);
-                    QT* out = dst + (lane >> 3) * p.a.os[1] + d;
+                        for (int k = 0; k < 8; ++k) row[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + (lane >> 3)) * 128 + ((e ^ (k * 4 + (lane >> 3))) & 7) * 16);
+                        QT* out = dst + (lane >> 3) * p.a.os[1] + d;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k, out += 4 * p.a.os[1])
-                        if (k * 4 + (lane >> 3) < left && d < D) *reinterpret_cast<uint4*>(out) = row[k];
+                        for (int k = 0; k < 8; ++k, out += 4 * p.a.os[1])
+                            if (k * 4 + (lane >> 3) < left && d < D) *reinterpret_cast<uint4*>(out) = row[k];
+                    }
                     __syncwarp();
                 }
             }
+            done += x.n > 0;
         }
     } else {
         fewer_registers<L::kLastRegs>();
@@ -584,7 +666,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         };
         const int ratio = p.a.H / p.a.Hkv;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<KV8>(p, item_of(r), order);
+            const Item x = item_at<MODE>(p, item_of(r), order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
             for (int t = 0; t < tiles; ++t) {
@@ -713,9 +795,9 @@ bool make_rows_map(CUtensorMap* tm, const void* ptr, const int64_t (&s)[3], int 
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename QT, int DP, bool KV8> int launch_tc(const CUtensorMap (&tm)[3], const TcParams& p, cudaStream_t st) {
-    using L = Tc<DP, KV8>;
-    auto kern = attention_tc_kernel<QT, DP, KV8>;
+template <typename QT, int DP, Mode MODE> int launch_tc(const CUtensorMap (&tm)[3], const TcParams& p, cudaStream_t st) {
+    using L = Tc<DP, MODE>;
+    auto kern = attention_tc_kernel<QT, DP, MODE>;
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
     const int sms = sm_count();
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
@@ -750,10 +832,38 @@ int b200q::attention_tc(int dtype, bool kv8, AttnParams& a, cudaStream_t st) {
                  !make_rows_map(&tm[2], a.v, a.vs, a.B, a.Lkv, a.Hkv, a.D)))
         return -203;
     const bool h = dtype == DT_F16, wide = a.D > 64;
-    if (kv8) return h ? (wide ? launch_tc<half, 128, true>(tm, p, st) : launch_tc<half, 64, true>(tm, p, st))
-                      : (wide ? launch_tc<bf16, 128, true>(tm, p, st) : launch_tc<bf16, 64, true>(tm, p, st));
-    return h ? (wide ? launch_tc<half, 128, false>(tm, p, st) : launch_tc<half, 64, false>(tm, p, st))
-             : (wide ? launch_tc<bf16, 128, false>(tm, p, st) : launch_tc<bf16, 64, false>(tm, p, st));
+    if (kv8) return h ? (wide ? launch_tc<half, 128, CACHE>(tm, p, st) : launch_tc<half, 64, CACHE>(tm, p, st))
+                      : (wide ? launch_tc<bf16, 128, CACHE>(tm, p, st) : launch_tc<bf16, 64, CACHE>(tm, p, st));
+    return h ? (wide ? launch_tc<half, 128, CROSS>(tm, p, st) : launch_tc<half, 64, CROSS>(tm, p, st))
+             : (wide ? launch_tc<bf16, 128, CROSS>(tm, p, st) : launch_tc<bf16, 64, CROSS>(tm, p, st));
+}
+
+bool b200q::attention_tc_takes_packed(const AttnParams& p) {
+    if (p.D > 128 || !(p.scale > 0.f)) return false;
+    // rows without a stride between them have no tensor map
+    return (p.rows == 1 || (p.qs[1] > 0 && p.ks[1] > 0 && p.vs[1] > 0)) && (p.H == 1 || p.qs[2] > 0) && p.ks[2] >= 0 && p.vs[2] >= 0 && (p.ks[2] == 0) == (p.vs[2] == 0);
+}
+
+int b200q::attention_tc_packed(int dtype, AttnParams& a, cudaStream_t st) {
+    const int tokens = 128 / a.pack, groups = a.H / a.pack;      // of a tile of 128 rows
+    a.tile_tokens = 2 * tokens;
+    const int64_t tiles = (int64_t)a.rows / a.tile_tokens + a.B;
+    if (tiles > INT32_MAX / 2 / groups) return -1;
+    TcParams p = {};
+    p.a = a, p.q_tiles = (int)tiles, p.items = (uint32_t)(tiles * groups), p.kv_head = a.ks[2] != 0;
+    CUtensorMap tm[3] = {};
+    EncodeTiledFn enc = encode_fn();
+    auto pitch = [](int64_t stride) { return (cuuint64_t)(stride ? stride * 2 : 16); };
+    // queries: a token's heads of a group next to one another, then the next token's, as a tile has them
+    const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)(a.qs[2] ? a.pack : 1), (cuuint64_t)a.rows, (cuuint64_t)(a.qs[2] ? groups : 1)};
+    const cuuint64_t strides[3] = {pitch(a.qs[2]), pitch(a.qs[1]), pitch(a.qs[2] * a.pack)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)a.pack, (cuuint32_t)tokens, 1}, estr[4] = {1, 1, 1, 1};
+    if (!enc || enc(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+        !make_rows_map(&tm[1], a.k, a.ks, 1, a.rows, a.Hkv, a.D) || !make_rows_map(&tm[2], a.v, a.vs, 1, a.rows, a.Hkv, a.D))
+        return -203;
+    if (dtype == DT_F16) return a.D > 64 ? launch_tc<half, 128, PACKED>(tm, p, st) : launch_tc<half, 64, PACKED>(tm, p, st);
+    return a.D > 64 ? launch_tc<bf16, 128, PACKED>(tm, p, st) : launch_tc<bf16, 64, PACKED>(tm, p, st);
 }
 
 int b200q::attention_status_read_clear(int* out) {

@@ -96,6 +96,7 @@ template <int NT> __global__ void __launch_bounds__(Few<NT>::kThreads) f8_few_ke
         tmem_alloc(smem_u32(tmem_s), L::kColumns);
         tmem_relinquish();
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -226,6 +227,7 @@ template <int BN> __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) f8_ti
         tmem_alloc(smem_u32(tmem_s), 512);
         tmem_relinquish();
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
