@@ -48,14 +48,15 @@ template <int DP, Mode MODE> struct Tc {
     static constexpr int kWords = kTail + 208, kInfo = kWords + kSlots * 16, kRowInfo = kInfo + kSlots * (KV8 ? 96 : 512);
     static constexpr int kOrder = kRowInfo + 2048, kEnd0 = kOrder + 128;
     // packed: for each of the two warps that look through V, item % 8: whether it found numbers that are none, and the first key with one for each column
-    static constexpr int kFound = kEnd0, kFrom = kFound + 64, kEnd = MODE == PACKED ? kFrom + 16 * DP * 4 : kEnd0, kSmem = kEnd + 1024;
+    // and the CTA's items (before that, the sequences by length)
+    static constexpr int kFound = kEnd0, kItems = kFound + 64, kFrom = kItems + 128 * 32, kEnd = MODE == PACKED ? kFrom + 16 * DP * 4 : kEnd0, kSmem = kEnd + 1024;
     static constexpr int kThreads = 512;
     // Quarters of a key tile whose products with V start before the softmax has the rest: what is left of them stands between it and the next
     // logits, which take p's place. 16384 rows, 2048 keys, 128 columns, two | three: 357 | 349 us; 4096 x 4096, 64 columns: 165 | 166.
     static constexpr int kEarly = DP > 64 ? 3 : 2;
     // Registers of the warpgroups (softmax twice, products and loads, codes or rows out): a softmax thread holds a row of 128 logits. Their
     // sum over the threads is what the launch has, 512 x 128.
-    static constexpr int kSoftmaxRegs = 184, kIssueRegs = KV8 ? 40 : 56, kLastRegs = KV8 ? 104 : 88;
+    static constexpr int kSoftmaxRegs = 184, kIssueRegs = KV8 ? 40 : MODE == PACKED ? 72 : 56, kLastRegs = KV8 ? 104 : MODE == PACKED ? 72 : 88;
     static_assert(2 * kSoftmaxRegs + kIssueRegs + kLastRegs == 4 * 128, "register split");
 };
 
@@ -110,28 +111,82 @@ struct TcParams {
     uint32_t items;
     int kv_batch, kv_head;   // 0: the batch's (the heads') keys and values are one
     int q_batch, q_head;
+    uint32_t first_slot;     // packed: this launch's first tile
 };
 struct Item {
-    int b, h, row0, rows, len, ql, seen, n;      // h: query head, kv head, or group of `pack` heads; rows from row0 on; n key tiles
-    int start, token0, live[2];                  // packed: the sequence's row, the item's first token in it, rows of the two tiles
+    int b, h, row0, rows, len, ql, seen, n;      // h: query head, or kv head of packed rows; rows from row0 on; n key tiles
 };
+// Packed sequences: an item of the CTA's list. h: group of `pack` heads; rows: of both tiles, live: of each; seen: keys; start: the sequence's row, token0:
+// the item's first token in it. All warps work the list out at the start, one item each at a time: found anew by every role, an item's numbers cost
+// registers that the roles do not have (8192 tokens, 32 / 8 heads of 128: 534 us, L2 traffic of spilled registers alone a quarter of all).
+struct PackedItem {
+    int n, rows, seen, h, start, token0, live[2];
+};
+constexpr int kListed = 128;                     // items to a CTA and launch
 // The item of a CTA's r-th round: the rounds run through the CTAs forwards and backwards in turn, so that where the items get smaller, as the
 // cache's do, the sums of a CTA's items come out alike.
 __device__ __forceinline__ uint32_t item_of(uint32_t r) { return r * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
-template <Mode MODE> __device__ __forceinline__ Item item_at(const TcParams& p, uint32_t i, const int* order) {
+// Up to 32 sequences in the order of their tiles' number, the longest first, so that items with most key tiles can come first. Causal: the
+// last tiles of the longest, then level by level of all that are as long, down to everybody's first: `before` counts the items before those levels
+// that this sequence and all longer ones have, and no shorter one. Otherwise the sequences one after the other. (Six sequences of up to 2049 tokens, 32 / 8
+// heads of 128: 121 us in the packed order.)
+struct Packed {
+    int start, len, tiles, before;
+};
+__device__ __forceinline__ void order_packed(const AttnParams& p, Packed* list) {      // one warp
+    const int lane = threadIdx.x & 31;
+    Packed x = {};
+    if (lane < p.B) {
+        x.start = offset_at(p, lane), x.len = max(0, offset_at(p, lane + 1) - x.start);
+        x.tiles = (x.len + p.tile_tokens - 1) / p.tile_tokens;
+    }
+    int rank = 0;
+    for (int j = 0; j < 32; ++j) {
+        const int other = __shfl_sync(0xffffffffu, x.tiles, j);
+        rank += other > x.tiles || (other == x.tiles && j < lane);
+    }
+    list[rank] = x;
+    __syncwarp();
+    const int mine = list[lane].tiles, next = lane < 31 ? list[lane + 1].tiles : 0, items = p.causal ? (mine - next) * (lane + 1) : mine;
+    int sum = items;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += other;
+    }
+    list[lane].before = sum - items;
+}
+__device__ __forceinline__ PackedTile ordered_tile(const AttnParams& p, int slot, const Packed* list) {      // a whole warp
+    const int k = __popc(__ballot_sync(0xffffffffu, list[threadIdx.x & 31].before <= slot)) - 1, at = slot - list[k].before;
+    const Packed x = list[p.causal ? at % (k + 1) : k];
+    const int tile = p.causal ? list[k].tiles - 1 - at / (k + 1) : at;
+    PackedTile y;
+    y.start = x.start, y.len = x.len;
+    y.token0 = tile < 0 || tile >= x.tiles ? x.len : tile * p.tile_tokens;
+    y.tokens = min(p.tile_tokens, y.len - y.token0);
+    return y;
+}
+__device__ __forceinline__ PackedItem packed_item(const TcParams& p, uint32_t i, const Packed* order) {      // a whole warp
+    const uint32_t groups = p.a.H / p.a.pack, slot = p.first_slot + i / groups;
+    const PackedTile y = p.a.B <= 32 ? ordered_tile(p.a, (int)slot, order) : packed_tile(p.a, p.q_tiles - 1 - (int)slot);
+    PackedItem x;
+    x.h = (int)(i % groups), x.start = (int)y.start, x.token0 = y.token0;
+    const int half = p.a.tile_tokens >> 1;
+    x.live[0] = min(y.tokens, half) * p.a.pack, x.live[1] = max(0, y.tokens - half) * p.a.pack;
+    x.rows = x.live[1] > 0 ? 128 + x.live[1] : x.live[0];
+    x.seen = p.a.causal ? y.token0 + y.tokens : y.len;
+    x.n = x.rows > 0 ? (x.seen + kTileKeys - 1) / kTileKeys : 0;
+    return x;
+}
+// A CTA's r-th item
+template <Mode MODE> __device__ __forceinline__ Item nth_item(const TcParams& p, uint32_t r, const int* order) {
     constexpr bool KV8 = MODE == CACHE;
     Item x;
-    if constexpr (MODE == PACKED) {      // a whole warp asks; the last tiles of a sequence, which see most keys, first
-        const uint32_t groups = p.a.H / p.a.pack, slot = i / groups;
-        const PackedTile y = packed_tile(p.a, p.q_tiles - 1 - (int)slot);
-        x.b = 0, x.h = (int)(i - slot * groups), x.row0 = 0, x.ql = 0, x.len = y.len, x.start = (int)y.start, x.token0 = y.token0;
-        const int half = p.a.tile_tokens >> 1;
-        x.live[0] = min(y.tokens, half) * p.a.pack, x.live[1] = max(0, y.tokens - half) * p.a.pack;
-        x.rows = x.live[1] > 0 ? 128 + x.live[1] : x.live[0];
-        x.seen = p.a.causal ? y.token0 + y.tokens : y.len;
-        x.n = x.rows > 0 ? (x.seen + kTileKeys - 1) / kTileKeys : 0;
+    if constexpr (MODE == PACKED) {
+        const PackedItem& y = reinterpret_cast<const PackedItem*>(order)[r];
+        x.b = x.row0 = x.ql = x.len = 0, x.h = y.h, x.rows = y.rows, x.seen = y.seen, x.n = y.n;
         return x;
     }
+    const uint32_t i = item_of(r);
     const uint32_t heads = KV8 ? p.a.Hkv : p.a.H;
     // Heads next to one another: together they read and write whole rows of Q and of the result. Cache: long sequences first, of each the
     // tiles with most keys.
@@ -199,7 +254,20 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     const uint32_t tmem = *tmem_s;
     pdl_wait();
     const int D = p.a.D;
-    int* order = reinterpret_cast<int*>(sm + L::kOrder);      // sequences by length, the longest first
+    int* order = reinterpret_cast<int*>(sm + (MODE == PACKED ? L::kItems : L::kOrder));      // sequences by length, the longest first; packed: the items
+    const PackedItem* items = reinterpret_cast<const PackedItem*>(order);
+    if constexpr (MODE == PACKED) {
+        Packed* by_length = reinterpret_cast<Packed*>(sm + L::kFrom);      // nobody has found anything yet
+        if (p.a.B <= 32) {
+            if (warp == 0) order_packed(p.a, by_length);
+            __syncthreads();
+        }
+        for (uint32_t r = warp; item_of(r) < p.items; r += L::kThreads / 32) {
+            const PackedItem x = packed_item(p, item_of(r), by_length);
+            if (lane == 0) reinterpret_cast<PackedItem*>(order)[r] = x;
+        }
+        __syncthreads();
+    }
     if (KV8 && p.a.B <= 32) {
         if (warp == 0) {
             const int mine = lane < p.a.B ? gload(p.a.kv_len + lane) : INT32_MIN;
@@ -223,7 +291,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t s_phase = 0, tile_no = 0, item_no = 0;
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<MODE>(p, item_of(r), order);
+            const Item x = nth_item<MODE>(p, r, order);
             if (x.n > 0 && t * 128 >= x.rows) {
                 tile_no += x.n;
                 continue;
@@ -232,7 +300,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             float m = -INFINITY, l = 0.f, factor = 1.f;
             // keys that this row sees
             const int bound = KV8 && p.a.causal ? x.len - x.ql + (x.row0 + t * 128 + row) / ratio + 1
-                            : MODE == PACKED && p.a.causal ? min(x.seen, x.token0 + t * (p.a.tile_tokens >> 1) + row / p.a.pack + 1) : x.seen;
+                            : MODE == PACKED && p.a.causal ? min(x.seen, items[r].token0 + t * (p.a.tile_tokens >> 1) + row / p.a.pack + 1) : x.seen;
             for (int j = 0; j < x.n; ++j, ++tile_no) {
                 if (!__all_sync(0xffffffffu, mbar_wait_moving(s_full + 8 * t, s_phase, abort_s, ST_TIMEOUT_TMEM_FULL, moving))) { ok = false; break; }
                 s_phase ^= 1;
@@ -394,7 +462,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             mbar_arrive(bar);
         };
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<MODE>(p, item_of(r), order);
+            const Item x = nth_item<MODE>(p, r, order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
             uint32_t ks = kv_no & 3, k_phase = kv_no >> 2 & 1;
@@ -462,7 +530,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         bool ok = true;
         auto wait = [&](uint32_t bar, uint32_t parity) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, ST_TIMEOUT_EMPTY)); };
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<MODE>(p, item_of(r), order);
+            const Item x = nth_item<MODE>(p, r, order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1, kvh = MODE == PACKED ? x.h * p.a.pack / (p.a.H / p.a.Hkv) : x.h / (p.a.H / p.a.Hkv);
             const uint32_t q_bytes = MODE == PACKED ? DP / 64 * 128 * (p.a.tile_tokens >> 1) * p.a.pack : L::kTile;
@@ -484,7 +552,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     mbar_arrive_expect_tx(kv_full + 8 * slot, L::kTile);
 #pragma unroll
                     for (int box = 0; box < DP / 64; ++box)
-                        tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, (MODE == PACKED ? x.start : 0) + j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
+                        tma_load_4d(base + L::kRing + slot * L::kTile + box * kBox, which ? &tmap_v : &tmap_k, box * 64, (MODE == PACKED ? items[r].start : 0) + j * kTileKeys, kvh * p.kv_head, x.b * p.kv_batch,
                                     kv_full + 8 * slot);
                 }
                 __syncwarp();
@@ -499,7 +567,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
                     for (int box = 0; box < DP / 64; ++box) {
                         const uint32_t dst = base + t * L::kTile + box * kBox;
-                        if (MODE == PACKED) tma_load_4d(dst, &tmap_q, box * 64, 0, x.start + x.token0 + t * (p.a.tile_tokens >> 1), x.h, q_full + 8 * t);
+                        if (MODE == PACKED) tma_load_4d(dst, &tmap_q, box * 64, 0, items[r].start + items[r].token0 + t * (p.a.tile_tokens >> 1), x.h, q_full + 8 * t);
                         else tma_load_4d(dst, &tmap_q, box * 64, x.row0 + t * 128, x.h * p.q_head, x.b * p.q_batch, q_full + 8 * t);
                     }
                 }
@@ -508,7 +576,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
             if (ok) load_kv(0, 1);
             ++tile_no;
             if (MODE == CROSS && lane == 0 && item_of(r + 1) < p.items) {      // the next item's queries to L2
-                const Item y = item_at<MODE>(p, item_of(r + 1), order);
+                const Item y = nth_item<MODE>(p, r + 1, order);
                 for (int t = 0; t < 2 && t * 128 < y.rows; ++t)
 #pragma unroll
                     for (int box = 0; box < DP / 64; ++box) tma_prefetch_4d(&tmap_q, box * 64, y.row0 + t * 128, y.h * p.q_head, y.b * p.q_batch);
@@ -524,7 +592,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t kv_no = 1, tile_no = 0, item_no = 0;
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<MODE>(p, item_of(r), order);
+            const Item x = nth_item<MODE>(p, r, order);
             if (x.n == 0) continue;
             bool noted = false;
             if (MODE == PACKED && lane == 0) found[(warp - 10) * 8 + (item_no + 1 & 7)] = 0;
@@ -534,7 +602,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                 const uint32_t* w = words + (tile_no & 3) * 4;
                 constexpr int kLanes = DP / 8;
                 const int piece = lane % kLanes;
-                if (MODE == PACKED && p.a.causal && (j + 1) * kTileKeys > x.token0 + 1) {
+                if (MODE == PACKED && p.a.causal && (j + 1) * kTileKeys > items[r].token0 + 1) {
                     // some of the item's rows see keys here that others do not: what would come through a weight of 0 is taken out and noted
                     uint8_t* tile = sm + L::kRing + slot * L::kTile + (piece >> 3) * kBox;
                     const int key0 = ((warp - 10) * 32 + lane) / kLanes, end = min(kTileKeys, x.seen - j * kTileKeys);
@@ -575,7 +643,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         uint32_t phase[2] = {}, item_no[2] = {}, done = 0;      // done: items of PACKED, none of which is without keys
         bool ok = true;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<MODE>(p, item_of(r), order);
+            const Item x = nth_item<MODE>(p, r, order);
+            const PackedItem& item = items[MODE == PACKED ? r : 0];
             for (int t = 0; t < 2 && t * 128 < x.rows; ++t) {
                 float inv = 0.f;
                 if (x.n > 0) {
@@ -586,56 +655,79 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     inv = l > 0.f || l != l ? 1.f / l : 0.f;      // 0: zeros, whatever the sums hold
                 }
                 // rows of this warp; none: nothing is stored
-                const int left = MODE == PACKED ? min(32, x.live[t] - quarter * 32) : min(32, x.rows - t * 128 - quarter * 32);
-                const int token0 = x.token0 + t * (p.a.tile_tokens >> 1);
-                const bool none = MODE == PACKED && p.a.causal && (found[done & 7] | found[8 + (done & 7)]) != 0;
-                QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + (x.row0 + t * 128 + quarter * 32) * p.a.os[1] + x.h * p.a.os[2];
-#pragma unroll
-                for (int q = 0; q < DP / 64; ++q) {
-                    uint32_t r[2][32];
-                    if (x.n > 0) {
-                        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 64, r[0]);
-                        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 64 + 32, r[1]);
+                const int left = MODE == PACKED ? min(32, item.live[t] - quarter * 32) : min(32, x.rows - t * 128 - quarter * 32);
+                if constexpr (MODE == PACKED) {      // 32 columns at a time, places worked out as they are needed: 64 would not fit beside them
+                    const bool none = p.a.causal && (found[done & 7] | found[8 + (done & 7)]) != 0;
+#pragma unroll 1
+                    for (int q = 0; q < DP / 32; ++q) {
+                        uint32_t v[32];
+                        tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 32, v);
                         tmem_ld_wait();
-                        if (q == DP / 64 - 1) {      // the next item's products may have O
+                        if (q == DP / 32 - 1) {      // the next item's products may have O
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(o_empty + 8 * t);
                         }
-                    }
-                    if (none) {      // columns of V with numbers that are none, from the row on that sees the first of them
-                        const int token = token0 + ((quarter * 32 + lane) * by_pack >> 16);
-                        for (int w = 0; w < 2; ++w)
-                            if (found[w * 8 + (done & 7)])
+                        if (none) {      // columns of V with numbers that are none, from the row on that sees the first of them
+                            const int token = item.token0 + t * (p.a.tile_tokens >> 1) + ((quarter * 32 + lane) * by_pack >> 16);
+                            for (int w = 0; w < 2; ++w)
+                                if (found[w * 8 + (done & 7)])
 #pragma unroll
-                                for (int e = 0; e < 64; ++e)
-                                    if (token >= from[(w * 8 + (done & 7)) * DP + q * 64 + e]) r[e >> 5][e & 31] = 0x7FC00000u;
-                    }
-                    if (__any_sync(0xffffffffu, inv == 0.f)) {      // no key seen: the columns may hold anything
-#pragma unroll
-                        for (int e = 0; e < 64; ++e) r[e >> 5][e & 31] = inv == 0.f ? 0u : r[e >> 5][e & 31];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        uint4 v;
-                        uint32_t* o = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            o[f] = pack2<QT>(__uint_as_float(r[e >> 2][(e & 3) * 8 + 2 * f]) * inv, __uint_as_float(r[e >> 2][(e & 3) * 8 + 2 * f + 1]) * inv);
-                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = v;
-                    }
-                    __syncwarp();
-                    const int e = lane & 7, d = q * 64 + e * 8;
-                    if constexpr (MODE == PACKED) {      // places worked out as they are needed: eight at a time would not fit beside the columns
-                        QT* out = reinterpret_cast<QT*>(p.a.out) + ((int64_t)x.start + token0) * p.a.os[1] + x.h * p.a.pack * p.a.os[2] + d;
-#pragma unroll 2
-                        for (int k = 0; k < 8; ++k) {
-                            const int r2 = k * 4 + (lane >> 3), at = quarter * 32 + r2, token = at * by_pack >> 16;
-                            if (r2 < left && d < D)
-                                *reinterpret_cast<uint4*>(out + token * p.a.os[1] + (at - token * p.a.pack) * p.a.os[2]) =
-                                    *reinterpret_cast<const uint4*>(stage + r2 * 128 + ((e ^ r2) & 7) * 16);
+                                    for (int e = 0; e < 32; ++e)
+                                        if (token >= from[(w * 8 + (done & 7)) * DP + q * 32 + e]) v[e] = 0x7FC00000u;
                         }
-                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint4 y;
+                            uint32_t* o = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+                            for (int f = 0; f < 4; ++f)      // (no weight at all: zeros, whatever the sums hold)
+                                o[f] = inv == 0.f ? 0u : pack2<QT>(__uint_as_float(v[e * 8 + 2 * f]) * inv, __uint_as_float(v[e * 8 + 2 * f + 1]) * inv);
+                            *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ (lane >> 1)) & 3) * 16) = y;
+                        }
+                        __syncwarp();
+                        const int e = lane & 3, d = q * 32 + e * 8;
+                        QT* out = reinterpret_cast<QT*>(p.a.out) + ((int64_t)item.start + item.token0 + t * (p.a.tile_tokens >> 1)) * p.a.os[1] +
+                                  item.h * p.a.pack * p.a.os[2] + d;
+#pragma unroll 2
+                        for (int k = 0; k < 4; ++k) {
+                            const int rr = k * 8 + (lane >> 2), at = quarter * 32 + rr, token = at * by_pack >> 16;
+                            if (rr < left && d < D)
+                                *reinterpret_cast<uint4*>(out + token * p.a.os[1] + (at - token * p.a.pack) * p.a.os[2]) =
+                                    *reinterpret_cast<const uint4*>(stage + rr * 64 + ((e ^ (rr >> 1)) & 3) * 16);
+                        }
+                        __syncwarp();
+                    }
+                } else {
+                    QT* dst = reinterpret_cast<QT*>(p.a.out) + x.b * p.a.os[0] + (x.row0 + t * 128 + quarter * 32) * p.a.os[1] + x.h * p.a.os[2];
+#pragma unroll
+                    for (int q = 0; q < DP / 64; ++q) {
+                        uint32_t r[2][32];
+                        if (x.n > 0) {
+                            tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 64, r[0]);
+                            tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * 128 + q * 64 + 32, r[1]);
+                            tmem_ld_wait();
+                            if (q == DP / 64 - 1) {      // the next item's products may have O
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(o_empty + 8 * t);
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, inv == 0.f)) {      // no key seen: the columns may hold anything
+#pragma unroll
+                            for (int e = 0; e < 64; ++e) r[e >> 5][e & 31] = inv == 0.f ? 0u : r[e >> 5][e & 31];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            uint4 v;
+                            uint32_t* o = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                            for (int f = 0; f < 4; ++f)
+                                o[f] = pack2<QT>(__uint_as_float(r[e >> 2][(e & 3) * 8 + 2 * f]) * inv, __uint_as_float(r[e >> 2][(e & 3) * 8 + 2 * f + 1]) * inv);
+                            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = v;
+                        }
+                        __syncwarp();
+                        const int e = lane & 7, d = q * 64 + e * 8;
                         uint4 row[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) row[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + (lane >> 3)) * 128 + ((e ^ (k * 4 + (lane >> 3))) & 7) * 16);
@@ -643,8 +735,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
 #pragma unroll
                         for (int k = 0; k < 8; ++k, out += 4 * p.a.os[1])
                             if (k * 4 + (lane >> 3) < left && d < D) *reinterpret_cast<uint4*>(out) = row[k];
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
             done += x.n > 0;
@@ -666,7 +758,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         };
         const int ratio = p.a.H / p.a.Hkv;
         for (uint32_t r = 0; item_of(r) < p.items && ok; ++r) {
-            const Item x = item_at<MODE>(p, item_of(r), order);
+            const Item x = nth_item<MODE>(p, r, order);
             if (x.n == 0) continue;
             const int tiles = x.rows > 128 ? 2 : 1;
             for (int t = 0; t < tiles; ++t) {
@@ -848,9 +940,11 @@ int b200q::attention_tc_packed(int dtype, AttnParams& a, cudaStream_t st) {
     const int tokens = 128 / a.pack, groups = a.H / a.pack;      // of a tile of 128 rows
     a.tile_tokens = 2 * tokens;
     const int64_t tiles = (int64_t)a.rows / a.tile_tokens + a.B;
+    const int sms = sm_count();
+    if (sms <= 0) return (int)cudaErrorInvalidDevice;
     if (tiles > INT32_MAX / 2 / groups) return -1;
     TcParams p = {};
-    p.a = a, p.q_tiles = (int)tiles, p.items = (uint32_t)(tiles * groups), p.kv_head = a.ks[2] != 0;
+    p.a = a, p.q_tiles = (int)tiles, p.kv_head = a.ks[2] != 0;
     CUtensorMap tm[3] = {};
     EncodeTiledFn enc = encode_fn();
     auto pitch = [](int64_t stride) { return (cuuint64_t)(stride ? stride * 2 : 16); };
@@ -862,8 +956,16 @@ int b200q::attention_tc_packed(int dtype, AttnParams& a, cudaStream_t st) {
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
         !make_rows_map(&tm[1], a.k, a.ks, 1, a.rows, a.Hkv, a.D) || !make_rows_map(&tm[2], a.v, a.vs, 1, a.rows, a.Hkv, a.D))
         return -203;
-    if (dtype == DT_F16) return a.D > 64 ? launch_tc<half, 128, PACKED>(tm, p, st) : launch_tc<half, 64, PACKED>(tm, p, st);
-    return a.D > 64 ? launch_tc<bf16, 128, PACKED>(tm, p, st) : launch_tc<bf16, 64, PACKED>(tm, p, st);
+    // as many launches as the lists take (one up to some 150 000 rows of 32 / 8 heads)
+    const int64_t most = (int64_t)kListed * sms / groups > 0 ? (int64_t)kListed * sms / groups : 1;
+    if (groups > (int64_t)kListed * sms) return -1;
+    for (int64_t first = 0; first < tiles; first += most) {
+        p.first_slot = (uint32_t)first, p.items = (uint32_t)((tiles - first < most ? tiles - first : most) * groups);
+        const int rc = dtype == DT_F16 ? (a.D > 64 ? launch_tc<half, 128, PACKED>(tm, p, st) : launch_tc<half, 64, PACKED>(tm, p, st))
+                                       : (a.D > 64 ? launch_tc<bf16, 128, PACKED>(tm, p, st) : launch_tc<bf16, 64, PACKED>(tm, p, st));
+        if (rc != 0) return rc;
+    }
+    return 0;
 }
 
 int b200q::attention_status_read_clear(int* out) {
