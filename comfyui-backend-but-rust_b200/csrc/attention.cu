@@ -10,7 +10,6 @@
 // half a step of each term, and below fp16's normal numbers at most 2^-25 of the largest p: keys far below the maximum may count in the sum of
 // p and not in the result.
 #include "attention.cuh"
-#include <cstdlib>
 
 namespace {
 
@@ -570,7 +569,7 @@ template <typename T> int launch_cross(AttnParams& p, cudaStream_t st) {
     return p.D <= 192 ? launch_tile<T, 192>(p, st) : launch_tile<T, 256>(p, st);
 }
 template <typename T> int launch_packed(AttnParams& p, cudaStream_t st) {
-    if (attention_tc_takes_packed(p) && !getenv("PACKED_TILE")) return attention_tc_packed(std::is_same<T, half>::value ? DT_F16 : DT_BF16, p, st);
+    if (attention_tc_takes_packed(p)) return attention_tc_packed(std::is_same<T, half>::value ? DT_F16 : DT_BF16, p, st);
     if (p.D <= 64) return launch_packed<T, 64>(p, st);
     if (p.D <= 128) return launch_packed<T, 128>(p, st);
     return p.D <= 192 ? launch_packed<T, 192>(p, st) : launch_packed<T, 256>(p, st);

@@ -932,6 +932,11 @@ int b200q::attention_tc(int dtype, bool kv8, AttnParams& a, cudaStream_t st) {
 
 bool b200q::attention_tc_takes_packed(const AttnParams& p) {
     if (p.D > 128 || !(p.scale > 0.f)) return false;
+    // Short sequences that tiles of 64 rows on every SM have done in a round or three take longer here, where an item begins and ends slowly. us here |
+    // there, heads of 128, 32 / 8: 1 x 64 tokens 12.2 | 9.1, 1 x 256 12.6 | 15.9, 40 x 20 16.1 | 25.9, 32 x 64 18.4 | 39.8; 12 heads of 64: 1 x 77 7.7 | 6.2,
+    // 16 x 40 11.0 | 7.6, 16 x 77 11.1 | 9.1, 64 x 77 26.8 | 30.4, 8 x 128 8.3 | 9.1, 1 x 333 11.0 | 11.9.
+    const int64_t tiles = ((int64_t)p.rows * p.pack / 64 + p.B / 2) * (p.H / p.pack);
+    if (p.rows <= 1536 && p.rows <= (int64_t)100 * p.B && tiles <= 400) return false;
     // rows without a stride between them have no tensor map
     return (p.rows == 1 || (p.qs[1] > 0 && p.ks[1] > 0 && p.vs[1] > 0)) && (p.H == 1 || p.qs[2] > 0) && p.ks[2] >= 0 && p.vs[2] >= 0 && (p.ks[2] == 0) == (p.vs[2] == 0);
 }

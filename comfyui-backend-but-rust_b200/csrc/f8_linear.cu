@@ -4,7 +4,7 @@
 //
 // Few tokens, f8_few_kernel: the weight's bytes are the bound. 128 rows of the weight are the product's M, the tokens its N, so that both operands
 // come straight from TMA; a cluster of CTAs shares a tile's K where there are few tiles and adds up in shared memory, in a fixed order.
-// Many tokens, f8_tile_kernel: 128 tokens by up to 256 outputs, a persistent CTA an SM. While the tensor cores multiply one block, two warpgroups
+// Many tokens, f8_tile_kernel: 256 tokens by 256 outputs, a persistent pair of CTAs. While the tensor cores multiply one block, two warpgroups
 // take the block before out of the other accumulator; an output row to a thread, whose scale is one number a block then.
 // Every wait is bounded; one that runs out is recorded in g_f8_status and the CTA unwinds.
 #include "f8.cuh"
@@ -197,42 +197,143 @@ template <int NT> __global__ void __launch_bounds__(Few<NT>::kThreads) f8_few_ke
 }
 
 // ---- many tokens ------------------------------------------------------------------------------------------------------------------------
-// Warps 0-3 and 4-7: sums of the left and the right half of a tile's columns, an output row to a thread; warp 8 loads, warp 9 issues.
-template <int BN> struct Tile {
-    static constexpr int kStage = kBox + BN * kBlock, kStages = BN == 256 ? 4 : 5, kBuffers = 512 / BN, kHalf = BN / 2;
+// A pair of CTAs on a tile of 256 tokens by 256 outputs: each has its 128 tokens' sums and loads its tokens' block and half of the weight's, which
+// the tensor cores read from both. (A CTA alone on 128 x 256 needs 48 KB a block instead of 32: from L2 the device has some 14 TB/s, which bound
+// that form to 0.5 us a block, the products' own 0.27.) Warps 0-3 and 4-7: sums of the left and the right half of a tile's columns, an output row to a
+// thread; warp 8 loads, warp 9 of the first CTA issues the products of both.
+struct Tile {
+    static constexpr int kStage = 2 * kBox, kStages = 6, kBuffers = 2, kColumns = 256, kHalf = 128;
     static constexpr int kStaging = kStages * kStage, kTail = kStaging + 8 * 4096, kSmem = kTail + 256 + 1024, kThreads = 384;
     // registers: 384 threads x 168 at launch; a sums' thread holds a row of kHalf sums and 64 columns on their way
     static constexpr int kSumRegs = 224, kRestRegs = 56;
+    static_assert(2 * kSumRegs + kRestRegs == 3 * 168, "register split");
 };
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128) : "memory");
+}
 
-template <int BN> __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
-                                                                                       const F8Params p) {
-    using L = Tile<BN>;
+// A warp's 32 rows of sums out, by way of its staging, so that a row's pieces are stored together
+__device__ __forceinline__ void rows_out(const F8Params& p, const uint64_t (&sum)[Tile::kHalf / 2], uint8_t* stage, int m0, int n0, int lane) {
+    constexpr int kCols = Tile::kHalf;
+    const int left = min(32, p.M - m0), esize = p.out_dt == DT_F32 ? 4 : 2;
+    if (left <= 0 || n0 >= p.N) return;
+    const bool whole = n0 + kCols <= p.N && p.out_stride * esize % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 &&
+                       (!p.bias || (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0);
+    if (whole && esize == 2 && !p.add) {
+#pragma unroll
+        for (int c = 0; c < kCols; c += 64) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) unpack_f32(sum[c / 2 + e * 4 + i], y[2 * i], y[2 * i + 1]);
+                if (p.bias) {
+                    float b[8];
+                    if (p.out_dt == DT_F16) load8<half>(reinterpret_cast<const half*>(p.bias) + n0 + c + e * 8, b);
+                    else load8<bf16>(reinterpret_cast<const bf16*>(p.bias) + n0 + c + e * 8, b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] += b[i];
+                }
+                *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) =
+                    p.out_dt == DT_F16 ? make_uint4(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]), pack2<half>(y[4], y[5]), pack2<half>(y[6], y[7]))
+                                       : make_uint4(pack2<bf16>(y[0], y[1]), pack2<bf16>(y[2], y[3]), pack2<bf16>(y[4], y[5]), pack2<bf16>(y[6], y[7]));
+            }
+            __syncwarp();
+            const int e = lane & 7;
+            uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (int64_t)(m0 + (lane >> 3)) * p.out_stride + n0 + c + e * 8;
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4*>(stage + (k * 4 + (lane >> 3)) * 128 + ((e ^ (k * 4 + (lane >> 3))) & 7) * 16);
+#pragma unroll
+            for (int k = 0; k < 8; ++k, out += 4 * p.out_stride)
+                if (k * 4 + (lane >> 3) < left) *reinterpret_cast<uint4*>(out) = v[k];
+            __syncwarp();
+        }
+        return;
+    }
+    // f32 rows, rows that are added to, ragged ones: 32 columns of f32 at a time
+#pragma unroll
+    for (int c = 0; c < kCols; c += 32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float4 v;
+            unpack_f32(sum[c / 2 + 2 * e], v.x, v.y), unpack_f32(sum[c / 2 + 2 * e + 1], v.z, v.w);
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = v;
+        }
+        __syncwarp();
+        if (whole) {
+            const int e = lane & 7, col = n0 + c + e * 4;
+            float b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = p.bias ? value_at(p.bias, p.out_dt, col + i) : 0.f;
+#pragma unroll 2
+            for (int k = 0; k < 8; ++k) {
+                const int r = k * 4 + (lane >> 3);
+                if (r >= left) break;
+                const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((e ^ r) & 7) * 16);
+                float y[4] = {v.x + b[0], v.y + b[1], v.z + b[2], v.w + b[3]};
+                const int64_t at = (int64_t)(m0 + r) * p.out_stride + col;
+                if (p.add)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] += value_at(p.out, p.out_dt, at + i);
+                if (esize == 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+                else
+                    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = p.out_dt == DT_F16 ? make_uint2(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]))
+                                                                                                            : make_uint2(pack2<bf16>(y[0], y[1]), pack2<bf16>(y[2], y[3]));
+            }
+        } else if (n0 + c + lane < p.N) {
+            const int col = n0 + c + lane;
+            const float b = p.bias ? value_at(p.bias, p.out_dt, col) : 0.f;
+#pragma unroll 2
+            for (int r = 0; r < left; ++r) {
+                float y = *reinterpret_cast<const float*>(stage + r * 128 + (((lane >> 2) ^ r) & 7) * 16 + (lane & 3) * 4) + b;
+                const int64_t at = (int64_t)(m0 + r) * p.out_stride + col;
+                if (p.add) y += value_at(p.out, p.out_dt, at);
+                put_value(p.out, p.out_dt, at, y);
+            }
+        }
+        __syncwarp();
+    }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile::kThreads, 1)
+f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Params p) {
+    using L = Tile;
     constexpr int kHalf = L::kHalf;
     extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;      // the same in both CTAs
     uint8_t* sm = smem_raw + (base - raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // full and t_empty: the first CTA's are used
     const uint32_t full = base + L::kTail, empty = full + 8 * L::kStages, t_full = empty + 8 * L::kStages, t_empty = t_full + 8 * L::kBuffers;
     uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 240);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
+    const uint32_t rank = cluster_ctarank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-        for (int i = 0; i < L::kBuffers; ++i) mbar_init(t_full + 8 * i, 1), mbar_init(t_empty + 8 * i, 8);
+        for (int i = 0; i < L::kBuffers; ++i) mbar_init(t_full + 8 * i, 1), mbar_init(t_empty + 8 * i, 16);
         *abort_s = 0;
         fence_mbar_init();
         prefetch_tmap(&tmap_x), prefetch_tmap(&tmap_w);
     }
     if (warp == 9) {
-        tmem_alloc(smem_u32(tmem_s), 512);
-        tmem_relinquish();
+        tmem_alloc_pair(smem_u32(tmem_s), 512);
+        tmem_relinquish_pair();
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    cluster_sync_all();      // the other CTA's barriers exist before anything signals them
     tc_fence_after();
     const uint32_t tmem = *tmem_s;
     pdl_wait();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (warp < 8) {
         more_registers<L::kSumRegs>();
         const int side = warp >> 2, quarter = warp & 3;
@@ -240,38 +341,32 @@ template <int BN> __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) f8_ti
         uint8_t* stage = sm + L::kStaging + warp * 4096;
         uint32_t no = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
-            const int m0 = tile % p.m_tiles * 128 + quarter * 32, n0 = tile / p.m_tiles * BN + side * kHalf;
+        for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
+            const int m0 = tile % p.m_tiles * 256 + (int)rank * 128 + quarter * 32, n0 = tile / p.m_tiles * L::kColumns + side * kHalf;
             const float* xs = p.xs + (int64_t)min(m0 + lane, p.M - 1) * p.groups;
             const float* ws = p.ws + (int64_t)(min(n0, p.N - 1) / 128) * p.groups;
             uint64_t sum[kHalf / 2] = {};
-            float now[4], next[4];      // scales of four blocks, requested four blocks ahead
-            auto request = [&](int g0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) next[i] = g0 + i < p.groups ? gload(xs + g0 + i) * gload(ws + g0 + i) : 0.f;
-            };
-            request(0);
+            // the scales of the block after next are on their way; their product is formed when it is needed, so that nobody waits for them
+            float x_scale[2] = {gload(xs), gload(xs + min(1, p.groups - 1))}, w_scale[2] = {gload(ws), gload(ws + min(1, p.groups - 1))};
             for (int g = 0; g < p.groups; ++g, ++no) {
-                if ((g & 3) == 0) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) now[i] = next[i];
-                    request(g + 4);
-                }
-                const uint64_t s = pack_f32(now[0], now[0]);
-                now[0] = now[1], now[1] = now[2], now[2] = now[3];
+                const float scale = x_scale[0] * w_scale[0];
+                const uint64_t s = pack_f32(scale, scale);
+                const int ahead = min(g + 2, p.groups - 1);
+                x_scale[0] = x_scale[1], w_scale[0] = w_scale[1];
+                x_scale[1] = gload(xs + ahead), w_scale[1] = gload(ws + ahead);
                 const uint32_t buf = no % L::kBuffers;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(t_full + 8 * buf, no / L::kBuffers & 1, abort_s, ST_TIMEOUT_TMEM_FULL)))) break;
                 tc_fence_after();
                 uint32_t t[2][32];
-                tmem_ld32(lanes + buf * BN, t[0]);
+                tmem_ld32(lanes + buf * L::kColumns, t[0]);
 #pragma unroll
                 for (int c = 0; c < kHalf; c += 32) {
                     tmem_ld_wait();
-                    if (c + 32 < kHalf) tmem_ld32(lanes + buf * BN + c + 32, t[(c >> 5) + 1 & 1]);
+                    if (c + 32 < kHalf) tmem_ld32(lanes + buf * L::kColumns + c + 32, t[(c >> 5) + 1 & 1]);
                     else {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(t_empty + 8 * buf);
+                        if (lane == 0) mbar_arrive_remote(mapa_shared(t_empty + 8 * buf, 0));
                     }
                     const uint32_t(&r)[32] = t[c >> 5 & 1];
 #pragma unroll
@@ -280,78 +375,33 @@ template <int BN> __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) f8_ti
                 }
             }
             if (!ok) break;
-            // ---- rows out: 32 columns of f32 at a time through this warp's staging, so that a row's pieces are stored together
-            const int esize = p.out_dt == DT_F32 ? 4 : 2;
-            const bool whole = n0 + kHalf <= p.N && (p.out_stride * esize) % (4 * esize) == 0 && (reinterpret_cast<uintptr_t>(p.out) % (4 * esize)) == 0;
-#pragma unroll
-            for (int c = 0; c < kHalf; c += 32) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float4 v;
-                    unpack_f32(sum[c / 2 + 2 * e], v.x, v.y), unpack_f32(sum[c / 2 + 2 * e + 1], v.z, v.w);
-                    *reinterpret_cast<float4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = v;
-                }
-                __syncwarp();
-                const int e = lane & 7, col = n0 + c + e * 4;
-                float b[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) b[i] = p.bias && col + i < p.N ? value_at(p.bias, p.out_dt, col + i) : 0.f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = k * 4 + (lane >> 3), row = m0 + r;
-                    if (row >= p.M) continue;
-                    const float4 v4 = *reinterpret_cast<const float4*>(stage + r * 128 + ((e ^ r) & 7) * 16);
-                    float y[4] = {v4.x + b[0], v4.y + b[1], v4.z + b[2], v4.w + b[3]};
-                    const int64_t at = (int64_t)row * p.out_stride + col;
-                    if (whole) {
-                        if (p.out_dt == DT_F32) {
-                            float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
-                            float4 o = make_float4(y[0], y[1], y[2], y[3]);
-                            if (p.add) {
-                                const float4 old = gload(dst);
-                                o.x += old.x, o.y += old.y, o.z += old.z, o.w += old.w;
-                            }
-                            *dst = o;
-                        } else {
-                            uint2* dst = reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at);
-                            if (p.add)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) y[i] += value_at(p.out, p.out_dt, at + i);
-                            *dst = p.out_dt == DT_F16 ? make_uint2(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]))
-                                                      : make_uint2(pack2<bf16>(y[0], y[1]), pack2<bf16>(y[2], y[3]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (col + i < p.N) put_value(p.out, p.out_dt, at + i, y[i] + (p.add ? value_at(p.out, p.out_dt, at + i) : 0.f));
-                    }
-                }
-                __syncwarp();
-            }
+            rows_out(p, sum, stage, m0, n0, lane);
         }
     } else {
         fewer_registers<L::kRestRegs>();
         if (warp == 8) {
             uint32_t no = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x)
+            for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
+                const int row_x = tile % p.m_tiles * 256 + (int)rank * 128, row_w = tile / p.m_tiles * L::kColumns + (int)rank * 128;
                 for (int g = 0; g < p.groups; ++g, ++no) {
                     const uint32_t stage = no % L::kStages;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * stage, (no / L::kStages & 1) ^ 1, abort_s, ST_TIMEOUT_EMPTY)))) break;
                     if (lane == 0) {
-                        const uint32_t at = base + stage * L::kStage;
-                        mbar_arrive_expect_tx(full + 8 * stage, L::kStage);
-                        tma_load_2d(at, &tmap_x, g * kBlock, tile % p.m_tiles * 128, full + 8 * stage);
-                        tma_load_2d(at + kBox, &tmap_w, g * kBlock, tile / p.m_tiles * BN, full + 8 * stage);
+                        const uint32_t at = base + stage * L::kStage, bar = mapa_shared(full + 8 * stage, 0);
+                        if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, 2 * L::kStage);
+                        tma_load_2d_pair(at, &tmap_x, g * kBlock, row_x, bar);
+                        tma_load_2d_pair(at + kBox, &tmap_w, g * kBlock, row_w, bar);
                     }
                     __syncwarp();
                 }
-        } else if (warp == 9) {
+            }
+        } else if (warp == 9 && rank == 0) {
             const bool one = elect_one();
             uint32_t no = 0;
             bool ok = true;
             auto wait = [&](uint32_t bar, uint32_t parity, int code) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, code)); };
-            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x)
+            for (int tile = pair; tile < p.tiles && ok; tile += pairs)
                 for (int g = 0; g < p.groups; ++g, ++no) {
                     const uint32_t stage = no % L::kStages, buf = no % L::kBuffers;
                     if (!wait(t_empty + 8 * buf, (no / L::kBuffers & 1) ^ 1, ST_TIMEOUT_TMEM_EMPTY) || !wait(full + 8 * stage, no / L::kStages & 1, ST_TIMEOUT_FULL)) break;
@@ -359,15 +409,27 @@ template <int BN> __global__ void __launch_bounds__(Tile<BN>::kThreads, 1) f8_ti
                     if (one) {
                         const uint32_t x = umma_desc_lo(base + stage * L::kStage), w = umma_desc_lo(base + stage * L::kStage + kBox);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) umma_f8(tmem + buf * BN, x + 2 * k, w + 2 * k, umma_idesc_f8(128, BN), k > 0);
-                        umma_commit(empty + 8 * stage);
-                        umma_commit(t_full + 8 * buf);
+                        for (int k = 0; k < 4; ++k) umma_f8_pair(tmem + buf * L::kColumns, x + 2 * k, w + 2 * k, umma_idesc_f8(256, L::kColumns), k > 0);
+                        umma_commit_pair(empty + 8 * stage);
+                        umma_commit_pair(t_full + 8 * buf);
                     }
                     __syncwarp();
                 }
         }
     }
-    leave(abort_s, warp == 9, tmem, 512);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();      // nobody leaves while the other may still signal its barriers or read its tiles
+    if (*abort_s != 0) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);      // leave time for copies and products still in flight, then report
+        if (threadIdx.x == 0) atomicCAS(&g_f8_status, 0, *abort_s);
+        __syncthreads();
+    }
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------------
@@ -393,17 +455,17 @@ template <int NT> int launch_few(const void* x, int64_t x_stride, const void* W,
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(256))) return (int)e;
     return launch_pdl_cluster(kern, dim3((unsigned)(p.tiles * p.splits)), L::kThreads, smem, st, p.splits, tx, tw, p);
 }
-template <int BN> int launch_tile(const void* x, int64_t x_stride, const void* W, F8Params& p, int sms, cudaStream_t st) {
-    using L = Tile<BN>;
+int launch_tile(const void* x, int64_t x_stride, const void* W, F8Params& p, int sms, cudaStream_t st) {
+    using L = Tile;
     CUtensorMap tx, tw;
-    if (!codes_map(&tx, x, x_stride, p.M, p.K, 128) || !codes_map(&tw, W, p.K, p.N, p.K, BN)) return -203;
-    p.m_tiles = (p.M + 127) / 128;
-    const int64_t tiles = (int64_t)p.m_tiles * ((p.N + BN - 1) / BN);
+    if (!codes_map(&tx, x, x_stride, p.M, p.K, 128) || !codes_map(&tw, W, p.K, p.N, p.K, 128)) return -203;
+    p.m_tiles = (p.M + 255) / 256;
+    const int64_t tiles = (int64_t)p.m_tiles * ((p.N + L::kColumns - 1) / L::kColumns);
     if (tiles > INT32_MAX / 2) return -1;      // and so does a tile a round further on
     p.tiles = (int)tiles;
-    auto kern = f8_tile_kernel<BN>;
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
-    return launch_pdl(kern, dim3((unsigned)(p.tiles < sms ? p.tiles : sms)), L::kThreads, L::kSmem, st, tx, tw, p);
+    if (cudaError_t e = cudaFuncSetAttribute(f8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
+    const int pairs = p.tiles < sms / 2 ? p.tiles : sms / 2;
+    return launch_pdl(f8_tile_kernel, dim3((unsigned)(2 * pairs)), L::kThreads, L::kSmem, st, tx, tw, p);
 }
 
 }  // namespace
@@ -437,7 +499,5 @@ GPU_API int gpu_f8_linear(const void* x, int64_t x_stride, const float* xs, cons
     if (M <= 64) return launch_few<64>(x, x_stride, W, p, st);
     const int sms = sm_count();
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
-    // tiles of 256 outputs where they fill the device
-    const int64_t wide = (int64_t)((M + 127) / 128) * ((N + 255) / 256);
-    return wide >= 2 * sms ? launch_tile<256>(x, x_stride, W, p, sms, st) : launch_tile<128>(x, x_stride, W, p, sms, st);
+    return launch_tile(x, x_stride, W, p, sms, st);
 }
