@@ -200,10 +200,12 @@ template <int NT> __global__ void __launch_bounds__(Few<NT>::kThreads) f8_few_ke
 // A pair of CTAs on a tile of 256 tokens by 256 outputs: each has its 128 tokens' sums and loads its tokens' block and half of the weight's, which
 // the tensor cores read from both. (A CTA alone on 128 x 256 needs 48 KB a block instead of 32: from L2 the device has some 14 TB/s, which bound
 // that form to 0.5 us a block, the products' own 0.27.) Warps 0-3 and 4-7: sums of the left and the right half of a tile's columns, an output row to a
-// thread; warp 8 loads, warp 9 of the first CTA issues the products of both.
+// thread; warp 8 loads, warp 9 of the first CTA issues the products of both, warps 10 and 11 bring in the scales.
 struct Tile {
-    static constexpr int kStage = 2 * kBox, kStages = 6, kBuffers = 2, kColumns = 256, kHalf = 128;
-    static constexpr int kStaging = kStages * kStage, kTail = kStaging + 8 * 4096, kSmem = kTail + 256 + 1024, kThreads = 384;
+    static constexpr int kStage = 2 * kBox, kStages = 5, kBuffers = 2, kColumns = 256, kHalf = 128, kChunk = 8;
+    // kChunk blocks' scales, twice: of 128 rows of x, of two blocks of the weight
+    static constexpr int kStaging = kStages * kStage, kXScales = kStaging + 8 * 4096, kWScales = kXScales + 2 * kChunk * 512, kTail = kWScales + 2 * kChunk * 8;
+    static constexpr int kSmem = kTail + 256 + 1024, kThreads = 384;
     // registers: 384 threads x 168 at launch; a sums' thread holds a row of kHalf sums and 64 columns on their way
     static constexpr int kSumRegs = 224, kRestRegs = 56;
     static_assert(2 * kSumRegs + kRestRegs == 3 * 168, "register split");
@@ -219,7 +221,7 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
 }
 
 // A warp's 32 rows of sums out, by way of its staging, so that a row's pieces are stored together
-__device__ __forceinline__ void rows_out(const F8Params& p, const uint64_t (&sum)[Tile::kHalf / 2], uint8_t* stage, int m0, int n0, int lane) {
+__device__ __forceinline__ void rows_out(const F8Params& p, const float (&sum)[Tile::kHalf], uint8_t* stage, int m0, int n0, int lane) {
     constexpr int kCols = Tile::kHalf;
     const int left = min(32, p.M - m0), esize = p.out_dt == DT_F32 ? 4 : 2;
     if (left <= 0 || n0 >= p.N) return;
@@ -232,7 +234,7 @@ __device__ __forceinline__ void rows_out(const F8Params& p, const uint64_t (&sum
             for (int e = 0; e < 8; ++e) {
                 float y[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) unpack_f32(sum[c / 2 + e * 4 + i], y[2 * i], y[2 * i + 1]);
+                for (int i = 0; i < 8; ++i) y[i] = sum[c + e * 8 + i];
                 if (p.bias) {
                     float b[8];
                     if (p.out_dt == DT_F16) load8<half>(reinterpret_cast<const half*>(p.bias) + n0 + c + e * 8, b);
@@ -261,11 +263,8 @@ __device__ __forceinline__ void rows_out(const F8Params& p, const uint64_t (&sum
 #pragma unroll
     for (int c = 0; c < kCols; c += 32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float4 v;
-            unpack_f32(sum[c / 2 + 2 * e], v.x, v.y), unpack_f32(sum[c / 2 + 2 * e + 1], v.z, v.w);
-            *reinterpret_cast<float4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = v;
-        }
+        for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = make_float4(sum[c + 4 * e], sum[c + 4 * e + 1], sum[c + 4 * e + 2], sum[c + 4 * e + 3]);
         __syncwarp();
         if (whole) {
             const int e = lane & 7, col = n0 + c + e * 4;
@@ -312,12 +311,15 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // full and t_empty: the first CTA's are used
     const uint32_t full = base + L::kTail, empty = full + 8 * L::kStages, t_full = empty + 8 * L::kStages, t_empty = t_full + 8 * L::kBuffers;
+    const uint32_t s_full = t_empty + 8 * L::kBuffers, s_empty = s_full + 16;
+    float *x_scales = reinterpret_cast<float*>(sm + L::kXScales), *w_scales = reinterpret_cast<float*>(sm + L::kWScales);      // [chunk % 2][block][row], [block][side]
     uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 240);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
     const uint32_t rank = cluster_ctarank();
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < L::kBuffers; ++i) mbar_init(t_full + 8 * i, 1), mbar_init(t_empty + 8 * i, 16);
+        for (int i = 0; i < 2; ++i) mbar_init(s_full + 8 * i, 2), mbar_init(s_empty + 8 * i, 8);
         *abort_s = 0;
         fence_mbar_init();
         prefetch_tmap(&tmap_x), prefetch_tmap(&tmap_w);
@@ -339,39 +341,40 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         const int side = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + side * kHalf;
         uint8_t* stage = sm + L::kStaging + warp * 4096;
-        uint32_t no = 0;
+        uint32_t no = 0, chunk = 0;
         bool ok = true;
         for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
             const int m0 = tile % p.m_tiles * 256 + (int)rank * 128 + quarter * 32, n0 = tile / p.m_tiles * L::kColumns + side * kHalf;
-            const float* xs = p.xs + (int64_t)min(m0 + lane, p.M - 1) * p.groups;
-            const float* ws = p.ws + (int64_t)(min(n0, p.N - 1) / 128) * p.groups;
-            uint64_t sum[kHalf / 2] = {};
-            // the scales of the block after next are on their way; their product is formed when it is needed, so that nobody waits for them
-            float x_scale[2] = {gload(xs), gload(xs + min(1, p.groups - 1))}, w_scale[2] = {gload(ws), gload(ws + min(1, p.groups - 1))};
+            float sum[kHalf] = {};
             for (int g = 0; g < p.groups; ++g, ++no) {
-                const float scale = x_scale[0] * w_scale[0];
-                const uint64_t s = pack_f32(scale, scale);
-                const int ahead = min(g + 2, p.groups - 1);
-                x_scale[0] = x_scale[1], w_scale[0] = w_scale[1];
-                x_scale[1] = gload(xs + ahead), w_scale[1] = gload(ws + ahead);
+                const int part = g % L::kChunk, at = (int)(chunk & 1) * L::kChunk + part;
+                if (part == 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (chunk & 1), chunk >> 1 & 1, abort_s, ST_TIMEOUT_UNPACK)))) break;
+                const float scale = x_scales[at * 128 + quarter * 32 + lane] * w_scales[at * 2 + side];
+                if (part == L::kChunk - 1 || g == p.groups - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty + 8 * (chunk & 1));
+                    ++chunk;
+                }
                 const uint32_t buf = no % L::kBuffers;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait(t_full + 8 * buf, no / L::kBuffers & 1, abort_s, ST_TIMEOUT_TMEM_FULL)))) break;
+                if (warp == 0 && lane == 0) mbar_arrive(empty + 8 * (no % L::kStages));      // the products have read the stage as well: one commit a block
                 tc_fence_after();
-                uint32_t t[2][32];
-                tmem_ld32(lanes + buf * L::kColumns, t[0]);
 #pragma unroll
-                for (int c = 0; c < kHalf; c += 32) {
+                for (int c = 0; c < kHalf; c += 64) {
+                    uint32_t t[64];
+                    tmem_ld32(lanes + buf * L::kColumns + c, reinterpret_cast<uint32_t(&)[32]>(t[0]));
+                    tmem_ld32(lanes + buf * L::kColumns + c + 32, reinterpret_cast<uint32_t(&)[32]>(t[32]));
                     tmem_ld_wait();
-                    if (c + 32 < kHalf) tmem_ld32(lanes + buf * L::kColumns + c + 32, t[(c >> 5) + 1 & 1]);
-                    else {
+                    if (c + 64 == kHalf) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_remote(mapa_shared(t_empty + 8 * buf, 0));
                     }
-                    const uint32_t(&r)[32] = t[c >> 5 & 1];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        sum[(c + e) / 2] = fma_f32x2(pack_f32(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), s, sum[(c + e) / 2]);
+                    for (int e = 0; e < 64; e += 2) {      // two sums an instruction (single ones: 288 us instead of 282, 4352 x 5120 -> 13824)
+                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(t[e]), __uint_as_float(t[e + 1])), make_float2(scale, scale), make_float2(sum[c + e], sum[c + e + 1]));
+                        sum[c + e] = y.x, sum[c + e + 1] = y.y;
+                    }
                 }
             }
             if (!ok) break;
@@ -396,6 +399,33 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
                     __syncwarp();
                 }
             }
+        } else if (warp >= 10) {
+            // ---- scales, kChunk blocks at a time, 64 rows a warp: rows of x lie groups * 4 bytes apart, 32 sectors to a load, which the sums' warps would
+            // wait for block by block (4352 x 5120 -> 13824: 291 us with their loads two blocks ahead)
+            uint32_t chunk = 0;
+            bool ok = true;
+            for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
+                const int m0 = tile % p.m_tiles * 256 + (int)rank * 128 + (warp - 10) * 64, n0 = tile / p.m_tiles * L::kColumns;
+                for (int g0 = 0; g0 < p.groups; g0 += L::kChunk, ++chunk) {
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_empty + 8 * (chunk & 1), (chunk >> 1 & 1) ^ 1, abort_s, ST_TIMEOUT_EMPTY)))) break;
+                    float v[2][L::kChunk], w = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < L::kChunk; ++e)
+                            v[i][e] = m0 + i * 32 + lane < p.M && g0 + e < p.groups ? gload(p.xs + (int64_t)(m0 + i * 32 + lane) * p.groups + g0 + e) : 0.f;
+                    if (warp == 10 && lane < 2 * L::kChunk && g0 + lane / 2 < p.groups && n0 + lane % 2 * kHalf < p.N)
+                        w = gload(p.ws + (int64_t)((n0 + lane % 2 * kHalf) / kBlock) * p.groups + g0 + lane / 2);
+                    const int at = (int)(chunk & 1) * L::kChunk;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < L::kChunk; ++e) x_scales[(at + e) * 128 + (warp - 10) * 64 + i * 32 + lane] = v[i][e];
+                    if (warp == 10 && lane < 2 * L::kChunk) w_scales[at * 2 + lane] = w;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_full + 8 * (chunk & 1));
+                }
+            }
         } else if (warp == 9 && rank == 0) {
             const bool one = elect_one();
             uint32_t no = 0;
@@ -404,13 +434,12 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             for (int tile = pair; tile < p.tiles && ok; tile += pairs)
                 for (int g = 0; g < p.groups; ++g, ++no) {
                     const uint32_t stage = no % L::kStages, buf = no % L::kBuffers;
-                    if (!wait(t_empty + 8 * buf, (no / L::kBuffers & 1) ^ 1, ST_TIMEOUT_TMEM_EMPTY) || !wait(full + 8 * stage, no / L::kStages & 1, ST_TIMEOUT_FULL)) break;
+                    if (!wait(full + 8 * stage, no / L::kStages & 1, ST_TIMEOUT_FULL) || !wait(t_empty + 8 * buf, (no / L::kBuffers & 1) ^ 1, ST_TIMEOUT_TMEM_EMPTY)) break;
                     tc_fence_after();
                     if (one) {
                         const uint32_t x = umma_desc_lo(base + stage * L::kStage), w = umma_desc_lo(base + stage * L::kStage + kBox);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) umma_f8_pair(tmem + buf * L::kColumns, x + 2 * k, w + 2 * k, umma_idesc_f8(256, L::kColumns), k > 0);
-                        umma_commit_pair(empty + 8 * stage);
                         umma_commit_pair(t_full + 8 * buf);
                     }
                     __syncwarp();
