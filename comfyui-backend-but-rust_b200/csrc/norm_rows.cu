@@ -43,107 +43,233 @@ template <typename T> __device__ __forceinline__ void store8(void* base, int64_t
     }
 }
 
-// A thread has V pieces of eight columns, `warps` * 32 pieces apart; sixteen lanes have a group of 128 columns.
-template <typename T, int PRO, int V> __global__ void __launch_bounds__(1024) norm_rows_kernel(const NormParams p) {
-    __shared__ float part[32];
-    const int threads = p.warps * 32, in_row = threadIdx.x % threads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x * (blockDim.x / threads) + threadIdx.x / threads, pieces = p.K / 8;
-    const bool there = row < p.M;
-    pdl_wait();
-    float y[V][8];
+inline int device_sms() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return n;
+}
+
+// Eight values as they lie in memory
+template <typename T> struct Raw {
+    static constexpr int kWords = sizeof(T) / 2;      // of 16 bytes
+    uint4 w[kWords];
+    __device__ __forceinline__ void load(const void* base, int64_t at) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int piece = in_row + i * threads;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[i][e] = 0.f;
-        if (there && piece < pieces) load8<T>(reinterpret_cast<const T*>(p.x) + row * p.x_stride + piece * 8, y[i]);
+        for (int i = 0; i < kWords; ++i) w[i] = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(base) + at) + i);
     }
-    if (PRO == PRO_SWIGLU) {
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f<T>(e[i]);
+    }
+    // The sum in T. Of 16-bit values directly: their f32 sum is exact, or the smaller one below half a step of the larger, which is the result either way
+    __device__ __forceinline__ void add(const Raw& o) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            uint32_t *x = &w[i].x, y[4] = {o.w[i].x, o.w[i].y, o.w[i].z, o.w[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (std::is_same<T, float>::value) x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(y[e]));
+                else if (std::is_same<T, half>::value) asm("add.rn.f16x2 %0, %0, %1;" : "+r"(x[e]) : "r"(y[e]));
+                else asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(x[e]) : "r"(y[e]));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void* base, int64_t at) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(reinterpret_cast<T*>(base) + at)[i] = w[i];
+    }
+};
+
+// Eight columns of a row on their way out: to `at`, of out's type; sixteen lanes have a group of 128 columns and all call this. `scale`: where the first
+// of them writes the group's, null for the others.
+__device__ __forceinline__ void emit(int out_dt, const float (&y)[8], uint8_t* at, float* scale, bool mine) {
+    if (out_dt == DT_E4M3) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float s = f8_scale(top), inv = __frcp_rn(s);
+        if (mine) {
+            *reinterpret_cast<uint2*>(at) =
+                make_uint2(e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv), e4m3x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv));
+            if (scale) *scale = s;
+        }
+    } else if (mine) {
+        if (out_dt == DT_F32) store8<float>(at, 0, y);
+        else if (out_dt == DT_F16) store8<half>(at, 0, y);
+        else store8<bf16>(at, 0, y);
+    }
+}
+__device__ __forceinline__ int out_size(int out_dt) { return out_dt == DT_E4M3 ? 1 : out_dt == DT_F32 ? 4 : 2; }
+
+// x / (1 + e^-x): e^-x as 2^(-x log2 e), the power and the reciprocal from the special function unit, 2^-22 each. The exponent's rounding is 2^-24 of it,
+// 2^-17 of the power where x is near -88: with f32 values that is taken into account, 16-bit ones and their codes do not show it. Below -87.3, where the
+// value is under 2e-36, it is 0; infinities and NaN as the formula has them.
+template <typename T> __device__ __forceinline__ float silu_fast(float x) {
+    constexpr float kHigh = 1.4426950216293335f, kLow = 1.9259629911266175e-8f, kEnd = 87.3f;      // log2 e; the reciprocal of 1 + e^kEnd is a normal number
+    float e, r;
+    if (std::is_same<T, float>::value) {
+        const float t = fminf(fmaxf(-x, -kEnd), kEnd), h = __fmul_rn(t, kHigh), rest = __fmaf_rn(t, kLow, __fmaf_rn(t, kHigh, -h));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
+        e = __fmaf_rn(e, rest * 0.6931471805599453f, e);
+    } else asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, kEnd) * kHigh));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return x * (x < -kEnd ? 0.f : r);
+}
+
+// Rows without a norm: sixteen lanes take a group of 128 columns, of every `step`-th row, whose values are on their way a row ahead; a CTA has
+// `wide` neighbouring groups of as many rows as fit. 4096 x 9728 bf16, SWIGLU: 107 us with expf and a division, 57 with rows and groups counted by one
+// number (41 instructions a value, the issue slots' limit).
+template <typename T, int PRO> __global__ void __launch_bounds__(256) group_rows_kernel(const NormParams p, const int wide, const int step) {
+    const int slot = threadIdx.x / 16, group = blockIdx.x * wide + slot % wide, piece = group * 16 + (threadIdx.x & 15), rows = blockDim.x / (16 * wide);
+    const bool in_row = piece < p.K / 8;
+    int row = slot < rows * wide ? blockIdx.y * rows + slot / wide : p.M;      // (whole warps: half of one may have nothing to do)
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)row * p.x_stride + piece * 8;
+    const int64_t next = (int64_t)step * p.x_stride, out_next = (int64_t)step * p.out_stride * out_size(p.out_dt);
+    const int groups = (p.K + 127) / 128;
+    uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + ((int64_t)row * p.out_stride + piece * 8) * out_size(p.out_dt);
+    float* scale = (threadIdx.x & 15) == 0 && p.scales ? p.scales + (int64_t)row * groups + group : nullptr;
+    pdl_wait();
+    Raw<T> a, b;
+    a.clear(), b.clear();
+    auto request = [&] {
+        if (in_row && row < p.M) {
+            a.load(x, 0);
+            if (PRO == PRO_SWIGLU) b.load(x, p.up_offset);
+        }
+    };
+    request();
+    while (__any_sync(0xffffffffu, row < p.M)) {
+        const bool mine = in_row && row < p.M;
+        float y[8];
+        a.values(y);
+        if (PRO == PRO_SWIGLU) {
+            float up[8];
+            b.values(up);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = silu_fast<T>(y[e]) * up[e];
+        }
+        row += step, x += next;
+        request();
+        if (!__any_sync(0xffffffffu, row < p.M)) pdl_trigger();
+        emit(p.out_dt, y, out, scale, mine);
+        out += out_next;
+        if (scale) scale += (int64_t)step * groups;
+    }
+}
+
+template <typename T, int V> constexpr bool ahead() { return sizeof(T) == 2 && V <= 2; }
+// RMS: a thread has V pieces of eight columns, `warps` * 32 pieces apart. A CTA takes rows in turn: weights stay in registers (read anew for every
+// row they are as many bytes as 16-bit rows and their stream), the next row's values are on their way while this one's sum goes round. With more than
+// two pieces a thread has no room for either.
+template <typename T, int V> __global__ void __launch_bounds__(V <= 2 ? 512 : 1024, V > 2 ? 1 : ahead<T, V>() ? 2 : 3) rms_rows_kernel(const NormParams p) {
+    constexpr bool kAhead = ahead<T, V>();
+    __shared__ __align__(16) float part[2][32];
+    const int threads = p.warps * 32, in_row = threadIdx.x % threads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = blockDim.x / threads, pieces = p.K / 8, step = gridDim.x * rows, groups = (p.K + 127) / 128;
+    if (threadIdx.x < 64) part[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+    if (p.warps > 1) __syncthreads();
+    const float by_k = 1.f / (float)p.K;
+    pdl_wait();
+    float w[kAhead ? V : 1][8];
+    auto weights = [&](float (&v)[8], int piece) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 1.f;
+        if (p.norm_w && piece < pieces) load8<float>(p.norm_w + piece * 8, v);
+    };
+    if (kAhead)
+#pragma unroll
+        for (int i = 0; i < V; ++i) weights(w[i], in_row + i * threads);
+    Raw<T> a[V], b[V];
+    auto request = [&](int row) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int piece = in_row + i * threads;
-            float up[8] = {};
-            if (there && piece < pieces) load8<T>(reinterpret_cast<const T*>(p.x) + row * p.x_stride + p.up_offset + piece * 8, up);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[i][e] = silu_f(y[i][e]) * up[e];
+            if (row < p.M && piece < pieces) {
+                a[i].load(p.x, row * p.x_stride + piece * 8);
+                if (p.resid) b[i].load(p.resid, row * p.resid_stride + piece * 8);
+            } else a[i].clear(), b[i].clear();
         }
-    }
-    if (PRO == PRO_RMS) {
-        if (p.resid) {
+    };
+    int row = blockIdx.x * rows + threadIdx.x / threads, turn = 0;
+    if (kAhead) request(row);
+    for (int first = blockIdx.x * rows; first < p.M; first += step, row += step, turn ^= 1) {
+        const bool there = row < p.M;
+        if (!kAhead) request(row);
+        float y[V][8], sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int piece = in_row + i * threads;
-                float s[8];
-                if (there && piece < pieces) {
-                    load8<T>(reinterpret_cast<const T*>(p.resid) + row * p.resid_stride + piece * 8, s);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[i][e] = rnd<T>(y[i][e] + s[e]);
-                    store8<T>(p.resid_out, row * p.resid_out_stride + piece * 8, y[i]);
-                }
+        for (int i = 0; i < V; ++i) {
+            const int piece = in_row + i * threads;
+            if (p.resid) {
+                a[i].add(b[i]);
+                if (there && piece < pieces) a[i].store(p.resid_out, row * p.resid_out_stride + piece * 8);
             }
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
+            a[i].values(y[i]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = __fmaf_rn(y[i][e], y[i][e], sum);
+        }
+        if (kAhead) request(row + step);      // (rows of this CTA alone: what another one writes is not read here)
         sum = warp_sum(sum);
         if (p.warps > 1) {
-            if (lane == 0) part[warp] = sum;
+            if (lane == 0) part[turn][warp] = sum;
             __syncthreads();
-            const int first = warp / p.warps * p.warps;
+            // (a row of its own CTA has all parts, zeros behind the last; several rows to a CTA have at most four warps each)
             sum = 0.f;
-            for (int w = 0; w < p.warps; ++w) sum += part[first + w];
+            if (rows == 1) {
+                const float4* all = reinterpret_cast<const float4*>(part[turn]);
+                for (int i = 0; i * 4 < p.warps; ++i) {
+                    const float4 v = all[i];
+                    sum += (v.x + v.y) + (v.z + v.w);
+                }
+            } else {
+                const int w0 = warp / p.warps * p.warps;
+                for (int i = 0; i < p.warps; ++i) sum += part[turn][w0 + i];
+            }
         }
-        const float r = rsqrtf(sum / (float)p.K + p.eps);
+        if (first + step >= p.M) pdl_trigger();
+        const float r = rsqrtf(__fmaf_rn(sum, by_k, p.eps));
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int piece = in_row + i * threads;
-            float w[8];
+            float v[8];
+            if (!kAhead) weights(v, piece);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = 1.f;
-            if (p.norm_w && piece < pieces) load8<float>(p.norm_w + piece * 8, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[i][e] = y[i][e] * r * w[e];
-        }
-    }
-    pdl_trigger();
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int piece = in_row + i * threads;
-        const bool mine = there && piece < pieces;
-        const int64_t at = row * p.out_stride + piece * 8;
-        if (p.out_dt == DT_E4M3) {
-            float top = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[i][e]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float s = f8_scale(top), inv = __frcp_rn(s);
-            if (mine) {
-                *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.out) + at) =
-                    make_uint2(e4m3x4(y[i][0] * inv, y[i][1] * inv, y[i][2] * inv, y[i][3] * inv), e4m3x4(y[i][4] * inv, y[i][5] * inv, y[i][6] * inv, y[i][7] * inv));
-                if ((piece & 15) == 0) p.scales[(int64_t)row * ((p.K + 127) / 128) + piece / 16] = s;
-            }
-        } else if (mine) {
-            if (p.out_dt == DT_F32) store8<float>(p.out, at, y[i]);
-            else if (p.out_dt == DT_F16) store8<half>(p.out, at, y[i]);
-            else store8<bf16>(p.out, at, y[i]);
+            for (int e = 0; e < 8; ++e) y[i][e] = y[i][e] * r * (kAhead ? w[kAhead ? i : 0][e] : v[e]);
+            emit(p.out_dt, y[i], reinterpret_cast<uint8_t*>(p.out) + (row * p.out_stride + piece * 8) * out_size(p.out_dt),
+                 (piece & 15) == 0 ? p.scales + (int64_t)row * groups + piece / 16 : nullptr, there && piece < pieces);
         }
     }
 }
 
-template <typename T, int PRO, int V> int launch_norm(NormParams& p, cudaStream_t st) {
-    const int pieces = p.K / 8;
-    p.warps = (pieces + 32 * V - 1) / (32 * V);
-    const int rows = p.warps >= 8 ? 1 : 8 / p.warps;      // to a CTA
-    return launch_pdl(norm_rows_kernel<T, PRO, V>, dim3((p.M + rows - 1) / rows), rows * p.warps * 32, 0, st, p);
+constexpr int kThreadsAhead = 1024;      // to an SM
+template <typename T, int PRO> int launch_groups(NormParams& p, cudaStream_t st) {
+    const int groups = (p.K + 127) / 128, columns = (groups + 15) / 16, wide = (groups + columns - 1) / columns;
+    const int rows = 16 / wide, sms = device_sms();      // rows to a CTA
+    if (sms <= 0) return (int)cudaErrorInvalidDevice;
+    const int threads = (rows * wide * 16 + 31) / 32 * 32;
+    const int64_t all = ((int64_t)p.M + rows - 1) / rows, some = (int64_t)sms * (2048 / threads) / columns, most = some < 1 ? 1 : some;
+    const int down = (int)(all < most ? all : most);
+    return launch_pdl(group_rows_kernel<T, PRO>, dim3(columns, down), threads, 0, st, p, wide, down * rows);
 }
-template <typename T, int PRO> int launch_norm(NormParams& p, cudaStream_t st) {
-    return p.K <= 4096 ? launch_norm<T, PRO, 1>(p, st) : p.K <= 16384 ? launch_norm<T, PRO, 2>(p, st) : launch_norm<T, PRO, 4>(p, st);
+template <typename T, int V> int launch_rms(NormParams& p, cudaStream_t st) {
+    const int pieces = p.K / 8, sms = device_sms();
+    if (sms <= 0) return (int)cudaErrorInvalidDevice;
+    p.warps = (pieces + 32 * V - 1) / (32 * V);
+    const int rows = p.warps >= 8 ? 1 : 8 / p.warps, ctas = (p.M + rows - 1) / rows;      // rows to a CTA
+    const int most = ahead<T, V>() ? sms * (kThreadsAhead / (rows * p.warps * 32)) : ctas;
+    return launch_pdl(rms_rows_kernel<T, V>, dim3(ctas < most ? ctas : most), rows * p.warps * 32, 0, st, p);
 }
 template <typename T> int launch_norm(int prologue, NormParams& p, cudaStream_t st) {
-    return prologue == PRO_PLAIN ? launch_norm<T, PRO_PLAIN>(p, st) : prologue == PRO_RMS ? launch_norm<T, PRO_RMS>(p, st) : launch_norm<T, PRO_SWIGLU>(p, st);
+    if (prologue == PRO_PLAIN) return launch_groups<T, PRO_PLAIN>(p, st);
+    if (prologue == PRO_SWIGLU) return launch_groups<T, PRO_SWIGLU>(p, st);
+    if (p.K <= (sizeof(T) == 4 ? 4096 : 1536)) return launch_rms<T, 1>(p, st);
+    return p.K <= 8192 ? launch_rms<T, 2>(p, st) : launch_rms<T, 4>(p, st);
 }
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------------
@@ -203,7 +329,7 @@ GPU_API int gpu_norm_rows(int dtype, int prologue, const void* x, int64_t x_stri
                           void* stream) {
     if (dtype < DT_F32 || dtype > DT_BF16 || out_dt < DT_F32 || out_dt > DT_E4M3) return -4;
     const bool f8 = out_dt == DT_E4M3;
-    if (M < 0 || K <= 0 || K % (f8 ? 16 : 8) != 0) return -1;
+    if (M < 0 || M > INT32_MAX - (1 << 20) || K <= 0 || K % (f8 ? 16 : 8) != 0) return -1;
     if (K > 32768) return -2;
     if ((prologue != PRO_PLAIN && prologue != PRO_RMS && prologue != PRO_SWIGLU) || (prologue != PRO_RMS && (resid || norm_w))) return -3;
     if (M == 0) return 0;
