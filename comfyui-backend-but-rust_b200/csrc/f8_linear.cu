@@ -145,6 +145,7 @@ template <int NT> __global__ void __launch_bounds__(Few<NT>::kThreads) f8_few_ke
             }
             __syncwarp();
         }
+        pdl_trigger();      // the last blocks are on their way: the next kernel's CTAs find room beside this one's and can set up
     } else {
         const bool one = elect_one();
         for (int g = 0; g < blocks; ++g) {
@@ -218,6 +219,16 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
         "mov.b64 db, {%2, %5};\n\t"
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
         ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128) : "memory");
+}
+
+// The mbarrier at this offset in both CTAs of the pair gets an arrival once the products that this thread issued are done; `mask`: the pair's ranks
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint16_t mask) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask) : "memory");
+}
+__device__ __forceinline__ float4 dsmem_f32x4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_shared(addr, rank)) : "memory");
+    return v;
 }
 
 // A warp's 32 rows of sums out, by way of its staging, so that a row's pieces are stored together
@@ -301,8 +312,8 @@ __device__ __forceinline__ void rows_out(const F8Params& p, const float (&sum)[T
     }
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile::kThreads, 1)
-f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Params p) {
+// Few tiles: a cluster of `splits` pairs on each, which share its K and add up in shared memory, in a fixed order.
+template <bool SPLIT> __global__ void __launch_bounds__(Tile::kThreads, 1) f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Params p) {
     using L = Tile;
     constexpr int kHalf = L::kHalf;
     extern __shared__ uint8_t smem_raw[];
@@ -315,7 +326,7 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     float *x_scales = reinterpret_cast<float*>(sm + L::kXScales), *w_scales = reinterpret_cast<float*>(sm + L::kWScales);      // [chunk % 2][block][row], [block][side]
     uint32_t* tmem_s = reinterpret_cast<uint32_t*>(sm + L::kTail + 240);
     volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
-    const uint32_t rank = cluster_ctarank();
+    const uint32_t in_cluster = cluster_ctarank(), rank = SPLIT ? in_cluster & 1 : in_cluster, leader = SPLIT ? in_cluster & ~1u : 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < L::kBuffers; ++i) mbar_init(t_full + 8 * i, 1), mbar_init(t_empty + 8 * i, 16);
@@ -335,7 +346,8 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     tc_fence_after();
     const uint32_t tmem = *tmem_s;
     pdl_wait();
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int pair = blockIdx.x / (SPLIT ? 2 * p.splits : 2), pairs = gridDim.x / (SPLIT ? 2 * p.splits : 2);      // (clusters; one tile each if they have several pairs)
+    const int g_first = SPLIT ? (int)(in_cluster >> 1) * p.per : 0, g_last = SPLIT ? min(g_first + p.per, p.groups) : p.groups;
     if (warp < 8) {
         more_registers<L::kSumRegs>();
         const int side = warp >> 2, quarter = warp & 3;
@@ -346,11 +358,11 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
             const int m0 = tile % p.m_tiles * 256 + (int)rank * 128 + quarter * 32, n0 = tile / p.m_tiles * L::kColumns + side * kHalf;
             float sum[kHalf] = {};
-            for (int g = 0; g < p.groups; ++g, ++no) {
-                const int part = g % L::kChunk, at = (int)(chunk & 1) * L::kChunk + part;
+            for (int g = g_first; g < g_last; ++g, ++no) {
+                const int part = (g - g_first) % L::kChunk, at = (int)(chunk & 1) * L::kChunk + part;
                 if (part == 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (chunk & 1), chunk >> 1 & 1, abort_s, ST_TIMEOUT_UNPACK)))) break;
                 const float scale = x_scales[at * 128 + quarter * 32 + lane] * w_scales[at * 2 + side];
-                if (part == L::kChunk - 1 || g == p.groups - 1) {
+                if (part == L::kChunk - 1 || g == g_last - 1) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s_empty + 8 * (chunk & 1));
                     ++chunk;
@@ -368,7 +380,7 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
                     if (c + 64 == kHalf) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_remote(mapa_shared(t_empty + 8 * buf, 0));
+                        if (lane == 0) mbar_arrive_remote(mapa_shared(t_empty + 8 * buf, leader));
                     }
 #pragma unroll
                     for (int e = 0; e < 64; e += 2) {      // two sums an instruction (single ones: 288 us instead of 282, 4352 x 5120 -> 13824)
@@ -378,7 +390,13 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
                 }
             }
             if (!ok) break;
-            rows_out(p, sum, stage, m0, n0, lane);
+            if (!SPLIT) rows_out(p, sum, stage, m0, n0, lane);
+            else {      // [row][256 columns] in pieces of four, over the stages: every product of the pair is done
+                const int row = quarter * 32 + lane;
+#pragma unroll
+                for (int e = 0; e < kHalf / 4; ++e)
+                    *reinterpret_cast<float4*>(sm + row * 1024 + ((side * (kHalf / 4) + e) ^ (row & 7)) * 16) = make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]);
+            }
         }
     } else {
         fewer_registers<L::kRestRegs>();
@@ -387,11 +405,11 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             bool ok = true;
             for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
                 const int row_x = tile % p.m_tiles * 256 + (int)rank * 128, row_w = tile / p.m_tiles * L::kColumns + (int)rank * 128;
-                for (int g = 0; g < p.groups; ++g, ++no) {
+                for (int g = g_first; g < g_last; ++g, ++no) {
                     const uint32_t stage = no % L::kStages;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * stage, (no / L::kStages & 1) ^ 1, abort_s, ST_TIMEOUT_EMPTY)))) break;
                     if (lane == 0) {
-                        const uint32_t at = base + stage * L::kStage, bar = mapa_shared(full + 8 * stage, 0);
+                        const uint32_t at = base + stage * L::kStage, bar = mapa_shared(full + 8 * stage, leader);
                         if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, 2 * L::kStage);
                         tma_load_2d_pair(at, &tmap_x, g * kBlock, row_x, bar);
                         tma_load_2d_pair(at + kBox, &tmap_w, g * kBlock, row_w, bar);
@@ -406,7 +424,7 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             bool ok = true;
             for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
                 const int m0 = tile % p.m_tiles * 256 + (int)rank * 128 + (warp - 10) * 64, n0 = tile / p.m_tiles * L::kColumns;
-                for (int g0 = 0; g0 < p.groups; g0 += L::kChunk, ++chunk) {
+                for (int g0 = g_first; g0 < g_last; g0 += L::kChunk, ++chunk) {
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait(s_empty + 8 * (chunk & 1), (chunk >> 1 & 1) ^ 1, abort_s, ST_TIMEOUT_EMPTY)))) break;
                     float v[2][L::kChunk], w = 0.f;
 #pragma unroll
@@ -432,7 +450,7 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             bool ok = true;
             auto wait = [&](uint32_t bar, uint32_t parity, int code) { return ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_s, code)); };
             for (int tile = pair; tile < p.tiles && ok; tile += pairs)
-                for (int g = 0; g < p.groups; ++g, ++no) {
+                for (int g = g_first; g < g_last; ++g, ++no) {
                     const uint32_t stage = no % L::kStages, buf = no % L::kBuffers;
                     if (!wait(full + 8 * stage, no / L::kStages & 1, ST_TIMEOUT_FULL) || !wait(t_empty + 8 * buf, (no / L::kBuffers & 1) ^ 1, ST_TIMEOUT_TMEM_EMPTY)) break;
                     tc_fence_after();
@@ -440,11 +458,45 @@ f8_tile_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
                         const uint32_t x = umma_desc_lo(base + stage * L::kStage), w = umma_desc_lo(base + stage * L::kStage + kBox);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) umma_f8_pair(tmem + buf * L::kColumns, x + 2 * k, w + 2 * k, umma_idesc_f8(256, L::kColumns), k > 0);
-                        umma_commit_pair(t_full + 8 * buf);
+                        commit_pair(t_full + 8 * buf, (uint16_t)(3u << leader));
                     }
                     __syncwarp();
                 }
         }
+    }
+    if (SPLIT) {
+        __syncwarp();
+        cluster_sync_all();
+        // the CTAs of a tile's 128 rows take turns over them, each adding up all of a row
+        const int m0 = pair % p.m_tiles * 256 + (int)rank * 128, n0 = pair / p.m_tiles * L::kColumns, left = min(128, p.M - m0);
+        const int esize = p.out_dt == DT_F32 ? 4 : 2;
+        const bool whole = p.out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * esize - 1)) == 0;
+        if (warp < 8 && pair < p.tiles)
+            for (int i = threadIdx.x + (int)(in_cluster >> 1) * 256; i < left * 64; i += 256 * p.splits) {
+                const int row = i >> 6, piece = i & 63, col = n0 + piece * 4;
+                if (col >= p.N) continue;
+                float y[4] = {};
+                for (int s = 0; s < p.splits; ++s) {
+                    const float4 v = dsmem_f32x4(base + row * 1024 + (piece ^ (row & 7)) * 16, 2 * s + rank);
+                    y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
+                }
+                const int64_t at = (int64_t)(m0 + row) * p.out_stride + col;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (col + e >= p.N) continue;
+                    if (p.bias) y[e] += value_at(p.bias, p.out_dt, col + e);
+                    if (p.add) y[e] += value_at(p.out, p.out_dt, at + e);
+                }
+                if (whole && col + 4 <= p.N) {
+                    if (esize == 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+                    else
+                        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = p.out_dt == DT_F16 ? make_uint2(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]))
+                                                                                                                : make_uint2(pack2<bf16>(y[0], y[1]), pack2<bf16>(y[2], y[3]));
+                } else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (col + e < p.N) put_value(p.out, p.out_dt, at + e, y[e]);
+            }
     }
     __syncwarp();
     tc_fence_before();
@@ -492,9 +544,15 @@ int launch_tile(const void* x, int64_t x_stride, const void* W, F8Params& p, int
     const int64_t tiles = (int64_t)p.m_tiles * ((p.N + L::kColumns - 1) / L::kColumns);
     if (tiles > INT32_MAX / 2) return -1;      // and so does a tile a round further on
     p.tiles = (int)tiles;
-    if (cudaError_t e = cudaFuncSetAttribute(f8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
-    const int pairs = p.tiles < sms / 2 ? p.tiles : sms / 2;
-    return launch_pdl(f8_tile_kernel, dim3((unsigned)(2 * pairs)), L::kThreads, L::kSmem, st, tx, tw, p);
+    // pairs to a tile: as many as the device has for it, four at most, with four blocks each
+    p.splits = 1;
+    while (p.splits < 4 && p.tiles * (p.splits + 1) <= sms / 2 && p.groups >= (p.splits + 1) * 4) ++p.splits;
+    p.per = (p.groups + p.splits - 1) / p.splits;
+    p.splits = (p.groups + p.per - 1) / p.per;
+    const int pairs = p.splits > 1 ? p.tiles * p.splits : p.tiles < sms / 2 ? p.tiles : sms / 2;
+    auto kern = p.splits > 1 ? f8_tile_kernel<true> : f8_tile_kernel<false>;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem)) return (int)e;
+    return launch_pdl_cluster(kern, dim3((unsigned)(2 * pairs)), L::kThreads, L::kSmem, st, 2 * p.splits, tx, tw, p);
 }
 
 }  // namespace
