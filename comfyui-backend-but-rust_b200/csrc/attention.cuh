@@ -38,20 +38,28 @@ struct PackedTile {
     int len, token0, tokens;   // its tokens, and those of the tile; none: a tile that nobody needs
 };
 __device__ __forceinline__ int offset_at(const AttnParams& p, int b) { return min(max(gload(p.offsets + b), 0), p.rows); }
-// A whole warp finds the tile, 32 sequences at a look
+// A whole warp finds the tile, 32 sequences at a look; up to 31 with one load for all that it has to know
 __device__ __forceinline__ PackedTile packed_tile(const AttnParams& p, int tile) {
     const int lane = threadIdx.x & 31;
-    int lo = 0, hi = p.B;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, b = lo + (lane + 1) * step;
-        const bool before = b < hi && offset_at(p, b) / p.tile_tokens + b <= tile;
-        lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
-        hi = min(hi, lo + step);
+    int lo = 0, start, end;
+    if (p.B < 32) {
+        const int mine = offset_at(p, min(lane, p.B));
+        lo = max(0, __popc(__ballot_sync(0xffffffffu, lane < p.B && mine / p.tile_tokens + lane <= tile)) - 1);
+        start = __shfl_sync(0xffffffffu, mine, lo), end = __shfl_sync(0xffffffffu, mine, lo + 1);
+    } else {
+        int hi = p.B;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32, b = lo + (lane + 1) * step;
+            const bool before = b < hi && offset_at(p, b) / p.tile_tokens + b <= tile;
+            lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+            hi = min(hi, lo + step);
+        }
+        start = offset_at(p, lo), end = offset_at(p, lo + 1);
     }
     PackedTile x;
-    const int start = offset_at(p, lo), ahead = tile - (start / p.tile_tokens + lo);
+    const int ahead = tile - (start / p.tile_tokens + lo);
     x.start = start;
-    x.len = ahead < 0 ? 0 : max(0, offset_at(p, lo + 1) - start);
+    x.len = ahead < 0 ? 0 : max(0, end - start);
     x.token0 = ahead < 0 || ahead > x.len / p.tile_tokens ? x.len : ahead * p.tile_tokens;
     x.tokens = min(p.tile_tokens, x.len - x.token0);
     return x;

@@ -91,7 +91,9 @@ template <int V> __device__ __forceinline__ void turned(const RotaryParams& p, f
 }
 
 // A group of `lanes` threads has a head, a thread of it one slot of 2 V values (several with V = 1); the next head's values are on their way. Measured
-// (us, floor at the copy's rate): 2 x 4179 tokens, 24 / 24 heads of 128, fp16, 50.3 (31.3) with 64-bit divisions for every head and nothing ahead.
+// (us, floor at the copy's rate): 2 x 4179 tokens, 24 / 24 heads of 128, fp16, 40.8 (31.3; 50.3 with
+// 64-bit divisions for every head and nothing ahead; 47.5 with a token's angles in registers, which leave room for fewer threads); 4096 tokens, 32 / 8 heads
+// of 128, bf16, 19.5 (12.8), heads normalised 25.3.
 template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, const int lanes) {
     extern __shared__ float2 turn[];      // [token][half]: cos, sin
     __shared__ int64_t row[4][kMaxTokens];      // of q, k and the results, where a token's row begins

@@ -416,6 +416,48 @@ def test_offsets_outside_the_rows(pkg, dev):
         assert torch.equal(got[:100], want[:100]) and bool((got[100:] == 0).all())
 
 
+@pytest.mark.parametrize("B", [1, 5, 40])
+def test_more_items_than_a_launch_lists(pkg, dev, B):
+    """Many heads of one row tile each: 512 groups fill a launch's lists with 37 tiles of 256 tokens; the next ones go to a second launch and a third."""
+    g = torch.Generator().manual_seed(B)
+    H, D = 512, 8
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    rows = 256 * (2 * (128 * sms // H) + 3) + 100
+    o = [0, *sorted(int(c) for c in torch.randint(0, rows + 1, (B - 1,), generator=g)), rows]
+    q, k, v = (torch.randn(rows, H, D, device=dev, dtype=torch.float16) for _ in range(3))
+    offsets = torch.tensor(o, dtype=torch.int32, device=dev)
+    got = pkg.attention.packed_attention(q, k, v, offsets)
+    for s, e in zip(o[:-1], o[1:]):              # a few heads and rows of every sequence, its ends among them
+        at = sorted({s, min(s + 300, e - 1), (s + e) // 2, e - 1}) if e > s else []
+        for h in (0, 255, 511):
+            for i in at:
+                seen = torch.ones(1, i + 1 - s, dtype=torch.bool, device=dev)
+                want, a, rest = _reference(q[i:i + 1, h].double(), k[s:i + 1, h].double(), v[s:i + 1, h].double(), seen, D ** -0.5)
+                _check_attention(got[i:i + 1, h], want, a, rest, _half(q.dtype))
+    again = q.clone()                            # onto the queries, launch after launch
+    pkg.attention.packed_attention(again, k, v, offsets, out=again)
+    assert torch.equal(again, got) and pkg.linear.kernel_status() == 0
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("H,Hkv,D", [(1, 1, 64), (8, 2, 128), (3, 1, 96)])
+def test_every_length_around_a_tiles_end(pkg, dev, H, Hkv, D, causal):
+    """One sequence of each length at which a tile of 128 or 256 rows, or of 128 keys, begins or ends, beside a long one that keeps the tiles full."""
+    g = torch.Generator().manual_seed(H)
+    ratio = H // Hkv
+    ends = sorted({n for t in (128 // ratio, 256 // ratio, 128, 256, 384) for n in (t - 1, t, t + 1)})
+    q, k, v = _packed(g, dev, torch.bfloat16, 1700, H, Hkv, D)
+    want = {}
+    for n in ends:
+        o, offsets = _offsets([n, 1700 - n], dev)
+        got = pkg.attention.packed_attention(q, k, v, offsets, causal=causal)
+        _check_packed(got[:n], q[:n], k[:n], v[:n], [0, n], causal)
+        want[n] = got[:n].clone()
+        o, offsets = _offsets([700, n], dev)     # the same rows elsewhere, and in another order of work
+        moved = [torch.cat((t[-700:], t[:n])) for t in (q, k, v)]
+        assert torch.equal(pkg.attention.packed_attention(*moved, offsets, causal=causal)[700:], want[n])
+
+
 def test_packed_attention_agrees_with_the_other_attentions(pkg, dev):
     """One sequence without a mask is cross attention to itself; over an int8 cache the same prompt is near."""
     g = torch.Generator().manual_seed(3)
@@ -578,6 +620,62 @@ def test_arguments_that_python_refuses(pkg, dev):
                  lambda: A.rotary(h(1, 2, 3, 264), None, i(1, 2), f(32).double())):
         with pytest.raises(pkg.ffi.GpuKernelError):
             call()
+
+
+def test_on_another_stream_than_the_tensors_own(pkg, dev):
+    """Calls go to the current stream, whichever made the tensors."""
+    L, A, F = pkg.linear, pkg.attention, pkg.ffi
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(200, 256, generator=g).bfloat16().to(dev)
+    w, ws = L.f8_requant((torch.randn(512, 256, generator=g) * 0.1).to(dev))
+    freq, _ = A.rope_frequencies(64, device=dev)
+    pos = torch.arange(200, dtype=torch.int32, device=dev)[None]
+    _, offsets = _offsets([150, 50], dev)
+
+    def run():
+        y = L.f8_linear(*L.norm_rows(x, F.PRO_RMS, eps=1e-6, out_dtype=F8), w, ws)
+        q, k = A.rotary(y[:, :256].view(1, 200, 4, 64), y[:, 256:384].view(1, 200, 2, 64), pos, freq)
+        return A.packed_attention(q[0], k[0], y[:, 384:].view(200, 2, 64), offsets)
+    want = run()
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_offsets_of_rows_beyond_32_bits(pkg, dev):
+    """Rows whose elements lie further than 2^31 from the first: 600 000 rows of 32 heads of 128."""
+    g = torch.Generator().manual_seed(12)
+    rows, H, D = 600000, 32, 128
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    q = torch.zeros(rows, H, D, dtype=torch.bfloat16, device=dev)
+    tail = (torch.randn(300, H, D, generator=g) * 2).bfloat16().to(dev)
+    q[-300:] = tail
+    kv = torch.zeros(rows, 1, D, dtype=torch.bfloat16, device=dev)
+    kv[-300:] = torch.randn(300, 1, D, generator=g).bfloat16().to(dev)
+    small = [0, 250, 300]
+    offsets = torch.tensor([rows - 300 + n for n in small], dtype=torch.int32, device=dev)      # the rows before belong to no sequence
+    pos = torch.arange(rows, dtype=torch.int32, device=dev)[None]
+    freq, _ = pkg.attention.rope_frequencies(D, device=dev)
+    turned, _ = pkg.attention.rotary(q[None], None, pos, freq)
+    want, _ = pkg.attention.rotary(tail[None], None, pos[:, -300:].contiguous(), freq)
+    assert torch.equal(turned[0, -300:], want[0])
+    out = pkg.attention.packed_attention(turned[0], kv, kv, offsets, out=turned[0])
+    ref = pkg.attention.packed_attention(want[0], kv[-300:].contiguous(), kv[-300:].contiguous(), torch.tensor(small, dtype=torch.int32, device=dev))
+    assert torch.equal(out[-300:], ref) and bool((out[:-300] == 0).all())
+    del turned, out
+    y = pkg.linear.norm_rows(q.view(rows, H * D), pkg.ffi.PRO_RMS, eps=1e-6)
+    z = pkg.linear.norm_rows(tail.view(300, H * D), pkg.ffi.PRO_RMS, eps=1e-6)
+    assert torch.equal(y[-300:], z) and bool((y[:-300] == 0).all())
+    del y
+    codes, s = pkg.linear.norm_rows(q.view(rows, H * D), pkg.ffi.PRO_PLAIN, out_dtype=F8)
+    w, ws = pkg.linear.f8_requant((torch.randn(256, H * D, generator=g) * 0.05).to(dev))
+    got = pkg.linear.f8_linear(codes, s, w, ws)
+    _check_linear(got[-300:], _values(codes[-300:], s[-300:], 1), _values(w, ws, 128), None, None, H * D)      # (fewer rows add up in another order)
+    assert bool((got[:-300] == 0).all())
 
 
 def test_nothing_to_do(pkg, dev):
