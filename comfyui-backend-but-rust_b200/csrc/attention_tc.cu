@@ -945,9 +945,10 @@ int b200q::attention_tc_packed(int dtype, AttnParams& a, cudaStream_t st) {
     const int tokens = 128 / a.pack, groups = a.H / a.pack;      // of a tile of 128 rows
     a.tile_tokens = 2 * tokens;
     const int64_t tiles = (int64_t)a.rows / a.tile_tokens + a.B;
+    if (tiles > INT32_MAX / 2 / groups) return -1;
     const int sms = sm_count();
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
-    if (tiles > INT32_MAX / 2 / groups) return -1;
+    if (groups > (int64_t)kListed * sms) return -1;
     TcParams p = {};
     p.a = a, p.q_tiles = (int)tiles, p.kv_head = a.ks[2] != 0;
     CUtensorMap tm[3] = {};
@@ -962,8 +963,7 @@ int b200q::attention_tc_packed(int dtype, AttnParams& a, cudaStream_t st) {
         !make_rows_map(&tm[1], a.k, a.ks, 1, a.rows, a.Hkv, a.D) || !make_rows_map(&tm[2], a.v, a.vs, 1, a.rows, a.Hkv, a.D))
         return -203;
     // as many launches as the lists take (one up to some 150 000 rows of 32 / 8 heads)
-    const int64_t most = (int64_t)kListed * sms / groups > 0 ? (int64_t)kListed * sms / groups : 1;
-    if (groups > (int64_t)kListed * sms) return -1;
+    const int64_t most = (int64_t)kListed * sms / groups;
     for (int64_t first = 0; first < tiles; first += most) {
         p.first_slot = (uint32_t)first, p.items = (uint32_t)((tiles - first < most ? tiles - first : most) * groups);
         const int rc = dtype == DT_F16 ? (a.D > 64 ? launch_tc<half, 128, PACKED>(tm, p, st) : launch_tc<half, 64, PACKED>(tm, p, st))

@@ -53,10 +53,6 @@ inline int device_sms() {
 template <typename T> struct Raw {
     static constexpr int kWords = sizeof(T) / 2;      // of 16 bytes
     uint4 w[kWords];
-    __device__ __forceinline__ void load(const void* base, int64_t at) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(base) + at) + i);
-    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
@@ -138,10 +134,14 @@ template <typename T, int PRO> __global__ void __launch_bounds__(256) group_rows
     pdl_wait();
     Raw<T> a, b;
     a.clear(), b.clear();
+    auto take = [](Raw<T>& r, const T* from) {
+#pragma unroll
+        for (int i = 0; i < Raw<T>::kWords; ++i) r.w[i] = gload(reinterpret_cast<const uint4*>(from) + i);
+    };
     auto request = [&] {
         if (in_row && row < p.M) {
-            a.load(x, 0);
-            if (PRO == PRO_SWIGLU) b.load(x, p.up_offset);
+            take(a, x);
+            if (PRO == PRO_SWIGLU) take(b, x + p.up_offset);
         }
     };
     request();
@@ -187,13 +187,17 @@ template <typename T, int V> __global__ void __launch_bounds__(V <= 2 ? 512 : 10
 #pragma unroll
         for (int i = 0; i < V; ++i) weights(w[i], in_row + i * threads);
     Raw<T> a[V], b[V];
+    auto take = [](Raw<T>& r, const T* from) {
+#pragma unroll
+        for (int i = 0; i < Raw<T>::kWords; ++i) r.w[i] = gload(reinterpret_cast<const uint4*>(from) + i);
+    };
     auto request = [&](int row) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int piece = in_row + i * threads;
             if (row < p.M && piece < pieces) {
-                a[i].load(p.x, row * p.x_stride + piece * 8);
-                if (p.resid) b[i].load(p.resid, row * p.resid_stride + piece * 8);
+                take(a[i], reinterpret_cast<const T*>(p.x) + row * p.x_stride + piece * 8);
+                if (p.resid) take(b[i], reinterpret_cast<const T*>(p.resid) + row * p.resid_stride + piece * 8);
             } else a[i].clear(), b[i].clear();
         }
     };
