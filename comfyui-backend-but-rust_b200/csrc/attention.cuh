@@ -69,6 +69,11 @@ template <typename T> __device__ __forceinline__ bool any_infinite(uint4 w) {
     const uint32_t top = std::is_same<T, half>::value ? 0x7C007C00u : 0x7F807F80u;
     return (__vcmpeq2(w.x & top, top) | __vcmpeq2(w.y & top, top) | __vcmpeq2(w.z & top, top) | __vcmpeq2(w.w & top, top)) != 0;
 }
+// sum += 0 * x in both halves: NaN once one of them is
+template <typename T> __device__ __forceinline__ void add_zero_times(uint32_t& sum, uint32_t x) {
+    if (std::is_same<T, half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(x), "r"(0));
+}
 // Takes them out of values of V that some rows of a tile see and others do not (a weight of 0 does not hide them in a product) and notes for each
 // of the eight columns the first key that had one: rows from that token on get NaN there.
 template <typename T> __device__ __forceinline__ uint4 without_infinite(uint4 w, int key, int* from) {

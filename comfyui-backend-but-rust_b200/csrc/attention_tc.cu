@@ -56,7 +56,7 @@ template <int DP, Mode MODE> struct Tc {
     static constexpr int kEarly = DP > 64 ? 3 : 2;
     // Registers of the warpgroups (softmax twice, products and loads, codes or rows out): a softmax thread holds a row of 128 logits. Their
     // sum over the threads is what the launch has, 512 x 128.
-    static constexpr int kSoftmaxRegs = 184, kIssueRegs = KV8 ? 40 : MODE == PACKED ? 72 : 56, kLastRegs = KV8 ? 104 : MODE == PACKED ? 72 : 88;
+    static constexpr int kSoftmaxRegs = MODE == PACKED ? 192 : 184, kIssueRegs = KV8 ? 40 : MODE == PACKED ? 64 : 56, kLastRegs = KV8 ? 104 : MODE == PACKED ? 64 : 88;
     static_assert(2 * kSoftmaxRegs + kIssueRegs + kLastRegs == 4 * 128, "register split");
 };
 
@@ -607,9 +607,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                     uint8_t* tile = sm + L::kRing + slot * L::kTile + (piece >> 3) * kBox;
                     const int key0 = ((warp - 10) * 32 + lane) / kLanes, end = min(kTileKeys, x.seen - j * kTileKeys);
                     auto at = [&](int key) { return reinterpret_cast<uint4*>(tile + key * 128 + ((piece ^ key) & 7) * 16); };
-                    bool bad = false;
-                    for (int key = key0; key < end; key += 64 / kLanes) bad |= any_infinite<QT>(*at(key));
-                    if (__any_sync(0xffffffffu, bad)) {
+                    uint32_t zero[2] = {};      // times 0 they are 0, or NaN that stays
+#pragma unroll 4
+                    for (int key = key0; key < end; key += 64 / kLanes) {
+                        const uint4 y = *at(key);
+                        add_zero_times<QT>(zero[0], y.x), add_zero_times<QT>(zero[1], y.y), add_zero_times<QT>(zero[0], y.z), add_zero_times<QT>(zero[1], y.w);
+                    }
+                    if (__any_sync(0xffffffffu, ((zero[0] | zero[1]) & 0x7FFF7FFFu) != 0)) {
                         int* first = from + ((warp - 10) * 8 + (item_no & 7)) * DP;
                         if (!noted) {
                             for (int c = lane; c < DP; c += 32) first[c] = INT32_MAX;
