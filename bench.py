@@ -114,6 +114,28 @@ def _setup_hbm(name, b, torch, dev, wl, I):
         b.q, b.k, b.v = (rnd(1, n, 24, 128).bfloat16() for n in (16384, 512, 512))
         b.qout = torch.empty_like(b.q)
         return None
+    if name in ("f8_linear", "f8_linear_prompt"):                # e4m3 blocks: one token, 2560 -> 19456 | 1024 tokens, 5120 -> 13824
+        M, K, N = (1, 2560, 19456) if name == "f8_linear" else (1024, 5120, 13824)
+        b.fw = I.f8_requant((rnd(N, K) * 0.03).bfloat16())
+        b.fx = I.norm_rows(rnd(M, K).bfloat16(), 1, eps=1e-6, out_dtype=torch.float8_e4m3fn)
+        b.fout = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        return N * K + N * K // 4096 + M * K + M * K // 32 + 2 * M * N
+    if name == "norm_rows":                                      # 16896 rows onto the residual stream, RMS, to e4m3
+        b.nx, b.nr, b.nw = rnd(16896, 5120).bfloat16(), rnd(16896, 5120).bfloat16(), rnd(5120)
+        b.nout = I.norm_rows(b.nx, 1, norm_w=b.nw, eps=1e-6, resid=b.nr, out_dtype=torch.float8_e4m3fn)
+        return 16896 * (5120 * 7 + 160) + 4 * 5120
+    if name == "rotary":                                         # 2 x 4096 tokens, 24 query and 24 key heads of 128
+        b.A = sys.modules[I.__package__ + ".attention"]
+        b.rq = rnd(2, 4096, 48, 128).bfloat16()
+        b.rf, b.rp = b.A.rope_frequencies(128, device=dev)[0], torch.arange(4096, dtype=torch.int32, device=dev).expand(2, -1).contiguous()
+        return 2 * 2 * b.rq.numel()
+    if name == "packed_attention":                               # prompts of 4096, 1000, 333 and 77 tokens, 32 / 8 heads of 128, causal
+        b.A = sys.modules[I.__package__ + ".attention"]
+        lens = (4096, 1000, 333, 77)
+        b.po = torch.tensor([sum(lens[:i]) for i in range(5)], dtype=torch.int32, device=dev)
+        b.q, b.k, b.v = (rnd(sum(lens), h, 128).bfloat16() for h in (32, 8, 8))
+        b.qout = torch.empty_like(b.q)
+        return None
     raise KeyError(name)
 
 
@@ -131,6 +153,11 @@ HBM_KERNELS = {
     "w4_linear_prompt": lambda b, I: I.w4_linear(b.qx, *b.q, out=b.qout),
     "kv8_attention": lambda b, I: b.A.kv8_attention(b.q, b.cache, b.table, b.lengths),
     "cross_attention": lambda b, I: b.A.cross_attention(b.q, b.k, b.v, out=b.qout),
+    "f8_linear": lambda b, I: I.f8_linear(*b.fx, *b.fw, out=b.fout),
+    "f8_linear_prompt": lambda b, I: I.f8_linear(*b.fx, *b.fw, out=b.fout),
+    "norm_rows": lambda b, I: I.norm_rows(b.nx, 1, norm_w=b.nw, eps=1e-6, resid=b.nr, out=b.nout[0], scales=b.nout[1]),
+    "rotary": lambda b, I: b.A.rotary(b.rq[:, :, :24], b.rq[:, :, 24:], b.rp, b.rf, q_out=b.rq[:, :, :24], k_out=b.rq[:, :, 24:]),
+    "packed_attention": lambda b, I: b.A.packed_attention(b.q, b.k, b.v, b.po, causal=True, out=b.qout),
     "pack_f32": lambda b, I: I.convrot_requant(b.hw, 0),
     "pack_bf16": lambda b, I: I.convrot_requant(b.hw, 0),
     "sd_quant": lambda b, I: I.sd_quant_rows(b.hx, 256),

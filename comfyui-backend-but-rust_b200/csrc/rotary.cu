@@ -71,7 +71,19 @@ template <int V> __device__ __forceinline__ void scaled(float (&u)[V], const flo
 #pragma unroll
     for (int e = 0; e < V; ++e) u[e] = u[e] * r * x.e[e];
 }
-template <int V> __device__ __forceinline__ void turned(const RotaryParams& p, float (&u)[V], float (&v)[V], const float2* cs) {
+// A token's cosines and sines: two pairs of a slot next to each other, then the same two of the next slot, so that neighbouring threads read neighbouring
+// 16 bytes (in the pairs' order a thread's 64 bytes meet its fourth neighbour's in the same banks)
+template <int V> __device__ __forceinline__ int turn_at(int f, int rotated) { return V == 1 ? f : (f % V / 2 * rotated + f / V) * 2 + f % 2; }
+template <int V> __device__ __forceinline__ void turned(const RotaryParams& p, float (&u)[V], float (&v)[V], const float2* at, int rotated) {
+    float2 cs[V];
+    if (V == 1) cs[0] = at[0];
+    else {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            const float4 two = reinterpret_cast<const float4*>(at)[e / 2 * rotated];
+            cs[e] = make_float2(two.x, two.y), cs[e + 1] = make_float2(two.z, two.w);
+        }
+    }
     if (p.interleaved && V > 1) {
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
@@ -91,11 +103,12 @@ template <int V> __device__ __forceinline__ void turned(const RotaryParams& p, f
 }
 
 // A group of `lanes` threads has a head, a thread of it one slot of 2 V values (several with V = 1); the next head's values are on their way. Measured
-// (us, floor at the copy's rate): 2 x 4179 tokens, 24 / 24 heads of 128, fp16, 40.8 (31.3; 50.3 with
+// (us, floor at the copy's rate): 2 x 4179 tokens, 24 / 24 heads of 128, fp16, 38.7 (31.3; before the table's order above 40.4, before that 50.3 with
 // 64-bit divisions for every head and nothing ahead; 47.5 with a token's angles in registers, which leave room for fewer threads); 4096 tokens, 32 / 8 heads
-// of 128, bf16, 19.5 (12.8), heads normalised 25.3.
+// of 128, bf16, 18.3 (12.8; 19.5), heads normalised 19.7 (26.3); 8192 tokens, 32 / 8 heads of 96, the first 40 values turned, normalised 53 (19.2): four
+// values at a time and 12 threads of 16.
 template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, const int lanes) {
-    extern __shared__ float2 turn[];      // [token][half]: cos, sin
+    extern __shared__ __align__(16) float2 turn[];      // [token][half]: cos, sin
     __shared__ int64_t row[4][kMaxTokens];      // of q, k and the results, where a token's row begins
     const int64_t tokens = (int64_t)p.B * p.L, first = (int64_t)blockIdx.x * p.tokens;
     const int here = (int)min((int64_t)p.tokens, tokens - first);
@@ -114,7 +127,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
         const double turns = (double)pos * gload(p.freq + f) * 0.15915494309189533577;
         float s, c;
         sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-        turn[i] = make_float2(c * p.scale, s * p.scale);
+        turn[t * p.half + turn_at<V>(f, p.half / V)] = make_float2(c * p.scale, s * p.scale);
     }
     __syncthreads();
     const int lane = threadIdx.x % lanes, slots = p.D / (2 * V), rotated = p.half / V, step = kThreads / lanes;
@@ -151,7 +164,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
             if (mine) x.values(u), y.values(v);
             T* dst = y_of(n);
             const float* w = p.norm[n.h >= p.H];
-            const float2* cs = turn + n.t * p.half + lane * V;
+            const float2* cs = turn + n.t * p.half + lane * 2;
             n.h += step;
             n.wrap(p.heads);
             request();
@@ -163,7 +176,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
                 const float r = factor(sum);
                 if (mine) scaled<V>(u, w + a, r), scaled<V>(v, w + b, r);
             }
-            if (lane < rotated) turned<V>(p, u, v, cs);
+            if (lane < rotated) turned<V>(p, u, v, cs, rotated);
             if (mine) {
                 Vec<T, V> o;
                 o.round(u), o.store(dst + a);
@@ -191,7 +204,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
             for (int s = lane; s < slots; s += lanes) {
                 read(s, a, b);
                 if (w) scaled<V>(u, w + a, r), scaled<V>(v, w + b, r);
-                if (s < rotated) turned<V>(p, u, v, turn + n.t * p.half + s);
+                if (s < rotated) turned<V>(p, u, v, turn + n.t * p.half + s, rotated);
                 x.round(u), x.store(dst + a);
                 y.round(v), y.store(dst + b);
             }
