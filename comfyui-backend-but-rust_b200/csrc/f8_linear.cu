@@ -50,6 +50,43 @@ __device__ __forceinline__ void put_value(void* p, int dt, int64_t i, float v) {
     else reinterpret_cast<bf16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+__device__ __forceinline__ float4 dsmem_f32x4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_shared(addr, rank)) : "memory");
+    return v;
+}
+// Four columns of sums that the CTAs `from`, from + by, ... of the cluster (kMost at most, p.splits in all) have at `addr`, in this order. All are on their way
+// at once: one after the other a row of 64 waits for each
+template <int kMost> __device__ __forceinline__ void add_up(const F8Params& p, uint32_t addr, uint32_t from, uint32_t by, float (&y)[4]) {
+    float4 v[kMost];
+#pragma unroll
+    for (int s = 0; s < kMost; ++s) v[s] = s < p.splits ? dsmem_f32x4(addr, from + s * by) : make_float4(0.f, 0.f, 0.f, 0.f);
+    y[0] = v[0].x, y[1] = v[0].y, y[2] = v[0].z, y[3] = v[0].w;
+#pragma unroll
+    for (int s = 1; s < kMost; ++s)
+        if (s < p.splits) y[0] += v[s].x, y[1] += v[s].y, y[2] += v[s].z, y[3] += v[s].w;
+}
+// Four columns of a row from `col` on: bias and what was there, and out; whole: rows of out begin on the four columns' bytes
+__device__ __forceinline__ bool whole_rows(const F8Params& p) { return p.out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (p.out_dt == DT_F32 ? 15 : 7)) == 0; }
+__device__ __forceinline__ void finish4(const F8Params& p, int row, int col, bool whole, float (&y)[4]) {
+    const int64_t at = (int64_t)row * p.out_stride + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= p.N) continue;
+        if (p.bias) y[e] += value_at(p.bias, p.out_dt, col + e);
+        if (p.add) y[e] += value_at(p.out, p.out_dt, at + e);
+    }
+    if (whole && col + 4 <= p.N) {
+        if (p.out_dt == DT_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+        else
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = p.out_dt == DT_F16 ? make_uint2(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]))
+                                                                                                    : make_uint2(pack2<bf16>(y[0], y[1]), pack2<bf16>(y[2], y[3]));
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.N) put_value(p.out, p.out_dt, at + e, y[e]);
+}
+
 // The end of a CTA: tensor memory back, a wait that ran out recorded
 __device__ __forceinline__ void leave(volatile int* abort_s, bool allocated, uint32_t tmem, uint32_t columns) {
     __syncwarp();
@@ -172,14 +209,13 @@ template <int NT> __global__ void __launch_bounds__(Few<NT>::kThreads) f8_few_ke
             for (int c = 0; c < NT; ++c) part[c * 128 + threadIdx.x] = sum[c];
         __syncwarp();
         cluster_sync_all();
-        if (warp < 4 && n < p.N)
-            for (int m = split; m < p.M; m += p.splits) {
-                float y = 0.f;
-                for (int s = 0; s < p.splits; ++s) y += dsmem_f32(smem_u32(part + m * 128 + threadIdx.x), s);
-                if (p.bias) y += value_at(p.bias, p.out_dt, n);
-                const int64_t at = m * p.out_stride + n;
-                if (p.add) y += value_at(p.out, p.out_dt, at);
-                put_value(p.out, p.out_dt, at, y);
+        const int col = tile * 128 + lane * 4;
+        const bool whole = whole_rows(p);
+        if (warp < 4 && col < p.N)      // a token to a warp
+            for (int m = split + warp * p.splits; m < p.M; m += 4 * p.splits) {
+                float y[4];
+                add_up<8>(p, smem_u32(part + m * 128 + lane * 4), 0, 1, y);
+                finish4(p, m, col, whole, y);
             }
         __syncwarp();
         cluster_sync_all();      // nobody leaves while its shared memory is read
@@ -224,11 +260,6 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
 // The mbarrier at this offset in both CTAs of the pair gets an arrival once the products that this thread issued are done; `mask`: the pair's ranks
 __device__ __forceinline__ void commit_pair(uint32_t bar, uint16_t mask) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask) : "memory");
-}
-__device__ __forceinline__ float4 dsmem_f32x4(uint32_t addr, uint32_t rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_shared(addr, rank)) : "memory");
-    return v;
 }
 
 // A warp's 32 rows of sums out, by way of its staging, so that a row's pieces are stored together
@@ -469,33 +500,15 @@ template <bool SPLIT> __global__ void __launch_bounds__(Tile::kThreads, 1) f8_ti
         cluster_sync_all();
         // the CTAs of a tile's 128 rows take turns over them, each adding up all of a row
         const int m0 = pair % p.m_tiles * 256 + (int)rank * 128, n0 = pair / p.m_tiles * L::kColumns, left = min(128, p.M - m0);
-        const int esize = p.out_dt == DT_F32 ? 4 : 2;
-        const bool whole = p.out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & (4 * esize - 1)) == 0;
+        const bool whole = whole_rows(p);
         if (warp < 8 && pair < p.tiles)
+#pragma unroll 2
             for (int i = threadIdx.x + (int)(in_cluster >> 1) * 256; i < left * 64; i += 256 * p.splits) {
                 const int row = i >> 6, piece = i & 63, col = n0 + piece * 4;
                 if (col >= p.N) continue;
-                float y[4] = {};
-                for (int s = 0; s < p.splits; ++s) {
-                    const float4 v = dsmem_f32x4(base + row * 1024 + (piece ^ (row & 7)) * 16, 2 * s + rank);
-                    y[0] += v.x, y[1] += v.y, y[2] += v.z, y[3] += v.w;
-                }
-                const int64_t at = (int64_t)(m0 + row) * p.out_stride + col;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (col + e >= p.N) continue;
-                    if (p.bias) y[e] += value_at(p.bias, p.out_dt, col + e);
-                    if (p.add) y[e] += value_at(p.out, p.out_dt, at + e);
-                }
-                if (whole && col + 4 <= p.N) {
-                    if (esize == 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
-                    else
-                        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = p.out_dt == DT_F16 ? make_uint2(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]))
-                                                                                                                : make_uint2(pack2<bf16>(y[0], y[1]), pack2<bf16>(y[2], y[3]));
-                } else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (col + e < p.N) put_value(p.out, p.out_dt, at + e, y[e]);
+                float y[4];
+                add_up<4>(p, base + row * 1024 + (piece ^ (row & 7)) * 16, rank, 2, y);
+                finish4(p, m0 + row, col, whole, y);
             }
     }
     __syncwarp();
