@@ -214,7 +214,7 @@ template <int NT> __global__ void __launch_bounds__(Few<NT>::kThreads) f8_few_ke
         if (warp < 4 && col < p.N)      // a token to a warp
             for (int m = split + warp * p.splits; m < p.M; m += 4 * p.splits) {
                 float y[4];
-                add_up<8>(p, smem_u32(part + m * 128 + lane * 4), 0, 1, y);
+                add_up<6>(p, smem_u32(part + m * 128 + lane * 4), 0, 1, y);
                 finish4(p, m, col, whole, y);
             }
         __syncwarp();
@@ -541,8 +541,11 @@ template <int NT> int launch_few(const void* x, int64_t x_stride, const void* W,
     CUtensorMap tx, tw;
     if (!codes_map(&tx, x, x_stride, p.M, p.K, NT) || !codes_map(&tw, W, p.K, p.N, p.K, 128)) return -203;
     p.tiles = (p.N + 127) / 128;
+    // CTAs to a tile: as many as find room beside one another, two to an SM, with four blocks each; six at most, for larger clusters leave SMs out (us with
+    // 4 | 5 | 6 | 7 | 8: 16 x 9728 -> 2560 8.7 | 8.4 | 8.0 | 8.9 | 8.5, 1 x 13824 -> 5120 14.3 | 14.0 | 13.9 | 19.4 | 18.1; 108 tiles, 1 | 2 | 3: 64 x 5120 -> 13824
+    // 27.3 | 20.2 | 26.8). More stages where an SM has one CTA: nothing.
     p.splits = 1;
-    while (p.splits < 8 && p.tiles * p.splits * 2 <= 296 && p.groups >= p.splits * 4) p.splits *= 2;
+    while (p.splits < 6 && (int64_t)p.tiles * (p.splits + 1) <= 296 && p.groups >= (p.splits + 1) * 4) ++p.splits;
     p.per = (p.groups + p.splits - 1) / p.splits;
     const int smem = L::smem(p.per);
     auto kern = f8_few_kernel<NT>;
