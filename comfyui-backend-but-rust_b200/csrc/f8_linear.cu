@@ -89,6 +89,21 @@ __device__ __forceinline__ void finish4(const F8Params& p, int row, int col, boo
             if (col + e < p.N) put_value(p.out, p.out_dt, at + e, y[e]);
 }
 
+// Four columns of a row as they lie in memory: loaded in one place, made numbers in another, so that nobody waits between the loads
+struct Four {
+    uint4 w;
+    __device__ __forceinline__ void load(const void* base, int dt, int64_t at) {
+        if (dt == DT_F32) w = gload(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + at));
+        else {
+            const uint2 v = gload(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(base) + at));
+            w = make_uint4(v.x, v.x >> 16, v.y, v.y >> 16);
+        }
+    }
+    __device__ __forceinline__ float value(int dt, uint32_t x) const {
+        return dt == DT_F32 ? __uint_as_float(x) : dt == DT_F16 ? __half2float(__ushort_as_half((uint16_t)x)) : __bfloat162float(__ushort_as_bfloat16((uint16_t)x));
+    }
+};
+
 // The end of a CTA: tensor memory back, a wait that ran out recorded
 __device__ __forceinline__ void leave(volatile int* abort_s, bool allocated, uint32_t tmem, uint32_t columns) {
     __syncwarp();
@@ -306,6 +321,11 @@ __device__ __forceinline__ void rows_out(const F8Params& p, const float (&sum)[T
     // f32 rows, rows that are added to, ragged ones: 32 columns of f32 at a time
 #pragma unroll
     for (int c = 0; c < kCols; c += 32) {
+        Four was[8] = {};      // what is added to: eight rows on their way at once (one after the other 4352 x 2560 -> 2560 in bf16 takes 88 us instead of 66)
+        if (whole && p.add)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k * 4 + (lane >> 3) < left) was[k].load(p.out, p.out_dt, (int64_t)(m0 + k * 4 + (lane >> 3)) * p.out_stride + n0 + c + (lane & 7) * 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             *reinterpret_cast<float4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) = make_float4(sum[c + 4 * e], sum[c + 4 * e + 1], sum[c + 4 * e + 2], sum[c + 4 * e + 3]);
@@ -315,16 +335,15 @@ __device__ __forceinline__ void rows_out(const F8Params& p, const float (&sum)[T
             float b[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) b[i] = p.bias ? value_at(p.bias, p.out_dt, col + i) : 0.f;
-#pragma unroll 2
+#pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int r = k * 4 + (lane >> 3);
-                if (r >= left) break;
+                if (r >= left) continue;
                 const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((e ^ r) & 7) * 16);
-                float y[4] = {v.x + b[0], v.y + b[1], v.z + b[2], v.w + b[3]};
+                const uint4 w = was[k].w;
+                const float y[4] = {v.x + b[0] + was[k].value(p.out_dt, w.x), v.y + b[1] + was[k].value(p.out_dt, w.y), v.z + b[2] + was[k].value(p.out_dt, w.z),
+                                    v.w + b[3] + was[k].value(p.out_dt, w.w)};
                 const int64_t at = (int64_t)(m0 + r) * p.out_stride + col;
-                if (p.add)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] += value_at(p.out, p.out_dt, at + i);
                 if (esize == 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
                 else
                     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = p.out_dt == DT_F16 ? make_uint2(pack2<half>(y[0], y[1]), pack2<half>(y[2], y[3]))
