@@ -209,6 +209,25 @@ def test_linear(pkg, dev, M, N, K):
     assert pkg.linear.kernel_status() == 0
 
 
+@pytest.mark.parametrize("M,tiles,width", [(5, n, 128) for n in (1, 22, 23, 44, 46, 58, 69, 90, 97, 149)] + [(40, n, 128) for n in (43, 57, 73)] +
+                         [(130, n, 256) for n in (1, 15, 16, 22, 23, 34, 35)] + [(482, 15, 256)])
+def test_linear_with_every_number_of_ctas_to_a_tile(pkg, dev, M, tiles, width):
+    """Sums of one to six CTAs and of one to four pairs, onto what is there and with a bias; widths whose last tile ends inside four columns too."""
+    g = torch.Generator().manual_seed(M + tiles)
+    K = 3200
+    for N in (tiles * width - 120, tiles * width - 1):
+        N = max(N, 1)
+        x, xs, w, ws = _operands(g, dev, M, N, K)
+        x64, w64 = _values(x, xs, 1), _values(w, ws, 128)
+        for dt in DT.values():
+            bias, base = torch.randn(N, generator=g).to(dt).to(dev), torch.randn(M + 1, N, generator=g).to(dt).to(dev)
+            out = base.clone()
+            pkg.linear.f8_linear(x, xs, w, ws, bias, out=out[:M], beta=1.0)
+            _check_linear(out[:M], x64, w64, bias, base[:M], K)
+            assert torch.equal(out[M], base[M])
+    assert pkg.linear.kernel_status() == 0
+
+
 @pytest.mark.parametrize("M", [1, 20, 50, 150, 700])
 def test_linear_on_strided_rows_and_into_a_slice(pkg, dev, M):
     g = torch.Generator().manual_seed(M)
