@@ -167,7 +167,7 @@ template <typename T, int PRO> __global__ void __launch_bounds__(256) group_rows
 template <typename T, int V> constexpr bool ahead() { return sizeof(T) == 2 && V <= 2; }
 // RMS: a thread has V pieces of eight columns, `warps` * 32 pieces apart. A CTA takes rows in turn: weights stay in registers (read anew for every
 // row they are as many bytes as 16-bit rows and their stream), the next row's values are on their way while this one's sum goes round. With more than
-// two pieces a thread has no room for either.
+// two pieces a thread has no room for either, nor with f32 rows: those CTAs have one turn, or several with more than kMostStep rows.
 template <typename T, int V> __global__ void __launch_bounds__(V <= 2 ? 512 : 1024, V > 2 ? 1 : ahead<T, V>() ? 2 : 3) rms_rows_kernel(const NormParams p) {
     constexpr bool kAhead = ahead<T, V>();
     __shared__ __align__(16) float part[2][32];
@@ -252,6 +252,7 @@ template <typename T, int V> __global__ void __launch_bounds__(V <= 2 ? 512 : 10
 }
 
 constexpr int kThreadsAhead = 1024;      // to an SM
+constexpr int kMostStep = 1 << 19;       // rows from a CTA's turn to its next: the last row's number and this one fit 32 bits (gpu_norm_rows leaves twice as much)
 template <typename T, int PRO> int launch_groups(NormParams& p, cudaStream_t st) {
     const int groups = (p.K + 127) / 128, columns = (groups + 15) / 16, wide = (groups + columns - 1) / columns;
     const int rows = 16 / wide, sms = device_sms();      // rows to a CTA
@@ -266,7 +267,7 @@ template <typename T, int V> int launch_rms(NormParams& p, cudaStream_t st) {
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
     p.warps = (pieces + 32 * V - 1) / (32 * V);
     const int rows = p.warps >= 8 ? 1 : 8 / p.warps, ctas = (p.M + rows - 1) / rows;      // rows to a CTA
-    const int most = ahead<T, V>() ? sms * (kThreadsAhead / (rows * p.warps * 32)) : ctas;
+    const int most = ahead<T, V>() ? sms * (kThreadsAhead / (rows * p.warps * 32)) : kMostStep / rows;
     return launch_pdl(rms_rows_kernel<T, V>, dim3(ctas < most ? ctas : most), rows * p.warps * 32, 0, st, p);
 }
 template <typename T> int launch_norm(int prologue, NormParams& p, cudaStream_t st) {
