@@ -62,6 +62,18 @@ template <typename T> struct Raw {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = to_f<T>(e[i]);
     }
+    // Whether one of them may be below `bound`, a negative number that T has. 16-bit values as whole numbers: what is more negative is larger
+    __device__ __forceinline__ bool below(float bound) const {
+        if constexpr (std::is_same<T, float>::value) {
+            float v[8];
+            values(v);
+            return fminf(fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), fminf(fminf(v[4], v[5]), fminf(v[6], v[7]))) < bound;
+        } else {
+            const T b = from_f<T>(bound);
+            const uint32_t most = __vmaxu2(__vmaxu2(w[0].x, w[0].y), __vmaxu2(w[0].z, w[0].w)), end = *reinterpret_cast<const uint16_t*>(&b);
+            return (most >> 16) > end || (most & 0xffffu) > end;
+        }
+    }
     // The sum in T. Of 16-bit values directly: their f32 sum is exact, or the smaller one below half a step of the larger, which is the result either way
     __device__ __forceinline__ void add(const Raw& o) {
 #pragma unroll
@@ -104,25 +116,42 @@ __device__ __forceinline__ void emit(int out_dt, const float (&y)[8], uint8_t* a
 }
 __device__ __forceinline__ int out_size(int out_dt) { return out_dt == DT_E4M3 ? 1 : out_dt == DT_F32 ? 4 : 2; }
 
-// x / (1 + e^-x): e^-x as 2^(-x log2 e), the power and the reciprocal from the special function unit, 2^-22 each. The exponent's rounding is 2^-24 of it,
-// 2^-17 of the power where x is near -88: with f32 values that is taken into account, 16-bit ones and their codes do not show it. Below -87.3, where the
-// value is under 2e-36, it is 0; infinities and NaN as the formula has them.
-template <typename T> __device__ __forceinline__ float silu_fast(float x) {
-    constexpr float kHigh = 1.4426950216293335f, kLow = 1.9259629911266175e-8f, kEnd = 87.3f;      // log2 e; the reciprocal of 1 + e^kEnd is a normal number
+// x / (1 + e^-x): e^-x as 2^h, h = -x log2 e, the power and the reciprocal from the special function unit, 2^-22.5 and 2^-23. Infinities and NaN as the
+// formula has them.
+//   16-bit rows to 16-bit rows or codes: h as it is rounded, with log2 e in f32, is 2^-23.7 of itself off, 2^-17.2 of the power where x is -87, far below half
+//   a step of either. Below -87.3 the reciprocal is no normal number and the value 0.
+//   f32 rows, or to f32 rows: what is left of the exponent is -x - h ln 2 (ln 2 in f32: 2^-22 of the power where x is -80) and is multiplied on: 2^-20 in all.
+//   Below kSiluFar the value is x e^x, by two halves that are normal numbers; seldom, so that eight values together are asked for one. 4096 x 9728 bf16 to e4m3:
+//   38.7 us the first way, 43.1 this way; 512 x 9728 f32, which wait for HBM, 8.7 and 9.0.
+constexpr float kSiluFar = -80.f;
+template <bool FINE> __device__ __forceinline__ float silu_near(float x) {
     float e, r;
-    if (std::is_same<T, float>::value) {
-        const float t = fminf(fmaxf(-x, -kEnd), kEnd), h = __fmul_rn(t, kHigh), rest = __fmaf_rn(t, kLow, __fmaf_rn(t, kHigh, -h));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
-        e = __fmaf_rn(e, rest * 0.6931471805599453f, e);
-    } else asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, kEnd) * kHigh));
+    const float t = FINE ? fmaxf(-x, kSiluFar) : -x, h = __fmul_rn(t, 1.4426950408889634f);      // (beyond 80 the power is nothing beside 1; infinity has no rest)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
+    if (FINE) e = __fmaf_rn(e, __fmaf_rn(h, -0.6931471805599453f, t), e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return x * (x < -kEnd ? 0.f : r);
+    return x * r;
+}
+template <typename T, bool FINE> __device__ __forceinline__ void silu8(const Raw<T>& a, float (&y)[8]) {
+    a.values(y);
+    const bool far = FINE && a.below(kSiluFar);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = silu_near<FINE>(y[e]);
+    if (far) {
+        float x[8];
+        a.values(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float half = expf(0.5f * x[e]);
+            if (x[e] < kSiluFar) y[e] = x[e] * half * half;
+        }
+    }
 }
 
 // Rows without a norm: sixteen lanes take a group of 128 columns, of every `step`-th row, whose values are on their way a row ahead; a CTA has
 // `wide` neighbouring groups of as many rows as fit. 4096 x 9728 bf16, SWIGLU: 107 us with expf and a division, 57 with rows and groups counted by one
 // number (41 instructions a value, the issue slots' limit).
-template <typename T, int PRO> __global__ void __launch_bounds__(256) group_rows_kernel(const NormParams p, const int wide, const int step) {
+template <typename T, int PRO, bool FINE> __global__ void __launch_bounds__(256) group_rows_kernel(const NormParams p, const int wide, const int step) {
     const int slot = threadIdx.x / 16, group = blockIdx.x * wide + slot % wide, piece = group * 16 + (threadIdx.x & 15), rows = blockDim.x / (16 * wide);
     const bool in_row = piece < p.K / 8;
     int row = slot < rows * wide ? blockIdx.y * rows + slot / wide : p.M;      // (whole warps: half of one may have nothing to do)
@@ -148,13 +177,13 @@ template <typename T, int PRO> __global__ void __launch_bounds__(256) group_rows
     while (__any_sync(0xffffffffu, row < p.M)) {
         const bool mine = in_row && row < p.M;
         float y[8];
-        a.values(y);
         if (PRO == PRO_SWIGLU) {
             float up[8];
+            silu8<T, FINE>(a, y);
             b.values(up);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = silu_fast<T>(y[e]) * up[e];
-        }
+            for (int e = 0; e < 8; ++e) y[e] *= up[e];
+        } else a.values(y);
         row += step, x += next;
         request();
         if (!__any_sync(0xffffffffu, row < p.M)) pdl_trigger();
@@ -253,14 +282,14 @@ template <typename T, int V> __global__ void __launch_bounds__(V <= 2 ? 512 : 10
 
 constexpr int kThreadsAhead = 1024;      // to an SM
 constexpr int kMostStep = 1 << 19;       // rows from a CTA's turn to its next: the last row's number and this one fit 32 bits (gpu_norm_rows leaves twice as much)
-template <typename T, int PRO> int launch_groups(NormParams& p, cudaStream_t st) {
+template <typename T, int PRO, bool FINE = false> int launch_groups(NormParams& p, cudaStream_t st) {
     const int groups = (p.K + 127) / 128, columns = (groups + 15) / 16, wide = (groups + columns - 1) / columns;
     const int rows = 16 / wide, sms = device_sms();      // rows to a CTA
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
     const int threads = (rows * wide * 16 + 31) / 32 * 32;
     const int64_t all = ((int64_t)p.M + rows - 1) / rows, some = (int64_t)sms * (2048 / threads) / columns, most = some < 1 ? 1 : some;
     const int down = (int)(all < most ? all : most);
-    return launch_pdl(group_rows_kernel<T, PRO>, dim3(columns, down), threads, 0, st, p, wide, down * rows);
+    return launch_pdl(group_rows_kernel<T, PRO, FINE>, dim3(columns, down), threads, 0, st, p, wide, down * rows);
 }
 template <typename T, int V> int launch_rms(NormParams& p, cudaStream_t st) {
     const int pieces = p.K / 8, sms = device_sms();
@@ -272,7 +301,7 @@ template <typename T, int V> int launch_rms(NormParams& p, cudaStream_t st) {
 }
 template <typename T> int launch_norm(int prologue, NormParams& p, cudaStream_t st) {
     if (prologue == PRO_PLAIN) return launch_groups<T, PRO_PLAIN>(p, st);
-    if (prologue == PRO_SWIGLU) return launch_groups<T, PRO_SWIGLU>(p, st);
+    if (prologue == PRO_SWIGLU) return sizeof(T) == 4 || p.out_dt == DT_F32 ? launch_groups<T, PRO_SWIGLU, true>(p, st) : launch_groups<T, PRO_SWIGLU, sizeof(T) == 4>(p, st);
     if (p.K <= (sizeof(T) == 4 ? 4096 : 1536)) return launch_rms<T, 1>(p, st);
     return p.K <= 8192 ? launch_rms<T, 2>(p, st) : launch_rms<T, 4>(p, st);
 }

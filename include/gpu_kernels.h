@@ -306,7 +306,8 @@ int gpu_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out
  *
  * gpu_norm_rows    rows [M, K] of dtype (f32, f16, bf16) on their way to the next linear: prologue PLAIN y = x; RMS, with a residual stream where resid is
  *                  given: s = x + resid in dtype, written to resid_out (may be resid or x itself), y = s / sqrt(mean(s^2) + eps) * norm_w (f32 [K], or NULL: 1);
- *                  SWIGLU y = silu(x[:, :K]) * x[:, up_offset : up_offset + K]. y, f32 until then, becomes out [M, K]: out_dt f32, f16, bf16
+ *                  SWIGLU y = silu(x[:, :K]) * x[:, up_offset : up_offset + K] (silu within 2^-20 of its value; 16-bit x to 16-bit out or codes: within 2^-17, and
+ *                  0 below -87.3). y, f32 until then, becomes out [M, K]: out_dt f32, f16, bf16
  *                  (K a multiple of 8), or GPU_DT_E4M3 with scales [M, ceil(K/128)]. K <= 32768 (-2); -3 prologue, or resid and norm_w without RMS; -4 types; -5 a
  *                  NULL, a row or norm_w off a 16-byte boundary.
  * gpu_f8_requant   w [N, K] (rows w_stride apart) -> codes [N, K] and ws.
