@@ -382,9 +382,9 @@ GPU_API int gpu_norm_rows(int dtype, int prologue, const void* x, int64_t x_stri
 
 GPU_API int gpu_f8_requant(int dtype, const void* w, int64_t w_stride, void* codes, float* scales, int64_t N, int K, void* stream) {
     if (dtype < DT_F32 || dtype > DT_BF16) return -4;
-    if (N < 0 || K <= 0 || K % 16 != 0) return -1;
+    if (N < 0 || N > (int64_t)1 << 38 || K <= 0 || K % 16 != 0) return -1;
     const int64_t groups = ((int64_t)K + 127) / 128, blocks = (N / 128 + (N % 128 != 0)) * groups;
-    if (N > (int64_t)1 << 40 || blocks > INT32_MAX) return -1;
+    if (blocks > INT32_MAX) return -1;
     if (N == 0) return 0;
     if (!w || !codes || !scales || off(w, 16) || off(codes, 16) || (N > 1 && (w_stride * (dtype == DT_F32 ? 4 : 2) % 16 != 0 || w_stride < K))) return -5;
     auto kern = dtype == DT_F32 ? f8_requant_kernel<float> : dtype == DT_F16 ? f8_requant_kernel<half> : f8_requant_kernel<bf16>;
@@ -394,7 +394,7 @@ GPU_API int gpu_f8_requant(int dtype, const void* w, int64_t w_stride, void* cod
 GPU_API int gpu_f8_dequant(int dtype, const void* codes, const float* scales, int block_rows, void* out, int64_t N, int K, void* stream) {
     if (dtype < DT_F32 || dtype > DT_BF16) return -4;
     if (N < 0 || K <= 0 || K % 16 != 0 || (block_rows != 1 && block_rows != 128)) return -1;
-    if (N > (int64_t)1 << 40 || N * K / 2048 > INT32_MAX - 1) return -1;
+    if (N > (int64_t)(INT32_MAX - 1) * 2048 / K) return -1;
     if (N == 0) return 0;
     if (!codes || !scales || !out || off(codes, 16) || off(out, 16)) return -5;
     const int64_t total = N * K;
