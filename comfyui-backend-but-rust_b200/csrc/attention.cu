@@ -222,7 +222,7 @@ template <typename T, int DP> int launch_packed(AttnParams& p, cudaStream_t st) 
     auto kern = attention_tile_kernel<T, DP, true>;
     p.tile_tokens = kRows / p.pack, p.splits = 1;
     const int64_t tiles = (int64_t)p.rows / p.tile_tokens + p.B;
-    if (tiles > INT32_MAX / (p.H / p.pack)) return -1;
+    if (tiles > INT32_MAX / (p.H / p.pack) || p.rows > (INT32_MAX - kRows) / p.pack) return -1;      // (rows of a tile are counted from the sequence's first)
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemPacked)) return (int)e;
     p.row_tiles = (int)tiles;
     return launch_pdl(kern, dim3((unsigned)(tiles * (p.H / p.pack))), kThreads, L::kSmemPacked, st, p);

@@ -283,7 +283,8 @@ int gpu_cross_attention(int dtype, const void* q, const void* k, const void* v, 
  * 8 up to 256. Sequence b is rows offsets[b] to offsets[b + 1] - 1 (int32 [B + 1], ascending; may be empty); with causal != 0 a row sees
  * itself and the rows of its sequence before it, otherwise all of them. Rows outside every sequence are not written. What a row does not see does not reach it,
  * NaN and infinities included; an infinity in v that it sees may show as NaN. p is rounded to q's type for its product with v, f32 otherwise. Needs no workspace.
- * out may be q itself and overlaps nothing else that the call reads. Errors as above. */
+ * out may be q itself and overlaps nothing else that the call reads. Errors as above; -1 too where D > 128 or scale <= 0 and rows * min(H / Hkv, 16) passes
+ * 31 bits. */
 int gpu_packed_attention(int dtype, const void* q, const void* k, const void* v, void* out, const int64_t* strides, const int32_t* offsets,
                          int causal, int B, int rows, int H, int Hkv, int D, float scale, void* stream);
 
