@@ -7,8 +7,7 @@
 // Many tokens, f8_tile_kernel: 256 tokens by 256 outputs, a persistent pair of CTAs. While the tensor cores multiply one block, two warpgroups
 // take the block before out of the other accumulator; an output row to a thread, whose scale is one number a block then.
 // Every wait is bounded; one that runs out is recorded in g_f8_status and the CTA unwinds.
-#include <mutex>
-
+#include "cluster_room.h"
 #include "f8.cuh"
 #include "mma.cuh"
 #include "umma16.cuh"
@@ -576,31 +575,25 @@ bool codes_map(CUtensorMap* tm, const void* ptr, int64_t stride, int rows, int K
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How many clusters of 2 .. 8 CTAs, one to an SM, the current device holds at once: asked of the runtime once per device, for few and many tokens. A cluster
-// lies in one group of SMs, so that there is room for fewer than the SMs' number says.
-template <bool MANY, typename... P> const int* clusters_at_once(void (*kern)(P...), int threads) {
+// Clusters of 2 .. 8 CTAs, one to an SM, that the current device holds at once, for few and many tokens. A cluster lies in one group of SMs, so that there
+// is room for fewer than the SMs' number says.
+template <bool MANY, typename... P> int clusters_at_once(void (*kern)(P...), int threads, const int** room) {
     constexpr int smem = 227 * 1024;      // an SM has one such CTA
-    static int count[64][9];
-    static std::mutex mu;
+    static ClusterRoom rooms;
     int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(mu);
-    int* c = count[dev & 63];
-    if (c[0] == 0) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
-            for (int i = 2; i <= 8; ++i) {
-                cudaLaunchConfig_t cfg = {};
-                cfg.gridDim = dim3(i), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
-                cudaLaunchAttribute at;
-                at.id = cudaLaunchAttributeClusterDimension;
-                at.val.clusterDim.x = (unsigned)i, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
-                cfg.attrs = &at, cfg.numAttrs = 1;
-                if (cudaOccupancyMaxActiveClusters(&c[i], kern, &cfg) != cudaSuccess) c[i] = 0;
-            }
-        (void)cudaGetLastError();
-        c[0] = 1;
-    }
-    return c;
+    if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+    const int rc = rooms.get(dev, [&](int ctas, int& n) {
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return (int)e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = (unsigned)ctas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+        cfg.attrs = &at, cfg.numAttrs = 1;
+        return (int)cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+    }, room);
+    if (rc != 0) (void)cudaGetLastError();      // the call returns it; no later launch is to find it
+    return rc;
 }
 
 template <int NT> int launch_few(const void* x, int64_t x_stride, const void* W, F8Params& p, cudaStream_t st) {
@@ -613,10 +606,12 @@ template <int NT> int launch_few(const void* x, int64_t x_stride, const void* W,
     // 1 x 13824 -> 5120 14.3 | 14.0 | 13.9 | 19.4 | 18.1). 16 x 4096, 4 | 5 | 6: 44 tiles 7.9 | 8.0 | 8.0, 46 8.0 | 8.1 | 12.0, 58 8.9 | 13.0. More stages where
     // an SM has one CTA: nothing.
     constexpr int kTwo = 113 * 1024;      // shared memory of a CTA, up to which an SM holds two
+    const int* room = nullptr;
+    if (int rc = clusters_at_once<false>(kern, L::kThreads, &room)) return rc;
     for (p.splits = 6; p.splits > 1; --p.splits) {
         if (p.groups < p.splits * 4) continue;
         const int to_sm = L::smem((p.groups + p.splits - 1) / p.splits) <= kTwo ? 2 : 1;
-        if (p.tiles <= to_sm * clusters_at_once<false>(kern, L::kThreads)[p.splits]) break;
+        if (p.tiles <= to_sm * room[p.splits]) break;
     }
     p.per = (p.groups + p.splits - 1) / p.splits;
     const int smem = L::smem(p.per);
@@ -633,7 +628,8 @@ int launch_tile(const void* x, int64_t x_stride, const void* W, F8Params& p, int
     p.tiles = (int)tiles;
     // pairs to a tile: as many as find room at once, four at most, with four blocks each (128 x 4096, us with 2 | 3 | 4: 15 tiles 18.0 | 15.0 | 13.6, 16 tiles
     // 18.1 | 15.3 | 25.0, 23 tiles 18.4 | 28.6)
-    const int* room = clusters_at_once<true>(f8_tile_kernel<true>, L::kThreads);
+    const int* room = nullptr;
+    if (int rc = clusters_at_once<true>(f8_tile_kernel<true>, L::kThreads, &room)) return rc;
     for (p.splits = 4; p.splits > 1 && (p.groups < p.splits * 4 || p.tiles > room[2 * p.splits]);) --p.splits;
     p.per = (p.groups + p.splits - 1) / p.splits;
     p.splits = (p.groups + p.per - 1) / p.per;
