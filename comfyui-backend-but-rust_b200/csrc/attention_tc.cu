@@ -232,9 +232,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     // for item n + 2 only behind what waited for item n's reader: l behind the logits of n + 2, which are issued behind the sums of n + 1, and those
     // wait for o_empty of n, which the rows' way out gives when it has read; powers behind q_empty of n + 1, whose logits are issued behind p of n.
     float* row_info = reinterpret_cast<float*>(sm + L::kRowInfo);
-    // packed: [warp][item % 8], [warp][item % 8][column]. A warp clears an item's flag an item ahead: by then the rows' way out is behind the item that
-    // had the place before, seven items back, for V of item n is loaded behind the sums of n - 2, and those begin when all the warps of the rows' way
-    // out have begun with n - 3.
+    // packed: [warp][item % 8], [warp][item % 8][column]. A warp clears the flag of item n + 1 at the start of item n. It has V of n - 1 behind it, which is
+    // loaded behind the sums of n - 3, and those begin when the rows' way out has begun its last reads of n - 4: it is through with n - 5, and the place was
+    // that of n - 7. tests/test_packed_ring_order.py goes through it.
     int *found = reinterpret_cast<int*>(sm + L::kFound), *from = reinterpret_cast<int*>(sm + L::kFrom);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(kv_full + 8 * i, KV8 ? 4 : 1), mbar_init(kv_empty + 8 * i, 1);
