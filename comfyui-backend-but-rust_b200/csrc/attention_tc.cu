@@ -383,6 +383,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
                         unpack_f32(KV8 ? add_f32x2(x, minus) : fma_f32x2(x, by, minus), a, b);
                         a = exp2_fast(a), b = exp2_fast(b);
                         const float wt = KV8 ? in[16 + q * 2 + (e >> 4)] : 0.f;
+                        // p to 16 bits for its product: the products take both operands in one type, and V's is q's (bf16 has no f16 partner, and p in two parts
+                        // would be the products twice). The sum l is of p in f32. 8192 tokens, 32 / 8 heads of 128, bf16: 2.2e-3 off the exact rows in the
+                        // norm, 1.6e-3 with p in f32, which is the result's own rounding; 16 captions in fp16 2.2e-4 and 2.0e-4.
                         sum[e >> 1 & 1] = KV8 ? fma_f32x2(pack_f32(a, b), pack_f32(wt, wt), sum[e >> 1 & 1]) : add_f32x2(pack_f32(a, b), sum[e >> 1 & 1]);
                         out[e >> 1] = pack2<T>(a, b);
                     }
@@ -939,8 +942,10 @@ int b200q::attention_tc(int dtype, bool kv8, AttnParams& a, cudaStream_t st) {
 bool b200q::attention_tc_takes_packed(const AttnParams& p) {
     if (p.D > 128 || !(p.scale > 0.f)) return false;
     // Short sequences that tiles of 64 rows on every SM have done in a round or three take longer here, where an item begins and ends slowly. us here |
-    // there, heads of 128, 32 / 8: 1 x 64 tokens 12.2 | 9.1, 1 x 256 12.6 | 15.9, 40 x 20 16.1 | 25.9, 32 x 64 18.4 | 39.8; 12 heads of 64: 1 x 77 7.7 | 6.2,
-    // 16 x 40 11.0 | 7.6, 16 x 77 11.1 | 9.1, 64 x 77 26.8 | 30.4, 8 x 128 8.3 | 9.1, 1 x 333 11.0 | 11.9.
+    // there, heads of 128, 32 / 8: 1 x 64 tokens 12.2 | 9.1, 8 x 64 12.4 | 11.0, 16 x 40 12.4 | 19.2, 1 x 256 13.0 | 15.8, 40 x 20 15.3 | 25.8, 32 x 64 18.4 | 39.8; 12 heads of 64:
+    // 1 x 77 7.3 | 6.2, 16 x 40 10.6 | 7.4, 16 x 77 10.7 | 8.8, 40 x 20 16.6 | 11.4, 64 x 77 26.8 | 30.4, 1 x 256 10.6 | 10.1, 1 x 333 11.0 | 11.9. The lengths lie on the device, so the rule
+    // goes by their mean, and a long prompt among short ones that it sends there is one CTA's work for each head: 200 + 7 x 60 tokens, 12 heads of 64, 11.3 | 10.2, 400 + 15 x 20
+    // 14.7 | 15.5, 700 + 15 x 20 17.9 | 23.9, 1441 + 15 x 4 27.7 | 48.1; 32 / 8 heads of 128, 128 + 7 x 60 12.4 | 13.9, 300 + 9 x 40 15.6 | 28.7.
     const int64_t tiles = ((int64_t)p.rows * p.pack / 64 + p.B / 2) * (p.H / p.pack);
     if (p.rows <= 1536 && p.rows <= (int64_t)100 * p.B && tiles <= 400) return false;
     // rows without a stride between them have no tensor map

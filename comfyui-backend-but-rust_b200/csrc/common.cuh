@@ -21,6 +21,15 @@ enum DType { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
 
 typedef __nv_bfloat16 bf16;
 
+// SMs of the current device; 0 where there is none
+namespace b200q {
+inline int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return n;
+}
+}  // namespace b200q
+
 // ---- programmatic dependent launch ------------------------------------------------------------------------------------
 // The linears of a block are ten to fifteen short kernels one after the other, and between two of them a stream idles for
 // the drain of the first, the launch of the second and its setup (barriers, tensor memory, tensor maps): 2 to 4 us. So every

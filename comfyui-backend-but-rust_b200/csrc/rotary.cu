@@ -220,10 +220,14 @@ template <typename T> int launch_rotary(RotaryParams& p, cudaStream_t st) {
     int lanes = 1;
     while (lanes < 32 && lanes < slots) lanes *= 2;
     const int64_t tokens = (int64_t)p.B * p.L;
+    if (tokens / kMaxTokens >= INT32_MAX) return -1;
+    const int sms = b200q::sm_count();
+    if (sms <= 0) return (int)cudaErrorInvalidDevice;
+    // Tokens to a CTA: as many as leave four CTAs an SM. us with 1 | 2 | 4, 32 / 8 normalised heads of 128: 592 tokens 4.9 | 4.9 | 5.9, 1184 8.6 | 6.8 | 8.5, 2368
+    // 16.5 | 13.1 | 11.5, 8192 52.6 | 40.8 | 35.8; of 96, 40 values turned: 1184 10.5 | 10.3 | 12.8, 2368 19.1 | 17.2 | 18.6, 8192 64 | 56 | 53.
     p.tokens = 1;
-    while (p.tokens < kMaxTokens && tokens >= (int64_t)p.tokens * 2 * 592) p.tokens *= 2;
+    while (p.tokens < kMaxTokens && tokens >= (int64_t)p.tokens * 2 * 4 * sms) p.tokens *= 2;
     const int64_t ctas = (tokens + p.tokens - 1) / p.tokens;
-    if (ctas > INT32_MAX) return -1;
     auto kern = V == 8 ? rotary_kernel<T, 8> : V == 4 ? rotary_kernel<T, 4> : rotary_kernel<T, 1>;
     return launch_pdl(kern, dim3((unsigned)ctas), kThreads, p.tokens * p.half * sizeof(float2), st, p, lanes);
 }

@@ -58,11 +58,5 @@ inline EncodeTiledFn encode_fn() {
     fn.store(f, std::memory_order_release);
     return f;
 }
-inline int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    return n;
-}
-
 
 }  // namespace b200q
