@@ -7,6 +7,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #define GPU_API extern "C" __attribute__((visibility("default")))
 
 // dtype codes of the C ABI (the reference's src/ffi.rs:11-13)
@@ -21,11 +23,16 @@ enum DType { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
 
 typedef __nv_bfloat16 bf16;
 
-// SMs of the current device; 0 where there is none
+// SMs of the current device, asked for once; 0 where there is none
 namespace b200q {
 inline int sm_count() {
+    static std::atomic<int> count[64];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::atomic<int>& c = count[dev & 63];
+    if ((n = c.load(std::memory_order_relaxed)) != 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    c.store(n, std::memory_order_relaxed);
     return n;
 }
 }  // namespace b200q
